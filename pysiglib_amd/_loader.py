@@ -114,6 +114,30 @@ CUSIG_SIG_TO_LOG_SIG_BACKPROP = _table("sig_to_log_sig_backprop_cuda", lambda r:
     POINTER(r), POINTER(r), POINTER(r), c_uint64, c_uint64, c_uint64, c_int, c_bool))
 
 
+# operators on token sequences: an element type code and the stream to enqueue on, addresses as plain integers
+SEQUENCE_DTYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
+
+
+def _sequence(name, letters):
+    """``letters``: p pointer or stream, i int, u uint64, s int64 stride, f float, b bool."""
+    kinds = {"p": ctypes.c_void_p, "i": c_int, "u": c_uint64, "s": ctypes.c_int64, "f": c_float, "b": c_bool}
+    fn = getattr(CUSIG, "cusig_amd_" + name)
+    fn.argtypes = tuple(kinds[x] for x in letters)
+    fn.restype = c_int
+    return fn
+
+
+CUSIG_LINEAR_RECURRENCE = _sequence("linear_recurrence", "ippppppuuuusspup")
+CUSIG_LINEAR_RECURRENCE_BACKPROP = _sequence("linear_recurrence_backprop", "ipppppppppuuuusspup")
+CUSIG_LINEAR_RECURRENCE_STEP = _sequence("linear_recurrence_step", "ippppuussp")
+CUSIG_LINEAR_RECURRENCE_WORKSPACE = _sequence("linear_recurrence_workspace", "iuu")
+CUSIG_LINEAR_RECURRENCE_WORKSPACE.restype = c_uint64
+CUSIG_NORM_ROTARY = _sequence("norm_rotary", "ipppppppppuuuuuussssfbp")
+CUSIG_NORM_ROTARY_BACKPROP = _sequence("norm_rotary_backprop", "ipppppppppppppuuuuuussssssssfbpup")
+CUSIG_NORM_ROTARY_BACKPROP_WORKSPACE = _sequence("norm_rotary_backprop_workspace", "u")
+CUSIG_NORM_ROTARY_BACKPROP_WORKSPACE.restype = c_uint64
+
+
 def last_error_message():
     msg = CUSIG.cusig_last_error_message()
     return msg.decode("utf-8", errors="replace") if msg else ""

@@ -1,0 +1,385 @@
+"""The layers of a sequence model (pysiglib_amd/sequence.py) against their formulas in 64 bits, written out step by step in
+NumPy, and their gradients also against differences of those.
+
+Tolerances follow from the number formats.  u = 2^-24, 2^-8, 2^-11 is the largest relative rounding error of float32,
+bfloat16 and float16; an output rounded once is off by u times its size.  What 32-bit sums add is bounded for each operator
+where it is used."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+DEV = "cuda:0"
+ROUND = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+U32 = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+# float16 values below the normal numbers are spaced evenly
+SMALL = {torch.float32: 1e-37, torch.bfloat16: 1e-37, torch.float16: 2.0 ** -25}
+
+
+@pytest.fixture(scope="module")
+def P():
+    import pysiglib_amd
+    return pysiglib_amd
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def within(got, want, bound, what):
+    """Every value within the bound; infinities and NaN in the same places."""
+    got = f64(got)
+    assert got.shape == want.shape, what
+    fine = np.isfinite(want)
+    assert (np.isnan(got) == np.isnan(want)).all(), what
+    assert (got[~fine & ~np.isnan(want)] == want[~fine & ~np.isnan(want)]).all(), what
+    over = np.abs(got - want)[fine] - np.broadcast_to(bound, want.shape)[fine]
+    assert over.size == 0 or over.max() <= 0, (what, float(over.max()), float(np.abs(got - want)[fine].max()))
+
+
+# ---- the recurrence ----
+
+def recurrence_oracle(x, g, h0, starts, grad=None, grad_final=None, h=None):
+    """Step by step in 64 bits over packed rows.  Returns the outputs and, for each, a bound of what 32-bit steps may add:
+    a step rounds the decay (relative error (4 + |2 g|) u: the argument's product and the exponential) and the sum, so
+    E_t = a_t E_{t-1} + (8 + 2 |g_t|) u M_t, with M the recurrence of the sizes; composing runs of steps adds roundings of
+    the same products, at most as many again."""
+    rows, channels = x.shape
+    a = np.exp(g)
+    out, err = np.zeros_like(x), np.zeros_like(x)
+    final = h0.copy()
+    final_err = np.zeros_like(h0)
+    for i in range(len(starts) - 1):
+        s, m, e = h0[i].copy(), np.abs(h0[i]), np.zeros(channels)
+        for t in range(starts[i], starts[i + 1]):
+            s = a[t] * s + x[t]
+            m = a[t] * m + np.abs(x[t])
+            step = 2 * U32 * (8 + 2 * np.abs(np.where(np.isfinite(g[t]), g[t], 0.0))) * m
+            e = a[t] * e + step
+            out[t], err[t] = s, e
+        final[i], final_err[i] = s, e
+    if grad is None:
+        return (out, final), (err, final_err)
+    prev = np.concatenate((np.zeros((1, channels)), h[:-1])) if rows else h
+    dx, dg, d0 = np.zeros_like(x), np.zeros_like(x), grad_final.copy()
+    ex, eg, e0 = np.zeros_like(x), np.zeros_like(x), np.zeros_like(h0)
+    for i in range(len(starts) - 1):
+        c, m, e = grad_final[i].copy(), np.abs(grad_final[i]), np.zeros(channels)
+        for t in range(starts[i + 1] - 1, starts[i] - 1, -1):
+            before = h0[i] if t == starts[i] else prev[t]
+            dx[t], ex[t] = grad[t] + c, e + U32 * (m + np.abs(grad[t]))
+            m = a[t] * (m + np.abs(grad[t]))
+            c = a[t] * (c + grad[t])
+            e = a[t] * e + 2 * U32 * (8 + 2 * np.abs(np.where(np.isfinite(g[t]), g[t], 0.0))) * m
+            dg[t], eg[t] = c * before, (e + 2 * U32 * np.abs(c)) * np.abs(before)
+        d0[i], e0[i] = c, e
+    return (out, final, dx, dg, d0), (err, final_err, ex, eg, e0)
+
+
+def recurrence_inputs(dtype, rows, channels, n, seed, low=-2.0):
+    rng = np.random.default_rng(seed)
+    rate = np.exp(rng.uniform(-6, 1, channels))
+    g = np.maximum(-rate * rng.exponential(size=(rows, 1)), low * 10)
+    x, grad = rng.standard_normal((rows, channels)), rng.standard_normal((rows, channels))
+    make = lambda v: torch.tensor(v, dtype=torch.float64).to(dtype)                      # noqa: E731
+    single = lambda: torch.tensor(rng.standard_normal((n, channels)), dtype=torch.float32)   # noqa: E731
+    return make(x), make(g), single(), make(grad), single()
+
+
+def check_recurrence(P, x, g, h0, grad, grad_final, starts, shape=None, offsets=None, with_states=True):
+    """shape: of the batched call, or None with offsets."""
+    dtype = x.dtype
+    put = lambda t: t.to(DEV).reshape(shape) if shape else t.to(DEV)                     # noqa: E731
+    state = lambda t: t.to(DEV).reshape(*shape[:-2], shape[-1]) if shape else t.to(DEV)  # noqa: E731
+    options = dict(offsets=None if offsets is None else torch.tensor(offsets, dtype=torch.int32, device=DEV))
+    if with_states:
+        options["initial_state"] = state(h0)
+    else:
+        h0, grad_final = torch.zeros_like(h0), torch.zeros_like(grad_final)
+    h, final = P.linear_recurrence(put(x), put(g), **options)
+    back = P.linear_recurrence_backprop(h, put(g), put(grad), grad_final=state(grad_final) if with_states else None, **options)
+    again = P.linear_recurrence(put(x), put(g), **options), P.linear_recurrence_backprop(
+        h, put(g), put(grad), grad_final=state(grad_final) if with_states else None, **options)
+    for one, two in zip((h, final, *back), (*again[0], *again[1])):
+        assert torch.equal(one.nan_to_num(), two.nan_to_num()), "the same inputs give the same bits"
+    want, bound = recurrence_oracle(f64(x), f64(g), f64(h0), starts, f64(grad), f64(grad_final), f64(h).reshape(x.shape))
+    u = ROUND[dtype]
+    for name, got, w, b in zip(("h", "final", "dx", "dg", "d0"), (h, final, *back), want, bound):
+        rounded = (u if name in ("h", "dx", "dg") else U32) * (np.abs(w) + b) + SMALL[dtype if name in ("h", "dx", "dg") else torch.float32]
+        within(got.reshape(w.shape), w, b + rounded, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,length,channels", [(1, 1, 1), (3, 1, 5), (2, 129, 33), (1, 700, 130), (5, 17, 16), (2, 300, 67),
+                                                   (1, 9000, 9), (1, 6000, 70)])
+def test_recurrence_batched(P, dtype, batch, length, channels):
+    inputs = recurrence_inputs(dtype, batch * length, channels, batch, seed=length)
+    check_recurrence(P, *inputs, [i * length for i in range(batch + 1)], shape=(batch, length, channels))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,channels", [([1], 3), ([0, 5, 0, 0, 1, 130, 0], 40), ([400, 1, 1, 1, 126, 2, 128, 129], 133),
+                                              ([7] * 300, 5), ([1] * 1500, 3), ([0, 0], 4)])
+@pytest.mark.parametrize("with_states", [True, False])
+def test_recurrence_packed(P, dtype, lengths, channels, with_states):
+    starts = [0]
+    for n in lengths:
+        starts.append(starts[-1] + n)
+    inputs = recurrence_inputs(dtype, starts[-1], channels, len(lengths), seed=len(lengths))
+    check_recurrence(P, *inputs, starts, offsets=starts, with_states=with_states)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_recurrence_decays_at_the_ends_of_their_range(P, dtype):
+    """-inf forgets the state (also one that is infinite, in the chunks behind it), 0 keeps it, growth keeps a zero state."""
+    rows, channels = 700, 20
+    x, g, h0, grad, gf = recurrence_inputs(dtype, rows, channels, 1, seed=3)
+    g[:, 0] = 0.0
+    g[::7, 1] = -float("inf")
+    g[:, 2] = -float("inf")
+    g[:, 3], x[:, 3], h0[:, 3] = 1.0, 0.0, 0.0
+    x[650:, 3] = 1e-3
+    g[650:, 3] = 0.0
+    grad[:, 3], gf[:, 3] = 0.0, 0.0
+    g[:, 4] = -60.0
+    check_recurrence(P, x, g, h0, grad, gf, [0, rows], shape=(1, rows, channels))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels", [(1, 1), (3, 7), (64, 256), (5, 1030)])
+def test_recurrence_step_follows_the_scan(P, dtype, rows, channels):
+    x, g, h0, _, _ = recurrence_inputs(dtype, rows * 3, channels, rows, seed=rows)
+    both = torch.cat((x, g), 1).to(DEV).reshape(3, rows, 2 * channels)         # parts of one projection
+    state = h0.to(DEV)
+    want, e = f64(h0), 0.0
+    for t in range(3):
+        got = P.linear_recurrence_step(both[t, :, :channels], both[t, :, channels:], state)
+        gt, xt = f64(both[t, :, channels:]), f64(both[t, :, :channels])
+        size = np.exp(gt) * np.abs(want) + np.abs(xt)
+        want = np.exp(gt) * want + xt
+        e = np.exp(gt) * e + (8 + 2 * np.abs(gt)) * U32 * size
+        within(state, want, e + SMALL[torch.float32], "state")
+        within(got, want, e + ROUND[dtype] * (np.abs(want) + e) + SMALL[dtype], "h")
+
+
+@pytest.mark.gpu
+def test_recurrence_gradients_are_differences(P):
+    """Along random directions: <gradient, v> is the central difference of the loss in 64 bits, whose error is the third
+    derivative's, below 1e-6 of the terms at a step of 1e-4."""
+    rows, channels, starts = 90, 6, [0, 40, 41, 90]
+    x, g, h0, grad, gf = recurrence_inputs(torch.float32, rows, channels, 3, seed=8)
+    offsets = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    h, _ = P.linear_recurrence(x.to(DEV), g.to(DEV), initial_state=h0.to(DEV), offsets=offsets)
+    dx, dg, d0 = P.linear_recurrence_backprop(h, g.to(DEV), grad.to(DEV), grad_final=gf.to(DEV), initial_state=h0.to(DEV), offsets=offsets)
+
+    def loss(x, g, h0):
+        (h, final), _ = recurrence_oracle(x, g, h0, starts)
+        return (h * f64(grad)).sum() + (final * f64(gf)).sum()
+
+    rng = np.random.default_rng(0)
+    at, grads = [f64(x), f64(g), f64(h0)], [f64(dx), f64(dg), f64(d0)]
+    for k in range(3):
+        for _ in range(3):
+            v = rng.standard_normal(at[k].shape)
+            up, down = list(at), list(at)
+            up[k], down[k] = at[k] + 1e-4 * v, at[k] - 1e-4 * v
+            want = (loss(*up) - loss(*down)) / 2e-4
+            size = np.abs(grads[k] * v).sum()
+            assert abs((grads[k] * v).sum() - want) <= 1e-5 * size, k
+
+
+@pytest.mark.gpu
+def test_recurrence_takes_rows_apart_and_other_streams(P):
+    x, g, h0, grad, gf = recurrence_inputs(torch.bfloat16, 2 * 150, 24, 2, seed=5)
+    dense = P.linear_recurrence(x.to(DEV).reshape(2, 150, 24), g.to(DEV).reshape(2, 150, 24))
+    both = torch.cat((g, x, grad), 1).to(DEV).reshape(2, 150, 72)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        parts = P.linear_recurrence(both[..., 24:48], both[..., :24])
+        back = P.linear_recurrence_backprop(parts[0], both[..., :24], both[..., 48:])
+    side.synchronize()
+    want = P.linear_recurrence_backprop(dense[0], g.to(DEV).reshape(2, 150, 24), grad.to(DEV).reshape(2, 150, 24))
+    turned = P.linear_recurrence(both[..., 24:48].transpose(0, 1).contiguous().transpose(0, 1), both[..., :24])
+    for a, b in zip((*parts, *back, *turned), (*dense, *want, *dense)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_recurrence_of_nothing(P):
+    for shape in [(0, 5, 3), (2, 0, 3), (2, 5, 0)]:
+        x = torch.zeros(shape, device=DEV)
+        start = torch.ones((shape[0], shape[2]), device=DEV)
+        h, final = P.linear_recurrence(x, x, initial_state=start)
+        assert h.shape == x.shape
+        if shape[1] == 0:
+            assert torch.equal(final, start)
+        dx, dg, d0 = P.linear_recurrence_backprop(h, x, x, grad_final=start)
+        assert d0.shape == start.shape
+        if shape[1] == 0:
+            assert torch.equal(d0, start)
+    assert P.linear_recurrence_step(torch.zeros((0, 4), device=DEV), torch.zeros((0, 4), device=DEV), torch.zeros((0, 4), device=DEV)).shape == (0, 4)
+
+
+# ---- norms and rotation ----
+
+def rotary_oracle(x, w, cos, sin, positions, interleaved, eps, grad=None):
+    rows, heads, dim = x.shape
+    half = cos.shape[1]
+    one = 2 * np.arange(half) if interleaved else np.arange(half)
+    two = one + 1 if interleaved else one + half
+    c, s = cos[positions][:, None], sin[positions][:, None]
+
+    def turn(y, s):
+        z = y.copy()
+        z[..., one], z[..., two] = y[..., one] * c - y[..., two] * s, y[..., two] * c + y[..., one] * s
+        return z
+
+    r = 1 / np.sqrt((x * x).mean(-1, keepdims=True) + eps)
+    y = turn(x * r * w, s)
+    if grad is None:
+        return y
+    g = turn(grad, -s)
+    u = g * w
+    dx = r * (u - x * r * r * (u * x).mean(-1, keepdims=True))
+    return y, dx, (g * x * r).sum((0, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,heads,kv,dim,rotary,interleaved", [
+    (1, 1, 1, 2, 2, False), (1, 1, 1, 2, 0, True), (5, 3, 1, 64, 64, False), (33, 8, 2, 128, 128, True), (7, 5, 5, 96, 48, False),
+    (7, 6, 3, 90, 34, True), (4, 2, 2, 90, 34, False), (3, 40, 8, 128, 128, False), (700, 4, 4, 32, 20, False), (3, 2, 1, 256, 256, False),
+    (2, 0, 3, 72, 72, True), (3, 2, 0, 40, 8, False), (2100, 2, 1, 16, 6, True)])
+def test_norm_rotary(P, dtype, tokens, heads, kv, dim, rotary, interleaved):
+    rng = np.random.default_rng(dim + tokens)
+    rows = torch.tensor(rng.standard_normal((tokens, heads + 2 * kv, dim))).to(dtype).to(DEV)
+    q, k = rows[:, :heads], rows[:, heads:heads + kv]
+    if heads:
+        q[0, 0] = 0.0                   # a head of zeros: the norm is eps alone
+    if heads > 1:
+        q[-1, 1] *= 100.0
+    grads = [torch.tensor(rng.standard_normal((tokens, n, dim))).to(dtype).to(DEV) for n in (heads, kv)]
+    weights = [torch.tensor(1 + 0.3 * rng.standard_normal(dim), dtype=torch.float32, device=DEV) for _ in range(2)]
+    cos, sin = P.rotary_tables(50, rotary, base=1000., device=DEV)
+    positions = torch.tensor(rng.integers(0, 50, tokens), dtype=torch.int32, device=DEV)
+    args = (q, k, *weights, cos, sin, positions)
+    out = P.norm_rotary(*args, eps=1e-5, interleaved=interleaved)
+    back = P.norm_rotary_backprop(*grads, *args, eps=1e-5, interleaved=interleaved)
+    again = P.norm_rotary_backprop(*grads, *args, eps=1e-5, interleaved=interleaved)
+    for a, b in zip(back, again):
+        assert torch.equal(a, b)
+    u = ROUND[dtype]
+    for i, (x, w, g) in enumerate(zip((q, k), weights, grads)):
+        want = rotary_oracle(f64(x), f64(w), f64(cos), f64(sin), f64(positions).astype(int), interleaved, 1e-5, f64(g))
+        # sums of dim terms in 32 bits and a dozen roundings on the way, of values no larger than the row's largest
+        f32 = (dim + 16) * U32
+        size = np.abs(want[0]).max(-1, keepdims=True) if dim else 0.0
+        within(out[i], want[0], u * np.abs(want[0]) + f32 * size + SMALL[dtype], "out")
+        # the second term cancels the first where the gradient is along x: their sizes count, not the difference's
+        r = 1 / np.sqrt((f64(x) ** 2).mean(-1, keepdims=True) + 1e-5)
+        terms = 2 * r * (np.abs(f64(g)).max(-1, keepdims=True) * 2 * np.abs(f64(w)).max()) * (1 + (np.abs(f64(x)) * r).max(-1, keepdims=True) ** 2)
+        within(back[i], want[1], u * np.abs(want[1]) + f32 * terms + SMALL[dtype], "dx")
+        # tokens * heads terms added in pieces: at most 64 roundings deep in a lane, 64 slots, 512 / 16 + 16 pieces
+        n = max(tokens * max(heads, kv), 1)
+        each = np.abs(f64(x) * r).max() * np.abs(f64(g)).max() * 2 if x.numel() else 0.0
+        within(back[2 + i], want[2], (f32 + min(n, 512) * U32) * n * each, "dw")
+
+
+@pytest.mark.gpu
+def test_norm_rotary_gradients_are_differences(P):
+    rng = np.random.default_rng(2)
+    tokens, heads, dim = 3, 2, 12
+    x = torch.tensor(rng.standard_normal((tokens, heads, dim)), dtype=torch.float32, device=DEV)
+    w = torch.tensor(1 + 0.3 * rng.standard_normal(dim), dtype=torch.float32, device=DEV)
+    g = torch.tensor(rng.standard_normal((tokens, heads, dim)), dtype=torch.float32, device=DEV)
+    cos, sin = P.rotary_tables(9, 8, device=DEV)
+    positions = torch.tensor([8, 0, 3], dtype=torch.int32, device=DEV)
+    dx, _, dw, _ = P.norm_rotary_backprop(g, g, x, x, w, w, cos, sin, positions)
+    loss = lambda x, w: (rotary_oracle(x, w, f64(cos), f64(sin), np.array([8, 0, 3]), False, 1e-6) * f64(g)).sum()   # noqa: E731
+    for _ in range(4):
+        v, z = rng.standard_normal(x.shape), rng.standard_normal(dim)
+        d = (loss(f64(x) + 1e-4 * v, f64(w)) - loss(f64(x) - 1e-4 * v, f64(w))) / 2e-4
+        assert abs((f64(dx) * v).sum() - d) <= 1e-5 * np.abs(f64(dx) * v).sum()
+        d = (loss(f64(x), f64(w) + 1e-4 * z) - loss(f64(x), f64(w) - 1e-4 * z)) / 2e-4
+        assert abs((f64(dw) * z).sum() - d) <= 1e-5 * np.abs(f64(dw) * z).sum()
+
+
+@pytest.mark.gpu
+def test_norm_rotary_outside_the_tables_and_of_nothing(P):
+    q, w = torch.ones((3, 2, 8), device=DEV), torch.ones(8, device=DEV)
+    cos, sin = P.rotary_tables(4, 4, device=DEV)
+    out, _ = P.norm_rotary(q, q, w, w, cos, sin, torch.tensor([0, 4, -1], dtype=torch.int32, device=DEV))
+    assert torch.isfinite(out[0]).all() and torch.isnan(out[1:]).all()
+    none = torch.ones((0, 2, 8), device=DEV)
+    at = torch.zeros(0, dtype=torch.int32, device=DEV)
+    assert P.norm_rotary(none, none, w, w, cos, sin, at)[0].shape == (0, 2, 8)
+    assert (P.norm_rotary_backprop(none, none, none, none, w, w, cos, sin, at)[2] == 0).all()
+
+
+# ---- refusals ----
+
+@pytest.mark.gpu
+def test_refusals(P):
+    x, s = torch.zeros((2, 3, 4), device=DEV), torch.zeros((2, 4), device=DEV)
+    with pytest.raises(TypeError):
+        P.linear_recurrence(x.double(), x.double())
+    with pytest.raises(TypeError):
+        P.linear_recurrence(x, x.half())
+    with pytest.raises(ValueError):
+        P.linear_recurrence(x, x[:, :2])
+    with pytest.raises(ValueError):
+        P.linear_recurrence(x[0, 0], x[0, 0])
+    with pytest.raises(ValueError):
+        P.linear_recurrence(x, x, initial_state=s[:1])
+    with pytest.raises(TypeError):
+        P.linear_recurrence(x, x, initial_state=s.half())
+    with pytest.raises(ValueError):
+        P.linear_recurrence(x, x, offsets=torch.zeros(3, dtype=torch.int32, device=DEV))
+    with pytest.raises(TypeError):
+        P.linear_recurrence(x[0], x[0], offsets=torch.zeros(3, dtype=torch.int64, device=DEV))
+    with pytest.raises(ValueError):
+        P.linear_recurrence(x[0], x[0], offsets=torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        P.linear_recurrence_backprop(x, x, x[:1])
+    with pytest.raises(ValueError):
+        P.linear_recurrence_step(s, s, torch.zeros((4, 2), device=DEV).t())
+    with pytest.raises(TypeError):
+        P.linear_recurrence_step(s, s, s.half())
+    q, w = torch.zeros((2, 3, 8), device=DEV), torch.ones(8, device=DEV)
+    cos, sin = P.rotary_tables(4, 8, device=DEV)
+    at = torch.zeros(2, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError):
+        P.norm_rotary(q, q[:1], w, w, cos, sin, at)
+    with pytest.raises(ValueError):
+        P.norm_rotary(q, q, w[:4], w, cos, sin, at)
+    with pytest.raises(TypeError):
+        P.norm_rotary(q, q, w.half(), w, cos, sin, at)
+    with pytest.raises(ValueError):
+        P.norm_rotary(q[..., :6], q[..., :6], w[:6], w[:6], cos, sin, at)
+    with pytest.raises(ValueError):
+        P.norm_rotary(q[..., :7], q[..., :7], w[:7], w[:7], cos, sin, at)
+    with pytest.raises(TypeError):
+        P.norm_rotary(q, q, w, w, cos, sin, at.long())
+    with pytest.raises(TypeError):
+        P.norm_rotary(q, q, w, w, cos, sin, at, interleaved=1)
+    with pytest.raises(ValueError):
+        P.norm_rotary_backprop(q[:, :2], q, q, q, w, w, cos, sin, at)
+
+
+def test_refuses_host_tensors(P):
+    x = torch.zeros((2, 3))
+    with pytest.raises(RuntimeError):
+        P.linear_recurrence(x, x)
+    with pytest.raises(TypeError):
+        P.linear_recurrence(np.zeros((2, 3)), x)
+    with pytest.raises(ValueError):
+        P.rotary_tables(4, 3, device="cpu")
+    cos, sin = P.rotary_tables(4, 6, base=100., scale=2., device="cpu")
+    want = np.arange(4)[:, None] / 2 * 100.0 ** (-np.arange(3) / 3)
+    assert np.abs(f64(cos) - np.cos(want)).max() <= U32 and np.abs(f64(sin) - np.sin(want)).max() <= U32
