@@ -137,6 +137,10 @@ CUSIG_NORM_ROTARY_BACKPROP = _sequence("norm_rotary_backprop", "ipppppppppppppuu
 CUSIG_NORM_ROTARY_BACKPROP_WORKSPACE = _sequence("norm_rotary_backprop_workspace", "u")
 CUSIG_NORM_ROTARY_BACKPROP_WORKSPACE.restype = c_uint64
 
+CUSIG_ATTENTION = _sequence("attention", "ippppppppuuuuuussssssfbpup")
+CUSIG_ATTENTION_WORKSPACE = _sequence("attention_workspace", "uuuuuu")
+CUSIG_ATTENTION_WORKSPACE.restype = c_uint64
+
 
 def last_error_message():
     msg = CUSIG.cusig_last_error_message()

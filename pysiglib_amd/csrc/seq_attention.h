@@ -1,0 +1,201 @@
+// Pieces shared by the attention kernels: matrix products of 32 x 32 x 16, tiles in shared memory that are read by rows and
+// transposed, the place of a block among packed sequences.
+//
+// Operand layouts of the product (64 lanes, lane = 32 h + m): A holds row m, B column m, both with the eight elements
+// k = 8 h .. 8 h + 7 of the summed axis; the result holds column m, its i-th value the row (i & 3) + 8 (i >> 2) + 4 h.  The
+// summed axis may go in any order that is the same in A and B: the eight results of a lane i = 8 s .. 8 s + 7 are therefore a
+// B operand as they stand, if A takes its elements from rows 16 s + 4 h + (0..3) and 16 s + 8 + 4 h + (0..3), which is what two
+// transposing reads of four rows each give.
+#pragma once
+#include "seq_common.h"
+
+#include <cmath>
+
+namespace seqamd {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+using Frag = T __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x16 product(Frag<bf16> a, Frag<bf16> b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 product(Frag<f16> a, Frag<f16> b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ f32x16 zeros16()
+{
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+    return z;
+}
+
+// row of the result's i-th value
+__device__ __forceinline__ int row_in(int i, int half) { return (i & 3) + 8 * (i >> 2) + 4 * half; }
+
+// the other half's value
+__device__ __forceinline__ float swapped(float x)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// A tile in shared memory: rows of DP 16-bit elements, in chunks of eight, whose places in the row are exchanged by the
+// row's number: the 8 rows of a read by rows and the 8 rows of a transposing read (each 64 bytes wide) then lie in
+// different banks (64 banks of 4 bytes).
+template <int DP>
+struct Tile {
+    static constexpr int kChunks = DP / 8, kRowBytes = DP * 2;
+    static __device__ __forceinline__ int swizzle(int row)
+    {
+        static_assert(DP == 64 || DP == 128, "");
+        return DP == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    }
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * kRowBytes + ((chunk ^ swizzle(row)) << 4); }
+};
+
+// An operand by rows: lane (h, m) takes eight elements of row m.  at[k]: byte in the tile for summed elements 16 k .. 16 k + 15
+template <int DP>
+struct RowRead {
+    int at[DP / 16];
+    __device__ __forceinline__ RowRead(int lane)
+    {
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) at[k] = Tile<DP>::at(lane & 31, 2 * k + (lane >> 5));
+    }
+    // row0: a multiple of 32
+    template <typename T>
+    __device__ __forceinline__ Frag<T> get(const char* tile, int row0, int k) const
+    {
+        return *reinterpret_cast<const Frag<T>*>(tile + row0 * Tile<DP>::kRowBytes + at[k]);
+    }
+};
+
+// A transposed operand: lane (h, m) takes column 32 b + m of the rows 16 s + 4 h + (0..3) and 16 s + 8 + 4 h + (0..3).
+// A transposing read takes 8 bytes from each of 16 lanes, four lanes to a row, and gives lane i column i of the four rows.
+template <int DP>
+struct ColumnRead {
+    int at[DP / 32][2];
+    __device__ __forceinline__ ColumnRead(int lane)
+    {
+        const int h = lane >> 5, group = (lane >> 4) & 1, i = lane & 15;
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) at[b][t] = Tile<DP>::at(8 * t + 4 * h + (i >> 2), 4 * b + 2 * group + ((i & 3) >> 1)) + (i & 1) * 8;
+    }
+    // row0: a multiple of 16
+    template <typename T>
+    __device__ __forceinline__ Frag<T> get(const char* tile, int row0, int b) const
+    {
+        typedef __attribute__((address_space(3))) i16x4* Shared;
+        struct {
+            i16x4 x[2];
+        } r;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) r.x[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared)(tile + row0 * Tile<DP>::kRowBytes + at[b][t]));
+        return __builtin_bit_cast(Frag<T>, r);
+    }
+};
+
+// eight results as an operand, rounded to nearest: the one rounding between the two products
+template <typename T>
+__device__ __forceinline__ Frag<T> rounded(const f32x16& x, int first)
+{
+    Frag<T> f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = T(x[first + i]);
+    return f;
+}
+
+// Packed sequences.  Offsets are read on the device and kept inside the tensors whatever they hold.
+struct Packed {
+    const int *q_offsets, *k_offsets, *k_lengths;
+    int64_t q_rows, k_rows;
+    int n;
+};
+
+struct Span {
+    int64_t q0, k0;      // first rows
+    int nq, nk;
+    int tile, seq;       // tile among the sequence's; seq < 0: none
+};
+
+__device__ __forceinline__ int64_t kept(int64_t x, int64_t low, int64_t high) { return x < low ? low : (x > high ? high : x); }
+
+__device__ __forceinline__ void span_of(const Packed& p, int seq, Span& s)
+{
+    s.seq = seq;
+    s.q0 = kept(p.q_offsets[seq], 0, p.q_rows);
+    s.nq = int(kept(p.q_offsets[seq + 1], s.q0, p.q_rows) - s.q0);
+    s.k0 = kept(p.k_offsets[seq], 0, p.k_rows);
+    const int64_t room = kept(p.k_offsets[seq + 1], s.k0, p.k_rows) - s.k0;
+    s.nk = int(p.k_lengths ? kept(p.k_lengths[seq], 0, room) : room);
+}
+
+// The `wanted`-th tile of `size` rows, counted over the sequences (of keys: by their keys); with `last_first` from the end.
+// The whole block (THREADS of it) calls it; `space`: THREADS / 64 + 4 ints.
+template <int THREADS>
+__device__ Span find_tile(const Packed& p, int size, int wanted, bool keys, bool last_first, int* space)
+{
+    Span s;
+    s.seq = -1;
+    if (p.n == 1) {
+        span_of(p, 0, s);
+        const int tiles = ((keys ? s.nk : s.nq) + size - 1) / size;
+        s.tile = last_first ? tiles - 1 - wanted : wanted;
+        if (wanted >= tiles) s.seq = -1;
+        return s;
+    }
+    // each thread counts the tiles of some sequences, then a sum over the threads before it
+    const int tid = threadIdx.x, each = (p.n + THREADS - 1) / THREADS;
+    const int first = tid * each < p.n ? tid * each : p.n, past = first + each < p.n ? first + each : p.n;
+    auto count = [&](int seq) {
+        Span one;
+        span_of(p, seq, one);
+        return ((keys ? one.nk : one.nq) + size - 1) / size;
+    };
+    int own = 0;
+    for (int i = first; i < past; ++i) own += count(i);
+    int upto = own;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+        const int left = __shfl_up(upto, m);
+        if ((tid & 63) >= m) upto += left;
+    }
+    int* const found = space + THREADS / 64;
+    if ((tid & 63) == 63) space[tid >> 6] = upto;
+    if (tid == 0) found[0] = -1;
+    __syncthreads();
+    int total = 0;
+    for (int w = 0; w < THREADS / 64; ++w) {
+        if (w < (tid >> 6)) upto += space[w];
+        total += space[w];
+    }
+    const int target = last_first ? total - 1 - wanted : wanted;
+    if (target >= upto - own && target < upto) {
+        int before = upto - own;
+        for (int i = first; i < past; ++i) {
+            const int c = count(i);
+            if (target < before + c) {
+                found[0] = i;
+                found[1] = target - before;
+                break;
+            }
+            before += c;
+        }
+    }
+    __syncthreads();
+    const int seq = found[0];
+    if (seq >= 0) {
+        span_of(p, seq, s);
+        s.tile = found[1];
+    }
+    return s;
+}
+
+// most tiles of `size` rows that n sequences with `rows` rows in all have
+inline int64_t most_tiles(int64_t rows, int64_t n, int64_t size) { return rows / size + (rows < n ? rows : n); }
+
+}  // namespace seqamd

@@ -1,0 +1,243 @@
+// Attention over packed sequences: O = softmax(scale Q K^T) V with a query's visible keys, forward.
+//
+// Mathematics.  One pass over the keys with the running maximum m and sum l of each query: a tile's scores S change them to
+// m' = max(m, max S), l' = 2^(m - m') l + sum 2^(S - m'), O' = 2^(m - m') O + 2^(S - m') V, and at the end O / l.  Queries see the
+// keys up to their own place, counted from the sequences' ends; a query that sees none gets 0 and a log-sum of -infinity.
+// Everything but the operands of the products is 32-bit; the weights 2^(S - m) are rounded to the inputs' type for the second
+// product, which is the only rounding before the last.
+//
+// The products are formed transposed, S^T = K Q^T and O^T = V^T P^T: a lane then holds scores of a single query, its maximum
+// and sum need one exchange between lanes, and the weights are the second product's operand where they stand.
+#include "seq_attention.h"
+
+namespace seqamd {
+namespace {
+
+struct AttentionArgs {
+    const void *q, *k, *v;
+    void* out;               // [q_rows][heads][dim]
+    float* lse;              // [q_rows][heads]
+    Packed packed;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+    int heads, kv_heads, dim, causal;
+    float scale;             // times log2(e)
+};
+
+constexpr int kKeys = 64;    // of a tile
+constexpr float kSlack = 8.0f;   // the maximum is taken over where it grew by more than this (in powers of two): weights stay below 2^8
+
+// WAVES waves of QB * 32 queries each
+template <typename T, int DP, int QB, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) attention_kernel(AttentionArgs p)
+{
+    constexpr int kThreads = WAVES * 64, kRows = 32 * QB * WAVES, kSlices = DP / 16, kBlocks = DP / 32;
+    constexpr int kTileBytes = kKeys * Tile<DP>::kRowBytes, kLoads = kKeys * Tile<DP>::kChunks / kThreads;
+    __shared__ __attribute__((aligned(16))) char s_tiles[2][2][kTileBytes];
+    __shared__ int s_space[WAVES + 4];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
+    // the heads that share keys and values follow each other at a distance of kv_heads: on the same die where that is a multiple of 8
+    const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
+    // the last tiles see the most keys: they begin first
+    const Span at = find_tile<kThreads>(p.packed, kRows, blockIdx.x / p.heads, false, true, s_space);
+    if (at.seq < 0) return;
+    const int q_first = at.tile * kRows, shift = at.nk - at.nq;
+    // keys that any query of the block sees
+    const int q_past = q_first + kRows < at.nq ? q_first + kRows : at.nq;
+    int keys = at.nk;
+    if (p.causal && q_past + shift < keys) keys = q_past + shift < 0 ? 0 : q_past + shift;
+    const int tiles = (keys + kKeys - 1) / kKeys;
+
+    const RowRead<DP> rows(lane);
+    const ColumnRead<DP> columns(lane);
+    int query[QB];
+    Frag<T> q[QB][kSlices];
+    f32x16 o[QB][kBlocks];
+    float top[QB], sum[QB];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        query[b] = q_first + (wave * QB + b) * 32 + (lane & 31);
+        const int row = query[b] < at.nq ? query[b] : at.nq - 1;
+        const T* from = static_cast<const T*>(p.q) + (at.q0 + row) * p.q_token + head * p.q_head;
+#pragma unroll
+        for (int k = 0; k < kSlices; ++k) {
+            const int d = 16 * k + 8 * half;
+            u32x4 x = {0, 0, 0, 0};
+            if (d < p.dim) __builtin_memcpy(&x, from + d, 16);
+            q[b][k] = __builtin_bit_cast(Frag<T>, x);
+        }
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d) o[b][d] = zeros16();
+        top[b] = -INFINITY;
+        sum[b] = 0.0f;
+    }
+
+    u32x4 next[2][kLoads];
+    auto fetch = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int e = i * kThreads + tid, row = e / Tile<DP>::kChunks, chunk = e % Tile<DP>::kChunks;
+            const int key = tile * kKeys + row < at.nk ? tile * kKeys + row : at.nk - 1;      // rows past the end are never used
+            next[0][i] = next[1][i] = u32x4{0, 0, 0, 0};
+            if (chunk * 8 < p.dim) {
+                __builtin_memcpy(&next[0][i], static_cast<const T*>(p.k) + (at.k0 + key) * p.k_token + kv * p.k_head + chunk * 8, 16);
+                __builtin_memcpy(&next[1][i], static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head + chunk * 8, 16);
+            }
+        }
+    };
+    auto put = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int e = i * kThreads + tid, to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
+            *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + to) = next[0][i];
+            *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + to) = next[1][i];
+        }
+    };
+    if (tiles) {
+        fetch(0);
+        put(0);
+    }
+    for (int tile = 0; tile < tiles; ++tile) {
+        __syncthreads();
+        if (tile + 1 < tiles) fetch(tile + 1);
+        const char *kt = s_tiles[tile & 1][0], *vt = s_tiles[tile & 1][1];
+        const int key0 = tile * kKeys;
+        f32x16 s[QB][kKeys / 32];
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) {
+#pragma unroll
+            for (int b = 0; b < QB; ++b) s[b][c] = zeros16();
+#pragma unroll
+            for (int k = 0; k < kSlices; ++k) {
+                const Frag<T> kf = rows.template get<T>(kt, 32 * c, k);
+#pragma unroll
+                for (int b = 0; b < QB; ++b) s[b][c] = product(kf, q[b][k], s[b][c]);
+            }
+        }
+        // a key is hidden past the sequence's end, or behind the query's place
+        const bool cut = key0 + kKeys > at.nk || (p.causal && key0 + kKeys - 1 > q_first + wave * QB * 32 + shift);
+        if (cut)
+#pragma unroll
+            for (int b = 0; b < QB; ++b) {
+                const int last = p.causal && query[b] + shift < at.nk - 1 ? query[b] + shift : at.nk - 1;
+#pragma unroll
+                for (int c = 0; c < kKeys / 32; ++c)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (key0 + 32 * c + row_in(i, half) > last) s[b][c][i] = -INFINITY;
+            }
+        Frag<T> w[QB][kKeys / 16];
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+            float most = s[b][0][0];
+#pragma unroll
+            for (int c = 0; c < kKeys / 32; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, s[b][c][i]);
+            most = fmaxf(most, swapped(most)) * p.scale;
+            if (__any(most > top[b] + kSlack || (top[b] == -INFINITY && most > top[b]))) {
+                const float now = fmaxf(top[b], most), shrink = top[b] == now ? 1.0f : exp2f(top[b] - now);
+                top[b] = now;
+                sum[b] *= shrink;
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[b][d][i] *= shrink;
+            }
+            const float base = top[b] == -INFINITY ? 0.0f : top[b];
+#pragma unroll
+            for (int c = 0; c < kKeys / 32; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[b][c][i] = __builtin_amdgcn_exp2f(fmaf(s[b][c][i], p.scale, -base));
+                    sum[b] += s[b][c][i];
+                }
+#pragma unroll
+            for (int c = 0; c < kKeys / 16; ++c) w[b][c] = rounded<T>(s[b][c / 2], 8 * (c & 1));
+        }
+#pragma unroll
+        for (int c = 0; c < kKeys / 16; ++c)
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) {
+                const Frag<T> vf = columns.template get<T>(vt, 16 * c, d);
+#pragma unroll
+                for (int b = 0; b < QB; ++b) o[b][d] = product(vf, w[b][c], o[b][d]);
+            }
+        if (tile + 1 < tiles) put((tile + 1) & 1);
+    }
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        const float total = sum[b] + swapped(sum[b]);
+        if (query[b] >= at.nq) continue;
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        const int64_t row = (at.q0 + query[b]) * p.heads + head;
+        if (half == 0) p.lse[row] = total == 0.0f ? -INFINITY : 0.69314718055994531f * (top[b] + log2f(total));
+        T* to = static_cast<T*>(p.out) + row * p.dim;
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int ch = 32 * d + row_in(i, half);
+                if (ch < p.dim) {
+                    float x[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[j] = o[b][d][i + j] * inv;
+                    Pack<T, 4> pack;
+                    pack.set(x);
+                    store_pack<T, 4>(to + ch, pack);
+                }
+            }
+    }
+}
+
+template <typename T, int DP>
+void forward(const AttentionArgs& p, hipStream_t stream)
+{
+        constexpr int QB = 1, WAVES = 8, kRows = 32 * QB * WAVES;
+    const int64_t blocks = most_tiles(p.packed.q_rows, p.packed.n, kRows) * p.heads;
+    require(blocks < (int64_t(1) << 31), "too many queries and heads");
+    hipLaunchKernelGGL((attention_kernel<T, DP, QB, WAVES>), dim3(unsigned(blocks)), dim3(WAVES * 64), 0, stream, p);
+    SIG_HIP(hipGetLastError());
+}
+
+}  // namespace
+}  // namespace seqamd
+
+using namespace seqamd;
+
+extern "C" {
+
+__attribute__((visibility("default"))) uint64_t cusig_amd_attention_workspace(uint64_t q_rows, uint64_t k_rows, uint64_t sequences, uint64_t heads,
+                                                                            uint64_t kv_heads, uint64_t dim) noexcept
+{
+    (void)q_rows, (void)k_rows, (void)sequences, (void)heads, (void)kv_heads, (void)dim;
+    return 0;
+}
+
+__attribute__((visibility("default"))) int cusig_amd_attention(
+    int dtype, const void* q, const void* k, const void* v, const int* q_offsets, const int* k_offsets, const int* k_lengths, void* out, float* lse,
+    uint64_t q_rows, uint64_t k_rows, uint64_t sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim, int64_t q_token, int64_t q_head, int64_t k_token,
+    int64_t k_head, int64_t v_token, int64_t v_head, float scale, bool causal, void* workspace, uint64_t workspace_bytes, void* stream) noexcept
+{
+    return sigamd::guarded([&] {
+        (void)workspace, (void)workspace_bytes;
+        require(q_rows < (uint64_t(1) << 31) && k_rows < (uint64_t(1) << 31) && sequences < (uint64_t(1) << 31), "too many rows or sequences");
+        require(dim >= 8 && dim <= 128 && dim % 8 == 0, "a head has 8 to 128 channels, a multiple of 8");
+        require(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads < (1u << 20), "heads are a multiple of the key heads");
+        require(scale > 0.0f && std::isfinite(scale), "the scale is positive and finite");
+        if (q_rows == 0 || sequences == 0) return;
+        AttentionArgs p{};
+        p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
+        p.packed = Packed{q_offsets, k_offsets, k_lengths, int64_t(q_rows), int64_t(k_rows), int(sequences)};
+        p.q_token = q_token, p.q_head = q_head, p.k_token = k_token, p.k_head = k_head, p.v_token = v_token, p.v_head = v_head;
+        p.heads = int(heads), p.kv_heads = int(kv_heads), p.dim = int(dim), p.causal = causal;
+        p.scale = scale * 1.44269504088896341f;
+        const hipStream_t s = static_cast<hipStream_t>(stream);
+        switch (dtype) {
+        case kBF16: dim <= 64 ? forward<bf16, 64>(p, s) : forward<bf16, 128>(p, s); break;
+        case kF16: dim <= 64 ? forward<f16, 64>(p, s) : forward<f16, 128>(p, s); break;
+        default: throw std::invalid_argument("attention takes bfloat16 or float16");
+        }
+    });
+}
+
+}  // extern "C"

@@ -13,7 +13,7 @@ import math
 
 import torch
 
-from ._loader import (CUSIG_LINEAR_RECURRENCE, CUSIG_LINEAR_RECURRENCE_BACKPROP, CUSIG_LINEAR_RECURRENCE_STEP,
+from ._loader import (CUSIG_ATTENTION, CUSIG_ATTENTION_WORKSPACE, CUSIG_LINEAR_RECURRENCE, CUSIG_LINEAR_RECURRENCE_BACKPROP, CUSIG_LINEAR_RECURRENCE_STEP,
                       CUSIG_LINEAR_RECURRENCE_WORKSPACE, CUSIG_NORM_ROTARY, CUSIG_NORM_ROTARY_BACKPROP,
                       CUSIG_NORM_ROTARY_BACKPROP_WORKSPACE, SEQUENCE_DTYPES)
 from .data_handlers import on_device
@@ -283,3 +283,55 @@ def norm_rotary_backprop(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin, pos
           positions.data_ptr(), dq.data_ptr(), dk.data_ptr(), dw.data_ptr(), dw.data_ptr() + 4 * dim, *sizes, gq_token, gq_head,
           gk_token, gk_head, eps, interleaved, space.data_ptr(), size)
     return dq, dk, dw[0], dw[1]
+
+
+def _attention_args(q, k, v, q_offsets, k_offsets, causal, scale):
+    check_type(causal, "causal", bool)
+    q, q_token, q_head = _heads(q, "q", None)
+    if q.dtype == torch.float32:
+        raise TypeError("q.dtype must be bfloat16 or float16, got torch.float32 instead")
+    dim, device = q.shape[2], q.device
+    k, k_token, k_head = _heads(k, "k", q, None, dim)
+    v, v_token, v_head = _heads(v, "v", q, k.shape[0], dim)
+    heads, kv_heads = q.shape[1], k.shape[1]
+    if v.shape[1] != kv_heads:
+        raise ValueError("k and v must have the same heads")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError("the heads of q must be a multiple of those of k, got " + str(heads) + " and " + str(kv_heads))
+    if dim < 8 or dim > 128 or dim % 8:
+        raise ValueError("q, k and v must have 8 to 128 channels to a head, a multiple of 8, got " + str(dim))
+    q_offsets, k_offsets = _offsets(q_offsets, "q_offsets", device), _offsets(k_offsets, "k_offsets", device)
+    if q_offsets.shape != k_offsets.shape:
+        raise ValueError("q_offsets and k_offsets must have the same length")
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError("scale must be positive and finite, got " + str(scale))
+    return (q, k, v, q_offsets, k_offsets, (q.shape[0], k.shape[0], q_offsets.shape[0] - 1, heads, kv_heads, dim),
+            (q_token, q_head, k_token, k_head, v_token, v_head, scale, causal))
+
+
+def attention(q, k, v, q_offsets, k_offsets, *, k_lengths=None, causal=True, scale=None):
+    """Softmax attention over packed sequences: query ``j`` of a sequence with ``n`` queries and ``m`` keys sees, with ``causal``,
+    the keys up to ``j + m - n`` (both count from the sequences' ends), otherwise all of them.  A query that sees no key gets 0.
+
+    ``q`` ``(rows, heads, dim)``, ``k`` and ``v`` ``(key rows, key heads, dim)``, bfloat16 or float16; ``heads`` is a multiple of the
+    key heads, which neighbouring heads share; ``dim`` a multiple of 8 up to 128.  ``q_offsets``, ``k_offsets``: where sequences
+    begin, see above.  ``k_lengths`` (int32, a number for each sequence): only that many keys from ``k_offsets[i]`` on are in
+    use, as in a cache with room for more: with one query to each sequence this is the form for single tokens.  ``scale`` of
+    the scores: ``dim ** -0.5`` where it is not given.
+
+    Returns ``(out, lse)``: ``out`` like ``q``, and the logarithm of the sum of exponentials of each query's scores, float32
+    ``(rows, heads)``.
+    """
+    q, k, v, q_offsets, k_offsets, sizes, rest = _attention_args(q, k, v, q_offsets, k_offsets, causal, scale)
+    device = q.device
+    if k_lengths is not None:
+        k_lengths = _other(k_lengths, "k_lengths", torch.int32, (sizes[2],), device)
+    out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device)
+    size = CUSIG_ATTENTION_WORKSPACE(*sizes)
+    space = _workspace(size, device) if size else None
+    _call(CUSIG_ATTENTION, "attention", device, _CODES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), q_offsets.data_ptr(),
+          k_offsets.data_ptr(), 0 if k_lengths is None else k_lengths.data_ptr(), out.data_ptr(), lse.data_ptr(), *sizes, *rest,
+          space.data_ptr() if size else 0, size)
+    return out, lse

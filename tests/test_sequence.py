@@ -34,8 +34,9 @@ def within(got, want, bound, what):
     fine = np.isfinite(want)
     assert (np.isnan(got) == np.isnan(want)).all(), what
     assert (got[~fine & ~np.isnan(want)] == want[~fine & ~np.isnan(want)]).all(), what
-    over = np.abs(got - want)[fine] - np.broadcast_to(bound, want.shape)[fine]
-    assert over.size == 0 or over.max() <= 0, (what, float(over.max()), float(np.abs(got - want)[fine].max()))
+    off = np.abs(got[fine] - want[fine])
+    over = off - np.broadcast_to(bound, want.shape)[fine]
+    assert over.size == 0 or over.max() <= 0, (what, float(over.max()), float(off.max()))
 
 
 # ---- the recurrence ----
@@ -322,6 +323,158 @@ def test_norm_rotary_outside_the_tables_and_of_nothing(P):
     assert (P.norm_rotary_backprop(none, none, none, none, w, w, cos, sin, at)[2] == 0).all()
 
 
+# ---- attention ----
+
+def starts_of(lengths):
+    out = [0]
+    for n in lengths:
+        out.append(out[-1] + n)
+    return out
+
+
+def attention_oracle(q, k, v, q_lengths, k_places, k_lengths, causal, scale, grad=None, u=0.0):
+    """One sequence and head after the other.  Returns (out, lse[, dq, dk, dv]) and a bound for each of them.
+
+    A score is a sum of dim products in 32 bits: off by e = (dim + 8) u32 scale |q||k|, so its weight by 2 e of its size; a
+    weight is rounded to the inputs' type (u) before the second product, and weights far below the largest by 2^-24 of that
+    (float16 has no smaller numbers); sums of n terms in 32 bits add (n + 16) u32 of their terms' sizes.  Backward, ds =
+    p (dp - delta) is rounded likewise, and delta comes from the rounded output: off by u times |grad||out|."""
+    heads, dim = q.shape[1:]
+    group = heads // k.shape[1]
+    out, lse = np.zeros_like(q), np.full(q.shape[:2], -np.inf)
+    b_out, b_lse = np.zeros_like(q), np.zeros(q.shape[:2])
+    grads = [np.zeros_like(t) for t in (q, k, v)]
+    bounds = [np.zeros_like(t) for t in (q, k, v)]
+    first = 0
+    for n, a in enumerate(q_lengths):
+        rows, cols = slice(first, first + a), slice(k_places[n], k_places[n] + k_lengths[n])
+        first += a
+        m = k_lengths[n]
+        if not m or not a:
+            continue
+        hidden = np.arange(m)[None] > np.arange(a)[:, None] + m - a if causal else np.zeros((a, m), bool)
+        for h in range(heads):
+            Q, K, V = q[rows, h], k[cols, h // group], v[cols, h // group]
+            score = np.where(hidden, -np.inf, Q @ K.T * scale)
+            e = (dim + 8) * U32 * scale * (np.abs(Q) @ np.abs(K).T)
+            top = score.max(1, keepdims=True)
+            top[top == -np.inf] = 0.0
+            w = np.exp(score - top)
+            total = w.sum(1, keepdims=True)
+            seen = total > 0
+            total[~seen] = 1.0
+            w = w / total
+            e = np.where(hidden, 0.0, e)
+            off = 2 * e.max(1, keepdims=True) + u + (m + 16) * U32
+            tiny = m * 2.0 ** -24 * np.abs(V).max()
+            out[rows, h] = w @ V
+            b_out[rows, h] = np.where(seen, 2 * off * (w @ np.abs(V)) + tiny, 0.0)
+            with np.errstate(divide="ignore"):
+                lse[rows, h] = np.where(seen, top + np.log(total), -np.inf)[:, 0]
+            b_lse[rows, h] = (off - u)[:, 0] + 4 * U32 * (np.abs(top[:, 0]) + 16)
+            if grad is None:
+                continue
+            G = grad[rows, h]
+            dp = G @ V.T
+            delta = (G * out[rows, h]).sum(1, keepdims=True)
+            ds = w * (dp - delta)
+            # |dp - delta| at its largest, and its own error: delta's, and 32-bit sums of dim terms
+            wrong = (u + (dim + 16) * U32) * (np.abs(G) * (np.abs(out[rows, h]) + b_out[rows, h])).sum(1, keepdims=True) + (
+                dim + 8) * U32 * (np.abs(G) @ np.abs(V).T) + (np.abs(G) * b_out[rows, h]).sum(1, keepdims=True)
+            b_ds = w * ((off + u) * (np.abs(dp) + np.abs(delta)) + wrong) + 2.0 ** -24 * (np.abs(dp) + np.abs(delta))
+            b_ds = np.where(hidden, 0.0, b_ds)
+            b_w = np.where(hidden, 0.0, w * (off + u) + 2.0 ** -24)
+            grads[0][rows, h] = ds @ K * scale
+            bounds[0][rows, h] = (b_ds + (m + 16) * U32 * np.abs(ds)) @ np.abs(K) * scale
+            grads[1][cols, h // group] += ds.T @ Q * scale
+            bounds[1][cols, h // group] += (b_ds + (a * group + 16) * U32 * np.abs(ds)).T @ np.abs(Q) * scale
+            grads[2][cols, h // group] += w.T @ G
+            bounds[2][cols, h // group] += (b_w + (a * group + 16) * U32 * w).T @ np.abs(G)
+    if grad is None:
+        return (out, lse), (b_out, b_lse)
+    return (out, lse, *grads), (b_out, b_lse, *bounds)
+
+
+def attention_inputs(dtype, q_rows, k_rows, heads, kv, dim, seed):
+    rng = np.random.default_rng(seed)
+    make = lambda rows, h, std: torch.tensor(std * rng.standard_normal((rows, h, dim))).to(dtype).to(DEV)      # noqa: E731
+    return make(q_rows, heads, 1.4), make(k_rows, kv, 1.4), make(k_rows, kv, 1.0), make(q_rows, heads, 1.0)
+
+
+HALVES = [torch.bfloat16, torch.float16]
+SEQUENCES = [([1], [1]), ([0, 3, 0], [0, 3, 0]), ([64], [64]), ([65, 1, 255, 256, 257, 31], None), ([700], None), ([2] * 70, None),
+             ([5, 1, 0, 7, 40], [130, 0, 9, 3, 33]), ([300], [290]), ([90], [500]), ([1, 1, 2], [900, 65, 64])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("queries,keys", SEQUENCES)
+@pytest.mark.parametrize("heads,kv,dim,causal", [(1, 1, 64, True), (4, 2, 128, True), (6, 1, 40, False), (3, 3, 96, True), (2, 2, 8, True),
+                                                 (8, 1, 128, False)])
+def test_attention(P, dtype, queries, keys, heads, kv, dim, causal):
+    keys = keys or queries
+    qs, ks = starts_of(queries), starts_of(keys)
+    q, k, v, _ = attention_inputs(dtype, qs[-1], ks[-1], heads, kv, dim, seed=dim + qs[-1])
+    offsets = [torch.tensor(s, dtype=torch.int32, device=DEV) for s in (qs, ks)]
+    out, lse = P.attention(q, k, v, *offsets, causal=causal)
+    u = ROUND[dtype]
+    want, bound = attention_oracle(f64(q), f64(k), f64(v), queries, ks, keys, causal, dim ** -0.5, u=u)
+    within(out, want[0], bound[0] + u * (np.abs(want[0]) + bound[0]) + SMALL[dtype], "out")
+    within(lse, want[1], bound[1], "lse")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("lengths,heads,kv,dim", [([1], 1, 1, 64), ([0, 5, 64, 65, 700, 33], 8, 2, 128), ([2500, 1, 3000], 12, 1, 40),
+                                                  ([129] * 40, 4, 4, 64), ([4100], 5, 1, 128), ([300, 0, 17], 48, 1, 64)])
+@pytest.mark.parametrize("queries", [1, 2, 5])
+def test_attention_against_a_cache(P, dtype, lengths, heads, kv, dim, queries):
+    """A few new tokens of each sequence, keys and values in a cache with room for more: what lies behind the lengths is
+    never looked at, here it is not a number."""
+    room, n = max(lengths) + 3, len(lengths)
+    q, k, v, _ = attention_inputs(dtype, n * queries, n * room, heads, kv, dim, seed=room)
+    for i, m in enumerate(lengths):
+        k[i * room + m:(i + 1) * room] = float("nan")
+        v[i * room + m:(i + 1) * room] = float("inf")
+    places = [i * room for i in range(n + 1)]
+    whole = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)         # noqa: E731
+    out, lse = P.attention(q, k, v, whole([i * queries for i in range(n + 1)]), whole(places), k_lengths=whole(lengths), scale=0.11)
+    again = P.attention(q, k, v, whole([i * queries for i in range(n + 1)]), whole(places), k_lengths=whole(lengths), scale=0.11)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    u = ROUND[dtype]
+    want, bound = attention_oracle(f64(q), f64(k), f64(v), [queries] * n, places, lengths, True, 0.11, u=u)
+    within(out, want[0], bound[0] + u * (np.abs(want[0]) + bound[0]) + SMALL[dtype], "out")
+    within(lse, want[1], bound[1], "lse")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+def test_attention_of_parts_of_a_projection_with_large_scores(P, dtype):
+    """Rows with gaps; scores in the hundreds, so that weights run from 1 to nothing and the maximum moves late."""
+    lengths, heads, kv, dim = [200, 77], 4, 2, 64
+    starts = starts_of(lengths)
+    rng = np.random.default_rng(4)
+    rows = torch.tensor(rng.standard_normal((277, heads + 2 * kv, dim))).to(dtype).to(DEV)
+    rows[:, :heads] *= 20.0
+    rows[150, heads:heads + kv] *= 30.0
+    offsets = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    q, k, v = rows[:, :heads], rows[:, heads:heads + kv], rows[:, heads + kv:]
+    out, lse = P.attention(q, k, v, offsets, offsets, causal=True)
+    u = ROUND[dtype]
+    want, bound = attention_oracle(f64(q), f64(k), f64(v), lengths, starts, lengths, True, dim ** -0.5, u=u)
+    within(out, want[0], bound[0] + u * (np.abs(want[0]) + bound[0]) + SMALL[dtype], "out")
+    within(lse, want[1], bound[1], "lse")
+
+
+@pytest.mark.gpu
+def test_attention_of_nothing(P):
+    q, k = torch.zeros((0, 2, 64), dtype=torch.bfloat16, device=DEV), torch.zeros((3, 1, 64), dtype=torch.bfloat16, device=DEV)
+    zero, at = torch.tensor([0, 0], dtype=torch.int32, device=DEV), torch.tensor([0, 3], dtype=torch.int32, device=DEV)
+    assert P.attention(q, k, k, zero, at)[0].shape == (0, 2, 64)
+    out, lse = P.attention(torch.ones((3, 2, 64), dtype=torch.bfloat16, device=DEV), k[:0], k[:0], at, zero)
+    assert (out == 0).all() and (lse == -float("inf")).all()
+
+
 # ---- refusals ----
 
 @pytest.mark.gpu
@@ -370,6 +523,19 @@ def test_refusals(P):
         P.norm_rotary(q, q, w, w, cos, sin, at, interleaved=1)
     with pytest.raises(ValueError):
         P.norm_rotary_backprop(q[:, :2], q, q, q, w, w, cos, sin, at)
+    q = torch.zeros((4, 4, 64), dtype=torch.float16, device=DEV)
+    k, at = q[:, :2], torch.tensor([0, 4], dtype=torch.int32, device=DEV)
+    assert P.attention(q, k, k, at, at)[0].shape == q.shape
+    for args in [(q.float(), k.float(), k.float(), at, at), (q, k.bfloat16(), k, at, at), (q, k, k, at.long(), at)]:
+        with pytest.raises(TypeError):
+            P.attention(*args)
+    for args in [(q, k, k[:, :1], at, at), (q, q[:, :3], q[:, :3], at, at), (q[..., :60], k[..., :60], k[..., :60], at, at), (q, k, k, at, at[:1]),
+                 (q, k, k[:2], at, at), (q[:, :0], k, k, at, at), (q.repeat(1, 1, 3), k.repeat(1, 1, 3), k.repeat(1, 1, 3), at, at)]:
+        with pytest.raises(ValueError):
+            P.attention(*args)
+    for options in [dict(scale=0.0), dict(scale=float("inf")), dict(k_lengths=at)]:
+        with pytest.raises(ValueError):
+            P.attention(q, k, k, at, at, **options)
 
 
 def test_refuses_host_tensors(P):
