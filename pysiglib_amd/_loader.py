@@ -140,6 +140,9 @@ CUSIG_NORM_ROTARY_BACKPROP_WORKSPACE.restype = c_uint64
 CUSIG_ATTENTION = _sequence("attention", "ippppppppuuuuuussssssfbpup")
 CUSIG_ATTENTION_WORKSPACE = _sequence("attention_workspace", "uuuuuu")
 CUSIG_ATTENTION_WORKSPACE.restype = c_uint64
+CUSIG_ATTENTION_BACKPROP = _sequence("attention_backprop", "ipppppppppppuuuuuussssssssfbpup")
+CUSIG_ATTENTION_BACKPROP_WORKSPACE = _sequence("attention_backprop_workspace", "uu")
+CUSIG_ATTENTION_BACKPROP_WORKSPACE.restype = c_uint64
 
 
 def last_error_message():

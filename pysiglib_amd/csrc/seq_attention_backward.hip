@@ -1,0 +1,422 @@
+// Gradients of the attention over packed sequences.
+//
+// Mathematics.  With the forward's log-sums, P = 2^(scale' S - lse') is formed again tile by tile.  delta = rowsum(dO . O),
+// dS = P . (dO V^T - delta), dQ = scale dS K, dK = scale dS^T Q, dV = P^T dO.
+//
+// Two kernels, one with its queries fixed (dQ and delta), one with its keys fixed (dK and dV, over all query heads that share
+// them): seven products instead of the five that one kernel would form, but every sum belongs to one block, so nothing is
+// added through memory in an order that changes from call to call.
+//
+// Keys fixed: a wave cannot hold sums, keys and values of 64 keys of 128 channels at once with two waves to a SIMD, so waves
+// work in pairs.  The first forms P of a tile of queries and adds to dV, the second, one tile behind, takes P from shared
+// memory, forms dS and adds to dK.  Operands are rounded to the inputs' type (P, dS), sums are 32-bit.
+#include "seq_attention.h"
+
+namespace seqamd {
+namespace {
+
+struct GradArgs {
+    const void *q, *k, *v, *out, *grad;       // out and grad: [q_rows][heads][dim]
+    const float* lse;
+    void *dq, *dk, *dv;                       // contiguous
+    float* delta;                             // [q_rows][heads]
+    unsigned* largest;                        // float16: bits of the largest |grad|, zero at the start
+    Packed packed;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, g_token, g_head;
+    int heads, kv_heads, dim, causal;
+    float scale, scale2;                      // scale2 = scale * log2(e)
+};
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+// float16 holds dS only near 1: it is formed from gradients multiplied by a power of two that brings the largest there
+__device__ __forceinline__ float towards_one(float largest)
+{
+    return largest > 0.0f && largest < INFINITY ? ldexpf(1.0f, -ilogbf(largest)) : 1.0f;
+}
+
+template <typename T>
+__device__ __forceinline__ Frag<T> load_row(const T* row, int d, int dim)
+{
+    u32x4 x = {0, 0, 0, 0};
+    if (d < dim) __builtin_memcpy(&x, row + d, 16);
+    return __builtin_bit_cast(Frag<T>, x);
+}
+
+// sums of a block's results, multiplied, to a row of `dim` values
+template <typename T, int DP>
+__device__ __forceinline__ void store_columns(T* to, const f32x16* x, float times, int dim, int half)
+{
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int ch = 32 * d + row_in(i, half);
+            if (ch < dim) {
+                float y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = x[d][i + j] * times;
+                Pack<T, 4> pack;
+                pack.set(y);
+                store_pack<T, 4>(to + ch, pack);
+            }
+        }
+}
+
+// ---- queries fixed: 32 to a wave ----
+template <typename T, int DP, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) dq_kernel(GradArgs p)
+{
+    constexpr int kThreads = WAVES * 64, kRows = 32 * WAVES, kKeys = 64, kSlices = DP / 16, kBlocks = DP / 32;
+    constexpr int kTileBytes = kKeys * Tile<DP>::kRowBytes, kLoads = kKeys * Tile<DP>::kChunks / kThreads;
+    __shared__ __attribute__((aligned(16))) char s_tiles[2][2][kTileBytes];
+    __shared__ int s_space[WAVES + 4];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
+    const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
+    const Span at = find_tile<kThreads>(p.packed, kRows, blockIdx.x / p.heads, false, true, s_space);
+    if (at.seq < 0) return;
+    const int q_first = at.tile * kRows, shift = at.nk - at.nq;
+    const int q_past = q_first + kRows < at.nq ? q_first + kRows : at.nq;
+    int keys = at.nk;
+    if (p.causal && q_past + shift < keys) keys = q_past + shift < 0 ? 0 : q_past + shift;
+    const int tiles = (keys + kKeys - 1) / kKeys;
+
+    const RowRead<DP> rows(lane);
+    const ColumnRead<DP> columns(lane);
+    const int query = q_first + wave * 32 + (lane & 31), row = query < at.nq ? query : at.nq - 1;
+    Frag<T> q[kSlices], g[kSlices];
+    float delta = 0.0f, largest = 0.0f;
+    {
+        const T* from = static_cast<const T*>(p.q) + (at.q0 + row) * p.q_token + head * p.q_head;
+        const T* grad = static_cast<const T*>(p.grad) + (at.q0 + row) * p.g_token + head * p.g_head;
+        const T* out = static_cast<const T*>(p.out) + ((at.q0 + row) * p.heads + head) * p.dim;
+#pragma unroll
+        for (int k = 0; k < kSlices; ++k) {
+            const int d = 16 * k + 8 * half;
+            q[k] = load_row<T>(from, d, p.dim);
+            g[k] = load_row<T>(grad, d, p.dim);
+            const Frag<T> y = load_row<T>(out, d, p.dim);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = static_cast<float>(g[k][i]);
+                delta = fmaf(x, static_cast<float>(y[i]), delta);
+                if constexpr (__is_same(T, f16)) largest = fmaxf(largest, fabsf(x));
+            }
+        }
+        delta += swapped(delta);
+    }
+    const int64_t place = (at.q0 + row) * p.heads + head;
+    if (query < at.nq && half == 0) p.delta[place] = delta;
+    float lift = 1.0f;
+    if constexpr (__is_same(T, f16)) {
+        largest = fmaxf(largest, swapped(largest));
+        lift = towards_one(largest);
+        float most = largest;
+#pragma unroll
+        for (int m = 1; m < 32; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+        if (lane == 0 && most < INFINITY) atomicMax(p.largest, __float_as_uint(most));       // bits of positive numbers ascend like them
+    }
+    const float lse = p.lse[place] == -INFINITY ? INFINITY : p.lse[place] * kLog2e;
+    const int last = p.causal && query + shift < at.nk - 1 ? query + shift : at.nk - 1;
+    f32x16 dq[kBlocks];
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d) dq[d] = zeros16();
+
+    u32x4 next[2][kLoads];
+    auto fetch = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int e = i * kThreads + tid, r = e / Tile<DP>::kChunks, chunk = e % Tile<DP>::kChunks;
+            const int key = tile * kKeys + r < at.nk ? tile * kKeys + r : at.nk - 1;
+            next[0][i] = next[1][i] = u32x4{0, 0, 0, 0};
+            if (chunk * 8 < p.dim) {
+                __builtin_memcpy(&next[0][i], static_cast<const T*>(p.k) + (at.k0 + key) * p.k_token + kv * p.k_head + chunk * 8, 16);
+                __builtin_memcpy(&next[1][i], static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head + chunk * 8, 16);
+            }
+        }
+    };
+    auto put = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int e = i * kThreads + tid, to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
+            *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + to) = next[0][i];
+            *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + to) = next[1][i];
+        }
+    };
+    if (tiles) {
+        fetch(0);
+        put(0);
+    }
+    for (int tile = 0; tile < tiles; ++tile) {
+        __syncthreads();
+        if (tile + 1 < tiles) fetch(tile + 1);
+        const char *kt = s_tiles[tile & 1][0], *vt = s_tiles[tile & 1][1];
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) {
+            const int key0 = tile * kKeys + 32 * c;
+            f32x16 s = zeros16(), dp = zeros16();
+#pragma unroll
+            for (int k = 0; k < kSlices; ++k) {
+                s = product(rows.template get<T>(kt, 32 * c, k), q[k], s);
+                dp = product(rows.template get<T>(vt, 32 * c, k), g[k], dp);
+            }
+            if (key0 + 32 > at.nk || (p.causal && key0 + 31 > q_first + wave * 32 + shift))
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (key0 + row_in(i, half) > last) s[i] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -lse));
+                s[i] = w * (__is_same(T, f16) ? lift * (dp[i] - delta) : dp[i] - delta);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const Frag<T> ds = rounded<T>(s, 8 * u);
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) dq[d] = product(columns.template get<T>(kt, 32 * c + 16 * u, d), ds, dq[d]);
+            }
+        }
+        if (tile + 1 < tiles) put((tile + 1) & 1);
+    }
+    if (query < at.nq) store_columns<T, DP>(static_cast<T*>(p.dq) + place * p.dim, dq, p.scale / lift, p.dim, half);
+}
+
+// ---- keys fixed: KB * 32 to a pair of waves, PAIRS pairs to a block ----
+template <typename T, int DP, int KB, int PAIRS>
+__global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
+{
+    constexpr int kThreads = PAIRS * 128, kRows = 32 * KB * PAIRS, kQueries = 32, kSlices = DP / 16, kBlocks = DP / 32;
+    constexpr int kTileBytes = kQueries * Tile<DP>::kRowBytes, kChunksAll = kQueries * Tile<DP>::kChunks, kLoads = (kChunksAll + kThreads - 1) / kThreads;
+    __shared__ __attribute__((aligned(16))) char s_tiles[3][2][kTileBytes];
+    __shared__ __attribute__((aligned(16))) float s_lse[3][kQueries], s_delta[3][kQueries];
+    __shared__ __attribute__((aligned(16))) u32x4 s_weights[2][PAIRS][KB][2][64];
+    __shared__ int s_space[PAIRS * 2 + 4];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6, pair = wave % PAIRS;
+    const bool second = wave >= PAIRS;
+    const int kv = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
+    const Span at = find_tile<kThreads>(p.packed, kRows, blockIdx.x / p.kv_heads, true, false, s_space);
+    if (at.seq < 0) return;
+    const int k_first = at.tile * kRows, shift = at.nk - at.nq;
+    // the first query that sees any of the block's keys
+    int q_begin = p.causal ? k_first - shift : 0;
+    q_begin = q_begin < 0 ? 0 : (q_begin > at.nq ? at.nq : q_begin);
+    const int tiles = (at.nq - q_begin + kQueries - 1) / kQueries, steps = tiles * group;
+
+    const RowRead<DP> rows(lane);
+    const ColumnRead<DP> columns(lane);
+    int key[KB];
+    Frag<T> fixed[KB][kSlices];         // keys, in the second wave values
+    f32x16 sums[KB][kBlocks];           // dV, in the second wave dK
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+        key[b] = k_first + (pair * KB + b) * 32 + (lane & 31);
+        const int64_t r = at.k0 + (key[b] < at.nk ? key[b] : at.nk - 1);
+        const T* from = second ? static_cast<const T*>(p.v) + r * p.v_token + kv * p.v_head : static_cast<const T*>(p.k) + r * p.k_token + kv * p.k_head;
+#pragma unroll
+        for (int k = 0; k < kSlices; ++k) fixed[b][k] = load_row<T>(from, 16 * k + 8 * half, p.dim);
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d) sums[b][d] = zeros16();
+    }
+    float lift = 1.0f;
+    if constexpr (__is_same(T, f16)) lift = towards_one(__uint_as_float(*p.largest));
+
+    u32x4 next[2][kLoads];
+    float next_lse = 0.0f, next_delta = 0.0f;
+    auto fetch = [&](int step) {
+        const int head = kv * group + step / tiles, q0 = q_begin + (step % tiles) * kQueries;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int e = i * kThreads + tid, r = e / Tile<DP>::kChunks, chunk = e % Tile<DP>::kChunks;
+            const int64_t row = at.q0 + (q0 + r < at.nq ? q0 + r : at.nq - 1);
+            next[0][i] = next[1][i] = u32x4{0, 0, 0, 0};
+            if (e < kChunksAll && chunk * 8 < p.dim) {
+                __builtin_memcpy(&next[0][i], static_cast<const T*>(p.q) + row * p.q_token + head * p.q_head + chunk * 8, 16);
+                __builtin_memcpy(&next[1][i], static_cast<const T*>(p.grad) + row * p.g_token + head * p.g_head + chunk * 8, 16);
+            }
+        }
+        if (tid < kQueries) {           // queries past the end, and those that see nothing, have no weights
+            next_lse = INFINITY;
+            next_delta = 0.0f;
+            if (q0 + tid < at.nq) {
+                const int64_t place = (at.q0 + q0 + tid) * p.heads + head;
+                const float l = p.lse[place];
+                next_lse = l == -INFINITY ? INFINITY : l * kLog2e;
+                next_delta = p.delta[place];
+            }
+        }
+    };
+    auto put = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int e = i * kThreads + tid;
+            if (e < kChunksAll) {
+                const int to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
+                *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + to) = next[0][i];
+                *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + to) = next[1][i];
+            }
+        }
+        if (tid < kQueries) {
+            s_lse[buffer][tid] = next_lse;
+            s_delta[buffer][tid] = next_delta;
+        }
+    };
+    if (steps) {
+        fetch(0);
+        put(0);
+    }
+    int now = 0, before = 2;            // buffers of this step and of the one before it
+    for (int step = 0; step <= steps && steps; ++step) {
+        __syncthreads();
+        const int after = now == 2 ? 0 : now + 1;
+        if (step + 1 < steps) fetch(step + 1);
+        if (!second && step < steps) {
+            const char *qt = s_tiles[now][0], *gt = s_tiles[now][1];
+            const int q0 = q_begin + (step % tiles) * kQueries;
+            f32x16 s[KB];
+#pragma unroll
+            for (int b = 0; b < KB; ++b) s[b] = zeros16();
+#pragma unroll
+            for (int k = 0; k < kSlices; ++k) {
+                const Frag<T> f = rows.template get<T>(qt, 0, k);
+#pragma unroll
+                for (int b = 0; b < KB; ++b) s[b] = product(f, fixed[b][k], s[b]);
+            }
+            float lse[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) lse[i] = s_lse[now][row_in(i, half)];
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                if (p.causal && q0 + shift < k_first + (pair * KB + b) * 32 + 31)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (key[b] > q0 + row_in(i, half) + shift) s[b][i] = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], p.scale2, -lse[i]));
+#pragma unroll
+                for (int u = 0; u < 2; ++u) s_weights[step & 1][pair][b][u][lane] = __builtin_bit_cast(u32x4, rounded<T>(s[b], 8 * u));
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) {
+                    const Frag<T> f = columns.template get<T>(gt, 16 * u, d);
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) sums[b][d] = product(f, rounded<T>(s[b], 8 * u), sums[b][d]);
+                }
+        }
+        if (second && step > 0) {
+            const char *qt = s_tiles[before][0], *gt = s_tiles[before][1];
+            f32x16 dp[KB];
+#pragma unroll
+            for (int b = 0; b < KB; ++b) dp[b] = zeros16();
+#pragma unroll
+            for (int k = 0; k < kSlices; ++k) {
+                const Frag<T> f = rows.template get<T>(gt, 0, k);
+#pragma unroll
+                for (int b = 0; b < KB; ++b) dp[b] = product(f, fixed[b][k], dp[b]);
+            }
+            float delta[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) delta[i] = s_delta[before][row_in(i, half)];
+            Frag<T> ds[KB][2];
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const Frag<T> w = __builtin_bit_cast(Frag<T>, s_weights[(step - 1) & 1][pair][b][u][lane]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float x = dp[b][8 * u + i] - delta[8 * u + i];
+                        ds[b][u][i] = T(static_cast<float>(w[i]) * (__is_same(T, f16) ? x * lift : x));
+                    }
+                }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) {
+                    const Frag<T> f = columns.template get<T>(qt, 16 * u, d);
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) sums[b][d] = product(f, ds[b][u], sums[b][d]);
+                }
+        }
+        if (step + 1 < steps) put(after);
+        before = now;
+        now = after;
+    }
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+        if (key[b] < at.nk) {
+            T* to = static_cast<T*>(second ? p.dk : p.dv) + ((at.k0 + key[b]) * p.kv_heads + kv) * p.dim;
+            store_columns<T, DP>(to, sums[b], second ? p.scale / lift : 1.0f, p.dim, half);
+        }
+}
+
+__global__ void clear_kernel(unsigned* largest) { *largest = 0; }
+
+template <typename T, int DP>
+void backward(const GradArgs& p, hipStream_t stream)
+{
+    constexpr int kWaves = 8, KB = 2, PAIRS = 4;
+    const int64_t q_blocks = most_tiles(p.packed.q_rows, p.packed.n, 32 * kWaves) * p.heads;
+    const int64_t k_blocks = most_tiles(p.packed.k_rows, p.packed.n, 32 * KB * PAIRS) * p.kv_heads;
+    require(q_blocks < (int64_t(1) << 31) && k_blocks < (int64_t(1) << 31), "too many queries and heads");
+    if (__is_same(T, f16)) {
+        hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(1), 0, stream, p.largest);
+        SIG_HIP(hipGetLastError());
+    }
+    if (q_blocks) {
+        hipLaunchKernelGGL((dq_kernel<T, DP, kWaves>), dim3(unsigned(q_blocks)), dim3(kWaves * 64), 0, stream, p);
+        SIG_HIP(hipGetLastError());
+    }
+    if (k_blocks) {
+        hipLaunchKernelGGL((dkv_kernel<T, DP, KB, PAIRS>), dim3(unsigned(k_blocks)), dim3(PAIRS * 128), 0, stream, p);
+        SIG_HIP(hipGetLastError());
+    }
+}
+
+constexpr uint64_t kHeadBytes = 256;
+
+}  // namespace
+}  // namespace seqamd
+
+using namespace seqamd;
+
+extern "C" {
+
+__attribute__((visibility("default"))) uint64_t cusig_amd_attention_backprop_workspace(uint64_t q_rows, uint64_t heads) noexcept
+{
+    return kHeadBytes + q_rows * heads * sizeof(float);
+}
+
+__attribute__((visibility("default"))) int cusig_amd_attention_backprop(
+    int dtype, const void* grad_out, const void* q, const void* k, const void* v, const void* out, const float* lse, const int* q_offsets,
+    const int* k_offsets, void* dq, void* dk, void* dv, uint64_t q_rows, uint64_t k_rows, uint64_t sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim,
+    int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, int64_t grad_token, int64_t grad_head, float scale,
+    bool causal, void* workspace, uint64_t workspace_bytes, void* stream) noexcept
+{
+    return sigamd::guarded([&] {
+        require(q_rows < (uint64_t(1) << 31) && k_rows < (uint64_t(1) << 31) && sequences < (uint64_t(1) << 31), "too many rows or sequences");
+        require(dim >= 8 && dim <= 128 && dim % 8 == 0, "a head has 8 to 128 channels, a multiple of 8");
+        require(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads < (1u << 20), "heads are a multiple of the key heads");
+        require(scale > 0.0f && std::isfinite(scale), "the scale is positive and finite");
+        require(workspace && workspace_bytes >= cusig_amd_attention_backprop_workspace(q_rows, heads), "the workspace is too small");
+        if (sequences == 0) return;
+        GradArgs p{};
+        p.q = q, p.k = k, p.v = v, p.out = out, p.grad = grad_out, p.lse = lse, p.dq = dq, p.dk = dk, p.dv = dv;
+        p.largest = static_cast<unsigned*>(workspace);
+        p.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + kHeadBytes);
+        p.packed = Packed{q_offsets, k_offsets, nullptr, int64_t(q_rows), int64_t(k_rows), int(sequences)};
+        p.q_token = q_token, p.q_head = q_head, p.k_token = k_token, p.k_head = k_head, p.v_token = v_token, p.v_head = v_head;
+        p.g_token = grad_token, p.g_head = grad_head;
+        p.heads = int(heads), p.kv_heads = int(kv_heads), p.dim = int(dim), p.causal = causal;
+        p.scale = scale, p.scale2 = scale * kLog2e;
+        const hipStream_t s = static_cast<hipStream_t>(stream);
+        switch (dtype) {
+        case kBF16: dim <= 64 ? backward<bf16, 64>(p, s) : backward<bf16, 128>(p, s); break;
+        case kF16: dim <= 64 ? backward<f16, 64>(p, s) : backward<f16, 128>(p, s); break;
+        default: throw std::invalid_argument("attention takes bfloat16 or float16");
+        }
+    });
+}
+
+}  // extern "C"

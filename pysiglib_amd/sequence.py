@@ -13,7 +13,8 @@ import math
 
 import torch
 
-from ._loader import (CUSIG_ATTENTION, CUSIG_ATTENTION_WORKSPACE, CUSIG_LINEAR_RECURRENCE, CUSIG_LINEAR_RECURRENCE_BACKPROP, CUSIG_LINEAR_RECURRENCE_STEP,
+from ._loader import (CUSIG_ATTENTION, CUSIG_ATTENTION_BACKPROP, CUSIG_ATTENTION_BACKPROP_WORKSPACE,
+                      CUSIG_ATTENTION_WORKSPACE, CUSIG_LINEAR_RECURRENCE, CUSIG_LINEAR_RECURRENCE_BACKPROP, CUSIG_LINEAR_RECURRENCE_STEP,
                       CUSIG_LINEAR_RECURRENCE_WORKSPACE, CUSIG_NORM_ROTARY, CUSIG_NORM_ROTARY_BACKPROP,
                       CUSIG_NORM_ROTARY_BACKPROP_WORKSPACE, SEQUENCE_DTYPES)
 from .data_handlers import on_device
@@ -335,3 +336,22 @@ def attention(q, k, v, q_offsets, k_offsets, *, k_lengths=None, causal=True, sca
           k_offsets.data_ptr(), 0 if k_lengths is None else k_lengths.data_ptr(), out.data_ptr(), lse.data_ptr(), *sizes, *rest,
           space.data_ptr() if size else 0, size)
     return out, lse
+
+
+def attention_backprop(grad_out, q, k, v, out, lse, q_offsets, k_offsets, *, causal=True, scale=None):
+    """Gradients of ``attention`` (whole sequences, without ``k_lengths``) from the gradient of ``out``, the inputs and both
+    outputs.  Returns ``(grad_q, grad_k, grad_v)``; the same inputs give the same bits."""
+    q, k, v, q_offsets, k_offsets, sizes, rest = _attention_args(q, k, v, q_offsets, k_offsets, causal, scale)
+    device, dtype = q.device, q.dtype
+    grad_out, g_token, g_head = _heads(grad_out, "grad_out", q, q.shape[0], q.shape[2])
+    if grad_out.shape != q.shape:
+        raise ValueError("grad_out must have the shape of q")
+    out = _other(out, "out", dtype, q.shape, device)
+    lse = _other(lse, "lse", torch.float32, q.shape[:2], device)
+    dq, dk, dv = (torch.empty(t.shape, dtype=dtype, device=device) for t in (q, k, v))
+    size = CUSIG_ATTENTION_BACKPROP_WORKSPACE(sizes[0], sizes[3])
+    space = _workspace(size, device)
+    _call(CUSIG_ATTENTION_BACKPROP, "attention_backprop", device, _CODES[dtype], grad_out.data_ptr(), q.data_ptr(), k.data_ptr(),
+          v.data_ptr(), out.data_ptr(), lse.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+          dv.data_ptr(), *sizes, *rest[:6], g_token, g_head, *rest[6:], space.data_ptr(), size)
+    return dq, dk, dv

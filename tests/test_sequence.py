@@ -425,6 +425,50 @@ def test_attention(P, dtype, queries, keys, heads, kv, dim, causal):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("queries,keys", SEQUENCES)
+@pytest.mark.parametrize("heads,kv,dim,causal", [(1, 1, 64, True), (4, 2, 128, True), (6, 1, 40, False), (3, 3, 96, True), (2, 1, 128, False)])
+def test_attention_gradients(P, dtype, queries, keys, heads, kv, dim, causal):
+    keys = keys or queries
+    qs, ks = starts_of(queries), starts_of(keys)
+    q, k, v, g = attention_inputs(dtype, qs[-1], ks[-1], heads, kv, dim, seed=dim + ks[-1])
+    offsets = [torch.tensor(s, dtype=torch.int32, device=DEV) for s in (qs, ks)]
+    out, lse = P.attention(q, k, v, *offsets, causal=causal)
+    got = P.attention_backprop(g, q, k, v, out, lse, *offsets, causal=causal)
+    again = P.attention_backprop(g, q, k, v, out, lse, *offsets, causal=causal)
+    u = ROUND[dtype]
+    want, bound = attention_oracle(f64(q), f64(k), f64(v), queries, ks, keys, causal, dim ** -0.5, grad=f64(g), u=u)
+    for name, x, y, w, b in zip(("dq", "dk", "dv"), got, again, want[2:], bound[2:]):
+        assert torch.equal(x, y), "the same inputs give the same bits"
+        within(x, w, b + u * (np.abs(w) + b) + SMALL[dtype], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -12])
+def test_attention_gradients_are_differences(P, size):
+    """Along random directions against central differences of the loss in 64 bits; small gradients as well, whose products
+    float16 does not hold.  Terms of a direction are off by a few roundings each, so their sum by 8 u of their 2-norm times
+    four standard deviations."""
+    lengths, heads, kv, dim = [40, 3, 70], 4, 2, 64
+    starts = starts_of(lengths)
+    q, k, v, g = attention_inputs(torch.float16, 113, 113, heads, kv, dim, seed=6)
+    g = g * size
+    offsets = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    out, lse = P.attention(q, k, v, offsets, offsets)
+    grads = [f64(t) for t in P.attention_backprop(g, q, k, v, out, lse, offsets, offsets)]
+    at = [f64(t) for t in (q, k, v)]
+    rng = np.random.default_rng(1)
+    loss = lambda x: (attention_oracle(*x, lengths, starts, lengths, True, dim ** -0.5)[0][0] * f64(g)).sum()       # noqa: E731
+    for i in range(3):
+        for _ in range(2):
+            z = rng.standard_normal(at[i].shape)
+            up, down = list(at), list(at)
+            up[i], down[i] = at[i] + 1e-4 * z, at[i] - 1e-4 * z
+            want = (loss(up) - loss(down)) / 2e-4
+            assert abs((grads[i] * z).sum() - want) <= 32 * ROUND[torch.float16] * np.sqrt(((grads[i] * z) ** 2).sum()), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("lengths,heads,kv,dim", [([1], 1, 1, 64), ([0, 5, 64, 65, 700, 33], 8, 2, 128), ([2500, 1, 3000], 12, 1, 40),
                                                   ([129] * 40, 4, 4, 64), ([4100], 5, 1, 128), ([300, 0, 17], 48, 1, 64)])
 @pytest.mark.parametrize("queries", [1, 2, 5])
@@ -533,6 +577,12 @@ def test_refusals(P):
                  (q, k, k[:2], at, at), (q[:, :0], k, k, at, at), (q.repeat(1, 1, 3), k.repeat(1, 1, 3), k.repeat(1, 1, 3), at, at)]:
         with pytest.raises(ValueError):
             P.attention(*args)
+    out, lse = P.attention(q, k, k, at, at)
+    for args in [(q[:2], q, k, k, out, lse), (k, q, k, k, out, lse), (q, q, k, k, out[:2], lse), (q, q, k, k, out, lse[:, :2])]:
+        with pytest.raises(ValueError):
+            P.attention_backprop(*args, at, at)
+    with pytest.raises(TypeError):
+        P.attention_backprop(q, q, k, k, out, lse.half(), at, at)
     for options in [dict(scale=0.0), dict(scale=float("inf")), dict(k_lengths=at)]:
         with pytest.raises(ValueError):
             P.attention(q, k, k, at, at, **options)
