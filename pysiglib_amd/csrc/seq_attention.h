@@ -134,16 +134,16 @@ __device__ __forceinline__ void span_of(const Packed& p, int seq, Span& s)
     s.nk = int(p.k_lengths ? kept(p.k_lengths[seq], 0, room) : room);
 }
 
-// The `wanted`-th tile of `size` rows, counted over the sequences (of keys: by their keys); with `last_first` from the end.
+// The `wanted`-th tile, counted over the sequences, each of which has count(span) of them; with `last_first` from the end.
 // The whole block (THREADS of it) calls it; `space`: THREADS / 64 + 4 ints.
-template <int THREADS>
-__device__ Span find_tile(const Packed& p, int size, int wanted, bool keys, bool last_first, int* space)
+template <int THREADS, typename F>
+__device__ Span find_tile(const Packed& p, int wanted, bool last_first, int* space, F&& count)
 {
     Span s;
     s.seq = -1;
     if (p.n == 1) {
         span_of(p, 0, s);
-        const int tiles = ((keys ? s.nk : s.nq) + size - 1) / size;
+        const int tiles = count(s);
         s.tile = last_first ? tiles - 1 - wanted : wanted;
         if (wanted >= tiles) s.seq = -1;
         return s;
@@ -151,13 +151,13 @@ __device__ Span find_tile(const Packed& p, int size, int wanted, bool keys, bool
     // each thread counts the tiles of some sequences, then a sum over the threads before it
     const int tid = threadIdx.x, each = (p.n + THREADS - 1) / THREADS;
     const int first = tid * each < p.n ? tid * each : p.n, past = first + each < p.n ? first + each : p.n;
-    auto count = [&](int seq) {
+    auto count_of = [&](int seq) {
         Span one;
         span_of(p, seq, one);
-        return ((keys ? one.nk : one.nq) + size - 1) / size;
+        return count(one);
     };
     int own = 0;
-    for (int i = first; i < past; ++i) own += count(i);
+    for (int i = first; i < past; ++i) own += count_of(i);
     int upto = own;
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) {
@@ -177,7 +177,7 @@ __device__ Span find_tile(const Packed& p, int size, int wanted, bool keys, bool
     if (target >= upto - own && target < upto) {
         int before = upto - own;
         for (int i = first; i < past; ++i) {
-            const int c = count(i);
+            const int c = count_of(i);
             if (target < before + c) {
                 found[0] = i;
                 found[1] = target - before;

@@ -19,7 +19,8 @@ struct AttentionArgs {
     float* lse;              // [q_rows][heads]
     Packed packed;
     int64_t q_token, q_head, k_token, k_head, v_token, v_head;
-    int heads, kv_heads, dim, causal;
+    float* parts;            // of the splits
+    int heads, kv_heads, dim, causal, splits;
     float scale;             // times log2(e)
 };
 
@@ -38,7 +39,7 @@ __global__ void __launch_bounds__(WAVES * 64) attention_kernel(AttentionArgs p)
     // the heads that share keys and values follow each other at a distance of kv_heads: on the same die where that is a multiple of 8
     const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
     // the last tiles see the most keys: they begin first
-    const Span at = find_tile<kThreads>(p.packed, kRows, blockIdx.x / p.heads, false, true, s_space);
+    const Span at = find_tile<kThreads>(p.packed, blockIdx.x / p.heads, true, s_space, [](const Span& s) { return (s.nq + kRows - 1) / kRows; });
     if (at.seq < 0) return;
     const int q_first = at.tile * kRows, shift = at.nk - at.nq;
     // keys that any query of the block sees
@@ -189,9 +190,261 @@ __global__ void __launch_bounds__(WAVES * 64) attention_kernel(AttentionArgs p)
     }
 }
 
+// ---- few queries to many keys: rows of a tile are the pairs (query, head) that share a key head ----
+// The four waves of a block take tiles of 32 keys in turn, each with its own maxima and sums, joined at the end; a sequence's
+// keys are cut into p.splits ranges that blocks take beside each other, joined by join_kernel.
 template <typename T, int DP>
-void forward(const AttentionArgs& p, hipStream_t stream)
+__global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
 {
+    constexpr int kSlices = DP / 16, kBlocks = DP / 32, kWaves = 4, kTile = 32;
+    constexpr int kTileBytes = kTile * Tile<DP>::kRowBytes, kLoads = kTile * Tile<DP>::kChunks / 64;
+    __shared__ __attribute__((aligned(16))) char s_tiles[kWaves][2][kTileBytes];
+    __shared__ float s_top[kWaves][32], s_sum[kWaves][32];
+    __shared__ int s_space[kWaves + 4];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
+    const int group = p.heads / p.kv_heads, kv = blockIdx.x % p.kv_heads, split = blockIdx.x / p.kv_heads % p.splits;
+    const Span at = find_tile<256>(p.packed, blockIdx.x / p.kv_heads / p.splits, false, s_space, [&](const Span& s) { return int((int64_t(s.nq) * group + 31) / 32); });
+    if (at.seq < 0) return;
+    const int pairs = at.nq * group, shift = at.nk - at.nq, pair = at.tile * 32 + (lane & 31);
+    const int own = pair < pairs ? pair : pairs - 1, query = own / group, head = kv * group + own % group;
+    // keys that any query of the tile sees, of those this split's
+    const int last_query = (at.tile * 32 + 31 < pairs ? at.tile * 32 + 31 : pairs - 1) / group;
+    int keys = p.causal && last_query + 1 + shift < at.nk ? last_query + 1 + shift : at.nk;
+    keys = keys < 0 ? 0 : keys;
+    const int each = ((keys + p.splits - 1) / p.splits + kTile - 1) / kTile * kTile;
+    const int begin = int64_t(split) * each < keys ? split * each : keys, past = begin + each < keys ? begin + each : keys;
+    const int tiles = (past - begin + kTile - 1) / kTile;
+
+    Frag<T> q[kSlices];
+    {
+        const T* from = static_cast<const T*>(p.q) + (at.q0 + query) * p.q_token + head * p.q_head;
+#pragma unroll
+        for (int k = 0; k < kSlices; ++k) {
+            const int d = 16 * k + 8 * half;
+            u32x4 x = {0, 0, 0, 0};
+            if (d < p.dim) __builtin_memcpy(&x, from + d, 16);
+            q[k] = __builtin_bit_cast(Frag<T>, x);
+        }
+    }
+    const RowRead<DP> rows(lane);
+    const ColumnRead<DP> columns(lane);
+    f32x16 o[kBlocks];
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d) o[d] = zeros16();
+    float top = -INFINITY, sum = 0.0f;
+    const int last = p.causal && query + shift < past - 1 ? query + shift : past - 1;
+
+    char *kt = s_tiles[wave][0], *vt = s_tiles[wave][1];
+    u32x4 next[2][kLoads];
+    auto fetch = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int e = i * 64 + lane, row = e / Tile<DP>::kChunks, chunk = e % Tile<DP>::kChunks;
+            const int at_key = begin + tile * kTile + row, key = at_key < past ? at_key : past - 1;
+            next[0][i] = next[1][i] = u32x4{0, 0, 0, 0};
+            if (chunk * 8 < p.dim) {
+                __builtin_memcpy(&next[0][i], static_cast<const T*>(p.k) + (at.k0 + key) * p.k_token + kv * p.k_head + chunk * 8, 16);
+                __builtin_memcpy(&next[1][i], static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head + chunk * 8, 16);
+            }
+        }
+    };
+    if (wave < tiles) fetch(wave);
+    for (int tile = wave; tile < tiles; tile += kWaves) {
+        // the wave's own tiles: shared memory serves a wave in order, no barrier is needed
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int e = i * 64 + lane, to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
+            *reinterpret_cast<u32x4*>(kt + to) = next[0][i];
+            *reinterpret_cast<u32x4*>(vt + to) = next[1][i];
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (tile + kWaves < tiles) fetch(tile + kWaves);
+        const int key0 = begin + tile * kTile;
+        f32x16 s = zeros16();
+#pragma unroll
+        for (int k = 0; k < kSlices; ++k) s = product(rows.template get<T>(kt, 0, k), q[k], s);
+        if (key0 + kTile > past || p.causal)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (key0 + row_in(i, half) > last) s[i] = -INFINITY;
+        float most = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
+        most = fmaxf(most, swapped(most)) * p.scale;
+        if (__any(most > top + kSlack || (top == -INFINITY && most > top))) {
+            const float now = fmaxf(top, most), shrink = top == now ? 1.0f : exp2f(top - now);
+            top = now;
+            sum *= shrink;
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= shrink;
+        }
+        const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale, -base));
+            sum += s[i];
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const Frag<T> w = rounded<T>(s, 8 * u);
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) o[d] = product(columns.template get<T>(vt, 16 * u, d), w, o[d]);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    // the waves' parts together: maxima and sums of all, then the weighted values, two waves into two, one into one
+    sum += swapped(sum);
+    if (half == 0) {
+        s_top[wave][lane] = top;
+        s_sum[wave][lane] = sum;
+    }
+    __syncthreads();
+    float most = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) most = fmaxf(most, s_top[w][lane & 31]);
+    const float base = most == -INFINITY ? 0.0f : most;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += s_sum[w][lane & 31] * exp2f(s_top[w][lane & 31] - base);
+    const float mine = exp2f(top - base);
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= mine;
+    float* const shared = reinterpret_cast<float*>(&s_tiles[0][0][0]);       // two parts of 64 lanes' sums, 64 KB at most
+    constexpr int kPart = kBlocks * 16 * 64;
+    static_assert(2 * kPart * sizeof(float) <= sizeof s_tiles, "");
+#pragma unroll
+    for (int step = 2; step > 0; step /= 2) {
+        __syncthreads();
+        if (wave >= step && wave < 2 * step)
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) shared[(wave - step) * kPart + (d * 16 + i) * 64 + lane] = o[d][i];
+        __syncthreads();
+        if (wave < step)
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] += shared[wave * kPart + (d * 16 + i) * 64 + lane];
+    }
+    if (wave || pair >= pairs) return;
+    const int64_t row = (at.q0 + query) * p.heads + head;
+    if (p.splits > 1) {
+        // [splits][q_rows * heads] of (maximum, sum), then [splits][q_rows * heads][dim]
+        const int64_t all = p.packed.q_rows * p.heads, place = split * all + row;
+        float* const to = p.parts + 2 * p.splits * all + place * p.dim;
+        if (half == 0) {
+            p.parts[2 * place] = most;
+            p.parts[2 * place + 1] = total;
+        }
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int ch = 32 * d + row_in(i, half);
+                if (ch < p.dim) {
+                    typedef float f32x4 __attribute__((ext_vector_type(4)));
+                    *reinterpret_cast<f32x4*>(to + ch) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+                }
+            }
+        return;
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    if (half == 0) p.lse[row] = total == 0.0f ? -INFINITY : 0.69314718055994531f * (most + log2f(total));
+    T* to = static_cast<T*>(p.out) + row * p.dim;
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int ch = 32 * d + row_in(i, half);
+            if (ch < p.dim) {
+                float x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = o[d][i + j] * inv;
+                Pack<T, 4> pack;
+                pack.set(x);
+                store_pack<T, 4>(to + ch, pack);
+            }
+        }
+}
+
+// the splits of one (query, head) to a wave, a lane to one or two channels pairwise
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(AttentionArgs p)
+{
+    const int64_t all = p.packed.q_rows * p.heads, row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= all) return;
+    float most = -INFINITY;
+    for (int s = lane; s < p.splits; s += 64) most = fmaxf(most, p.parts[2 * (s * all + row)]);
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+    const float base = most == -INFINITY ? 0.0f : most;
+    const float* from = p.parts + 2 * p.splits * all + row * p.dim;
+    float total = 0.0f, x[2] = {0.0f, 0.0f};
+    const bool in = 2 * lane < p.dim;
+    for (int s = 0; s < p.splits; ++s) {
+        const int64_t place = s * all + row;
+        const float w = exp2f(p.parts[2 * place] - base);
+        total += w * p.parts[2 * place + 1];
+        if (in) {
+            x[0] = fmaf(w, from[s * all * p.dim + 2 * lane], x[0]);
+            x[1] = fmaf(w, from[s * all * p.dim + 2 * lane + 1], x[1]);
+        }
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    if (lane == 0) p.lse[row] = total == 0.0f ? -INFINITY : 0.69314718055994531f * (most + log2f(total));
+    if (in) {
+        x[0] *= inv;
+        x[1] *= inv;
+        Pack<T, 2> pack;
+        pack.set(x);
+        store_pack<T, 2>(static_cast<T*>(p.out) + row * p.dim + 2 * lane, pack);
+    }
+}
+
+// How a call is cut.  few: pairs of (query, head) in tiles of 32 instead of a head's queries in tiles of 256.
+struct Cut {
+    bool few;
+    int splits;
+    int64_t tiles;           // of pairs
+};
+
+Cut cut_of(int64_t q_rows, int64_t k_rows, int64_t n, int64_t heads, int64_t kv_heads)
+{
+    Cut c;
+    const int64_t group = heads / kv_heads;
+    c.few = q_rows * group <= 128 * n;
+    c.tiles = most_tiles(q_rows * group, q_rows < n ? q_rows : n, 32);
+    // ranges of 256 keys and more, until there are about 16 blocks for each of the 256 compute units
+    const int64_t by_blocks = 4096 / (c.tiles * kv_heads ? c.tiles * kv_heads : 1), by_keys = k_rows / n / 256;
+    const int64_t splits = by_blocks < by_keys ? by_blocks : by_keys;
+    c.splits = c.few ? int(splits < 1 ? 1 : (splits > 256 ? 256 : splits)) : 1;
+    return c;
+}
+
+size_t parts_bytes(const Cut& c, int64_t q_rows, int64_t heads, int64_t dim)
+{
+    return c.splits > 1 ? size_t(c.splits) * q_rows * heads * (dim + 2) * sizeof(float) : 0;
+}
+
+template <typename T, int DP>
+void forward(const AttentionArgs& p, const Cut& cut, hipStream_t stream)
+{
+    if (cut.few) {
+        const int64_t blocks = cut.tiles * p.kv_heads * p.splits, rows = p.packed.q_rows * p.heads;
+        require(blocks < (int64_t(1) << 31) && rows < (int64_t(1) << 32), "too many queries and heads");
+        hipLaunchKernelGGL((few_kernel<T, DP>), dim3(unsigned(blocks)), dim3(256), 0, stream, p);
+        SIG_HIP(hipGetLastError());
+        if (p.splits > 1) {
+            hipLaunchKernelGGL((join_kernel<T>), dim3(unsigned((rows + 3) / 4)), dim3(256), 0, stream, p);
+            SIG_HIP(hipGetLastError());
+        }
+        return;
+    }
         constexpr int QB = 1, WAVES = 8, kRows = 32 * QB * WAVES;
     const int64_t blocks = most_tiles(p.packed.q_rows, p.packed.n, kRows) * p.heads;
     require(blocks < (int64_t(1) << 31), "too many queries and heads");
@@ -209,8 +462,8 @@ extern "C" {
 __attribute__((visibility("default"))) uint64_t cusig_amd_attention_workspace(uint64_t q_rows, uint64_t k_rows, uint64_t sequences, uint64_t heads,
                                                                             uint64_t kv_heads, uint64_t dim) noexcept
 {
-    (void)q_rows, (void)k_rows, (void)sequences, (void)heads, (void)kv_heads, (void)dim;
-    return 0;
+    if (!sequences || !kv_heads || !heads || heads % kv_heads) return 0;
+    return parts_bytes(cut_of(int64_t(q_rows), int64_t(k_rows), int64_t(sequences), int64_t(heads), int64_t(kv_heads)), int64_t(q_rows), int64_t(heads), int64_t(dim));
 }
 
 __attribute__((visibility("default"))) int cusig_amd_attention(
@@ -219,7 +472,6 @@ __attribute__((visibility("default"))) int cusig_amd_attention(
     int64_t k_head, int64_t v_token, int64_t v_head, float scale, bool causal, void* workspace, uint64_t workspace_bytes, void* stream) noexcept
 {
     return sigamd::guarded([&] {
-        (void)workspace, (void)workspace_bytes;
         require(q_rows < (uint64_t(1) << 31) && k_rows < (uint64_t(1) << 31) && sequences < (uint64_t(1) << 31), "too many rows or sequences");
         require(dim >= 8 && dim <= 128 && dim % 8 == 0, "a head has 8 to 128 channels, a multiple of 8");
         require(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads < (1u << 20), "heads are a multiple of the key heads");
@@ -231,10 +483,14 @@ __attribute__((visibility("default"))) int cusig_amd_attention(
         p.q_token = q_token, p.q_head = q_head, p.k_token = k_token, p.k_head = k_head, p.v_token = v_token, p.v_head = v_head;
         p.heads = int(heads), p.kv_heads = int(kv_heads), p.dim = int(dim), p.causal = causal;
         p.scale = scale * 1.44269504088896341f;
+        const Cut cut = cut_of(p.packed.q_rows, p.packed.k_rows, p.packed.n, p.heads, p.kv_heads);
+        require(workspace_bytes >= parts_bytes(cut, p.packed.q_rows, p.heads, p.dim) && (workspace || cut.splits == 1), "the workspace is too small");
+        p.parts = static_cast<float*>(workspace);
+        p.splits = cut.splits;
         const hipStream_t s = static_cast<hipStream_t>(stream);
         switch (dtype) {
-        case kBF16: dim <= 64 ? forward<bf16, 64>(p, s) : forward<bf16, 128>(p, s); break;
-        case kF16: dim <= 64 ? forward<f16, 64>(p, s) : forward<f16, 128>(p, s); break;
+        case kBF16: dim <= 64 ? forward<bf16, 64>(p, cut, s) : forward<bf16, 128>(p, cut, s); break;
+        case kF16: dim <= 64 ? forward<f16, 64>(p, cut, s) : forward<f16, 128>(p, cut, s); break;
         default: throw std::invalid_argument("attention takes bfloat16 or float16");
         }
     });

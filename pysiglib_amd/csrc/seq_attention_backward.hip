@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(WAVES * 64) dq_kernel(GradArgs p)
     __shared__ int s_space[WAVES + 4];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
-    const Span at = find_tile<kThreads>(p.packed, kRows, blockIdx.x / p.heads, false, true, s_space);
+    const Span at = find_tile<kThreads>(p.packed, blockIdx.x / p.heads, true, s_space, [](const Span& s) { return (s.nq + kRows - 1) / kRows; });
     if (at.seq < 0) return;
     const int q_first = at.tile * kRows, shift = at.nk - at.nq;
     const int q_past = q_first + kRows < at.nq ? q_first + kRows : at.nq;
@@ -114,7 +114,9 @@ __global__ void __launch_bounds__(WAVES * 64) dq_kernel(GradArgs p)
         float most = largest;
 #pragma unroll
         for (int m = 1; m < 32; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
-        if (lane == 0 && most < INFINITY) atomicMax(p.largest, __float_as_uint(most));       // bits of positive numbers ascend like them
+        // bits of positive numbers ascend like them; most waves find a larger one there and leave the address alone
+        if (lane == 0 && most < INFINITY && __float_as_uint(most) > __hip_atomic_load(p.largest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+            atomicMax(p.largest, __float_as_uint(most));
     }
     const float lse = p.lse[place] == -INFINITY ? INFINITY : p.lse[place] * kLog2e;
     const int last = p.causal && query + shift < at.nk - 1 ? query + shift : at.nk - 1;
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6, pair = wave % PAIRS;
     const bool second = wave >= PAIRS;
     const int kv = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
-    const Span at = find_tile<kThreads>(p.packed, kRows, blockIdx.x / p.kv_heads, true, false, s_space);
+    const Span at = find_tile<kThreads>(p.packed, blockIdx.x / p.kv_heads, false, s_space, [](const Span& s) { return (s.nk + kRows - 1) / kRows; });
     if (at.seq < 0) return;
     const int k_first = at.tile * kRows, shift = at.nk - at.nq;
     // the first query that sees any of the block's keys
