@@ -134,53 +134,110 @@ __device__ __forceinline__ void span_of(const Packed& p, int seq, Span& s)
     s.nk = int(p.k_lengths ? kept(p.k_lengths[seq], 0, room) : room);
 }
 
-// The `wanted`-th tile, counted over the sequences, each of which has count(span) of them; with `last_first` from the end.
-// The whole block (THREADS of it) calls it; `space`: THREADS / 64 + 4 ints.
+__device__ __forceinline__ int wave_sum(int x)
+{
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m);
+    return x;
+}
+
+__device__ __forceinline__ int wave_max(int x)
+{
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) x = max(x, __shfl_xor(x, m));
+    return x;
+}
+
+// inclusive sum over the lanes
+__device__ __forceinline__ int wave_scan(int x)
+{
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+        const int left = __shfl_up(x, m);
+        if (int(threadIdx.x & 63) >= m) x += left;
+    }
+    return x;
+}
+
+// In which order tiles are handed out, from the dearest to the cheapest where up to 64 sequences allow it: by their distance
+// from the sequence's first tile (a causal tile of queries sees the keys before it), or from its last (a tile of keys is
+// seen by the queries behind it).
+enum class Dear { kLast, kFirst };
+
+// The `wanted`-th tile over all sequences, each of which has count(span) of them.  The whole block (THREADS of it) calls it;
+// `space`: THREADS / 64 + 4 ints.
 template <int THREADS, typename F>
-__device__ Span find_tile(const Packed& p, int wanted, bool last_first, int* space, F&& count)
+__device__ Span find_tile(const Packed& p, int wanted, Dear dear, int* space, F&& count)
 {
     Span s;
     s.seq = -1;
-    if (p.n == 1) {
-        span_of(p, 0, s);
-        const int tiles = count(s);
-        s.tile = last_first ? tiles - 1 - wanted : wanted;
-        if (wanted >= tiles) s.seq = -1;
-        return s;
-    }
-    // each thread counts the tiles of some sequences, then a sum over the threads before it
-    const int tid = threadIdx.x, each = (p.n + THREADS - 1) / THREADS;
-    const int first = tid * each < p.n ? tid * each : p.n, past = first + each < p.n ? first + each : p.n;
     auto count_of = [&](int seq) {
         Span one;
         span_of(p, seq, one);
         return count(one);
     };
+    const int tid = threadIdx.x, lane = tid & 63;
+    if (p.n == 1) {
+        span_of(p, 0, s);
+        const int tiles = count(s);
+        s.tile = dear == Dear::kLast ? tiles - 1 - wanted : wanted;
+        if (wanted >= tiles) s.seq = -1;
+        return s;
+    }
+    if (p.n <= 64) {
+        // a sequence to a lane.  Level by level (a level: the tiles at the same distance), the levels below r hold
+        // sum of min(tiles, r); r by bisection, bit by bit
+        const int tiles = lane < p.n ? count_of(lane) : 0;
+        const int target = wave_sum(tiles) - 1 - wanted;
+        if (target < 0) return s;
+        const int most = wave_max(tiles);
+        int level = 0, below = 0;
+        for (int bit = 31 - __clz(most); bit >= 0; --bit) {
+            const int r = level + (1 << bit), c = wave_sum(min(tiles, r));
+            if (c <= target) level = r, below = c;
+        }
+        const unsigned long long there = __ballot(tiles > level), mine = 1ull << lane;
+        const int seq = __ffsll(__ballot((there & mine) && __popcll(there & (mine - 1)) == target - below)) - 1;
+        span_of(p, seq, s);
+        s.tile = dear == Dear::kLast ? level : __shfl(tiles, seq) - 1 - level;
+        return s;
+    }
+    if (p.n <= 512) {
+        // up to eight sequences to a lane, one after the other
+        const int each = (p.n + 63) / 64, first = min(lane * each, p.n), past = min(first + each, p.n);
+        int own = 0;
+        for (int i = first; i < past; ++i) own += count_of(i);
+        const int upto = wave_scan(own), total = __shfl(upto, 63), target = total - 1 - wanted;
+        if (target < 0) return s;
+        const int holder = __ffsll(__ballot(target < upto)) - 1;
+        int left = target - __shfl(upto - own, holder), seq = min(holder * each, p.n - 1), tiles = count_of(seq);
+        while (left >= tiles) {
+            left -= tiles;
+            tiles = count_of(++seq);
+        }
+        span_of(p, seq, s);
+        s.tile = dear == Dear::kLast ? left : tiles - 1 - left;
+        return s;
+    }
+    // each thread counts the tiles of some sequences, then a sum over the threads before it
+    const int each = (p.n + THREADS - 1) / THREADS;
+    const int first = min(tid * each, p.n), past = min(first + each, p.n);
     int own = 0;
     for (int i = first; i < past; ++i) own += count_of(i);
-    int upto = own;
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        const int left = __shfl_up(upto, m);
-        if ((tid & 63) >= m) upto += left;
-    }
+    int upto = wave_scan(own);
     int* const found = space + THREADS / 64;
-    if ((tid & 63) == 63) space[tid >> 6] = upto;
+    if (lane == 63) space[tid >> 6] = upto;
     if (tid == 0) found[0] = -1;
     __syncthreads();
-    int total = 0;
-    for (int w = 0; w < THREADS / 64; ++w) {
+    for (int w = 0; w < THREADS / 64; ++w)
         if (w < (tid >> 6)) upto += space[w];
-        total += space[w];
-    }
-    const int target = last_first ? total - 1 - wanted : wanted;
-    if (target >= upto - own && target < upto) {
+    if (wanted >= upto - own && wanted < upto) {
         int before = upto - own;
         for (int i = first; i < past; ++i) {
             const int c = count_of(i);
-            if (target < before + c) {
+            if (wanted < before + c) {
                 found[0] = i;
-                found[1] = target - before;
+                found[1] = wanted - before;
                 break;
             }
             before += c;

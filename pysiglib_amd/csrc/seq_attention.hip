@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(WAVES * 64) attention_kernel(AttentionArgs p)
     // the heads that share keys and values follow each other at a distance of kv_heads: on the same die where that is a multiple of 8
     const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
     // the last tiles see the most keys: they begin first
-    const Span at = find_tile<kThreads>(p.packed, blockIdx.x / p.heads, true, s_space, [](const Span& s) { return (s.nq + kRows - 1) / kRows; });
+    const Span at = find_tile<kThreads>(p.packed, blockIdx.x / p.heads, Dear::kLast, s_space, [](const Span& s) { return (s.nq + kRows - 1) / kRows; });
     if (at.seq < 0) return;
     const int q_first = at.tile * kRows, shift = at.nk - at.nq;
     // keys that any query of the block sees
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
     __shared__ int s_space[kWaves + 4];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     const int group = p.heads / p.kv_heads, kv = blockIdx.x % p.kv_heads, split = blockIdx.x / p.kv_heads % p.splits;
-    const Span at = find_tile<256>(p.packed, blockIdx.x / p.kv_heads / p.splits, false, s_space, [&](const Span& s) { return int((int64_t(s.nq) * group + 31) / 32); });
+    const Span at = find_tile<256>(p.packed, blockIdx.x / p.kv_heads / p.splits, Dear::kLast, s_space, [&](const Span& s) { return int((int64_t(s.nq) * group + 31) / 32); });
     if (at.seq < 0) return;
     const int pairs = at.nq * group, shift = at.nk - at.nq, pair = at.tile * 32 + (lane & 31);
     const int own = pair < pairs ? pair : pairs - 1, query = own / group, head = kv * group + own % group;

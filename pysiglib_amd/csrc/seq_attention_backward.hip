@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(WAVES * 64) dq_kernel(GradArgs p)
     __shared__ int s_space[WAVES + 4];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
-    const Span at = find_tile<kThreads>(p.packed, blockIdx.x / p.heads, true, s_space, [](const Span& s) { return (s.nq + kRows - 1) / kRows; });
+    const Span at = find_tile<kThreads>(p.packed, blockIdx.x / p.heads, Dear::kLast, s_space, [](const Span& s) { return (s.nq + kRows - 1) / kRows; });
     if (at.seq < 0) return;
     const int q_first = at.tile * kRows, shift = at.nk - at.nq;
     const int q_past = q_first + kRows < at.nq ? q_first + kRows : at.nq;
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6, pair = wave % PAIRS;
     const bool second = wave >= PAIRS;
     const int kv = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
-    const Span at = find_tile<kThreads>(p.packed, blockIdx.x / p.kv_heads, false, s_space, [](const Span& s) { return (s.nk + kRows - 1) / kRows; });
+    const Span at = find_tile<kThreads>(p.packed, blockIdx.x / p.kv_heads, Dear::kFirst, s_space, [](const Span& s) { return (s.nk + kRows - 1) / kRows; });
     if (at.seq < 0) return;
     const int k_first = at.tile * kRows, shift = at.nk - at.nq;
     // the first query that sees any of the block's keys
@@ -358,7 +358,7 @@ __global__ void clear_kernel(unsigned* largest) { *largest = 0; }
 template <typename T, int DP>
 void backward(const GradArgs& p, hipStream_t stream)
 {
-    constexpr int kWaves = 8, KB = 2, PAIRS = 4;
+    constexpr int kWaves = 8, KB = 1, PAIRS = 4;
     const int64_t q_blocks = most_tiles(p.packed.q_rows, p.packed.n, 32 * kWaves) * p.heads;
     const int64_t k_blocks = most_tiles(p.packed.k_rows, p.packed.n, 32 * KB * PAIRS) * p.kv_heads;
     require(q_blocks < (int64_t(1) << 31) && k_blocks < (int64_t(1) << 31), "too many queries and heads");
