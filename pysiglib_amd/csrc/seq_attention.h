@@ -114,6 +114,15 @@ struct Packed {
     const int *q_offsets, *k_offsets, *k_lengths;
     int64_t q_rows, k_rows;
     int n;
+    const int* map;      // more than kMapped sequences: the number of tiles, then (sequence, tile) of each, see map_kernel
+};
+
+constexpr int kMapped = 256;
+
+// How a sequence is cut into tiles: by its keys, or by its queries times `mult`
+struct Tiling {
+    bool keys;
+    int size, mult;
 };
 
 struct Span {
@@ -159,24 +168,36 @@ __device__ __forceinline__ int wave_scan(int x)
     return x;
 }
 
+// a lane's span, for all
+__device__ __forceinline__ Span taken(const Span& own, int lane, int seq, int tile)
+{
+    Span s;
+    s.q0 = __shfl(int(own.q0), lane);
+    s.k0 = __shfl(int(own.k0), lane);
+    s.nq = __shfl(own.nq, lane);
+    s.nk = __shfl(own.nk, lane);
+    s.seq = seq;
+    s.tile = tile;
+    return s;
+}
+
 // In which order tiles are handed out, from the dearest to the cheapest where up to 64 sequences allow it: by their distance
 // from the sequence's first tile (a causal tile of queries sees the keys before it), or from its last (a tile of keys is
 // seen by the queries behind it).
 enum class Dear { kLast, kFirst };
 
-// The `wanted`-th tile over all sequences, each of which has count(span) of them.  The whole block (THREADS of it) calls it;
-// `space`: THREADS / 64 + 4 ints.
-template <int THREADS, typename F>
-__device__ Span find_tile(const Packed& p, int wanted, Dear dear, int* space, F&& count)
+__device__ __forceinline__ int tiles_of(const Tiling& t, const Span& s)
+{
+    return t.keys ? (s.nk + t.size - 1) / t.size : int((int64_t(s.nq) * t.mult + t.size - 1) / t.size);
+}
+
+// The `wanted`-th tile over all sequences; each wave finds it by itself.
+__device__ __forceinline__ Span find_tile(const Packed& p, const Tiling& how, int wanted, Dear dear)
 {
     Span s;
     s.seq = -1;
-    auto count_of = [&](int seq) {
-        Span one;
-        span_of(p, seq, one);
-        return count(one);
-    };
-    const int tid = threadIdx.x, lane = tid & 63;
+    auto count = [&](const Span& one) { return tiles_of(how, one); };
+    const int lane = threadIdx.x & 63;
     if (p.n == 1) {
         span_of(p, 0, s);
         const int tiles = count(s);
@@ -187,7 +208,9 @@ __device__ Span find_tile(const Packed& p, int wanted, Dear dear, int* space, F&
     if (p.n <= 64) {
         // a sequence to a lane.  Level by level (a level: the tiles at the same distance), the levels below r hold
         // sum of min(tiles, r); r by bisection, bit by bit
-        const int tiles = lane < p.n ? count_of(lane) : 0;
+        Span own{};
+        if (lane < p.n) span_of(p, lane, own);
+        const int tiles = lane < p.n ? count(own) : 0;
         const int target = wave_sum(tiles) - 1 - wanted;
         if (target < 0) return s;
         const int most = wave_max(tiles);
@@ -197,62 +220,89 @@ __device__ Span find_tile(const Packed& p, int wanted, Dear dear, int* space, F&
             if (c <= target) level = r, below = c;
         }
         const unsigned long long there = __ballot(tiles > level), mine = 1ull << lane;
-        const int seq = __ffsll(__ballot((there & mine) && __popcll(there & (mine - 1)) == target - below)) - 1;
-        span_of(p, seq, s);
-        s.tile = dear == Dear::kLast ? level : __shfl(tiles, seq) - 1 - level;
-        return s;
+        const int holder = __ffsll(__ballot((there & mine) && __popcll(there & (mine - 1)) == target - below)) - 1;
+        return taken(own, holder, holder, dear == Dear::kLast ? level : __shfl(tiles, holder) - 1 - level);
     }
-    if (p.n <= 512) {
-        // up to eight sequences to a lane, one after the other
-        const int each = (p.n + 63) / 64, first = min(lane * each, p.n), past = min(first + each, p.n);
-        int own = 0;
-        for (int i = first; i < past; ++i) own += count_of(i);
-        const int upto = wave_scan(own), total = __shfl(upto, 63), target = total - 1 - wanted;
+    if (p.n <= kMapped) {
+        // up to four sequences to a lane, one after the other
+        const int each = (p.n + 63) / 64;
+        Span own[4];
+        int tiles[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int seq = lane * each + i;
+            const bool is = i < each && seq < p.n;
+            if (is) span_of(p, seq, own[i]);
+            else own[i] = Span{};
+            tiles[i] = is ? count(own[i]) : 0;
+            sum += tiles[i];
+        }
+        const int upto = wave_scan(sum), target = __shfl(upto, 63) - 1 - wanted;
         if (target < 0) return s;
         const int holder = __ffsll(__ballot(target < upto)) - 1;
-        int left = target - __shfl(upto - own, holder), seq = min(holder * each, p.n - 1), tiles = count_of(seq);
-        while (left >= tiles) {
-            left -= tiles;
-            tiles = count_of(++seq);
-        }
-        span_of(p, seq, s);
-        s.tile = dear == Dear::kLast ? left : tiles - 1 - left;
-        return s;
-    }
-    // each thread counts the tiles of some sequences, then a sum over the threads before it
-    const int each = (p.n + THREADS - 1) / THREADS;
-    const int first = min(tid * each, p.n), past = min(first + each, p.n);
-    int own = 0;
-    for (int i = first; i < past; ++i) own += count_of(i);
-    int upto = wave_scan(own);
-    int* const found = space + THREADS / 64;
-    if (lane == 63) space[tid >> 6] = upto;
-    if (tid == 0) found[0] = -1;
-    __syncthreads();
-    for (int w = 0; w < THREADS / 64; ++w)
-        if (w < (tid >> 6)) upto += space[w];
-    if (wanted >= upto - own && wanted < upto) {
-        int before = upto - own;
-        for (int i = first; i < past; ++i) {
-            const int c = count_of(i);
-            if (wanted < before + c) {
-                found[0] = i;
-                found[1] = wanted - before;
-                break;
+        int left = target - (upto - sum), which = 0, there = tiles[0];
+        Span one = own[0];
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+            if (which == i - 1 && left >= there) {
+                left -= there;
+                which = i;
+                there = tiles[i];
+                one = own[i];
             }
-            before += c;
+        return taken(one, holder, holder * each + __shfl(which, holder), __shfl(dear == Dear::kLast ? left : there - 1 - left, holder));
+    }
+    const int target = p.map[0] - 1 - wanted;
+    if (target < 0) return s;
+    const int seq = p.map[2 + 2 * target], tile = p.map[3 + 2 * target];
+    span_of(p, seq, s);
+    s.tile = tile;
+    if (dear == Dear::kFirst) s.tile = count(s) - 1 - tile;
+    return s;
+}
+
+// The tiles of many sequences, listed once for all blocks of the kernels behind it: a block to a tiling.
+struct MapArgs {
+    Packed packed;
+    Tiling how[2];
+    int* map[2];
+    unsigned* clear;         // a word to be cleared, or null
+};
+
+constexpr int kMapThreads = 1024;
+
+static __global__ void __launch_bounds__(kMapThreads) map_kernel(MapArgs p)
+{
+    __shared__ int s_sums[kMapThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const Tiling how = blockIdx.x ? p.how[1] : p.how[0];
+    int* const map = blockIdx.x ? p.map[1] : p.map[0];
+    if (p.clear && blockIdx.x == 0 && tid == 0) *p.clear = 0;
+    if (!map) return;
+    int done = 0;
+    for (int base = 0; base < p.packed.n; base += kMapThreads) {
+        Span one{};
+        if (base + tid < p.packed.n) span_of(p.packed, base + tid, one);
+        const int own = base + tid < p.packed.n ? tiles_of(how, one) : 0, upto = wave_scan(own);
+        __syncthreads();
+        if (lane == 63) s_sums[tid >> 6] = upto;
+        __syncthreads();
+        int before = done + upto - own;
+        for (int w = 0; w < kMapThreads / 64; ++w) {
+            if (w < (tid >> 6)) before += s_sums[w];
+            done += s_sums[w];
+        }
+        for (int i = 0; i < own; ++i) {
+            map[2 + 2 * (before + i)] = base + tid;
+            map[3 + 2 * (before + i)] = i;
         }
     }
-    __syncthreads();
-    const int seq = found[0];
-    if (seq >= 0) {
-        span_of(p, seq, s);
-        s.tile = found[1];
-    }
-    return s;
+    if (tid == 0) map[0] = done;
 }
 
 // most tiles of `size` rows that n sequences with `rows` rows in all have
 inline int64_t most_tiles(int64_t rows, int64_t n, int64_t size) { return rows / size + (rows < n ? rows : n); }
+
+inline size_t map_bytes(int64_t tiles, int64_t n) { return n > kMapped ? (size_t(tiles + 1) * 2 * sizeof(int) + 255) / 256 * 256 : 0; }
 
 }  // namespace seqamd

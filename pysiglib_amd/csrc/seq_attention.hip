@@ -24,22 +24,20 @@ struct AttentionArgs {
     float scale;             // times log2(e)
 };
 
-constexpr int kKeys = 64;    // of a tile
 constexpr float kSlack = 8.0f;   // the maximum is taken over where it grew by more than this (in powers of two): weights stay below 2^8
 
-// WAVES waves of QB * 32 queries each
-template <typename T, int DP, int QB, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64) attention_kernel(AttentionArgs p)
+// WAVES waves of 32 queries each, tiles of kKeys keys
+template <typename T, int DP, int WAVES, int kKeys>
+__global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel(AttentionArgs p)
 {
-    constexpr int kThreads = WAVES * 64, kRows = 32 * QB * WAVES, kSlices = DP / 16, kBlocks = DP / 32;
+    constexpr int QB = 1, kThreads = WAVES * 64, kRows = 32 * WAVES, kSlices = DP / 16, kBlocks = DP / 32;
     constexpr int kTileBytes = kKeys * Tile<DP>::kRowBytes, kLoads = kKeys * Tile<DP>::kChunks / kThreads;
     __shared__ __attribute__((aligned(16))) char s_tiles[2][2][kTileBytes];
-    __shared__ int s_space[WAVES + 4];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     // the heads that share keys and values follow each other at a distance of kv_heads: on the same die where that is a multiple of 8
     const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
     // the last tiles see the most keys: they begin first
-    const Span at = find_tile<kThreads>(p.packed, blockIdx.x / p.heads, Dear::kLast, s_space, [](const Span& s) { return (s.nq + kRows - 1) / kRows; });
+    const Span at = find_tile(p.packed, Tiling{false, kRows, 1}, blockIdx.x / p.heads, Dear::kLast);
     if (at.seq < 0) return;
     const int q_first = at.tile * kRows, shift = at.nk - at.nq;
     // keys that any query of the block sees
@@ -102,67 +100,70 @@ __global__ void __launch_bounds__(WAVES * 64) attention_kernel(AttentionArgs p)
         if (tile + 1 < tiles) fetch(tile + 1);
         const char *kt = s_tiles[tile & 1][0], *vt = s_tiles[tile & 1][1];
         const int key0 = tile * kKeys;
-        f32x16 s[QB][kKeys / 32];
+        // a wave whose queries see none of the tile has nothing to do
+        if (!p.causal || key0 <= q_first + wave * QB * 32 + QB * 32 - 1 + shift) {
+            f32x16 s[QB][kKeys / 32];
 #pragma unroll
-        for (int c = 0; c < kKeys / 32; ++c) {
+            for (int c = 0; c < kKeys / 32; ++c) {
 #pragma unroll
-            for (int b = 0; b < QB; ++b) s[b][c] = zeros16();
+                for (int b = 0; b < QB; ++b) s[b][c] = zeros16();
 #pragma unroll
-            for (int k = 0; k < kSlices; ++k) {
-                const Frag<T> kf = rows.template get<T>(kt, 32 * c, k);
+                for (int k = 0; k < kSlices; ++k) {
+                    const Frag<T> kf = rows.template get<T>(kt, 32 * c, k);
 #pragma unroll
-                for (int b = 0; b < QB; ++b) s[b][c] = product(kf, q[b][k], s[b][c]);
+                    for (int b = 0; b < QB; ++b) s[b][c] = product(kf, q[b][k], s[b][c]);
+                }
             }
-        }
-        // a key is hidden past the sequence's end, or behind the query's place
-        const bool cut = key0 + kKeys > at.nk || (p.causal && key0 + kKeys - 1 > q_first + wave * QB * 32 + shift);
-        if (cut)
+            // a key is hidden past the sequence's end, or behind the query's place
+            const bool cut = key0 + kKeys > at.nk || (p.causal && key0 + kKeys - 1 > q_first + wave * QB * 32 + shift);
+            if (cut)
+#pragma unroll
+                for (int b = 0; b < QB; ++b) {
+                    const int last = p.causal && query[b] + shift < at.nk - 1 ? query[b] + shift : at.nk - 1;
+#pragma unroll
+                    for (int c = 0; c < kKeys / 32; ++c)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (key0 + 32 * c + row_in(i, half) > last) s[b][c][i] = -INFINITY;
+                }
+            Frag<T> w[QB][kKeys / 16];
 #pragma unroll
             for (int b = 0; b < QB; ++b) {
-                const int last = p.causal && query[b] + shift < at.nk - 1 ? query[b] + shift : at.nk - 1;
+                float most = s[b][0][0];
 #pragma unroll
                 for (int c = 0; c < kKeys / 32; ++c)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (key0 + 32 * c + row_in(i, half) > last) s[b][c][i] = -INFINITY;
-            }
-        Frag<T> w[QB][kKeys / 16];
+                    for (int i = 0; i < 16; ++i) most = fmaxf(most, s[b][c][i]);
+                most = fmaxf(most, swapped(most)) * p.scale;
+                if (__any(most > top[b] + kSlack || (top[b] == -INFINITY && most > top[b]))) {
+                    const float now = fmaxf(top[b], most), shrink = top[b] == now ? 1.0f : exp2f(top[b] - now);
+                    top[b] = now;
+                    sum[b] *= shrink;
 #pragma unroll
-        for (int b = 0; b < QB; ++b) {
-            float most = s[b][0][0];
+                    for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-            for (int c = 0; c < kKeys / 32; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) most = fmaxf(most, s[b][c][i]);
-            most = fmaxf(most, swapped(most)) * p.scale;
-            if (__any(most > top[b] + kSlack || (top[b] == -INFINITY && most > top[b]))) {
-                const float now = fmaxf(top[b], most), shrink = top[b] == now ? 1.0f : exp2f(top[b] - now);
-                top[b] = now;
-                sum[b] *= shrink;
-#pragma unroll
-                for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[b][d][i] *= shrink;
-            }
-            const float base = top[b] == -INFINITY ? 0.0f : top[b];
-#pragma unroll
-            for (int c = 0; c < kKeys / 32; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[b][c][i] = __builtin_amdgcn_exp2f(fmaf(s[b][c][i], p.scale, -base));
-                    sum[b] += s[b][c][i];
+                        for (int i = 0; i < 16; ++i) o[b][d][i] *= shrink;
                 }
+                const float base = top[b] == -INFINITY ? 0.0f : top[b];
 #pragma unroll
-            for (int c = 0; c < kKeys / 16; ++c) w[b][c] = rounded<T>(s[b][c / 2], 8 * (c & 1));
-        }
+                for (int c = 0; c < kKeys / 32; ++c)
 #pragma unroll
-        for (int c = 0; c < kKeys / 16; ++c)
+                    for (int i = 0; i < 16; ++i) {
+                        s[b][c][i] = __builtin_amdgcn_exp2f(fmaf(s[b][c][i], p.scale, -base));
+                        sum[b] += s[b][c][i];
+                    }
 #pragma unroll
-            for (int d = 0; d < kBlocks; ++d) {
-                const Frag<T> vf = columns.template get<T>(vt, 16 * c, d);
-#pragma unroll
-                for (int b = 0; b < QB; ++b) o[b][d] = product(vf, w[b][c], o[b][d]);
+                for (int c = 0; c < kKeys / 16; ++c) w[b][c] = rounded<T>(s[b][c / 2], 8 * (c & 1));
             }
+#pragma unroll
+            for (int c = 0; c < kKeys / 16; ++c)
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) {
+                    const Frag<T> vf = columns.template get<T>(vt, 16 * c, d);
+#pragma unroll
+                    for (int b = 0; b < QB; ++b) o[b][d] = product(vf, w[b][c], o[b][d]);
+                }
+        }
         if (tile + 1 < tiles) put((tile + 1) & 1);
     }
 #pragma unroll
@@ -200,10 +201,9 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
     constexpr int kTileBytes = kTile * Tile<DP>::kRowBytes, kLoads = kTile * Tile<DP>::kChunks / 64;
     __shared__ __attribute__((aligned(16))) char s_tiles[kWaves][2][kTileBytes];
     __shared__ float s_top[kWaves][32], s_sum[kWaves][32];
-    __shared__ int s_space[kWaves + 4];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     const int group = p.heads / p.kv_heads, kv = blockIdx.x % p.kv_heads, split = blockIdx.x / p.kv_heads % p.splits;
-    const Span at = find_tile<256>(p.packed, blockIdx.x / p.kv_heads / p.splits, Dear::kLast, s_space, [&](const Span& s) { return int((int64_t(s.nq) * group + 31) / 32); });
+    const Span at = find_tile(p.packed, Tiling{false, 32, group}, blockIdx.x / p.kv_heads / p.splits, Dear::kLast);
     if (at.seq < 0) return;
     const int pairs = at.nq * group, shift = at.nk - at.nq, pair = at.tile * 32 + (lane & 31);
     const int own = pair < pairs ? pair : pairs - 1, query = own / group, head = kv * group + own % group;
@@ -406,29 +406,39 @@ __global__ void __launch_bounds__(256) join_kernel(AttentionArgs p)
     }
 }
 
-// How a call is cut.  few: pairs of (query, head) in tiles of 32 instead of a head's queries in tiles of 256.
+// How a call is cut.  few: pairs of (query, head) in tiles of 32 instead of a head's queries in tiles of 32 to a wave.
 struct Cut {
     bool few;
-    int splits;
-    int64_t tiles;           // of pairs
+    int waves, splits;
+    int64_t tiles;           // over all sequences, at most
+    size_t map, parts;       // bytes of workspace
 };
 
-Cut cut_of(int64_t q_rows, int64_t k_rows, int64_t n, int64_t heads, int64_t kv_heads)
+Cut cut_of(int64_t q_rows, int64_t k_rows, int64_t n, int64_t heads, int64_t kv_heads, int64_t dim)
 {
     Cut c;
     const int64_t group = heads / kv_heads;
-    c.few = q_rows * group <= 128 * n;
-    c.tiles = most_tiles(q_rows * group, q_rows < n ? q_rows : n, 32);
-    // ranges of 256 keys and more, until there are about 16 blocks for each of the 256 compute units
-    const int64_t by_blocks = 4096 / (c.tiles * kv_heads ? c.tiles * kv_heads : 1), by_keys = k_rows / n / 256;
-    const int64_t splits = by_blocks < by_keys ? by_blocks : by_keys;
-    c.splits = c.few ? int(splits < 1 ? 1 : (splits > 256 ? 256 : splits)) : 1;
+    const int64_t queries = q_rows / n, keys = k_rows / n;         // of a sequence, on average
+    // One tile for the pairs of all heads that share keys: against keys enough to cut in ranges, or for a handful of queries
+    // (4000 sequences of 4, 16 heads on 4: 109 us, by heads 268; 1000 of 16: 66 us, by heads 41)
+    c.few = (queries * group < 64 && keys >= 256) || (queries * group < 32 && group > 1);
+    // Small blocks for short sequences (16 heads on 4 of 64 channels, 16000 tokens in sequences of 64: 2 waves 34 us, 8 waves
+    // 69; of 400: 55 and 64; of 1000: 88 and 82.  32 heads on 8 of 128, 8000 tokens in sequences of 100: 2 waves 64 us, 4 waves
+    // 73; of 1000: 138, 128, 8 waves 152; one of 8192: 8 waves 597, 4 waves 621)
+    c.waves = dim <= 64 ? (queries <= 512 ? 2 : 8) : (queries <= 200 ? 2 : (queries <= 2048 ? 4 : 8));
+    c.splits = 1;
+    if (c.few) {
+        c.tiles = most_tiles(q_rows * group, q_rows < n ? q_rows : n, 32);
+        // ranges of 256 keys and more, until there are about 16 blocks for each of the 256 compute units
+        const int64_t by_blocks = 4096 / (c.tiles * kv_heads ? c.tiles * kv_heads : 1), by_keys = k_rows / n / 256;
+        const int64_t splits = by_blocks < by_keys ? by_blocks : by_keys;
+        c.splits = int(splits < 1 ? 1 : (splits > 256 ? 256 : splits));
+    } else {
+        c.tiles = most_tiles(q_rows, n, 32 * c.waves);
+    }
+    c.map = map_bytes(c.tiles, n);
+    c.parts = c.splits > 1 ? size_t(c.splits) * q_rows * heads * (dim + 2) * sizeof(float) : 0;
     return c;
-}
-
-size_t parts_bytes(const Cut& c, int64_t q_rows, int64_t heads, int64_t dim)
-{
-    return c.splits > 1 ? size_t(c.splits) * q_rows * heads * (dim + 2) * sizeof(float) : 0;
 }
 
 template <typename T, int DP>
@@ -445,10 +455,14 @@ void forward(const AttentionArgs& p, const Cut& cut, hipStream_t stream)
         }
         return;
     }
-        constexpr int QB = 1, WAVES = 8, kRows = 32 * QB * WAVES;
-    const int64_t blocks = most_tiles(p.packed.q_rows, p.packed.n, kRows) * p.heads;
+    const int64_t blocks = cut.tiles * p.heads;
     require(blocks < (int64_t(1) << 31), "too many queries and heads");
-    hipLaunchKernelGGL((attention_kernel<T, DP, QB, WAVES>), dim3(unsigned(blocks)), dim3(WAVES * 64), 0, stream, p);
+    const dim3 grid(static_cast<unsigned>(blocks));
+    switch (cut.waves) {
+    case 2: hipLaunchKernelGGL((attention_kernel<T, DP, 2, 32>), grid, dim3(128), 0, stream, p); break;
+    case 4: hipLaunchKernelGGL((attention_kernel<T, 128, 4, 64>), grid, dim3(256), 0, stream, p); break;
+    default: hipLaunchKernelGGL((attention_kernel<T, DP, 8, 64>), grid, dim3(512), 0, stream, p); break;
+    }
     SIG_HIP(hipGetLastError());
 }
 
@@ -463,7 +477,8 @@ __attribute__((visibility("default"))) uint64_t cusig_amd_attention_workspace(ui
                                                                             uint64_t kv_heads, uint64_t dim) noexcept
 {
     if (!sequences || !kv_heads || !heads || heads % kv_heads) return 0;
-    return parts_bytes(cut_of(int64_t(q_rows), int64_t(k_rows), int64_t(sequences), int64_t(heads), int64_t(kv_heads)), int64_t(q_rows), int64_t(heads), int64_t(dim));
+    const Cut c = cut_of(int64_t(q_rows), int64_t(k_rows), int64_t(sequences), int64_t(heads), int64_t(kv_heads), int64_t(dim));
+    return c.map + c.parts;
 }
 
 __attribute__((visibility("default"))) int cusig_amd_attention(
@@ -479,15 +494,24 @@ __attribute__((visibility("default"))) int cusig_amd_attention(
         if (q_rows == 0 || sequences == 0) return;
         AttentionArgs p{};
         p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
-        p.packed = Packed{q_offsets, k_offsets, k_lengths, int64_t(q_rows), int64_t(k_rows), int(sequences)};
+        p.packed = Packed{q_offsets, k_offsets, k_lengths, int64_t(q_rows), int64_t(k_rows), int(sequences), nullptr};
         p.q_token = q_token, p.q_head = q_head, p.k_token = k_token, p.k_head = k_head, p.v_token = v_token, p.v_head = v_head;
         p.heads = int(heads), p.kv_heads = int(kv_heads), p.dim = int(dim), p.causal = causal;
         p.scale = scale * 1.44269504088896341f;
-        const Cut cut = cut_of(p.packed.q_rows, p.packed.k_rows, p.packed.n, p.heads, p.kv_heads);
-        require(workspace_bytes >= parts_bytes(cut, p.packed.q_rows, p.heads, p.dim) && (workspace || cut.splits == 1), "the workspace is too small");
-        p.parts = static_cast<float*>(workspace);
+        const Cut cut = cut_of(p.packed.q_rows, p.packed.k_rows, p.packed.n, p.heads, p.kv_heads, p.dim);
+        require(workspace_bytes >= cut.map + cut.parts && (workspace || cut.map + cut.parts == 0), "the workspace is too small");
+        p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + cut.map);
         p.splits = cut.splits;
         const hipStream_t s = static_cast<hipStream_t>(stream);
+        if (cut.map) {
+            p.packed.map = static_cast<const int*>(workspace);
+            MapArgs m{};
+            m.packed = p.packed;
+            m.how[0] = cut.few ? Tiling{false, 32, p.heads / p.kv_heads} : Tiling{false, 32 * cut.waves, 1};
+            m.map[0] = static_cast<int*>(workspace);
+            hipLaunchKernelGGL(map_kernel, dim3(1), dim3(kMapThreads), 0, s, m);
+            SIG_HIP(hipGetLastError());
+        }
         switch (dtype) {
         case kBF16: dim <= 64 ? forward<bf16, 64>(p, cut, s) : forward<bf16, 128>(p, cut, s); break;
         case kF16: dim <= 64 ? forward<f16, 64>(p, cut, s) : forward<f16, 128>(p, cut, s); break;

@@ -21,7 +21,7 @@ struct GradArgs {
     void *dq, *dk, *dv;                       // contiguous
     float* delta;                             // [q_rows][heads]
     unsigned* largest;                        // float16: bits of the largest |grad|, zero at the start
-    Packed packed;
+    Packed packed, k_packed;                  // the second with the map of tiles of keys
     int64_t q_token, q_head, k_token, k_head, v_token, v_head, g_token, g_head;
     int heads, kv_heads, dim, causal;
     float scale, scale2;                      // scale2 = scale * log2(e)
@@ -70,10 +70,9 @@ __global__ void __launch_bounds__(WAVES * 64) dq_kernel(GradArgs p)
     constexpr int kThreads = WAVES * 64, kRows = 32 * WAVES, kKeys = 64, kSlices = DP / 16, kBlocks = DP / 32;
     constexpr int kTileBytes = kKeys * Tile<DP>::kRowBytes, kLoads = kKeys * Tile<DP>::kChunks / kThreads;
     __shared__ __attribute__((aligned(16))) char s_tiles[2][2][kTileBytes];
-    __shared__ int s_space[WAVES + 4];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
-    const Span at = find_tile<kThreads>(p.packed, blockIdx.x / p.heads, Dear::kLast, s_space, [](const Span& s) { return (s.nq + kRows - 1) / kRows; });
+    const Span at = find_tile(p.packed, Tiling{false, kRows, 1}, blockIdx.x / p.heads, Dear::kLast);
     if (at.seq < 0) return;
     const int q_first = at.tile * kRows, shift = at.nk - at.nq;
     const int q_past = q_first + kRows < at.nq ? q_first + kRows : at.nq;
@@ -192,11 +191,10 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
     __shared__ __attribute__((aligned(16))) char s_tiles[3][2][kTileBytes];
     __shared__ __attribute__((aligned(16))) float s_lse[3][kQueries], s_delta[3][kQueries];
     __shared__ __attribute__((aligned(16))) u32x4 s_weights[2][PAIRS][KB][2][64];
-    __shared__ int s_space[PAIRS * 2 + 4];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6, pair = wave % PAIRS;
     const bool second = wave >= PAIRS;
     const int kv = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
-    const Span at = find_tile<kThreads>(p.packed, blockIdx.x / p.kv_heads, Dear::kFirst, s_space, [](const Span& s) { return (s.nk + kRows - 1) / kRows; });
+    const Span at = find_tile(p.k_packed, Tiling{true, kRows, 1}, blockIdx.x / p.kv_heads, Dear::kFirst);
     if (at.seq < 0) return;
     const int k_first = at.tile * kRows, shift = at.nk - at.nq;
     // the first query that sees any of the block's keys
@@ -353,30 +351,57 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
         }
 }
 
-__global__ void clear_kernel(unsigned* largest) { *largest = 0; }
+constexpr uint64_t kHeadBytes = 256;
+constexpr int kQueryWaves = 8, kPairs = 4;
+
+struct Space {
+    size_t q_map, k_map, all;
+};
+
+Space space_of(int64_t q_rows, int64_t k_rows, int64_t n, int64_t heads)
+{
+    Space s;
+    s.q_map = map_bytes(most_tiles(q_rows, n, 32 * kQueryWaves), n);
+    s.k_map = map_bytes(most_tiles(k_rows, n, 32 * kPairs), n);
+    s.all = kHeadBytes + s.q_map + s.k_map + size_t(q_rows) * heads * sizeof(float);
+    return s;
+}
 
 template <typename T, int DP>
-void backward(const GradArgs& p, hipStream_t stream)
+void backward(GradArgs& p, void* workspace, hipStream_t stream)
 {
-    constexpr int kWaves = 8, KB = 1, PAIRS = 4;
-    const int64_t q_blocks = most_tiles(p.packed.q_rows, p.packed.n, 32 * kWaves) * p.heads;
-    const int64_t k_blocks = most_tiles(p.packed.k_rows, p.packed.n, 32 * KB * PAIRS) * p.kv_heads;
+    const Space space = space_of(p.packed.q_rows, p.packed.k_rows, p.packed.n, p.heads);
+    char* const at = static_cast<char*>(workspace);
+    p.largest = reinterpret_cast<unsigned*>(at);
+    p.delta = reinterpret_cast<float*>(at + kHeadBytes + space.q_map + space.k_map);
+    const int64_t q_blocks = most_tiles(p.packed.q_rows, p.packed.n, 32 * kQueryWaves) * p.heads;
+    const int64_t k_blocks = most_tiles(p.packed.k_rows, p.packed.n, 32 * kPairs) * p.kv_heads;
     require(q_blocks < (int64_t(1) << 31) && k_blocks < (int64_t(1) << 31), "too many queries and heads");
-    if (__is_same(T, f16)) {
-        hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(1), 0, stream, p.largest);
+    p.k_packed = p.packed;
+    if (space.q_map || __is_same(T, f16)) {
+        MapArgs m{};
+        m.packed = p.packed;
+        m.clear = p.largest;
+        if (space.q_map) {
+            m.how[0] = Tiling{false, 32 * kQueryWaves, 1};
+            m.how[1] = Tiling{true, 32 * kPairs, 1};
+            m.map[0] = reinterpret_cast<int*>(at + kHeadBytes);
+            m.map[1] = reinterpret_cast<int*>(at + kHeadBytes + space.q_map);
+            p.packed.map = m.map[0];
+            p.k_packed.map = m.map[1];
+        }
+        hipLaunchKernelGGL(map_kernel, dim3(space.q_map ? 2 : 1), dim3(space.q_map ? kMapThreads : 64), 0, stream, m);
         SIG_HIP(hipGetLastError());
     }
     if (q_blocks) {
-        hipLaunchKernelGGL((dq_kernel<T, DP, kWaves>), dim3(unsigned(q_blocks)), dim3(kWaves * 64), 0, stream, p);
+        hipLaunchKernelGGL((dq_kernel<T, DP, kQueryWaves>), dim3(unsigned(q_blocks)), dim3(kQueryWaves * 64), 0, stream, p);
         SIG_HIP(hipGetLastError());
     }
     if (k_blocks) {
-        hipLaunchKernelGGL((dkv_kernel<T, DP, KB, PAIRS>), dim3(unsigned(k_blocks)), dim3(PAIRS * 128), 0, stream, p);
+        hipLaunchKernelGGL((dkv_kernel<T, DP, 1, kPairs>), dim3(unsigned(k_blocks)), dim3(kPairs * 128), 0, stream, p);
         SIG_HIP(hipGetLastError());
     }
 }
-
-constexpr uint64_t kHeadBytes = 256;
 
 }  // namespace
 }  // namespace seqamd
@@ -385,9 +410,9 @@ using namespace seqamd;
 
 extern "C" {
 
-__attribute__((visibility("default"))) uint64_t cusig_amd_attention_backprop_workspace(uint64_t q_rows, uint64_t heads) noexcept
+__attribute__((visibility("default"))) uint64_t cusig_amd_attention_backprop_workspace(uint64_t q_rows, uint64_t k_rows, uint64_t sequences, uint64_t heads) noexcept
 {
-    return kHeadBytes + q_rows * heads * sizeof(float);
+    return space_of(int64_t(q_rows), int64_t(k_rows), int64_t(sequences), int64_t(heads)).all;
 }
 
 __attribute__((visibility("default"))) int cusig_amd_attention_backprop(
@@ -401,21 +426,19 @@ __attribute__((visibility("default"))) int cusig_amd_attention_backprop(
         require(dim >= 8 && dim <= 128 && dim % 8 == 0, "a head has 8 to 128 channels, a multiple of 8");
         require(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads < (1u << 20), "heads are a multiple of the key heads");
         require(scale > 0.0f && std::isfinite(scale), "the scale is positive and finite");
-        require(workspace && workspace_bytes >= cusig_amd_attention_backprop_workspace(q_rows, heads), "the workspace is too small");
+        require(workspace && workspace_bytes >= cusig_amd_attention_backprop_workspace(q_rows, k_rows, sequences, heads), "the workspace is too small");
         if (sequences == 0) return;
         GradArgs p{};
         p.q = q, p.k = k, p.v = v, p.out = out, p.grad = grad_out, p.lse = lse, p.dq = dq, p.dk = dk, p.dv = dv;
-        p.largest = static_cast<unsigned*>(workspace);
-        p.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + kHeadBytes);
-        p.packed = Packed{q_offsets, k_offsets, nullptr, int64_t(q_rows), int64_t(k_rows), int(sequences)};
+        p.packed = Packed{q_offsets, k_offsets, nullptr, int64_t(q_rows), int64_t(k_rows), int(sequences), nullptr};
         p.q_token = q_token, p.q_head = q_head, p.k_token = k_token, p.k_head = k_head, p.v_token = v_token, p.v_head = v_head;
         p.g_token = grad_token, p.g_head = grad_head;
         p.heads = int(heads), p.kv_heads = int(kv_heads), p.dim = int(dim), p.causal = causal;
         p.scale = scale, p.scale2 = scale * kLog2e;
         const hipStream_t s = static_cast<hipStream_t>(stream);
         switch (dtype) {
-        case kBF16: dim <= 64 ? backward<bf16, 64>(p, s) : backward<bf16, 128>(p, s); break;
-        case kF16: dim <= 64 ? backward<f16, 64>(p, s) : backward<f16, 128>(p, s); break;
+        case kBF16: dim <= 64 ? backward<bf16, 64>(p, workspace, s) : backward<bf16, 128>(p, workspace, s); break;
+        case kF16: dim <= 64 ? backward<f16, 64>(p, workspace, s) : backward<f16, 128>(p, workspace, s); break;
         default: throw std::invalid_argument("attention takes bfloat16 or float16");
         }
     });

@@ -403,7 +403,8 @@ def attention_inputs(dtype, q_rows, k_rows, heads, kv, dim, seed):
 
 HALVES = [torch.bfloat16, torch.float16]
 SEQUENCES = [([1], [1]), ([0, 3, 0], [0, 3, 0]), ([64], [64]), ([65, 1, 255, 256, 257, 31], None), ([700], None), ([2] * 70, None),
-             ([5, 1, 0, 7, 40], [130, 0, 9, 3, 33]), ([300], [290]), ([90], [500]), ([1, 1, 2], [900, 65, 64])]
+             ([5, 1, 0, 7, 40], [130, 0, 9, 3, 33]), ([300], [290]), ([90], [500]), ([1, 1, 2], [900, 65, 64]), ([33, 0, 1] * 100, None),
+             ([600, 530], None), ([2200], None)]
 
 
 @pytest.mark.gpu
