@@ -141,7 +141,7 @@ CUSIG_ATTENTION = _sequence("attention", "ippppppppuuuuuussssssfbpup")
 CUSIG_ATTENTION_WORKSPACE = _sequence("attention_workspace", "uuuuuu")
 CUSIG_ATTENTION_WORKSPACE.restype = c_uint64
 CUSIG_ATTENTION_BACKPROP = _sequence("attention_backprop", "ipppppppppppuuuuuussssssssfbpup")
-CUSIG_ATTENTION_BACKPROP_WORKSPACE = _sequence("attention_backprop_workspace", "uuuu")
+CUSIG_ATTENTION_BACKPROP_WORKSPACE = _sequence("attention_backprop_workspace", "uuuuu")
 CUSIG_ATTENTION_BACKPROP_WORKSPACE.restype = c_uint64
 
 

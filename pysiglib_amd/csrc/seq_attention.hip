@@ -32,6 +32,7 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
 {
     constexpr int QB = 1, kThreads = WAVES * 64, kRows = 32 * WAVES, kSlices = DP / 16, kBlocks = DP / 32;
     constexpr int kTileBytes = kKeys * Tile<DP>::kRowBytes, kLoads = kKeys * Tile<DP>::kChunks / kThreads;
+    static_assert(kLoads * kThreads == kKeys * Tile<DP>::kChunks, "");
     __shared__ __attribute__((aligned(16))) char s_tiles[2][2][kTileBytes];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     // the heads that share keys and values follow each other at a distance of kv_heads: on the same die where that is a multiple of 8

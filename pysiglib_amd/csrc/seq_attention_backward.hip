@@ -63,12 +63,13 @@ __device__ __forceinline__ void store_columns(T* to, const f32x16* x, float time
         }
 }
 
-// ---- queries fixed: 32 to a wave ----
-template <typename T, int DP, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64) dq_kernel(GradArgs p)
+// ---- queries fixed: 32 to a wave, tiles of kKeys keys ----
+template <typename T, int DP, int WAVES, int kKeys>
+__global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) dq_kernel(GradArgs p)
 {
-    constexpr int kThreads = WAVES * 64, kRows = 32 * WAVES, kKeys = 64, kSlices = DP / 16, kBlocks = DP / 32;
+    constexpr int kThreads = WAVES * 64, kRows = 32 * WAVES, kSlices = DP / 16, kBlocks = DP / 32;
     constexpr int kTileBytes = kKeys * Tile<DP>::kRowBytes, kLoads = kKeys * Tile<DP>::kChunks / kThreads;
+    static_assert(kLoads * kThreads == kKeys * Tile<DP>::kChunks, "");
     __shared__ __attribute__((aligned(16))) char s_tiles[2][2][kTileBytes];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
@@ -155,6 +156,7 @@ __global__ void __launch_bounds__(WAVES * 64) dq_kernel(GradArgs p)
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c) {
             const int key0 = tile * kKeys + 32 * c;
+            if (p.causal && key0 > q_first + wave * 32 + 31 + shift) continue;       // none of the wave's queries sees these
             f32x16 s = zeros16(), dp = zeros16();
 #pragma unroll
             for (int k = 0; k < kSlices; ++k) {
@@ -352,17 +354,33 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 }
 
 constexpr uint64_t kHeadBytes = 256;
-constexpr int kQueryWaves = 8, kPairs = 4;
+
+// Blocks by the average length of the sequences (times of whole calls; 16 heads on 4 of 64 channels, 16000 tokens, and 32 on 8 of
+// 128, 8000 tokens).  Waves of the kernel with its queries fixed: 64 channels, in sequences of 16: 2 waves 140 us, 4 waves 166, 8
+// waves 272; of 1000: 404, 324, 334.  128 channels, of 64: 184, 194, 247; of 1000: 560, 535, 550; one of 8192: 2442, 2338, 2302.
+// Pairs of the kernel with its keys fixed: 64 channels, in sequences of 2000: 1 pair 908 us, 2 pairs 799, 4 pairs 910;
+// 128 channels, of 1000: 790, 537, 548; one of 8192: 3753, 2335, 2235.
+struct Blocks {
+    int waves, pairs;
+};
+
+Blocks blocks_of(int64_t q_rows, int64_t k_rows, int64_t n, int64_t dim)
+{
+    const int64_t queries = q_rows / n, keys = k_rows / n;
+    if (dim <= 64) return Blocks{queries <= 50 ? 2 : 4, 2};
+    return Blocks{queries <= 200 ? 2 : (queries <= 2048 ? 4 : 8), keys <= 4096 ? 2 : 4};
+}
 
 struct Space {
     size_t q_map, k_map, all;
 };
 
-Space space_of(int64_t q_rows, int64_t k_rows, int64_t n, int64_t heads)
+Space space_of(int64_t q_rows, int64_t k_rows, int64_t n, int64_t heads, int64_t dim)
 {
+    const Blocks b = blocks_of(q_rows, k_rows, n, dim);
     Space s;
-    s.q_map = map_bytes(most_tiles(q_rows, n, 32 * kQueryWaves), n);
-    s.k_map = map_bytes(most_tiles(k_rows, n, 32 * kPairs), n);
+    s.q_map = map_bytes(most_tiles(q_rows, n, 32 * b.waves), n);
+    s.k_map = map_bytes(most_tiles(k_rows, n, 32 * b.pairs), n);
     s.all = kHeadBytes + s.q_map + s.k_map + size_t(q_rows) * heads * sizeof(float);
     return s;
 }
@@ -370,12 +388,13 @@ Space space_of(int64_t q_rows, int64_t k_rows, int64_t n, int64_t heads)
 template <typename T, int DP>
 void backward(GradArgs& p, void* workspace, hipStream_t stream)
 {
-    const Space space = space_of(p.packed.q_rows, p.packed.k_rows, p.packed.n, p.heads);
+    const Blocks b = blocks_of(p.packed.q_rows, p.packed.k_rows, p.packed.n, p.dim);
+    const Space space = space_of(p.packed.q_rows, p.packed.k_rows, p.packed.n, p.heads, p.dim);
     char* const at = static_cast<char*>(workspace);
     p.largest = reinterpret_cast<unsigned*>(at);
     p.delta = reinterpret_cast<float*>(at + kHeadBytes + space.q_map + space.k_map);
-    const int64_t q_blocks = most_tiles(p.packed.q_rows, p.packed.n, 32 * kQueryWaves) * p.heads;
-    const int64_t k_blocks = most_tiles(p.packed.k_rows, p.packed.n, 32 * kPairs) * p.kv_heads;
+    const int64_t q_blocks = most_tiles(p.packed.q_rows, p.packed.n, 32 * b.waves) * p.heads;
+    const int64_t k_blocks = most_tiles(p.packed.k_rows, p.packed.n, 32 * b.pairs) * p.kv_heads;
     require(q_blocks < (int64_t(1) << 31) && k_blocks < (int64_t(1) << 31), "too many queries and heads");
     p.k_packed = p.packed;
     if (space.q_map || __is_same(T, f16)) {
@@ -383,8 +402,8 @@ void backward(GradArgs& p, void* workspace, hipStream_t stream)
         m.packed = p.packed;
         m.clear = p.largest;
         if (space.q_map) {
-            m.how[0] = Tiling{false, 32 * kQueryWaves, 1};
-            m.how[1] = Tiling{true, 32 * kPairs, 1};
+            m.how[0] = Tiling{false, 32 * b.waves, 1};
+            m.how[1] = Tiling{true, 32 * b.pairs, 1};
             m.map[0] = reinterpret_cast<int*>(at + kHeadBytes);
             m.map[1] = reinterpret_cast<int*>(at + kHeadBytes + space.q_map);
             p.packed.map = m.map[0];
@@ -394,11 +413,18 @@ void backward(GradArgs& p, void* workspace, hipStream_t stream)
         SIG_HIP(hipGetLastError());
     }
     if (q_blocks) {
-        hipLaunchKernelGGL((dq_kernel<T, DP, kQueryWaves>), dim3(unsigned(q_blocks)), dim3(kQueryWaves * 64), 0, stream, p);
+        const dim3 grid(static_cast<unsigned>(q_blocks));
+        switch (b.waves) {
+        case 2: hipLaunchKernelGGL((dq_kernel<T, DP, 2, 32>), grid, dim3(128), 0, stream, p); break;
+        case 4: hipLaunchKernelGGL((dq_kernel<T, DP, 4, DP / 2>), grid, dim3(256), 0, stream, p); break;
+        default: hipLaunchKernelGGL((dq_kernel<T, 128, 8, 64>), grid, dim3(512), 0, stream, p); break;
+        }
         SIG_HIP(hipGetLastError());
     }
     if (k_blocks) {
-        hipLaunchKernelGGL((dkv_kernel<T, DP, 1, kPairs>), dim3(unsigned(k_blocks)), dim3(kPairs * 128), 0, stream, p);
+        const dim3 grid(static_cast<unsigned>(k_blocks));
+        if (b.pairs == 2) hipLaunchKernelGGL((dkv_kernel<T, DP, 1, 2>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((dkv_kernel<T, 128, 1, 4>), grid, dim3(512), 0, stream, p);
         SIG_HIP(hipGetLastError());
     }
 }
@@ -410,9 +436,9 @@ using namespace seqamd;
 
 extern "C" {
 
-__attribute__((visibility("default"))) uint64_t cusig_amd_attention_backprop_workspace(uint64_t q_rows, uint64_t k_rows, uint64_t sequences, uint64_t heads) noexcept
+__attribute__((visibility("default"))) uint64_t cusig_amd_attention_backprop_workspace(uint64_t q_rows, uint64_t k_rows, uint64_t sequences, uint64_t heads, uint64_t dim) noexcept
 {
-    return space_of(int64_t(q_rows), int64_t(k_rows), int64_t(sequences), int64_t(heads)).all;
+    return sequences ? space_of(int64_t(q_rows), int64_t(k_rows), int64_t(sequences), int64_t(heads), int64_t(dim)).all : kHeadBytes;
 }
 
 __attribute__((visibility("default"))) int cusig_amd_attention_backprop(
@@ -426,7 +452,7 @@ __attribute__((visibility("default"))) int cusig_amd_attention_backprop(
         require(dim >= 8 && dim <= 128 && dim % 8 == 0, "a head has 8 to 128 channels, a multiple of 8");
         require(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads < (1u << 20), "heads are a multiple of the key heads");
         require(scale > 0.0f && std::isfinite(scale), "the scale is positive and finite");
-        require(workspace && workspace_bytes >= cusig_amd_attention_backprop_workspace(q_rows, k_rows, sequences, heads), "the workspace is too small");
+        require(workspace && workspace_bytes >= cusig_amd_attention_backprop_workspace(q_rows, k_rows, sequences, heads, dim), "the workspace is too small");
         if (sequences == 0) return;
         GradArgs p{};
         p.q = q, p.k = k, p.v = v, p.out = out, p.grad = grad_out, p.lse = lse, p.dq = dq, p.dk = dk, p.dv = dv;

@@ -349,7 +349,7 @@ def attention_backprop(grad_out, q, k, v, out, lse, q_offsets, k_offsets, *, cau
     out = _other(out, "out", dtype, q.shape, device)
     lse = _other(lse, "lse", torch.float32, q.shape[:2], device)
     dq, dk, dv = (torch.empty(t.shape, dtype=dtype, device=device) for t in (q, k, v))
-    size = CUSIG_ATTENTION_BACKPROP_WORKSPACE(*sizes[:4])
+    size = CUSIG_ATTENTION_BACKPROP_WORKSPACE(*sizes[:4], sizes[5])
     space = _workspace(size, device)
     _call(CUSIG_ATTENTION_BACKPROP, "attention_backprop", device, _CODES[dtype], grad_out.data_ptr(), q.data_ptr(), k.data_ptr(),
           v.data_ptr(), out.data_ptr(), lse.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), dq.data_ptr(), dk.data_ptr(),
