@@ -99,6 +99,16 @@ struct ColumnRead {
     }
 };
 
+// The operand is there from here on: a load that is still under way when a loop begins would be waited for in each turn of
+// it, with all loads of that turn that are meant to go on meanwhile.
+template <typename T>
+__device__ __forceinline__ void arrive(Frag<T>& f)
+{
+    u32x4 w = __builtin_bit_cast(u32x4, f);
+    asm volatile("" : "+v"(w));
+    f = __builtin_bit_cast(Frag<T>, w);
+}
+
 // eight results as an operand, rounded to nearest: the one rounding between the two products
 template <typename T>
 __device__ __forceinline__ Frag<T> rounded(const f32x16& x, int first)

@@ -77,11 +77,9 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
         for (int i = 0; i < kLoads; ++i) {
             const int e = i * kThreads + tid, row = e / Tile<DP>::kChunks, chunk = e % Tile<DP>::kChunks;
             const int key = tile * kKeys + row < at.nk ? tile * kKeys + row : at.nk - 1;      // rows past the end are never used
-            next[0][i] = next[1][i] = u32x4{0, 0, 0, 0};
-            if (chunk * 8 < p.dim) {
-                __builtin_memcpy(&next[0][i], static_cast<const T*>(p.k) + (at.k0 + key) * p.k_token + kv * p.k_head + chunk * 8, 16);
-                __builtin_memcpy(&next[1][i], static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head + chunk * 8, 16);
-            }
+            const int ch = chunk * 8 < p.dim ? chunk * 8 : p.dim - 8;      // nor are channels: theirs of the queries are zero
+            __builtin_memcpy(&next[0][i], static_cast<const T*>(p.k) + (at.k0 + key) * p.k_token + kv * p.k_head + ch, 16);
+            __builtin_memcpy(&next[1][i], static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head + ch, 16);
         }
     };
     auto put = [&](int buffer) {
@@ -96,6 +94,10 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
         fetch(0);
         put(0);
     }
+#pragma unroll
+    for (int b = 0; b < QB; ++b)
+#pragma unroll
+        for (int k = 0; k < kSlices; ++k) arrive<T>(q[b][k]);
     for (int tile = 0; tile < tiles; ++tile) {
         __syncthreads();
         if (tile + 1 < tiles) fetch(tile + 1);
@@ -242,14 +244,14 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
         for (int i = 0; i < kLoads; ++i) {
             const int e = i * 64 + lane, row = e / Tile<DP>::kChunks, chunk = e % Tile<DP>::kChunks;
             const int at_key = begin + tile * kTile + row, key = at_key < past ? at_key : past - 1;
-            next[0][i] = next[1][i] = u32x4{0, 0, 0, 0};
-            if (chunk * 8 < p.dim) {
-                __builtin_memcpy(&next[0][i], static_cast<const T*>(p.k) + (at.k0 + key) * p.k_token + kv * p.k_head + chunk * 8, 16);
-                __builtin_memcpy(&next[1][i], static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head + chunk * 8, 16);
-            }
+            const int ch = chunk * 8 < p.dim ? chunk * 8 : p.dim - 8;
+            __builtin_memcpy(&next[0][i], static_cast<const T*>(p.k) + (at.k0 + key) * p.k_token + kv * p.k_head + ch, 16);
+            __builtin_memcpy(&next[1][i], static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head + ch, 16);
         }
     };
     if (wave < tiles) fetch(wave);
+#pragma unroll
+    for (int k = 0; k < kSlices; ++k) arrive<T>(q[k]);
     for (int tile = wave; tile < tiles; tile += kWaves) {
         // the wave's own tiles: shared memory serves a wave in order, no barrier is needed
 #pragma unroll

@@ -130,11 +130,9 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) dq_kernel(GradAr
         for (int i = 0; i < kLoads; ++i) {
             const int e = i * kThreads + tid, r = e / Tile<DP>::kChunks, chunk = e % Tile<DP>::kChunks;
             const int key = tile * kKeys + r < at.nk ? tile * kKeys + r : at.nk - 1;
-            next[0][i] = next[1][i] = u32x4{0, 0, 0, 0};
-            if (chunk * 8 < p.dim) {
-                __builtin_memcpy(&next[0][i], static_cast<const T*>(p.k) + (at.k0 + key) * p.k_token + kv * p.k_head + chunk * 8, 16);
-                __builtin_memcpy(&next[1][i], static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head + chunk * 8, 16);
-            }
+            const int ch = chunk * 8 < p.dim ? chunk * 8 : p.dim - 8;      // channels past the end meet zeros, or are not stored
+            __builtin_memcpy(&next[0][i], static_cast<const T*>(p.k) + (at.k0 + key) * p.k_token + kv * p.k_head + ch, 16);
+            __builtin_memcpy(&next[1][i], static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head + ch, 16);
         }
     };
     auto put = [&](int buffer) {
@@ -148,6 +146,11 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) dq_kernel(GradAr
     if (tiles) {
         fetch(0);
         put(0);
+    }
+#pragma unroll
+    for (int k = 0; k < kSlices; ++k) {
+        arrive<T>(q[k]);
+        arrive<T>(g[k]);
     }
     for (int tile = 0; tile < tiles; ++tile) {
         __syncthreads();
@@ -189,7 +192,8 @@ template <typename T, int DP, int KB, int PAIRS>
 __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 {
     constexpr int kThreads = PAIRS * 128, kRows = 32 * KB * PAIRS, kQueries = 32, kSlices = DP / 16, kBlocks = DP / 32;
-    constexpr int kTileBytes = kQueries * Tile<DP>::kRowBytes, kChunksAll = kQueries * Tile<DP>::kChunks, kLoads = (kChunksAll + kThreads - 1) / kThreads;
+    constexpr int kTileBytes = kQueries * Tile<DP>::kRowBytes, kLoads = kQueries * Tile<DP>::kChunks / kThreads;
+    static_assert(kLoads * kThreads == kQueries * Tile<DP>::kChunks, "");
     __shared__ __attribute__((aligned(16))) char s_tiles[3][2][kTileBytes];
     __shared__ __attribute__((aligned(16))) float s_lse[3][kQueries], s_delta[3][kQueries];
     __shared__ __attribute__((aligned(16))) u32x4 s_weights[2][PAIRS][KB][2][64];
@@ -223,49 +227,45 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
     if constexpr (__is_same(T, f16)) lift = towards_one(__uint_as_float(*p.largest));
 
     u32x4 next[2][kLoads];
-    float next_lse = 0.0f, next_delta = 0.0f;
+    float next_lse, next_delta;
+    bool next_in;
     auto fetch = [&](int step) {
         const int head = kv * group + step / tiles, q0 = q_begin + (step % tiles) * kQueries;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int e = i * kThreads + tid, r = e / Tile<DP>::kChunks, chunk = e % Tile<DP>::kChunks;
             const int64_t row = at.q0 + (q0 + r < at.nq ? q0 + r : at.nq - 1);
-            next[0][i] = next[1][i] = u32x4{0, 0, 0, 0};
-            if (e < kChunksAll && chunk * 8 < p.dim) {
-                __builtin_memcpy(&next[0][i], static_cast<const T*>(p.q) + row * p.q_token + head * p.q_head + chunk * 8, 16);
-                __builtin_memcpy(&next[1][i], static_cast<const T*>(p.grad) + row * p.g_token + head * p.g_head + chunk * 8, 16);
-            }
+            const int ch = chunk * 8 < p.dim ? chunk * 8 : p.dim - 8;
+            __builtin_memcpy(&next[0][i], static_cast<const T*>(p.q) + row * p.q_token + head * p.q_head + ch, 16);
+            __builtin_memcpy(&next[1][i], static_cast<const T*>(p.grad) + row * p.g_token + head * p.g_head + ch, 16);
         }
-        if (tid < kQueries) {           // queries past the end, and those that see nothing, have no weights
-            next_lse = INFINITY;
-            next_delta = 0.0f;
-            if (q0 + tid < at.nq) {
-                const int64_t place = (at.q0 + q0 + tid) * p.heads + head;
-                const float l = p.lse[place];
-                next_lse = l == -INFINITY ? INFINITY : l * kLog2e;
-                next_delta = p.delta[place];
-            }
-        }
+        const int mine = q0 + tid % kQueries;
+        const int64_t place = (at.q0 + (mine < at.nq ? mine : at.nq - 1)) * p.heads + head;
+        next_lse = p.lse[place];
+        next_delta = p.delta[place];
+        next_in = mine < at.nq;
     };
     auto put = [&](int buffer) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int e = i * kThreads + tid;
-            if (e < kChunksAll) {
-                const int to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
-                *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + to) = next[0][i];
-                *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + to) = next[1][i];
-            }
+            const int e = i * kThreads + tid, to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
+            *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + to) = next[0][i];
+            *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + to) = next[1][i];
         }
-        if (tid < kQueries) {
-            s_lse[buffer][tid] = next_lse;
-            s_delta[buffer][tid] = next_delta;
+        if (tid < kQueries) {           // queries past the end, and those that see nothing, have no weights
+            const bool none = !next_in || next_lse == -INFINITY;
+            s_lse[buffer][tid] = none ? INFINITY : next_lse * kLog2e;
+            s_delta[buffer][tid] = none ? 0.0f : next_delta;
         }
     };
     if (steps) {
         fetch(0);
         put(0);
     }
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int k = 0; k < kSlices; ++k) arrive<T>(fixed[b][k]);
     int now = 0, before = 2;            // buffers of this step and of the one before it
     for (int step = 0; step <= steps && steps; ++step) {
         __syncthreads();
