@@ -34,6 +34,10 @@ __device__ __forceinline__ f32x16 zeros16()
 // row of the result's i-th value
 __device__ __forceinline__ int row_in(int i, int half) { return (i & 3) + 8 * (i >> 2) + 4 * half; }
 
+// The larger value; NaN where there is one, so that the compiler need not quieten its operands first, an instruction for each
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float larger(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
+
 // the other half's value
 __device__ __forceinline__ float swapped(float x)
 {
@@ -109,6 +113,14 @@ __device__ __forceinline__ void arrive(Frag<T>& f)
     f = __builtin_bit_cast(Frag<T>, w);
 }
 
+// 16 bytes at a byte offset from an address that is the same for the whole wave
+__device__ __forceinline__ u32x4 load_at(const char* base, unsigned offset)
+{
+    u32x4 x;
+    __builtin_memcpy(&x, base + offset, 16);
+    return x;
+}
+
 // eight results as an operand, rounded to nearest: the one rounding between the two products
 template <typename T>
 __device__ __forceinline__ Frag<T> rounded(const f32x16& x, int first)
@@ -117,6 +129,35 @@ __device__ __forceinline__ Frag<T> rounded(const f32x16& x, int first)
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = T(x[first + i]);
     return f;
+}
+
+// eight elements of a row as an operand, zeros behind its end
+template <typename T>
+__device__ __forceinline__ Frag<T> load_row(const T* row, int d, int dim)
+{
+    u32x4 x = {0, 0, 0, 0};
+    if (d < dim) __builtin_memcpy(&x, row + d, 16);
+    return __builtin_bit_cast(Frag<T>, x);
+}
+
+// a lane's column of results, multiplied, as a row of `dim` values
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(T* to, const f32x16* x, float times, int dim, int half)
+{
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int ch = 32 * d + row_in(i, half);
+            if (ch < dim) {
+                float y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = x[d][i + j] * times;
+                Pack<T, 4> pack;
+                pack.set(y);
+                store_pack<T, 4>(to + ch, pack);
+            }
+        }
 }
 
 // Packed sequences.  Offsets are read on the device and kept inside the tensors whatever they hold.
@@ -201,8 +242,7 @@ __device__ __forceinline__ int tiles_of(const Tiling& t, const Span& s)
     return t.keys ? (s.nk + t.size - 1) / t.size : int((int64_t(s.nq) * t.mult + t.size - 1) / t.size);
 }
 
-// The `wanted`-th tile over all sequences; each wave finds it by itself.
-__device__ __forceinline__ Span find_tile(const Packed& p, const Tiling& how, int wanted, Dear dear)
+__device__ __forceinline__ Span any_tile(const Packed& p, const Tiling& how, int wanted, Dear dear)
 {
     Span s;
     s.seq = -1;
@@ -268,6 +308,20 @@ __device__ __forceinline__ Span find_tile(const Packed& p, const Tiling& how, in
     span_of(p, seq, s);
     s.tile = tile;
     if (dear == Dear::kFirst) s.tile = count(s) - 1 - tile;
+    return s;
+}
+
+// The `wanted`-th tile over all sequences; each wave finds it by itself, and holds it in scalar registers.
+__device__ __forceinline__ Span find_tile(const Packed& p, const Tiling& how, int wanted, Dear dear)
+{
+    const Span v = any_tile(p, how, wanted, dear);
+    Span s;
+    s.q0 = __builtin_amdgcn_readfirstlane(int(v.q0));
+    s.k0 = __builtin_amdgcn_readfirstlane(int(v.k0));
+    s.nq = __builtin_amdgcn_readfirstlane(v.nq);
+    s.nk = __builtin_amdgcn_readfirstlane(v.nk);
+    s.tile = __builtin_amdgcn_readfirstlane(v.tile);
+    s.seq = __builtin_amdgcn_readfirstlane(v.seq);
     return s;
 }
 

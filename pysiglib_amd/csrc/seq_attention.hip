@@ -30,11 +30,11 @@ constexpr float kSlack = 8.0f;   // the maximum is taken over where it grew by m
 template <typename T, int DP, int WAVES, int kKeys>
 __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel(AttentionArgs p)
 {
-    constexpr int QB = 1, kThreads = WAVES * 64, kRows = 32 * WAVES, kSlices = DP / 16, kBlocks = DP / 32;
+    constexpr int kThreads = WAVES * 64, kRows = 32 * WAVES, kSlices = DP / 16, kBlocks = DP / 32;
     constexpr int kTileBytes = kKeys * Tile<DP>::kRowBytes, kLoads = kKeys * Tile<DP>::kChunks / kThreads;
     static_assert(kLoads * kThreads == kKeys * Tile<DP>::kChunks, "");
     __shared__ __attribute__((aligned(16))) char s_tiles[2][2][kTileBytes];
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the heads that share keys and values follow each other at a distance of kv_heads: on the same die where that is a multiple of 8
     const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
     // the last tiles see the most keys: they begin first
@@ -49,45 +49,141 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
 
     const RowRead<DP> rows(lane);
     const ColumnRead<DP> columns(lane);
-    int query[QB];
-    Frag<T> q[QB][kSlices];
-    f32x16 o[QB][kBlocks];
-    float top[QB], sum[QB];
+    const int query = q_first + wave * 32 + (lane & 31);
+    Frag<T> q[kSlices];
+    f32x16 o[kBlocks];
+    float top = -INFINITY, sum = 0.0f;
+    {
+        const T* from = static_cast<const T*>(p.q) + (at.q0 + min(query, at.nq - 1)) * p.q_token + head * p.q_head;
 #pragma unroll
-    for (int b = 0; b < QB; ++b) {
-        query[b] = q_first + (wave * QB + b) * 32 + (lane & 31);
-        const int row = query[b] < at.nq ? query[b] : at.nq - 1;
-        const T* from = static_cast<const T*>(p.q) + (at.q0 + row) * p.q_token + head * p.q_head;
-#pragma unroll
-        for (int k = 0; k < kSlices; ++k) {
-            const int d = 16 * k + 8 * half;
-            u32x4 x = {0, 0, 0, 0};
-            if (d < p.dim) __builtin_memcpy(&x, from + d, 16);
-            q[b][k] = __builtin_bit_cast(Frag<T>, x);
-        }
-#pragma unroll
-        for (int d = 0; d < kBlocks; ++d) o[b][d] = zeros16();
-        top[b] = -INFINITY;
-        sum[b] = 0.0f;
+        for (int k = 0; k < kSlices; ++k) q[k] = load_row<T>(from, 16 * k + 8 * half, p.dim);
     }
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d) o[d] = zeros16();
 
+    // A tile's rows at fixed offsets from its first: only the last tile, whose rows may end early, forms them anew
     u32x4 next[2][kLoads];
-    auto fetch = [&](int tile) {
+    unsigned k_at[kLoads], v_at[kLoads];
+    auto offsets = [&](unsigned* to, int64_t token, int left) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int e = i * kThreads + tid, row = e / Tile<DP>::kChunks, chunk = e % Tile<DP>::kChunks;
-            const int key = tile * kKeys + row < at.nk ? tile * kKeys + row : at.nk - 1;      // rows past the end are never used
-            const int ch = chunk * 8 < p.dim ? chunk * 8 : p.dim - 8;      // nor are channels: theirs of the queries are zero
-            __builtin_memcpy(&next[0][i], static_cast<const T*>(p.k) + (at.k0 + key) * p.k_token + kv * p.k_head + ch, 16);
-            __builtin_memcpy(&next[1][i], static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head + ch, 16);
+            const int e = i * kThreads + tid, row = min(e / Tile<DP>::kChunks, left - 1), ch = min(e % Tile<DP>::kChunks * 8, p.dim - 8);
+            to[i] = unsigned((row * int(token) + ch) * int(sizeof(T)));        // rows past the end have no weight, channels meet zeros or are not stored
         }
     };
-    auto put = [&](int buffer) {
+    const char* const k_base = reinterpret_cast<const char*>(static_cast<const T*>(p.k) + at.k0 * p.k_token + kv * p.k_head);
+    const char* const v_base = reinterpret_cast<const char*>(static_cast<const T*>(p.v) + at.k0 * p.v_token + kv * p.v_head);
+    offsets(k_at, p.k_token, min(at.nk, kKeys));
+    offsets(v_at, p.v_token, min(at.nk, kKeys));
+    auto fetch = [&](int tile) __attribute__((always_inline)) {
+        if ((tile + 1) * kKeys > at.nk) {
+            offsets(k_at, p.k_token, at.nk - tile * kKeys);
+            offsets(v_at, p.v_token, at.nk - tile * kKeys);
+        }
+        const char *kp = k_base + tile * int64_t(kKeys * sizeof(T)) * p.k_token, *vp = v_base + tile * int64_t(kKeys * sizeof(T)) * p.v_token;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            next[0][i] = load_at(kp, k_at[i]);
+            next[1][i] = load_at(vp, v_at[i]);
+        }
+    };
+    auto put = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int e = i * kThreads + tid, to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
-            *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + to) = next[0][i];
-            *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + to) = next[1][i];
+            *reinterpret_cast<u32x4*>(s_tiles[tile & 1][0] + to) = next[0][i];
+            *reinterpret_cast<u32x4*>(s_tiles[tile & 1][1] + to) = next[1][i];
+        }
+    };
+    f32x16 s[kKeys / 32];
+    Frag<T> w[kKeys / 16];
+    // 128 channels: operands are read a group ahead of the products that take them, the compiler would read each right before
+    // its product and wait (two waves to a SIMD; 8192 tokens, 32 heads: 548 us, without 580).  64 channels: four waves to a SIMD
+    // hide the waits, and the registers read ahead into would cost one of them (365 us, without 350).
+    constexpr bool kAhead = DP == 128;
+    auto scores = [&](int tile) __attribute__((always_inline)) {
+        const char* kt = s_tiles[tile & 1][0];
+        constexpr int kGroup = kKeys == 64 ? 2 : 4, kGroups = kSlices / kGroup;
+        Frag<T> f[2][kGroup][kKeys / 32];
+        auto read = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k)
+#pragma unroll
+                for (int c = 0; c < kKeys / 32; ++c) f[g & 1][k][c] = rows.template get<T>(kt, 32 * c, g * kGroup + k);
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) s[c] = zeros16();
+        read(0);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            if (g + 1 < kGroups) read(g + 1);
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k)
+#pragma unroll
+                for (int c = 0; c < kKeys / 32; ++c) s[c] = product(f[g & 1][k][c], q[g * kGroup + k], s[c]);
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto weights = [&](int tile) __attribute__((always_inline)) {
+        const int key0 = tile * kKeys;
+        // a key is hidden past the sequence's end, or behind the query's place
+        if (key0 + kKeys > at.nk || (p.causal && key0 + kKeys - 1 > q_first + wave * 32 + shift)) {
+            const int last = p.causal && query + shift < at.nk - 1 ? query + shift : at.nk - 1;
+#pragma unroll
+            for (int c = 0; c < kKeys / 32; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (key0 + 32 * c + row_in(i, half) > last) s[c][i] = -INFINITY;
+        }
+        float part[4];           // chains of their own: each waits for itself alone
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part[j] = larger(s[0][j], s[0][j + 4], s[0][j + 8]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part[j] = kKeys == 64 ? larger(part[j], s[0][j + 12], s[kKeys / 32 - 1][j]) : larger(part[j], s[0][j + 12]);
+        if constexpr (kKeys == 64)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) part[j] = larger(larger(part[j], s[1][j + 4], s[1][j + 8]), s[1][j + 12]);
+        float most = larger(larger(part[0], part[1], part[2]), part[3]);
+        most = larger(most, swapped(most)) * p.scale;
+        if (__any(most > top + kSlack || (top == -INFINITY && most > top))) {
+            const float now = fmaxf(top, most), shrink = top == now ? 1.0f : exp2f(top - now);
+            top = now;
+            sum *= shrink;
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= shrink;
+        }
+        const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part[j] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[c][i] = __builtin_amdgcn_exp2f(fmaf(s[c][i], p.scale, -base));
+                part[i & 3] += s[c][i];
+            }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+        for (int c = 0; c < kKeys / 16; ++c) w[c] = rounded<T>(s[c / 2], 8 * (c & 1));
+    };
+    auto values = [&](int tile) __attribute__((always_inline)) {
+        const char* vt = s_tiles[tile & 1][1];
+        Frag<T> f[2][kBlocks];
+        auto read = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) f[c & 1][d] = columns.template get<T>(vt, 16 * c, d);
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
+        };
+        read(0);
+#pragma unroll
+        for (int c = 0; c < kKeys / 16; ++c) {
+            if (c + 1 < kKeys / 16) read(c + 1);
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) o[d] = product(f[c & 1][d], w[c], o[d]);
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
         }
     };
     if (tiles) {
@@ -95,103 +191,23 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
         put(0);
     }
 #pragma unroll
-    for (int b = 0; b < QB; ++b)
-#pragma unroll
-        for (int k = 0; k < kSlices; ++k) arrive<T>(q[b][k]);
+    for (int k = 0; k < kSlices; ++k) arrive<T>(q[k]);
     for (int tile = 0; tile < tiles; ++tile) {
         __syncthreads();
         if (tile + 1 < tiles) fetch(tile + 1);
-        const char *kt = s_tiles[tile & 1][0], *vt = s_tiles[tile & 1][1];
-        const int key0 = tile * kKeys;
-        // a wave whose queries see none of the tile has nothing to do
-        if (!p.causal || key0 <= q_first + wave * QB * 32 + QB * 32 - 1 + shift) {
-            f32x16 s[QB][kKeys / 32];
-#pragma unroll
-            for (int c = 0; c < kKeys / 32; ++c) {
-#pragma unroll
-                for (int b = 0; b < QB; ++b) s[b][c] = zeros16();
-#pragma unroll
-                for (int k = 0; k < kSlices; ++k) {
-                    const Frag<T> kf = rows.template get<T>(kt, 32 * c, k);
-#pragma unroll
-                    for (int b = 0; b < QB; ++b) s[b][c] = product(kf, q[b][k], s[b][c]);
-                }
-            }
-            // a key is hidden past the sequence's end, or behind the query's place
-            const bool cut = key0 + kKeys > at.nk || (p.causal && key0 + kKeys - 1 > q_first + wave * QB * 32 + shift);
-            if (cut)
-#pragma unroll
-                for (int b = 0; b < QB; ++b) {
-                    const int last = p.causal && query[b] + shift < at.nk - 1 ? query[b] + shift : at.nk - 1;
-#pragma unroll
-                    for (int c = 0; c < kKeys / 32; ++c)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (key0 + 32 * c + row_in(i, half) > last) s[b][c][i] = -INFINITY;
-                }
-            Frag<T> w[QB][kKeys / 16];
-#pragma unroll
-            for (int b = 0; b < QB; ++b) {
-                float most = s[b][0][0];
-#pragma unroll
-                for (int c = 0; c < kKeys / 32; ++c)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) most = fmaxf(most, s[b][c][i]);
-                most = fmaxf(most, swapped(most)) * p.scale;
-                if (__any(most > top[b] + kSlack || (top[b] == -INFINITY && most > top[b]))) {
-                    const float now = fmaxf(top[b], most), shrink = top[b] == now ? 1.0f : exp2f(top[b] - now);
-                    top[b] = now;
-                    sum[b] *= shrink;
-#pragma unroll
-                    for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[b][d][i] *= shrink;
-                }
-                const float base = top[b] == -INFINITY ? 0.0f : top[b];
-#pragma unroll
-                for (int c = 0; c < kKeys / 32; ++c)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        s[b][c][i] = __builtin_amdgcn_exp2f(fmaf(s[b][c][i], p.scale, -base));
-                        sum[b] += s[b][c][i];
-                    }
-#pragma unroll
-                for (int c = 0; c < kKeys / 16; ++c) w[b][c] = rounded<T>(s[b][c / 2], 8 * (c & 1));
-            }
-#pragma unroll
-            for (int c = 0; c < kKeys / 16; ++c)
-#pragma unroll
-                for (int d = 0; d < kBlocks; ++d) {
-                    const Frag<T> vf = columns.template get<T>(vt, 16 * c, d);
-#pragma unroll
-                    for (int b = 0; b < QB; ++b) o[b][d] = product(vf, w[b][c], o[b][d]);
-                }
+        if (!p.causal || tile * kKeys <= q_first + wave * 32 + 31 + shift) {       // else none of the wave's queries sees any of the tile
+            scores(tile);
+            weights(tile);
+            values(tile);
         }
-        if (tile + 1 < tiles) put((tile + 1) & 1);
+        if (tile + 1 < tiles) put(tile + 1);
     }
-#pragma unroll
-    for (int b = 0; b < QB; ++b) {
-        const float total = sum[b] + swapped(sum[b]);
-        if (query[b] >= at.nq) continue;
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        const int64_t row = (at.q0 + query[b]) * p.heads + head;
-        if (half == 0) p.lse[row] = total == 0.0f ? -INFINITY : 0.69314718055994531f * (top[b] + log2f(total));
-        T* to = static_cast<T*>(p.out) + row * p.dim;
-#pragma unroll
-        for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int ch = 32 * d + row_in(i, half);
-                if (ch < p.dim) {
-                    float x[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[j] = o[b][d][i + j] * inv;
-                    Pack<T, 4> pack;
-                    pack.set(x);
-                    store_pack<T, 4>(to + ch, pack);
-                }
-            }
-    }
+    const float total = sum + swapped(sum);
+    if (query >= at.nq) return;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const int64_t row = (at.q0 + query) * p.heads + head;
+    if (half == 0) p.lse[row] = total == 0.0f ? -INFINITY : 0.69314718055994531f * (top + log2f(total));
+    store_row<T, DP>(static_cast<T*>(p.out) + row * p.dim, o, inv, p.dim, half);
 }
 
 // ---- few queries to many keys: rows of a tile are the pairs (query, head) that share a key head ----
@@ -204,7 +220,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
     constexpr int kTileBytes = kTile * Tile<DP>::kRowBytes, kLoads = kTile * Tile<DP>::kChunks / 64;
     __shared__ __attribute__((aligned(16))) char s_tiles[kWaves][2][kTileBytes];
     __shared__ float s_top[kWaves][32], s_sum[kWaves][32];
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = p.heads / p.kv_heads, kv = blockIdx.x % p.kv_heads, split = blockIdx.x / p.kv_heads % p.splits;
     const Span at = find_tile(p.packed, Tiling{false, 32, group}, blockIdx.x / p.kv_heads / p.splits, Dear::kLast);
     if (at.seq < 0) return;
@@ -222,12 +238,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
     {
         const T* from = static_cast<const T*>(p.q) + (at.q0 + query) * p.q_token + head * p.q_head;
 #pragma unroll
-        for (int k = 0; k < kSlices; ++k) {
-            const int d = 16 * k + 8 * half;
-            u32x4 x = {0, 0, 0, 0};
-            if (d < p.dim) __builtin_memcpy(&x, from + d, 16);
-            q[k] = __builtin_bit_cast(Frag<T>, x);
-        }
+        for (int k = 0; k < kSlices; ++k) q[k] = load_row<T>(from, 16 * k + 8 * half, p.dim);
     }
     const RowRead<DP> rows(lane);
     const ColumnRead<DP> columns(lane);
@@ -270,10 +281,11 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 if (key0 + row_in(i, half) > last) s[i] = -INFINITY;
-        float most = s[0];
+        float most = larger(s[0], s[1], s[2]);
 #pragma unroll
-        for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
-        most = fmaxf(most, swapped(most)) * p.scale;
+        for (int i = 3; i < 15; i += 2) most = larger(most, s[i], s[i + 1]);
+        most = larger(most, s[15]);
+        most = larger(most, swapped(most)) * p.scale;
         if (__any(most > top + kSlack || (top == -INFINITY && most > top))) {
             const float now = fmaxf(top, most), shrink = top == now ? 1.0f : exp2f(top - now);
             top = now;
@@ -357,21 +369,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     if (half == 0) p.lse[row] = total == 0.0f ? -INFINITY : 0.69314718055994531f * (most + log2f(total));
-    T* to = static_cast<T*>(p.out) + row * p.dim;
-#pragma unroll
-    for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int ch = 32 * d + row_in(i, half);
-            if (ch < p.dim) {
-                float x[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = o[d][i + j] * inv;
-                Pack<T, 4> pack;
-                pack.set(x);
-                store_pack<T, 4>(to + ch, pack);
-            }
-        }
+    store_row<T, DP>(static_cast<T*>(p.out) + row * p.dim, o, inv, p.dim, half);
 }
 
 // the splits of one (query, head) to a wave, a lane to one or two channels pairwise

@@ -35,43 +35,15 @@ __device__ __forceinline__ float towards_one(float largest)
     return largest > 0.0f && largest < INFINITY ? ldexpf(1.0f, -ilogbf(largest)) : 1.0f;
 }
 
-template <typename T>
-__device__ __forceinline__ Frag<T> load_row(const T* row, int d, int dim)
-{
-    u32x4 x = {0, 0, 0, 0};
-    if (d < dim) __builtin_memcpy(&x, row + d, 16);
-    return __builtin_bit_cast(Frag<T>, x);
-}
-
-// sums of a block's results, multiplied, to a row of `dim` values
-template <typename T, int DP>
-__device__ __forceinline__ void store_columns(T* to, const f32x16* x, float times, int dim, int half)
-{
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int ch = 32 * d + row_in(i, half);
-            if (ch < dim) {
-                float y[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = x[d][i + j] * times;
-                Pack<T, 4> pack;
-                pack.set(y);
-                store_pack<T, 4>(to + ch, pack);
-            }
-        }
-}
-
 // ---- queries fixed: 32 to a wave, tiles of kKeys keys ----
 template <typename T, int DP, int WAVES, int kKeys>
-__global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) dq_kernel(GradArgs p)
+__global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 3 : 2) dq_kernel(GradArgs p)
 {
     constexpr int kThreads = WAVES * 64, kRows = 32 * WAVES, kSlices = DP / 16, kBlocks = DP / 32;
     constexpr int kTileBytes = kKeys * Tile<DP>::kRowBytes, kLoads = kKeys * Tile<DP>::kChunks / kThreads;
     static_assert(kLoads * kThreads == kKeys * Tile<DP>::kChunks, "");
     __shared__ __attribute__((aligned(16))) char s_tiles[2][2][kTileBytes];
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
     const Span at = find_tile(p.packed, Tiling{false, kRows, 1}, blockIdx.x / p.heads, Dear::kLast);
     if (at.seq < 0) return;
@@ -125,22 +97,59 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) dq_kernel(GradAr
     for (int d = 0; d < kBlocks; ++d) dq[d] = zeros16();
 
     u32x4 next[2][kLoads];
-    auto fetch = [&](int tile) {
+    unsigned k_at[kLoads], v_at[kLoads];
+    auto offsets = [&](int left) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int e = i * kThreads + tid, r = e / Tile<DP>::kChunks, chunk = e % Tile<DP>::kChunks;
-            const int key = tile * kKeys + r < at.nk ? tile * kKeys + r : at.nk - 1;
-            const int ch = chunk * 8 < p.dim ? chunk * 8 : p.dim - 8;      // channels past the end meet zeros, or are not stored
-            __builtin_memcpy(&next[0][i], static_cast<const T*>(p.k) + (at.k0 + key) * p.k_token + kv * p.k_head + ch, 16);
-            __builtin_memcpy(&next[1][i], static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head + ch, 16);
+            const int e = i * kThreads + tid, r = min(e / Tile<DP>::kChunks, left - 1), ch = min(e % Tile<DP>::kChunks * 8, p.dim - 8);
+            k_at[i] = unsigned((r * int(p.k_token) + ch) * int(sizeof(T)));
+            v_at[i] = unsigned((r * int(p.v_token) + ch) * int(sizeof(T)));
         }
     };
-    auto put = [&](int buffer) {
+    const char* const k_base = reinterpret_cast<const char*>(static_cast<const T*>(p.k) + at.k0 * p.k_token + kv * p.k_head);
+    const char* const v_base = reinterpret_cast<const char*>(static_cast<const T*>(p.v) + at.k0 * p.v_token + kv * p.v_head);
+    offsets(kKeys);
+    auto fetch = [&](int tile) __attribute__((always_inline)) {
+        if ((tile + 1) * kKeys > at.nk) offsets(at.nk - tile * kKeys);
+        const char *kp = k_base + tile * int64_t(kKeys * sizeof(T)) * p.k_token, *vp = v_base + tile * int64_t(kKeys * sizeof(T)) * p.v_token;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            next[0][i] = load_at(kp, k_at[i]);
+            next[1][i] = load_at(vp, v_at[i]);
+        }
+    };
+    auto put = [&](int buffer) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int e = i * kThreads + tid, to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
             *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + to) = next[0][i];
             *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + to) = next[1][i];
+        }
+    };
+    constexpr bool kAhead = DP == 128;
+    // S^T and dP^T of 32 keys; 128 channels: operands are read a group ahead, as in the forward
+    auto pair_products = [&](const char* kt, const char* vt, int row0, f32x16& s, f32x16& dp) __attribute__((always_inline)) {
+        constexpr int kGroup = 1, kGroups = kSlices / kGroup;
+        Frag<T> kf[2][kGroup], vf[2][kGroup];
+        auto read = [&](int n) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k) {
+                kf[n & 1][k] = rows.template get<T>(kt, row0, n * kGroup + k);
+                vf[n & 1][k] = rows.template get<T>(vt, row0, n * kGroup + k);
+            }
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
+        };
+        s = zeros16(), dp = zeros16();
+        read(0);
+#pragma unroll
+        for (int n = 0; n < kGroups; ++n) {
+            if (n + 1 < kGroups) read(n + 1);
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k) {
+                s = product(kf[n & 1][k], q[n * kGroup + k], s);
+                dp = product(vf[n & 1][k], g[n * kGroup + k], dp);
+            }
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
         }
     };
     if (tiles) {
@@ -160,12 +169,8 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) dq_kernel(GradAr
         for (int c = 0; c < kKeys / 32; ++c) {
             const int key0 = tile * kKeys + 32 * c;
             if (p.causal && key0 > q_first + wave * 32 + 31 + shift) continue;       // none of the wave's queries sees these
-            f32x16 s = zeros16(), dp = zeros16();
-#pragma unroll
-            for (int k = 0; k < kSlices; ++k) {
-                s = product(rows.template get<T>(kt, 32 * c, k), q[k], s);
-                dp = product(rows.template get<T>(vt, 32 * c, k), g[k], dp);
-            }
+            f32x16 s, dp;
+            pair_products(kt, vt, 32 * c, s, dp);
             if (key0 + 32 > at.nk || (p.causal && key0 + 31 > q_first + wave * 32 + shift))
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
@@ -175,29 +180,36 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) dq_kernel(GradAr
                 const float w = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -lse));
                 s[i] = w * (__is_same(T, f16) ? lift * (dp[i] - delta) : dp[i] - delta);
             }
+            Frag<T> f[2][kBlocks];
+            auto read = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) f[u][d] = columns.template get<T>(kt, 32 * c + 16 * u, d);
+            };
+            read(0);
+            read(1);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const Frag<T> ds = rounded<T>(s, 8 * u);
 #pragma unroll
-                for (int d = 0; d < kBlocks; ++d) dq[d] = product(columns.template get<T>(kt, 32 * c + 16 * u, d), ds, dq[d]);
+                for (int d = 0; d < kBlocks; ++d) dq[d] = product(f[u][d], ds, dq[d]);
             }
         }
         if (tile + 1 < tiles) put((tile + 1) & 1);
     }
-    if (query < at.nq) store_columns<T, DP>(static_cast<T*>(p.dq) + place * p.dim, dq, p.scale / lift, p.dim, half);
+    if (query < at.nq) store_row<T, DP>(static_cast<T*>(p.dq) + place * p.dim, dq, p.scale / lift, p.dim, half);
 }
 
-// ---- keys fixed: KB * 32 to a pair of waves, PAIRS pairs to a block ----
-template <typename T, int DP, int KB, int PAIRS>
+// ---- keys fixed: 32 to a pair of waves, PAIRS pairs to a block; queries in steps of kQueries ----
+template <typename T, int DP, int PAIRS, int kQueries>
 __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 {
-    constexpr int kThreads = PAIRS * 128, kRows = 32 * KB * PAIRS, kQueries = 32, kSlices = DP / 16, kBlocks = DP / 32;
+    constexpr int kThreads = PAIRS * 128, kRows = 32 * PAIRS, kSlices = DP / 16, kBlocks = DP / 32, kParts = kQueries / 32;
     constexpr int kTileBytes = kQueries * Tile<DP>::kRowBytes, kLoads = kQueries * Tile<DP>::kChunks / kThreads;
     static_assert(kLoads * kThreads == kQueries * Tile<DP>::kChunks, "");
     __shared__ __attribute__((aligned(16))) char s_tiles[3][2][kTileBytes];
     __shared__ __attribute__((aligned(16))) float s_lse[3][kQueries], s_delta[3][kQueries];
-    __shared__ __attribute__((aligned(16))) u32x4 s_weights[2][PAIRS][KB][2][64];
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6, pair = wave % PAIRS;
+    __shared__ __attribute__((aligned(16))) u32x4 s_weights[2][PAIRS][kParts][2][64];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave % PAIRS;
     const bool second = wave >= PAIRS;
     const int kv = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
     const Span at = find_tile(p.k_packed, Tiling{true, kRows, 1}, blockIdx.x / p.kv_heads, Dear::kFirst);
@@ -210,18 +222,16 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 
     const RowRead<DP> rows(lane);
     const ColumnRead<DP> columns(lane);
-    int key[KB];
-    Frag<T> fixed[KB][kSlices];         // keys, in the second wave values
-    f32x16 sums[KB][kBlocks];           // dV, in the second wave dK
-#pragma unroll
-    for (int b = 0; b < KB; ++b) {
-        key[b] = k_first + (pair * KB + b) * 32 + (lane & 31);
-        const int64_t r = at.k0 + (key[b] < at.nk ? key[b] : at.nk - 1);
+    const int key0 = k_first + pair * 32, key = key0 + (lane & 31);
+    Frag<T> fixed[kSlices];             // keys, in the second wave values
+    f32x16 sums[kBlocks];               // dV, in the second wave dK
+    {
+        const int64_t r = at.k0 + min(key, at.nk - 1);
         const T* from = second ? static_cast<const T*>(p.v) + r * p.v_token + kv * p.v_head : static_cast<const T*>(p.k) + r * p.k_token + kv * p.k_head;
 #pragma unroll
-        for (int k = 0; k < kSlices; ++k) fixed[b][k] = load_row<T>(from, 16 * k + 8 * half, p.dim);
+        for (int k = 0; k < kSlices; ++k) fixed[k] = load_row<T>(from, 16 * k + 8 * half, p.dim);
 #pragma unroll
-        for (int d = 0; d < kBlocks; ++d) sums[b][d] = zeros16();
+        for (int d = 0; d < kBlocks; ++d) sums[d] = zeros16();
     }
     float lift = 1.0f;
     if constexpr (__is_same(T, f16)) lift = towards_one(__uint_as_float(*p.largest));
@@ -229,23 +239,23 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
     u32x4 next[2][kLoads];
     float next_lse, next_delta;
     bool next_in;
-    auto fetch = [&](int step) {
-        const int head = kv * group + step / tiles, q0 = q_begin + (step % tiles) * kQueries;
+    auto fetch = [&](int head, int tile) __attribute__((always_inline)) {
+        const int q0 = q_begin + tile * kQueries, left = at.nq - q0 - 1;
+        const char* qp = reinterpret_cast<const char*>(static_cast<const T*>(p.q) + (at.q0 + q0) * p.q_token + head * p.q_head);
+        const char* gp = reinterpret_cast<const char*>(static_cast<const T*>(p.grad) + (at.q0 + q0) * p.g_token + head * p.g_head);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int e = i * kThreads + tid, r = e / Tile<DP>::kChunks, chunk = e % Tile<DP>::kChunks;
-            const int64_t row = at.q0 + (q0 + r < at.nq ? q0 + r : at.nq - 1);
-            const int ch = chunk * 8 < p.dim ? chunk * 8 : p.dim - 8;
-            __builtin_memcpy(&next[0][i], static_cast<const T*>(p.q) + row * p.q_token + head * p.q_head + ch, 16);
-            __builtin_memcpy(&next[1][i], static_cast<const T*>(p.grad) + row * p.g_token + head * p.g_head + ch, 16);
+            const int e = i * kThreads + tid, r = min(e / Tile<DP>::kChunks, left), ch = min(e % Tile<DP>::kChunks * 8, p.dim - 8);
+            next[0][i] = load_at(qp, unsigned((r * int(p.q_token) + ch) * int(sizeof(T))));
+            next[1][i] = load_at(gp, unsigned((r * int(p.g_token) + ch) * int(sizeof(T))));
         }
-        const int mine = q0 + tid % kQueries;
-        const int64_t place = (at.q0 + (mine < at.nq ? mine : at.nq - 1)) * p.heads + head;
-        next_lse = p.lse[place];
-        next_delta = p.delta[place];
-        next_in = mine < at.nq;
+        const int64_t first = (at.q0 + q0) * p.heads + head;
+        const int mine = tid % kQueries, place = min(mine, left) * p.heads;
+        next_lse = p.lse[first + place];
+        next_delta = p.delta[first + place];
+        next_in = mine <= left;
     };
-    auto put = [&](int buffer) {
+    auto put = [&](int buffer) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int e = i * kThreads + tid, to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
@@ -258,117 +268,115 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
             s_delta[buffer][tid] = none ? 0.0f : next_delta;
         }
     };
+    constexpr bool kAhead = DP == 128;
+    // 32 rows of a tile times the fixed operand; 128 channels: operands are read a group ahead, as in the forward
+    auto by_rows = [&](const char* tile, int row0) __attribute__((always_inline)) {
+        constexpr int kGroup = 4, kGroups = kSlices / kGroup;
+        Frag<T> f[2][kGroup];
+        auto read = [&](int n) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k) f[n & 1][k] = rows.template get<T>(tile, row0, n * kGroup + k);
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
+        };
+        f32x16 x = zeros16();
+        read(0);
+#pragma unroll
+        for (int n = 0; n < kGroups; ++n) {
+            if (n + 1 < kGroups) read(n + 1);
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k) x = product(f[n & 1][k], fixed[n * kGroup + k], x);
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
+        }
+        return x;
+    };
+    // adds the columns of 32 rows times the two operands
+    auto by_columns = [&](const char* tile, int row0, const Frag<T>* w) __attribute__((always_inline)) {
+        Frag<T> f[2][kBlocks];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) f[u][d] = columns.template get<T>(tile, row0 + 16 * u, d);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) sums[d] = product(f[u][d], w[u], sums[d]);
+    };
     if (steps) {
-        fetch(0);
+        fetch(kv * group, 0);
         put(0);
     }
 #pragma unroll
-    for (int b = 0; b < KB; ++b)
-#pragma unroll
-        for (int k = 0; k < kSlices; ++k) arrive<T>(fixed[b][k]);
+    for (int k = 0; k < kSlices; ++k) arrive<T>(fixed[k]);
     int now = 0, before = 2;            // buffers of this step and of the one before it
+    int head = kv * group, tile = 0;    // of this step
     for (int step = 0; step <= steps && steps; ++step) {
         __syncthreads();
         const int after = now == 2 ? 0 : now + 1;
-        if (step + 1 < steps) fetch(step + 1);
+        const int q0 = q_begin + tile * kQueries;
+        if (++tile == tiles) tile = 0, ++head;
+        if (step + 1 < steps) fetch(head, tile);
         if (!second && step < steps) {
-            const char *qt = s_tiles[now][0], *gt = s_tiles[now][1];
-            const int q0 = q_begin + (step % tiles) * kQueries;
-            f32x16 s[KB];
 #pragma unroll
-            for (int b = 0; b < KB; ++b) s[b] = zeros16();
-#pragma unroll
-            for (int k = 0; k < kSlices; ++k) {
-                const Frag<T> f = rows.template get<T>(qt, 0, k);
-#pragma unroll
-                for (int b = 0; b < KB; ++b) s[b] = product(f, fixed[b][k], s[b]);
-            }
-            float lse[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) lse[i] = s_lse[now][row_in(i, half)];
-#pragma unroll
-            for (int b = 0; b < KB; ++b) {
-                if (p.causal && q0 + shift < k_first + (pair * KB + b) * 32 + 31)
+            for (int c = 0; c < kParts; ++c) {
+                f32x16 s = by_rows(s_tiles[now][0], 32 * c);
+                if (p.causal && q0 + 32 * c + shift < key0 + 31)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (key[b] > q0 + row_in(i, half) + shift) s[b][i] = -INFINITY;
+                        if (key > q0 + 32 * c + row_in(i, half) + shift) s[i] = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], p.scale2, -lse[i]));
-#pragma unroll
-                for (int u = 0; u < 2; ++u) s_weights[step & 1][pair][b][u][lane] = __builtin_bit_cast(u32x4, rounded<T>(s[b], 8 * u));
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int d = 0; d < kBlocks; ++d) {
-                    const Frag<T> f = columns.template get<T>(gt, 16 * u, d);
-#pragma unroll
-                    for (int b = 0; b < KB; ++b) sums[b][d] = product(f, rounded<T>(s[b], 8 * u), sums[b][d]);
-                }
-        }
-        if (second && step > 0) {
-            const char *qt = s_tiles[before][0], *gt = s_tiles[before][1];
-            f32x16 dp[KB];
-#pragma unroll
-            for (int b = 0; b < KB; ++b) dp[b] = zeros16();
-#pragma unroll
-            for (int k = 0; k < kSlices; ++k) {
-                const Frag<T> f = rows.template get<T>(gt, 0, k);
-#pragma unroll
-                for (int b = 0; b < KB; ++b) dp[b] = product(f, fixed[b][k], dp[b]);
-            }
-            float delta[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) delta[i] = s_delta[before][row_in(i, half)];
-            Frag<T> ds[KB][2];
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
+                for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -s_lse[now][32 * c + row_in(i, half)]));
+                Frag<T> w[2];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const Frag<T> w = __builtin_bit_cast(Frag<T>, s_weights[(step - 1) & 1][pair][b][u][lane]);
+                    w[u] = rounded<T>(s, 8 * u);
+                    s_weights[step & 1][pair][c][u][lane] = __builtin_bit_cast(u32x4, w[u]);
+                }
+                by_columns(s_tiles[now][1], 32 * c, w);
+            }
+        }
+        if (second && step > 0) {
+#pragma unroll
+            for (int c = 0; c < kParts; ++c) {
+                const f32x16 dp = by_rows(s_tiles[before][1], 32 * c);
+                Frag<T> ds[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const Frag<T> w = __builtin_bit_cast(Frag<T>, s_weights[(step - 1) & 1][pair][c][u][lane]);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float x = dp[b][8 * u + i] - delta[8 * u + i];
-                        ds[b][u][i] = T(static_cast<float>(w[i]) * (__is_same(T, f16) ? x * lift : x));
+                        const float x = dp[8 * u + i] - s_delta[before][32 * c + row_in(8 * u + i, half)];
+                        ds[u][i] = T(static_cast<float>(w[i]) * (__is_same(T, f16) ? x * lift : x));
                     }
                 }
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int d = 0; d < kBlocks; ++d) {
-                    const Frag<T> f = columns.template get<T>(qt, 16 * u, d);
-#pragma unroll
-                    for (int b = 0; b < KB; ++b) sums[b][d] = product(f, ds[b][u], sums[b][d]);
-                }
+                by_columns(s_tiles[before][0], 32 * c, ds);
+            }
         }
         if (step + 1 < steps) put(after);
         before = now;
         now = after;
     }
-#pragma unroll
-    for (int b = 0; b < KB; ++b)
-        if (key[b] < at.nk) {
-            T* to = static_cast<T*>(second ? p.dk : p.dv) + ((at.k0 + key[b]) * p.kv_heads + kv) * p.dim;
-            store_columns<T, DP>(to, sums[b], second ? p.scale / lift : 1.0f, p.dim, half);
-        }
+    if (key < at.nk)
+        store_row<T, DP>(static_cast<T*>(second ? p.dk : p.dv) + ((at.k0 + key) * p.kv_heads + kv) * p.dim, sums, second ? p.scale / lift : 1.0f, p.dim, half);
 }
 
 constexpr uint64_t kHeadBytes = 256;
 
-// Blocks by the average length of the sequences (times of whole calls; 16 heads on 4 of 64 channels, 16000 tokens, and 32 on 8 of
-// 128, 8000 tokens).  Waves of the kernel with its queries fixed: 64 channels, in sequences of 16: 2 waves 140 us, 4 waves 166, 8
-// waves 272; of 1000: 404, 324, 334.  128 channels, of 64: 184, 194, 247; of 1000: 560, 535, 550; one of 8192: 2442, 2338, 2302.
-// Pairs of the kernel with its keys fixed: 64 channels, in sequences of 2000: 1 pair 908 us, 2 pairs 799, 4 pairs 910;
-// 128 channels, of 1000: 790, 537, 548; one of 8192: 3753, 2335, 2235.
+// Blocks by the average length of the sequences, from times of whole calls (16 heads on 4 of 64 channels, 16000 tokens, and 32 on
+// 8 of 128, 8000 tokens).
+// Queries fixed, waves of a block: 64 channels, sequences of 16: 2 waves 140 us, 4 waves 166; of 1000: 404 and 324.  128
+// channels, of 16: 2 waves 178 us, 8 waves 232; of 400: 4 waves 250; of 2000: 4 waves 466 us, 8 waves 480; one of 8192: 8 waves 1934 us.
+// Keys fixed: 64 channels, 2 pairs, sequences of 16: steps of 32 queries 94 us, of 64 132; of 400: 150 and 139; of 8192: 895
+// and 804.  128 channels, of 64: 2 pairs and 32 queries 172 us, 4 pairs and 64 queries 191; of 1000: 493 and 498; 4 of 1600 to
+// 2047: 546 and 508; two of 4096: 1057 and 955.
 struct Blocks {
-    int waves, pairs;
+    int waves, pairs, queries;
 };
 
 Blocks blocks_of(int64_t q_rows, int64_t k_rows, int64_t n, int64_t dim)
 {
     const int64_t queries = q_rows / n, keys = k_rows / n;
-    if (dim <= 64) return Blocks{queries <= 50 ? 2 : 4, 2};
-    return Blocks{queries <= 200 ? 2 : (queries <= 2048 ? 4 : 8), keys <= 4096 ? 2 : 4};
+    if (dim <= 64) return Blocks{queries <= 50 ? 2 : 4, 2, keys <= 200 ? 32 : 64};
+    return Blocks{queries <= 200 ? 2 : (queries <= 2048 ? 4 : 8), keys <= 700 ? 2 : 4, keys <= 700 ? 32 : 64};
 }
 
 struct Space {
@@ -416,15 +424,15 @@ void backward(GradArgs& p, void* workspace, hipStream_t stream)
         const dim3 grid(static_cast<unsigned>(q_blocks));
         switch (b.waves) {
         case 2: hipLaunchKernelGGL((dq_kernel<T, DP, 2, 32>), grid, dim3(128), 0, stream, p); break;
-        case 4: hipLaunchKernelGGL((dq_kernel<T, DP, 4, DP / 2>), grid, dim3(256), 0, stream, p); break;
-        default: hipLaunchKernelGGL((dq_kernel<T, 128, 8, 64>), grid, dim3(512), 0, stream, p); break;
+        case 4: hipLaunchKernelGGL((dq_kernel<T, DP, 4, 32>), grid, dim3(256), 0, stream, p); break;
+        default: hipLaunchKernelGGL((dq_kernel<T, 128, 8, 32>), grid, dim3(512), 0, stream, p); break;
         }
         SIG_HIP(hipGetLastError());
     }
     if (k_blocks) {
         const dim3 grid(static_cast<unsigned>(k_blocks));
-        if (b.pairs == 2) hipLaunchKernelGGL((dkv_kernel<T, DP, 1, 2>), grid, dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL((dkv_kernel<T, 128, 1, 4>), grid, dim3(512), 0, stream, p);
+        if (b.queries == 32) hipLaunchKernelGGL((dkv_kernel<T, DP, 2, 32>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((dkv_kernel<T, DP, DP == 64 ? 2 : 4, 64>), grid, dim3(DP == 64 ? 256 : 512), 0, stream, p);
         SIG_HIP(hipGetLastError());
     }
 }
