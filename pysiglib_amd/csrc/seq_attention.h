@@ -168,7 +168,7 @@ struct Packed {
     const int* map;      // more than kMapped sequences: the number of tiles, then (sequence, tile) of each, see map_kernel
 };
 
-constexpr int kMapped = 256;
+constexpr int kMapped = 64;
 
 // How a sequence is cut into tiles: by its keys, or by its queries times `mult`
 struct Tiling {
@@ -255,7 +255,7 @@ __device__ __forceinline__ Span any_tile(const Packed& p, const Tiling& how, int
         if (wanted >= tiles) s.seq = -1;
         return s;
     }
-    if (p.n <= 64) {
+    if (p.n <= kMapped) {
         // a sequence to a lane.  Level by level (a level: the tiles at the same distance), the levels below r hold
         // sum of min(tiles, r); r by bisection, bit by bit
         Span own{};
@@ -272,35 +272,6 @@ __device__ __forceinline__ Span any_tile(const Packed& p, const Tiling& how, int
         const unsigned long long there = __ballot(tiles > level), mine = 1ull << lane;
         const int holder = __ffsll(__ballot((there & mine) && __popcll(there & (mine - 1)) == target - below)) - 1;
         return taken(own, holder, holder, dear == Dear::kLast ? level : __shfl(tiles, holder) - 1 - level);
-    }
-    if (p.n <= kMapped) {
-        // up to four sequences to a lane, one after the other
-        const int each = (p.n + 63) / 64;
-        Span own[4];
-        int tiles[4], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int seq = lane * each + i;
-            const bool is = i < each && seq < p.n;
-            if (is) span_of(p, seq, own[i]);
-            else own[i] = Span{};
-            tiles[i] = is ? count(own[i]) : 0;
-            sum += tiles[i];
-        }
-        const int upto = wave_scan(sum), target = __shfl(upto, 63) - 1 - wanted;
-        if (target < 0) return s;
-        const int holder = __ffsll(__ballot(target < upto)) - 1;
-        int left = target - (upto - sum), which = 0, there = tiles[0];
-        Span one = own[0];
-#pragma unroll
-        for (int i = 1; i < 4; ++i)
-            if (which == i - 1 && left >= there) {
-                left -= there;
-                which = i;
-                there = tiles[i];
-                one = own[i];
-            }
-        return taken(one, holder, holder * each + __shfl(which, holder), __shfl(dear == Dear::kLast ? left : there - 1 - left, holder));
     }
     const int target = p.map[0] - 1 - wanted;
     if (target < 0) return s;

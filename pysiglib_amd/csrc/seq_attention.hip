@@ -384,21 +384,31 @@ __global__ void __launch_bounds__(256) join_kernel(AttentionArgs p)
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
     const float base = most == -INFINITY ? 0.0f : most;
-    const float* from = p.parts + 2 * p.splits * all + row * p.dim;
+    const int ch = min(2 * lane, p.dim - 2);
+    const float* from = p.parts + 2 * p.splits * all + row * p.dim + ch;
     float total = 0.0f, x[2] = {0.0f, 0.0f};
-    const bool in = 2 * lane < p.dim;
-    for (int s = 0; s < p.splits; ++s) {
-        const int64_t place = s * all + row;
-        const float w = exp2f(p.parts[2 * place] - base);
-        total += w * p.parts[2 * place + 1];
-        if (in) {
-            x[0] = fmaf(w, from[s * all * p.dim + 2 * lane], x[0]);
-            x[1] = fmaf(w, from[s * all * p.dim + 2 * lane + 1], x[1]);
+    for (int first = 0; first < p.splits; first += 64) {
+        // a split's maximum and sum to a lane; then the splits' values, whose loads wait for nothing
+        float w = 0.0f;
+        if (first + lane < p.splits) {
+            const int64_t place = (first + lane) * all + row;
+            w = exp2f(p.parts[2 * place] - base);
+            total += w * p.parts[2 * place + 1];
+        }
+        const int count = min(64, p.splits - first);
+#pragma unroll 8
+        for (int s = 0; s < count; ++s) {
+            const float ws = __shfl(w, s);
+            const Pack<float, 2> v = load_pack<float, 2>(from + (first + s) * all * p.dim);
+            x[0] = fmaf(ws, v.get(0), x[0]);
+            x[1] = fmaf(ws, v.get(1), x[1]);
         }
     }
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) total += __shfl_xor(total, m);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     if (lane == 0) p.lse[row] = total == 0.0f ? -INFINITY : 0.69314718055994531f * (most + log2f(total));
-    if (in) {
+    if (2 * lane < p.dim) {
         x[0] *= inv;
         x[1] *= inv;
         Pack<T, 2> pack;

@@ -9,7 +9,8 @@
 //
 // Keys fixed: a wave cannot hold sums, keys and values of 64 keys of 128 channels at once with two waves to a SIMD, so waves
 // work in pairs.  The first forms P of a tile of queries and adds to dV, the second, one tile behind, takes P from shared
-// memory, forms dS and adds to dK.  Operands are rounded to the inputs' type (P, dS), sums are 32-bit.
+// memory, forms dS and adds to dK.  Operands are rounded to the inputs' type (P, dS), sums are 32-bit.  In shared memory P is a
+// float16 whatever that type: in [0, 1] these are eight times as fine as bfloat16 at the same size.
 #include "seq_attention.h"
 
 namespace seqamd {
@@ -28,6 +29,7 @@ struct GradArgs {
 };
 
 constexpr float kLog2e = 1.44269504088896341f;
+constexpr int kExact = 512;               // keys up to which delta is summed from its definition
 
 // float16 holds dS only near 1: it is formed from gradients multiplied by a power of two that brings the largest there
 __device__ __forceinline__ float towards_one(float largest)
@@ -78,7 +80,6 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 3 : 2) dq_kernel(GradAr
         delta += swapped(delta);
     }
     const int64_t place = (at.q0 + row) * p.heads + head;
-    if (query < at.nq && half == 0) p.delta[place] = delta;
     float lift = 1.0f;
     if constexpr (__is_same(T, f16)) {
         largest = fmaxf(largest, swapped(largest));
@@ -108,9 +109,8 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 3 : 2) dq_kernel(GradAr
     };
     const char* const k_base = reinterpret_cast<const char*>(static_cast<const T*>(p.k) + at.k0 * p.k_token + kv * p.k_head);
     const char* const v_base = reinterpret_cast<const char*>(static_cast<const T*>(p.v) + at.k0 * p.v_token + kv * p.v_head);
-    offsets(kKeys);
     auto fetch = [&](int tile) __attribute__((always_inline)) {
-        if ((tile + 1) * kKeys > at.nk) offsets(at.nk - tile * kKeys);
+        if (tile == 0 || (tile + 1) * kKeys > at.nk) offsets(min(at.nk - tile * kKeys, kKeys));
         const char *kp = k_base + tile * int64_t(kKeys * sizeof(T)) * p.k_token, *vp = v_base + tile * int64_t(kKeys * sizeof(T)) * p.v_token;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
@@ -161,20 +161,44 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 3 : 2) dq_kernel(GradAr
         arrive<T>(q[k]);
         arrive<T>(g[k]);
     }
-    for (int tile = 0; tile < tiles; ++tile) {
+    auto hide = [&](f32x16& s, int key0) __attribute__((always_inline)) {
+        if (key0 + 32 > at.nk || (p.causal && key0 + 31 > q_first + wave * 32 + shift))
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (key0 + row_in(i, half) > last) s[i] = -INFINITY;
+    };
+    int buffer = 0;
+    // The output's rounding makes delta wrong by u |dO| |O|, which matters where few keys share the weight: dS, differences from
+    // delta, is as small there as that.  Queries with up to kExact keys go over them twice, first to sum P dP, which is delta.
+    if (keys <= kExact && tiles) {
+        float exact = 0.0f;
+        for (int tile = 0; tile < tiles; ++tile, buffer ^= 1) {
+            __syncthreads();
+            fetch(tile + 1 < tiles ? tile + 1 : 0);
+#pragma unroll 1
+            for (int c = 0; c < kKeys / 32; ++c) {
+                const int key0 = tile * kKeys + 32 * c;
+                f32x16 s, dp;
+                pair_products(s_tiles[buffer][0], s_tiles[buffer][1], 32 * c, s, dp);
+                hide(s, key0);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) exact = fmaf(__builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -lse)), dp[i], exact);
+            }
+            put(buffer ^ 1);
+        }
+        delta = exact + swapped(exact);
+    }
+    for (int tile = 0; tile < tiles; ++tile, buffer ^= 1) {
         __syncthreads();
         if (tile + 1 < tiles) fetch(tile + 1);
-        const char *kt = s_tiles[tile & 1][0], *vt = s_tiles[tile & 1][1];
+        const char *kt = s_tiles[buffer][0], *vt = s_tiles[buffer][1];
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c) {
             const int key0 = tile * kKeys + 32 * c;
             if (p.causal && key0 > q_first + wave * 32 + 31 + shift) continue;       // none of the wave's queries sees these
             f32x16 s, dp;
             pair_products(kt, vt, 32 * c, s, dp);
-            if (key0 + 32 > at.nk || (p.causal && key0 + 31 > q_first + wave * 32 + shift))
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (key0 + row_in(i, half) > last) s[i] = -INFINITY;
+            hide(s, key0);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float w = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -lse));
@@ -194,8 +218,9 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 3 : 2) dq_kernel(GradAr
                 for (int d = 0; d < kBlocks; ++d) dq[d] = product(f[u][d], ds, dq[d]);
             }
         }
-        if (tile + 1 < tiles) put((tile + 1) & 1);
+        if (tile + 1 < tiles) put(buffer ^ 1);
     }
+    if (query < at.nq && half == 0) p.delta[place] = delta;
     if (query < at.nq) store_row<T, DP>(static_cast<T*>(p.dq) + place * p.dim, dq, p.scale / lift, p.dim, half);
 }
 
@@ -329,7 +354,7 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     w[u] = rounded<T>(s, 8 * u);
-                    s_weights[step & 1][pair][c][u][lane] = __builtin_bit_cast(u32x4, w[u]);
+                    s_weights[step & 1][pair][c][u][lane] = __builtin_bit_cast(u32x4, rounded<f16>(s, 8 * u));
                 }
                 by_columns(s_tiles[now][1], 32 * c, w);
             }
@@ -341,7 +366,7 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
                 Frag<T> ds[2];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const Frag<T> w = __builtin_bit_cast(Frag<T>, s_weights[(step - 1) & 1][pair][c][u][lane]);
+                    const Frag<f16> w = __builtin_bit_cast(Frag<f16>, s_weights[(step - 1) & 1][pair][c][u][lane]);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float x = dp[8 * u + i] - s_delta[before][32 * c + row_in(8 * u + i, half)];
@@ -363,7 +388,7 @@ constexpr uint64_t kHeadBytes = 256;
 
 // Blocks by the average length of the sequences, from times of whole calls (16 heads on 4 of 64 channels, 16000 tokens, and 32 on
 // 8 of 128, 8000 tokens).
-// Queries fixed, waves of a block: 64 channels, sequences of 16: 2 waves 140 us, 4 waves 166; of 1000: 404 and 324.  128
+// Queries fixed, waves of a block: 64 channels, sequences of 64: 2 waves 92 us, 4 waves 100; of 250: 135 and 130; of 1000: 404 and 324.  128
 // channels, of 16: 2 waves 178 us, 8 waves 232; of 400: 4 waves 250; of 2000: 4 waves 466 us, 8 waves 480; one of 8192: 8 waves 1934 us.
 // Keys fixed: 64 channels, 2 pairs, sequences of 16: steps of 32 queries 94 us, of 64 132; of 400: 150 and 139; of 8192: 895
 // and 804.  128 channels, of 64: 2 pairs and 32 queries 172 us, 4 pairs and 64 queries 191; of 1000: 493 and 498; 4 of 1600 to
@@ -375,7 +400,7 @@ struct Blocks {
 Blocks blocks_of(int64_t q_rows, int64_t k_rows, int64_t n, int64_t dim)
 {
     const int64_t queries = q_rows / n, keys = k_rows / n;
-    if (dim <= 64) return Blocks{queries <= 50 ? 2 : 4, 2, keys <= 200 ? 32 : 64};
+    if (dim <= 64) return Blocks{queries <= 150 ? 2 : 4, 2, keys <= 200 ? 32 : 64};
     return Blocks{queries <= 200 ? 2 : (queries <= 2048 ? 4 : 8), keys <= 700 ? 2 : 4, keys <= 700 ? 32 : 64};
 }
 
