@@ -130,7 +130,7 @@ def _sequence(name, letters):
 CUSIG_LINEAR_RECURRENCE = _sequence("linear_recurrence", "ippppppuuuusspup")
 CUSIG_LINEAR_RECURRENCE_BACKPROP = _sequence("linear_recurrence_backprop", "ipppppppppuuuusspup")
 CUSIG_LINEAR_RECURRENCE_STEP = _sequence("linear_recurrence_step", "ippppuussp")
-CUSIG_LINEAR_RECURRENCE_WORKSPACE = _sequence("linear_recurrence_workspace", "iuu")
+CUSIG_LINEAR_RECURRENCE_WORKSPACE = _sequence("linear_recurrence_workspace", "iuuu")
 CUSIG_LINEAR_RECURRENCE_WORKSPACE.restype = c_uint64
 CUSIG_NORM_ROTARY = _sequence("norm_rotary", "ipppppppppuuuuuussssfbp")
 CUSIG_NORM_ROTARY_BACKPROP = _sequence("norm_rotary_backprop", "ipppppppppppppuuuuuussssssssfbpup")

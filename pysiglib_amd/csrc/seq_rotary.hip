@@ -228,20 +228,24 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(RotaryArgs p)
     }
 }
 
-// a block to 16 channels of one of the two: 16 threads for each add up every 16th piece
+// a block to 4 channels: 64 threads for each add up every 64th piece, then each other's sums
 __global__ void __launch_bounds__(kThreads) weights_kernel(const float* parts, int pieces, int dim, float* dqw, float* dkw)
 {
-    __shared__ float s_sum[16][17];
-    const int ch = threadIdx.x % 16, row = threadIdx.x / 16, e = blockIdx.x * 16 + ch;
+    __shared__ float s_sum[64][4];
+    const int ch = threadIdx.x % 4, row = threadIdx.x / 4, e = blockIdx.x * 4 + ch;
     float sum = 0.0f;
     if (e < 2 * dim)
-        for (int n = row; n < pieces; n += 16) sum += parts[int64_t(n) * 2 * dim + e];
+#pragma unroll
+        for (int i = 0; i < kPieces / 64; ++i) {
+            const int n = row + 64 * i;
+            if (n < pieces) sum += parts[int64_t(n) * 2 * dim + e];
+        }
     s_sum[row][ch] = sum;
-    __syncthreads();
-    if (row == 0 && e < 2 * dim) {
-        for (int n = 1; n < 16; ++n) sum += s_sum[n][ch];
-        (e < dim ? dqw : dkw)[e < dim ? e : e - dim] = sum;
+    for (int half = 32; half; half /= 2) {
+        __syncthreads();
+        if (row < half) s_sum[row][ch] += s_sum[row + half][ch];
     }
+    if (row == 0 && e < 2 * dim) (e < dim ? dqw : dkw)[e < dim ? e : e - dim] = s_sum[0][ch];
 }
 
 constexpr int kUnit = 4;
@@ -277,7 +281,7 @@ void launch(RotaryArgs& p, bool back, float* dqw, float* dkw, hipStream_t stream
     const int pieces = blocks < kPieces ? int(blocks) : kPieces;
     hipLaunchKernelGGL((backward_kernel<T, kUnit, G, NEAR>), dim3(pieces), dim3(kThreads), 0, stream, p);
     SIG_HIP(hipGetLastError());
-    hipLaunchKernelGGL(weights_kernel, dim3((2 * p.dim + 15) / 16), dim3(kThreads), 0, stream, p.parts, pieces, p.dim, dqw, dkw);
+    hipLaunchKernelGGL(weights_kernel, dim3((2 * p.dim + 3) / 4), dim3(kThreads), 0, stream, p.parts, pieces, p.dim, dqw, dkw);
     SIG_HIP(hipGetLastError());
 }
 
@@ -300,7 +304,7 @@ void run(int dtype, RotaryArgs& p, bool interleaved, bool back, float* dqw, floa
     require(p.heads >= 0 && p.kv_heads >= 0 && p.heads + p.kv_heads < (1 << 20) && p.tokens < (int64_t(1) << 31), "too many heads or tokens");
     if (p.tokens == 0 || p.heads + p.kv_heads == 0) {
         if (back) {        // no pieces: zeros
-            hipLaunchKernelGGL(weights_kernel, dim3((2 * p.dim + 15) / 16), dim3(kThreads), 0, static_cast<hipStream_t>(stream), p.parts, 0, p.dim, dqw, dkw);
+            hipLaunchKernelGGL(weights_kernel, dim3((2 * p.dim + 3) / 4), dim3(kThreads), 0, static_cast<hipStream_t>(stream), p.parts, 0, p.dim, dqw, dkw);
             SIG_HIP(hipGetLastError());
         }
         return;

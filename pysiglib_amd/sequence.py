@@ -23,6 +23,7 @@ from .param_checks import check_type
 
 _CODES = {getattr(torch, name): code for name, code in SEQUENCE_DTYPES.items()}
 _stream_of = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _tensor(value, name, rank=None, like=None):
@@ -50,7 +51,7 @@ def _other(value, name, dtype, shape, device):
         raise TypeError(name + " must be a torch tensor, got " + type(value).__name__ + " instead")
     if value.dtype != dtype:
         raise TypeError(name + ".dtype must be " + str(dtype) + ", got " + str(value.dtype) + " instead")
-    if tuple(value.shape) != tuple(shape):
+    if value.shape != shape:
         raise ValueError(name + " must have shape " + str(tuple(shape)) + ", got " + str(tuple(value.shape)))
     if value.device != device:
         raise ValueError(name + " must be on " + str(device) + ", got " + str(value.device))
@@ -71,8 +72,11 @@ def _offsets(value, name, device):
 
 def _call(fn, name, device, *args):
     index = device.index
-    with on_device(device):
+    if index == _current_device():
         code = fn(*args, _stream_of(index))
+    else:
+        with on_device(device):
+            code = fn(*args, _stream_of(index))
     if code:
         raise Exception("Error in pysiglib." + name + ": " + err_msg(code))
 
@@ -80,6 +84,8 @@ def _call(fn, name, device, *args):
 def _rows(x):
     """A tensor of rank 2 or more as rows a fixed distance apart: (tensor that holds them, distance)."""
     shape = x.shape
+    if x.is_contiguous():
+        return x, shape[-1]
     if x.stride(-1) == 1 or shape[-1] <= 1:
         step = x.stride(-2)
         want = step
@@ -137,11 +143,11 @@ def linear_recurrence(x, log_decay, *, initial_state=None, offsets=None):
     x, x_step = _rows(x)
     log_decay, decay_step = _rows(log_decay)
     code = _CODES[x.dtype]
-    size = CUSIG_LINEAR_RECURRENCE_WORKSPACE(code, rows, channels)
-    space = _workspace(size, device)
+    size = CUSIG_LINEAR_RECURRENCE_WORKSPACE(code, rows, n, channels)
+    space = _workspace(size, device) if size else None
     _call(CUSIG_LINEAR_RECURRENCE, "linear_recurrence", device, code, x.data_ptr(), log_decay.data_ptr(),
           0 if initial_state is None else initial_state.data_ptr(), h.data_ptr(), final.data_ptr(), at, n, length, rows, channels,
-          x_step, decay_step, space.data_ptr(), size)
+          x_step, decay_step, space.data_ptr() if size else 0, size)
     return h, final
 
 
@@ -172,12 +178,12 @@ def linear_recurrence_backprop(h, log_decay, grad_h, *, grad_final=None, initial
     log_decay, decay_step = _rows(log_decay)
     grad_h, grad_step = _rows(grad_h)
     code = _CODES[h.dtype]
-    size = CUSIG_LINEAR_RECURRENCE_WORKSPACE(code, rows, channels)
-    space = _workspace(size, device)
+    size = CUSIG_LINEAR_RECURRENCE_WORKSPACE(code, rows, n, channels)
+    space = _workspace(size, device) if size else None
     _call(CUSIG_LINEAR_RECURRENCE_BACKPROP, "linear_recurrence_backprop", device, code, h.data_ptr(), log_decay.data_ptr(),
           grad_h.data_ptr(), 0 if grad_final is None else grad_final.data_ptr(),
           0 if initial_state is None else initial_state.data_ptr(), dx.data_ptr(), dg.data_ptr(), d0.data_ptr(), at, n, length,
-          rows, channels, decay_step, grad_step, space.data_ptr(), size)
+          rows, channels, decay_step, grad_step, space.data_ptr() if size else 0, size)
     return dx, dg, d0
 
 

@@ -123,7 +123,8 @@ def test_recurrence_batched(P, dtype, batch, length, channels):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lengths,channels", [([1], 3), ([0, 5, 0, 0, 1, 130, 0], 40), ([400, 1, 1, 1, 126, 2, 128, 129], 133),
-                                              ([7] * 300, 5), ([1] * 1500, 3), ([0, 0], 4)])
+                                              ([7] * 300, 5), ([1] * 1500, 3), ([0, 0], 4),
+                                              ([3000, 0, 2500, 0], 40), ([5000], 2)])
 @pytest.mark.parametrize("with_states", [True, False])
 def test_recurrence_packed(P, dtype, lengths, channels, with_states):
     starts = [0]
