@@ -342,6 +342,81 @@ CUSIG_AMD_API void cusig_amd_force_partition(int tail, int k) CUSIG_AMD_NOEXCEPT
 CUSIG_AMD_API int cusig_amd_kernel_choice(int backward, int is_f64, uint64_t dimension, uint64_t degree,
                                           int* tail, int* k, int* specialised) CUSIG_AMD_NOEXCEPT;
 
+/* ---- Layers of a sequence model over path features (no counterpart in the reference) ----
+ * These entry points enqueue on `stream` and return without waiting; inputs are ordered before them, consumers after them, by
+ * the stream.  They allocate nothing: scratch is the caller's (`workspace`, of at least the size its query function gives,
+ * aligned to 256 bytes; it may be null where that is 0) and is free again when the enqueued work has ended.  Nothing is kept
+ * between calls; calls on different streams with scratch of their own run beside each other, and all of them can be captured
+ * into a HIP graph.  The same inputs give the same bits.
+ * dtype: 0 float32, 1 bfloat16, 2 float16; sums, states, norms and statistics are 32-bit whatever it is.
+ * Strides count elements; the last axis is contiguous.  Packed sequences: `offsets` are sequences + 1 ascending int32 row numbers on
+ * the device, sequence i has the rows offsets[i] to offsets[i + 1].  They are not read on the host; numbers outside the tensors
+ * are cut to them, rows that belong to no sequence are not written. */
+
+/* h_t = exp(log_decay_t) h_{t-1} + x_t for each channel.  x, log_decay, h [rows, channels] (h contiguous), offsets, or null: `sequences`
+ * of `length` rows each.  initial_state (may be null: zero) and final_state float32 [sequences, channels].  Rows of at most 2^20
+ * elements. */
+CUSIG_AMD_API int cusig_amd_linear_recurrence(int dtype, const void* x, const void* log_decay, const float* initial_state, void* h,
+                                              float* final_state, const int* offsets, uint64_t sequences, uint64_t length,
+                                              uint64_t rows, uint64_t channels, int64_t x_stride, int64_t log_decay_stride,
+                                              void* workspace, uint64_t workspace_bytes, void* stream) CUSIG_AMD_NOEXCEPT;
+CUSIG_AMD_API uint64_t cusig_amd_linear_recurrence_workspace(int dtype, uint64_t rows, uint64_t sequences,
+                                                             uint64_t channels) CUSIG_AMD_NOEXCEPT;
+/* Its gradients, from the output h (contiguous) and the gradients of both outputs (grad_final may be null: zero); grad_x and
+ * grad_log_decay contiguous, grad_initial float32 [sequences, channels].  The same workspace. */
+CUSIG_AMD_API int cusig_amd_linear_recurrence_backprop(int dtype, const void* h, const void* log_decay, const void* grad_h,
+                                                       const float* grad_final, const float* initial_state, void* grad_x,
+                                                       void* grad_log_decay, float* grad_initial, const int* offsets,
+                                                       uint64_t sequences, uint64_t length, uint64_t rows, uint64_t channels,
+                                                       int64_t log_decay_stride, int64_t grad_stride, void* workspace,
+                                                       uint64_t workspace_bytes, void* stream) CUSIG_AMD_NOEXCEPT;
+/* One step of it: state [rows, channels] float32 becomes exp(log_decay) state + x, and h the same rounded. */
+CUSIG_AMD_API int cusig_amd_linear_recurrence_step(int dtype, const void* x, const void* log_decay, float* state, void* h, uint64_t rows,
+                                                   uint64_t channels, int64_t x_stride, int64_t log_decay_stride,
+                                                   void* stream) CUSIG_AMD_NOEXCEPT;
+
+/* Root-mean-square norm of every head of q [tokens, heads, dim] and k [tokens, kv_heads, dim] with a weight for each channel, then
+ * the first rotary_dim channels turned in pairs by cos and sin [table, rotary_dim / 2] at the token's position: channels i and
+ * i + rotary_dim / 2, or 2 i and 2 i + 1 (interleaved).  Weights and tables float32; q_out and k_out contiguous; dim even, at most
+ * 256.  A position outside the table gives NaN. */
+CUSIG_AMD_API int cusig_amd_norm_rotary(int dtype, const void* q, const void* k, const float* q_weight, const float* k_weight,
+                                        const float* cos, const float* sin, const int* positions, void* q_out, void* k_out,
+                                        uint64_t tokens, uint64_t heads, uint64_t kv_heads, uint64_t dim, uint64_t rotary_dim,
+                                        uint64_t table, int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head, float eps,
+                                        bool interleaved, void* stream) CUSIG_AMD_NOEXCEPT;
+CUSIG_AMD_API uint64_t cusig_amd_norm_rotary_backprop_workspace(uint64_t dim) CUSIG_AMD_NOEXCEPT;
+CUSIG_AMD_API int cusig_amd_norm_rotary_backprop(int dtype, const void* grad_q, const void* grad_k, const void* q, const void* k,
+                                                 const float* q_weight, const float* k_weight, const float* cos, const float* sin,
+                                                 const int* positions, void* dq, void* dk, float* dq_weight, float* dk_weight,
+                                                 uint64_t tokens, uint64_t heads, uint64_t kv_heads, uint64_t dim,
+                                                 uint64_t rotary_dim, uint64_t table, int64_t q_token, int64_t q_head,
+                                                 int64_t k_token, int64_t k_head, int64_t grad_q_token, int64_t grad_q_head,
+                                                 int64_t grad_k_token, int64_t grad_k_head, float eps, bool interleaved,
+                                                 void* workspace, uint64_t workspace_bytes, void* stream) CUSIG_AMD_NOEXCEPT;
+
+/* Softmax attention over packed sequences, bfloat16 or float16: q [q_rows, heads, dim], k and v [k_rows, kv_heads, dim]; heads / kv_heads
+ * neighbouring heads share keys and values; dim a multiple of 8 up to 128.  causal: query j of n sees the keys up to j + m - n of
+ * m.  k_lengths (may be null): keys in use from each sequence's first on, as in a cache.  out [q_rows, heads, dim] and lse float32
+ * [q_rows, heads] (the logarithm of the sum of exponentials), contiguous; 0 and -infinity where a query sees no key. */
+CUSIG_AMD_API int cusig_amd_attention(int dtype, const void* q, const void* k, const void* v, const int* q_offsets,
+                                      const int* k_offsets, const int* k_lengths, void* out, float* lse, uint64_t q_rows,
+                                      uint64_t k_rows, uint64_t sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim,
+                                      int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token,
+                                      int64_t v_head, float scale, bool causal, void* workspace, uint64_t workspace_bytes,
+                                      void* stream) CUSIG_AMD_NOEXCEPT;
+CUSIG_AMD_API uint64_t cusig_amd_attention_workspace(uint64_t q_rows, uint64_t k_rows, uint64_t sequences, uint64_t heads,
+                                                     uint64_t kv_heads, uint64_t dim) CUSIG_AMD_NOEXCEPT;
+/* Its gradients (whole sequences), dq, dk and dv contiguous. */
+CUSIG_AMD_API int cusig_amd_attention_backprop(int dtype, const void* grad_out, const void* q, const void* k, const void* v,
+                                               const void* out, const float* lse, const int* q_offsets, const int* k_offsets,
+                                               void* dq, void* dk, void* dv, uint64_t q_rows, uint64_t k_rows, uint64_t sequences,
+                                               uint64_t heads, uint64_t kv_heads, uint64_t dim, int64_t q_token, int64_t q_head,
+                                               int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                                               int64_t grad_token, int64_t grad_head, float scale, bool causal, void* workspace,
+                                               uint64_t workspace_bytes, void* stream) CUSIG_AMD_NOEXCEPT;
+CUSIG_AMD_API uint64_t cusig_amd_attention_backprop_workspace(uint64_t q_rows, uint64_t k_rows, uint64_t sequences, uint64_t heads,
+                                                              uint64_t dim) CUSIG_AMD_NOEXCEPT;
+
 #ifdef __cplusplus
 }
 #endif

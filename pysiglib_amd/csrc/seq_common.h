@@ -2,6 +2,7 @@
 // each other, argument checks.  These operators take their scratch from the caller and only enqueue on the caller's stream.
 #pragma once
 #include "sig_host.h"
+#include "../../include/cusig_amd.h"
 
 #include <cstdint>
 

@@ -156,3 +156,71 @@ def log_sig(path, degree, *, time_aug=False, lead_lag=False, end_time=1., method
     """Differentiable ``log_sig``: the differentiable signature followed by the differentiable ``sig_to_log_sig``."""
     sig_ = sig(path, degree, time_aug=time_aug, lead_lag=lead_lag, end_time=end_time, scalar_term=scalar_term)
     return sig_to_log_sig(sig_, path.shape[-1], degree, time_aug=time_aug, lead_lag=lead_lag, method=method)
+
+
+class LinearRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, log_decay, initial_state, offsets):
+        from .sequence import linear_recurrence as _recurrence
+        h, final = _recurrence(x, log_decay, initial_state=initial_state, offsets=offsets)
+        ctx.save_for_backward(h, log_decay, initial_state, offsets)
+        ctx.set_materialize_grads(False)
+        return h, final
+
+    @staticmethod
+    def backward(ctx, grad_h, grad_final):
+        from .sequence import linear_recurrence_backprop as _recurrence_backprop
+        h, log_decay, initial_state, offsets = ctx.saved_tensors
+        grad_h = torch.zeros_like(h) if grad_h is None else grad_h
+        dx, dg, d0 = _recurrence_backprop(h, log_decay, grad_h, grad_final=grad_final, initial_state=initial_state,
+                                          offsets=offsets)
+        return dx, dg, d0 if initial_state is not None else None, None
+
+
+def linear_recurrence(x, log_decay, *, initial_state=None, offsets=None):
+    """Differentiable ``linear_recurrence``."""
+    return LinearRecurrence.apply(x, log_decay, initial_state, offsets)
+
+
+class NormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+        from .sequence import norm_rotary as _norm_rotary
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.args = (eps, interleaved)
+        return _norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, eps=eps, interleaved=interleaved)
+
+    @staticmethod
+    def backward(ctx, grad_q, grad_k):
+        from .sequence import norm_rotary_backprop as _norm_rotary_backprop
+        eps, interleaved = ctx.args
+        grads = _norm_rotary_backprop(grad_q, grad_k, *ctx.saved_tensors, eps=eps, interleaved=interleaved)
+        return (*grads, None, None, None, None, None)
+
+
+def norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, *, eps=1e-6, interleaved=False):
+    """Differentiable ``norm_rotary`` (with respect to queries, keys and both weights)."""
+    return NormRotary.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+
+
+class Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, q_offsets, k_offsets, causal, scale):
+        from .sequence import attention as _attention
+        out, lse = _attention(q, k, v, q_offsets, k_offsets, causal=causal, scale=scale)
+        ctx.save_for_backward(q, k, v, out, lse, q_offsets, k_offsets)
+        ctx.args = (causal, scale)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        from .sequence import attention_backprop as _attention_backprop
+        q, k, v, out, lse, q_offsets, k_offsets = ctx.saved_tensors
+        causal, scale = ctx.args
+        return (*_attention_backprop(grad_out, q, k, v, out, lse, q_offsets, k_offsets, causal=causal, scale=scale), None, None,
+                None, None)
+
+
+def attention(q, k, v, q_offsets, k_offsets, *, causal=True, scale=None):
+    """Differentiable ``attention`` of whole sequences; the output alone, without the sums' logarithms."""
+    return Attention.apply(q, k, v, q_offsets, k_offsets, causal, scale)

@@ -521,6 +521,98 @@ def test_attention_of_nothing(P):
     assert (out == 0).all() and (lse == -float("inf")).all()
 
 
+# ---- through autograd, and all together ----
+
+@pytest.mark.gpu
+def test_autograd_gives_the_gradients(P):
+    lengths, heads, kv, dim = [40, 7, 0, 130], 4, 2, 64
+    starts = starts_of(lengths)
+    offsets = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    q, k, v, g = attention_inputs(torch.bfloat16, 177, 177, heads, kv, dim, seed=1)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = P.torch_api.attention(*leaves, offsets, offsets, scale=0.2)
+    out.backward(g)
+    same, lse = P.attention(q, k, v, offsets, offsets, scale=0.2)
+    assert torch.equal(out, same)
+    for x, y in zip(leaves, P.attention_backprop(g, q, k, v, same, lse, offsets, offsets, scale=0.2)):
+        assert torch.equal(x.grad, y)
+    w = [torch.rand(dim, device=DEV).requires_grad_(True) for _ in range(2)]
+    cos, sin = P.rotary_tables(200, dim, device=DEV)
+    at = torch.arange(177, dtype=torch.int32, device=DEV)
+    leaves = [q.clone().requires_grad_(True), k.clone().requires_grad_(True), *w]
+    a, b = P.torch_api.norm_rotary(*leaves, cos, sin, at, interleaved=True)
+    (a.float().sum() + 2 * b.float().sum()).backward()
+    want = P.norm_rotary_backprop(torch.ones_like(q), torch.full_like(k, 2.0), q, k, w[0].detach(), w[1].detach(), cos, sin, at, interleaved=True)
+    for x, y in zip(leaves, want):
+        assert torch.equal(x.grad, y)
+    x, gate, h0, grad, gf = (t.to(DEV) for t in recurrence_inputs(torch.float16, 177, 20, 4, seed=2))
+    leaves = [t.clone().requires_grad_(True) for t in (x, gate, h0)]
+    h, final = P.torch_api.linear_recurrence(leaves[0], leaves[1], initial_state=leaves[2], offsets=offsets)
+    torch.autograd.backward([h, final], [grad, gf])
+    for t, y in zip(leaves, P.linear_recurrence_backprop(h.detach(), gate, grad, grad_final=gf, initial_state=h0, offsets=offsets)):
+        assert torch.equal(t.grad, y)
+    leaf = x.clone().requires_grad_(True)
+    _, final = P.torch_api.linear_recurrence(leaf, gate, offsets=offsets)
+    final.sum().backward()
+    want = P.linear_recurrence_backprop(P.linear_recurrence(x, gate, offsets=offsets)[0], gate, torch.zeros_like(x),
+                                        grad_final=torch.ones_like(final), offsets=offsets)[0]
+    assert torch.equal(leaf.grad, want)
+
+
+@pytest.mark.gpu
+def test_the_example_learns_and_serves(P):
+    import importlib.util
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location("stream_model", os.path.join(root, "examples", "stream_model.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    torch.manual_seed(0)
+    gen = torch.Generator().manual_seed(0)
+    model = example.StreamModel()
+    losses = example.train(model, 30, gen, say=lambda line: None)
+    assert sum(losses[-5:]) < 0.8 * sum(losses[:5]) and model.mix.weight.grad.abs().max() > 0
+    worst, size = example.serve(model, gen)
+    # both ways round to bfloat16 in a dozen places, at different ones inside the attention
+    assert worst <= 32 * ROUND[torch.bfloat16] * max(size, 1.0)
+
+
+@pytest.mark.gpu
+def test_a_captured_graph_replays(P):
+    """Serving captures its step: every replay gives what the same calls give outside the graph."""
+    n, heads, kv, dim, room = 4, 8, 2, 128, 700
+    q, k, v, _ = attention_inputs(torch.bfloat16, n, n * room, heads, kv, dim, seed=9)
+    whole = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)         # noqa: E731
+    queries, places, lengths = whole(range(n + 1)), whole([i * room for i in range(n + 1)]), whole([700, 1, 333, 64])
+    w = torch.ones(dim, device=DEV)
+    cos, sin = P.rotary_tables(room, dim, device=DEV)
+    state, decay = torch.zeros((n, heads * dim), device=DEV), torch.full((n, heads * dim), -0.1, dtype=torch.bfloat16, device=DEV)
+
+    def step():
+        a, _ = P.norm_rotary(q, q[:, :kv], w, w, cos, sin, lengths - 1)
+        out, lse = P.attention(a, k, v, queries, places, k_lengths=lengths)
+        scan = P.linear_recurrence(out.flatten(1)[None].expand(3, n, heads * dim).reshape(1, 3 * n, heads * dim), decay.repeat(3, 1)[None])[0]
+        return out, lse, scan, P.linear_recurrence_step(out.flatten(1), decay, state)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for turn in range(4):
+        q.copy_(torch.randn_like(q))
+        lengths.copy_(whole([700 - 100 * turn, 1 + turn, 333, 64]))
+        state.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        state.zero_()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), turn
+
+
 # ---- refusals ----
 
 @pytest.mark.gpu
