@@ -10,6 +10,7 @@
 #include "seq_common.h"
 
 #include <cmath>
+#include <initializer_list>
 
 namespace seqamd {
 
@@ -160,6 +161,45 @@ __device__ __forceinline__ void store_row(T* to, const f32x16* x, float times, i
         }
 }
 
+// Values that are not finite, at keys that some queries of a tile do not see: a weight of zero times them would not be zero.  Tiles
+// with hidden keys are put into shared memory with zeros in their place; which keys had them is noted, and what they are is
+// added at the end for the queries that see them.
+template <typename T>
+__device__ __forceinline__ unsigned not_finite(unsigned two)
+{
+    constexpr unsigned kLow = __is_same(T, bf16) ? 0x7f80u : 0x7c00u, kBoth = kLow << 16 | kLow;
+    const unsigned e = two & kBoth;
+    return ((e & 0xffffu) == kLow ? 0xffffu : 0u) | ((e >> 16) == kLow ? 0xffff0000u : 0u);
+}
+
+// zeros in their place; returns whether there were any
+template <typename T>
+__device__ __forceinline__ bool take_them_out(u32x4& x)
+{
+    unsigned any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned m = not_finite<T>(x[i]);
+        x[i] &= ~m;
+        any |= m;
+    }
+    return any != 0;
+}
+
+// adds the values that are not finite of the row `v` to a lane's column of sums
+template <typename T, int DP>
+__device__ __forceinline__ void add_them(const T* v, int dim, int half, f32x16* o)
+{
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int ch = 32 * d + row_in(i, half);
+            const float x = ch < dim ? static_cast<float>(v[ch]) : 0.0f;
+            if (!__builtin_isfinite(x)) o[d][i] += x;
+        }
+}
+
 // Packed sequences.  Offsets are read on the device and kept inside the tensors whatever they hold.
 struct Packed {
     const int *q_offsets, *k_offsets, *k_lengths;
@@ -301,6 +341,7 @@ struct MapArgs {
     Packed packed;
     Tiling how[2];
     int* map[2];
+    int room[2];             // tiles that a map holds: offsets that do not ascend could name more
     unsigned* clear;         // a word to be cleared, or null
 };
 
@@ -312,6 +353,7 @@ static __global__ void __launch_bounds__(kMapThreads) map_kernel(MapArgs p)
     const int tid = threadIdx.x, lane = tid & 63;
     const Tiling how = blockIdx.x ? p.how[1] : p.how[0];
     int* const map = blockIdx.x ? p.map[1] : p.map[0];
+    const int room = blockIdx.x ? p.room[1] : p.room[0];
     if (p.clear && blockIdx.x == 0 && tid == 0) *p.clear = 0;
     if (!map) return;
     int done = 0;
@@ -327,12 +369,18 @@ static __global__ void __launch_bounds__(kMapThreads) map_kernel(MapArgs p)
             if (w < (tid >> 6)) before += s_sums[w];
             done += s_sums[w];
         }
-        for (int i = 0; i < own; ++i) {
+        for (int i = 0; i < own && before + i < room; ++i) {
             map[2 + 2 * (before + i)] = base + tid;
             map[3 + 2 * (before + i)] = i;
         }
     }
-    if (tid == 0) map[0] = done;
+    if (tid == 0) map[0] = min(done, room);
+}
+
+// offsets of a tile's rows are 32-bit
+inline void check_strides(std::initializer_list<int64_t> tokens)
+{
+    for (const int64_t t : tokens) require(t >= 0 && t < (int64_t(1) << 23), "tokens are at most 2^23 elements apart");
 }
 
 // most tiles of `size` rows that n sequences with `rows` rows in all have

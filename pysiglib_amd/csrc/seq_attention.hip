@@ -34,6 +34,8 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
     constexpr int kTileBytes = kKeys * Tile<DP>::kRowBytes, kLoads = kKeys * Tile<DP>::kChunks / kThreads;
     static_assert(kLoads * kThreads == kKeys * Tile<DP>::kChunks, "");
     __shared__ __attribute__((aligned(16))) char s_tiles[2][2][kTileBytes];
+    constexpr int kHiding = kRows / kKeys + 2;       // tiles that hide keys from some queries of the block, at most
+    __shared__ unsigned s_bad[kHiding][kKeys / 32];  // their keys whose values are not finite
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the heads that share keys and values follow each other at a distance of kv_heads: on the same die where that is a multiple of 8
     const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
@@ -87,7 +89,16 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
             next[1][i] = load_at(vp, v_at[i]);
         }
     };
+    // a key is hidden past the sequence's end, or behind a query's place: from any of the queries from `first` on
+    auto hides = [&](int tile, int first) { return tile * kKeys + kKeys > at.nk || (p.causal && tile * kKeys + kKeys - 1 > first + shift); };
+    const int hiding = min(p.causal ? max(q_first + shift + 1, 0) / kKeys : tiles, tiles - 1);       // the first such tile, or one before it
     auto put = [&](int tile) __attribute__((always_inline)) {
+        if (hides(tile, q_first))
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int row = (i * kThreads + tid) / Tile<DP>::kChunks;
+                if (take_them_out<T>(next[1][i])) atomicOr(&s_bad[tile - hiding][row / 32], 1u << row % 32);
+            }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int e = i * kThreads + tid, to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
@@ -95,6 +106,7 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
             *reinterpret_cast<u32x4*>(s_tiles[tile & 1][1] + to) = next[1][i];
         }
     };
+    const int last = p.causal && query + shift < at.nk - 1 ? query + shift : at.nk - 1;
     f32x16 s[kKeys / 32];
     Frag<T> w[kKeys / 16];
     // 128 channels: operands are read a group ahead of the products that take them, the compiler would read each right before
@@ -127,9 +139,7 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
     };
     auto weights = [&](int tile) __attribute__((always_inline)) {
         const int key0 = tile * kKeys;
-        // a key is hidden past the sequence's end, or behind the query's place
-        if (key0 + kKeys > at.nk || (p.causal && key0 + kKeys - 1 > q_first + wave * 32 + shift)) {
-            const int last = p.causal && query + shift < at.nk - 1 ? query + shift : at.nk - 1;
+        if (hides(tile, q_first + wave * 32)) {
 #pragma unroll
             for (int c = 0; c < kKeys / 32; ++c)
 #pragma unroll
@@ -186,6 +196,9 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
             if (kAhead) __builtin_amdgcn_sched_barrier(0);
         }
     };
+    if (tid < kHiding)
+        for (unsigned& bad : s_bad[tid]) bad = 0;
+    __syncthreads();
     if (tiles) {
         fetch(0);
         put(0);
@@ -202,6 +215,12 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
         }
         if (tile + 1 < tiles) put(tile + 1);
     }
+    for (int tile = hiding; tile < tiles; ++tile)
+        for (int part = 0; part < kKeys / 32; ++part)
+            for (unsigned bad = s_bad[tile - hiding][part]; __builtin_expect(bad != 0, 0); bad &= bad - 1) {
+                const int key = tile * kKeys + 32 * part + __ffs(bad) - 1;
+                if (key <= last) add_them<T, DP>(static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head, p.dim, half, o);
+            }
     const float total = sum + swapped(sum);
     if (query >= at.nq) return;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
@@ -220,6 +239,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
     constexpr int kTileBytes = kTile * Tile<DP>::kRowBytes, kLoads = kTile * Tile<DP>::kChunks / 64;
     __shared__ __attribute__((aligned(16))) char s_tiles[kWaves][2][kTileBytes];
     __shared__ float s_top[kWaves][32], s_sum[kWaves][32];
+    __shared__ unsigned s_bad[4];            // of the tiles that hide keys from some of the pairs: keys whose values are not finite
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = p.heads / p.kv_heads, kv = blockIdx.x % p.kv_heads, split = blockIdx.x / p.kv_heads % p.splits;
     const Span at = find_tile(p.packed, Tiling{false, 32, group}, blockIdx.x / p.kv_heads / p.splits, Dear::kLast);
@@ -260,10 +280,20 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
             __builtin_memcpy(&next[1][i], static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head + ch, 16);
         }
     };
+    const int first_query = at.tile * 32 / group;
+    auto hides = [&](int tile) { return (tile + 1) * kTile > past - begin || (p.causal && begin + (tile + 1) * kTile - 1 > first_query + shift); };
+    const int hiding = min(p.causal ? max(first_query + shift + 1 - begin, 0) / kTile : tiles, tiles - 1);      // the first of them, or one before it
+    if (tid < 4) s_bad[tid] = 0;
+    __syncthreads();
     if (wave < tiles) fetch(wave);
 #pragma unroll
     for (int k = 0; k < kSlices; ++k) arrive<T>(q[k]);
     for (int tile = wave; tile < tiles; tile += kWaves) {
+        const bool hidden = hides(tile);
+        if (hidden)
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                if (take_them_out<T>(next[1][i])) atomicOr(&s_bad[tile - hiding], 1u << (i * 64 + lane) / Tile<DP>::kChunks);
         // the wave's own tiles: shared memory serves a wave in order, no barrier is needed
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
@@ -277,7 +307,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
         f32x16 s = zeros16();
 #pragma unroll
         for (int k = 0; k < kSlices; ++k) s = product(rows.template get<T>(kt, 0, k), q[k], s);
-        if (key0 + kTile > past || p.causal)
+        if (hidden)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 if (key0 + row_in(i, half) > last) s[i] = -INFINITY;
@@ -346,6 +376,11 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
                 for (int i = 0; i < 16; ++i) o[d][i] += shared[wave * kPart + (d * 16 + i) * 64 + lane];
     }
     if (wave || pair >= pairs) return;
+    for (int tile = hiding; tile < tiles; ++tile)
+        for (unsigned bad = s_bad[tile - hiding]; __builtin_expect(bad != 0, 0); bad &= bad - 1) {
+            const int key = begin + tile * kTile + __ffs(bad) - 1;
+            if (key <= last) add_them<T, DP>(static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head, p.dim, half, o);
+        }
     const int64_t row = (at.q0 + query) * p.heads + head;
     if (p.splits > 1) {
         // [splits][q_rows * heads] of (maximum, sum), then [splits][q_rows * heads][dim]
@@ -396,13 +431,14 @@ __global__ void __launch_bounds__(256) join_kernel(AttentionArgs p)
             total += w * p.parts[2 * place + 1];
         }
         const int count = min(64, p.splits - first);
-#pragma unroll 8
-        for (int s = 0; s < count; ++s) {
-            const float ws = __shfl(w, s);
-            const Pack<float, 2> v = load_pack<float, 2>(from + (first + s) * all * p.dim);
-            x[0] = fmaf(ws, v.get(0), x[0]);
-            x[1] = fmaf(ws, v.get(1), x[1]);
-        }
+        for (int s = 0; s < count; s += 8)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float ws = __shfl(w, s + j);              // zero past the last split
+                const Pack<float, 2> v = load_pack<float, 2>(from + min(first + s + j, p.splits - 1) * all * p.dim);
+                x[0] = fmaf(ws, v.get(0), x[0]);
+                x[1] = fmaf(ws, v.get(1), x[1]);
+            }
     }
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) total += __shfl_xor(total, m);
@@ -502,7 +538,9 @@ __attribute__((visibility("default"))) int cusig_amd_attention(
         require(dim >= 8 && dim <= 128 && dim % 8 == 0, "a head has 8 to 128 channels, a multiple of 8");
         require(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads < (1u << 20), "heads are a multiple of the key heads");
         require(scale > 0.0f && std::isfinite(scale), "the scale is positive and finite");
+        check_strides({q_token, k_token, v_token});
         if (q_rows == 0 || sequences == 0) return;
+        require(q && q_offsets && k_offsets && out && lse && (k_rows == 0 || (k && v)), "a tensor is missing");
         AttentionArgs p{};
         p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse;
         p.packed = Packed{q_offsets, k_offsets, k_lengths, int64_t(q_rows), int64_t(k_rows), int(sequences), nullptr};
@@ -520,6 +558,7 @@ __attribute__((visibility("default"))) int cusig_amd_attention(
             m.packed = p.packed;
             m.how[0] = cut.few ? Tiling{false, 32, p.heads / p.kv_heads} : Tiling{false, 32 * cut.waves, 1};
             m.map[0] = static_cast<int*>(workspace);
+            m.room[0] = int(cut.tiles);
             hipLaunchKernelGGL(map_kernel, dim3(1), dim3(kMapThreads), 0, s, m);
             SIG_HIP(hipGetLastError());
         }

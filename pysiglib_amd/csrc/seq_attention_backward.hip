@@ -439,6 +439,8 @@ void backward(GradArgs& p, void* workspace, hipStream_t stream)
             m.how[1] = Tiling{true, 32 * b.pairs, 1};
             m.map[0] = reinterpret_cast<int*>(at + kHeadBytes);
             m.map[1] = reinterpret_cast<int*>(at + kHeadBytes + space.q_map);
+            m.room[0] = int(most_tiles(p.packed.q_rows, p.packed.n, 32 * b.waves));
+            m.room[1] = int(most_tiles(p.packed.k_rows, p.packed.n, 32 * b.pairs));
             p.packed.map = m.map[0];
             p.k_packed.map = m.map[1];
         }
@@ -486,7 +488,9 @@ __attribute__((visibility("default"))) int cusig_amd_attention_backprop(
         require(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads < (1u << 20), "heads are a multiple of the key heads");
         require(scale > 0.0f && std::isfinite(scale), "the scale is positive and finite");
         require(workspace && workspace_bytes >= cusig_amd_attention_backprop_workspace(q_rows, k_rows, sequences, heads, dim), "the workspace is too small");
+        check_strides({q_token, k_token, v_token, grad_token});
         if (sequences == 0) return;
+        require(q_offsets && k_offsets && (q_rows == 0 || (grad_out && q && out && lse && dq)) && (k_rows == 0 || (k && v && dk && dv)), "a tensor is missing");
         GradArgs p{};
         p.q = q, p.k = k, p.v = v, p.out = out, p.grad = grad_out, p.lse = lse, p.dq = dq, p.dk = dk, p.dv = dv;
         p.packed = Packed{q_offsets, k_offsets, nullptr, int64_t(q_rows), int64_t(k_rows), int(sequences), nullptr};

@@ -570,6 +570,7 @@ void scan(ScanArgs p, void* workspace, size_t bytes, hipStream_t stream)
 {
     using S = Shape<T>;
     if (p.n * p.channels == 0) return;
+    require(p.end && (p.rows == 0 || (p.gate && p.in && p.out && (!BACK || (p.h && p.out2)))), "a tensor is missing");
     const Plan plan = plan_of<T, BACK>(p.rows, p.n, p.channels);
     const size_t need = scan_workspace<T, BACK>(p.rows, p.n, p.channels);
     require(bytes >= need && (workspace || need == 0), "the workspace is too small");
@@ -682,6 +683,7 @@ __attribute__((visibility("default"))) int cusig_amd_linear_recurrence_step(
     return sigamd::guarded([&] {
         check_scan(rows, channels, rows, 1, nullptr);
         if (rows * channels == 0) return;
+        require(x && log_decay && state && h, "a tensor is missing");
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
             constexpr int V = 4;

@@ -309,6 +309,8 @@ void run(int dtype, RotaryArgs& p, bool interleaved, bool back, float* dqw, floa
         }
         return;
     }
+    require(p.qw && p.kw && p.positions && (p.rotary == 0 || (p.cos && p.sin)), "a tensor is missing");
+    require((p.heads == 0 || (p.q && p.oq && (!back || p.gq))) && (p.kv_heads == 0 || (p.k && p.ok && (!back || p.gk))), "a tensor is missing");
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
         if (interleaved) by_lanes<T, true>(p, back, dqw, dkw, static_cast<hipStream_t>(stream));

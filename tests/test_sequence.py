@@ -513,6 +513,60 @@ def test_attention_of_parts_of_a_projection_with_large_scores(P, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("lengths,past,heads,kv,dim", [([300, 70, 5], 0, 4, 2, 64), ([700], 0, 2, 1, 128), ([900], 0, 2, 2, 40), ([5, 3], 400, 4, 2, 128),
+                                                       ([1, 12], 300, 2, 1, 64)])
+def test_attention_with_values_that_are_not_finite(P, dtype, lengths, past, heads, kv, dim):
+    """A value that is infinite or not a number reaches the queries that see its key, and no others; so does a key."""
+    keys = [n + past for n in lengths]
+    qs, ks = starts_of(lengths), starts_of(keys)
+    q, k, v, _ = attention_inputs(dtype, qs[-1], ks[-1], heads, kv, dim, seed=qs[-1])
+    offsets = [torch.tensor(s, dtype=torch.int32, device=DEV) for s in (qs, ks)]
+    clean, _ = P.attention(q, k, v, *offsets)
+    for n in range(len(lengths)):
+        for back, ch, x in [(1, 0, float("nan")), (2, dim - 1, float("inf")), (lengths[n] // 2 + 1, 5, -float("inf"))]:
+            if back <= keys[n]:
+                v[ks[n + 1] - back, 0, ch] = x
+    out, lse = P.attention(q, k, v, *offsets)
+    assert torch.isfinite(lse).all()
+    values, group = f64(v), heads // kv
+    want, touched = f64(clean).copy(), np.zeros(out.shape, bool)
+    for n, a in enumerate(lengths):
+        for j in range(a):
+            row, seen = qs[n] + j, slice(ks[n], ks[n + 1] - a + j + 1)
+            bad = np.where(np.isfinite(values[seen, 0]), 0.0, values[seen, 0])
+            with np.errstate(invalid="ignore"):
+                total = bad.sum(0)
+            touched[row, :group] = total != 0
+            want[row, :group] = np.where(total != 0, total, want[row, :group])
+    got = f64(out)
+    assert (np.isnan(got) == np.isnan(want)).all() and (got[touched & ~np.isnan(want)] == want[touched & ~np.isnan(want)]).all()
+    assert (got[~touched] == want[~touched]).all()
+    k[ks[-1] - 1] = float("nan")
+    out, _ = P.attention(q, k, torch.nan_to_num(v, 0.0, 0.0, 0.0), *offsets)
+    assert torch.isfinite(out[:-1]).all() and torch.isnan(out[-1]).all()
+
+
+@pytest.mark.gpu
+def test_offsets_that_do_not_ascend_stay_inside(P):
+    """Offsets are not read on the host: whatever they hold, nothing is read or written outside the tensors."""
+    rng = np.random.default_rng(3)
+    rows = 300
+    q, k, v, g = attention_inputs(torch.float16, rows, rows, 2, 1, 64, seed=3)
+    x = torch.zeros((rows, 40), dtype=torch.bfloat16, device=DEV)
+    for n in (1, 5, 64, 65, 400):
+        offsets = torch.tensor(rng.integers(-1000, 1000, n + 1), dtype=torch.int32, device=DEV)
+        offsets[n // 2] = 0
+        offsets[n // 2 + 1] = rows
+        out, lse = P.attention(q, k, v, offsets, offsets)
+        P.attention(q, k, v, offsets, offsets, k_lengths=offsets[:-1].contiguous())
+        P.attention_backprop(g, q, k, v, out, torch.zeros_like(lse), offsets, offsets)
+        P.linear_recurrence(x, x, offsets=offsets)
+        P.linear_recurrence_backprop(x, x, x, offsets=offsets)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
 def test_attention_of_nothing(P):
     q, k = torch.zeros((0, 2, 64), dtype=torch.bfloat16, device=DEV), torch.zeros((3, 1, 64), dtype=torch.bfloat16, device=DEV)
     zero, at = torch.tensor([0, 0], dtype=torch.int32, device=DEV), torch.tensor([0, 3], dtype=torch.int32, device=DEV)
@@ -693,3 +747,33 @@ def test_refuses_host_tensors(P):
     cos, sin = P.rotary_tables(4, 6, base=100., scale=2., device="cpu")
     want = np.arange(4)[:, None] / 2 * 100.0 ** (-np.arange(3) / 3)
     assert np.abs(f64(cos) - np.cos(want)).max() <= U32 and np.abs(f64(sin) - np.sin(want)).max() <= U32
+
+
+def test_the_entry_points_report_what_is_wrong(P):
+    """Straight calls of the C entry points that never reach the GPU: status 2 and a message, nothing thrown."""
+    from pysiglib_amd import _loader as L
+    assert L.CUSIG_LINEAR_RECURRENCE(7, 0, 0, 0, 0, 0, 0, 1, 1, 1, 1, 1, 1, 0, 0, 0) == 2
+    assert L.CUSIG_LINEAR_RECURRENCE(0, 0, 0, 0, 0, 0, 0, 1, 1, 1, 1, 1, 1, 0, 0, 0) == 2 and "missing" in L.last_error_message()
+    assert L.CUSIG_LINEAR_RECURRENCE(0, 8, 8, 0, 8, 8, 0, 3, 1, 1, 1, 1, 1, 0, 0, 0) == 2
+    assert L.CUSIG_LINEAR_RECURRENCE(0, 8, 8, 0, 8, 8, 0, 1, 100000, 100000, 8, 8, 8, 0, 0, 0) == 2 and "workspace" in L.last_error_message()
+    assert L.CUSIG_LINEAR_RECURRENCE(0, 8, 8, 0, 8, 8, 0, 1, 5000, 5000, 8, 1 << 21, 8, 8, 1 << 40, 0) == 2 and "2^20" in L.last_error_message()
+    assert L.CUSIG_LINEAR_RECURRENCE_STEP(0, 0, 0, 0, 0, 1, 1, 1, 1, 0) == 2
+    assert L.CUSIG_LINEAR_RECURRENCE(0, 0, 0, 0, 0, 0, 0, 0, 5, 0, 8, 8, 8, 0, 0, 0) == 0
+    rotary = [0, 8, 8, 8, 8, 8, 8, 8, 8, 8, 2, 2, 2, 8, 8, 4, 16, 8, 16, 8, 1e-6, False, 0]
+    for at, value, text in [(13, 300, "too many"), (13, 9, "even"), (14, 3, "even"), (14, 16, "too many"), (5, 0, "missing"), (1, 0, "missing")]:
+        args = list(rotary)
+        args[at] = value
+        assert L.CUSIG_NORM_ROTARY(*args) == 2 and text in L.last_error_message(), (at, value)
+    attention = [1, 8, 8, 8, 8, 8, 0, 8, 8, 4, 4, 1, 2, 1, 64, 128, 64, 64, 64, 64, 64, 0.1, True, 0, 0, 0]
+    for at, value, text in [(0, 0, "bfloat16"), (14, 60, "multiple of 8"), (14, 136, "multiple of 8"), (13, 0, "heads"), (12, 3, None), (21, 0.0, "scale"),
+                            (15, 1 << 23, "apart"), (7, 0, "missing"), (1, 0, "missing")]:
+        args = list(attention)
+        args[at] = value
+        if at == 12:
+            args[13] = 2
+        assert L.CUSIG_ATTENTION(*args) == 2 and (text is None or text in L.last_error_message()), (at, value)
+    many = list(attention)
+    many[11], many[9], many[10] = 100, 100000, 100000        # the list of the sequences' tiles needs room
+    assert L.CUSIG_ATTENTION_WORKSPACE(100000, 100000, 100, 2, 1, 64) > 0
+    assert L.CUSIG_ATTENTION(*many) == 2 and "workspace" in L.last_error_message()
+    assert L.CUSIG_ATTENTION_WORKSPACE(4, 4, 0, 2, 1, 64) == 0 and L.CUSIG_ATTENTION_BACKPROP_WORKSPACE(4, 4, 0, 2, 64) > 0
