@@ -163,7 +163,7 @@ __device__ __forceinline__ void store_row(T* to, const f32x16* x, float times, i
 
 // Values that are not finite, at keys that some queries of a tile do not see: a weight of zero times them would not be zero.  Tiles
 // with hidden keys are put into shared memory with zeros in their place; which keys had them is noted, and what they are is
-// added at the end for the queries that see them.
+// added to the stored rows of the queries that see them.
 template <typename T>
 __device__ __forceinline__ unsigned not_finite(unsigned two)
 {
@@ -186,18 +186,16 @@ __device__ __forceinline__ bool take_them_out(u32x4& x)
     return any != 0;
 }
 
-// adds the values that are not finite of the row `v` to a lane's column of sums
-template <typename T, int DP>
-__device__ __forceinline__ void add_them(const T* v, int dim, int half, f32x16* o)
+// Adds the values that are not finite of the row `v` to the channels of a stored row that a lane has stored (in memory and out of
+// line: a rare case takes no registers from the common one)
+template <typename T, typename O>
+__device__ __attribute__((noinline)) void add_them(const T* v, O* to, int dim, int half)
 {
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int ch = 32 * d + row_in(i, half);
-            const float x = ch < dim ? static_cast<float>(v[ch]) : 0.0f;
-            if (!__builtin_isfinite(x)) o[d][i] += x;
-        }
+#pragma unroll 1
+    for (int ch = 4 * half; ch < dim; ch += (ch & 3) == 3 ? 5 : 1) {
+        const float x = static_cast<float>(v[ch]);
+        if (!__builtin_isfinite(x)) to[ch] = O(static_cast<float>(to[ch]) + x);
+    }
 }
 
 // Packed sequences.  Offsets are read on the device and kept inside the tensors whatever they hold.

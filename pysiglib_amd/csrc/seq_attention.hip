@@ -35,8 +35,11 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
     static_assert(kLoads * kThreads == kKeys * Tile<DP>::kChunks, "");
     __shared__ __attribute__((aligned(16))) char s_tiles[2][2][kTileBytes];
     constexpr int kHiding = kRows / kKeys + 2;       // tiles that hide keys from some queries of the block, at most
-    __shared__ unsigned s_bad[kHiding][kKeys / 32];  // their keys whose values are not finite
+    __shared__ unsigned s_bad[kHiding][kKeys / 32], s_any;       // their keys whose values are not finite, and whether there are any
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (tid < kHiding)
+        for (unsigned& bad : s_bad[tid]) bad = 0;
+    if (tid == 0) s_any = 0;
     // the heads that share keys and values follow each other at a distance of kv_heads: on the same die where that is a multiple of 8
     const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
     // the last tiles see the most keys: they begin first
@@ -89,21 +92,29 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
             next[1][i] = load_at(vp, v_at[i]);
         }
     };
-    // a key is hidden past the sequence's end, or behind a query's place: from any of the queries from `first` on
-    auto hides = [&](int tile, int first) { return tile * kKeys + kKeys > at.nk || (p.causal && tile * kKeys + kKeys - 1 > first + shift); };
-    const int hiding = min(p.causal ? max(q_first + shift + 1, 0) / kKeys : tiles, tiles - 1);       // the first such tile, or one before it
+    // A key is hidden past the sequence's end, or behind a query's place.  Tiles from `hiding` on hide some from some of the block's
+    // queries, from `hiding_wave` on from some of the wave's; from `unseen` on the wave's queries see none of them.
+    const int hiding = min(at.nk, p.causal ? max(q_first + shift + 1, 0) : at.nk) / kKeys;
+    const int hiding_wave = min(at.nk, p.causal ? max(q_first + wave * 32 + shift + 1, 0) : at.nk) / kKeys;
+    const int unseen = p.causal ? min(max(q_first + wave * 32 + 31 + shift + kKeys, 0) / kKeys, tiles) : tiles;
     auto put = [&](int tile) __attribute__((always_inline)) {
-        if (hides(tile, q_first))
+        auto place = [&](int i) { return Tile<DP>::at((i * kThreads + tid) / Tile<DP>::kChunks, (i * kThreads + tid) % Tile<DP>::kChunks); };
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) *reinterpret_cast<u32x4*>(s_tiles[tile & 1][0] + place(i)) = next[0][i];
+        if (tile >= hiding) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const int row = (i * kThreads + tid) / Tile<DP>::kChunks;
-                if (take_them_out<T>(next[1][i])) atomicOr(&s_bad[tile - hiding][row / 32], 1u << row % 32);
+                u32x4 x = next[1][i];
+                if (take_them_out<T>(x)) {
+                    atomicOr(&s_bad[tile - hiding][row / 32], 1u << row % 32);
+                    s_any = 1;
+                }
+                *reinterpret_cast<u32x4*>(s_tiles[tile & 1][1] + place(i)) = x;
             }
+        } else {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int e = i * kThreads + tid, to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
-            *reinterpret_cast<u32x4*>(s_tiles[tile & 1][0] + to) = next[0][i];
-            *reinterpret_cast<u32x4*>(s_tiles[tile & 1][1] + to) = next[1][i];
+            for (int i = 0; i < kLoads; ++i) *reinterpret_cast<u32x4*>(s_tiles[tile & 1][1] + place(i)) = next[1][i];
         }
     };
     const int last = p.causal && query + shift < at.nk - 1 ? query + shift : at.nk - 1;
@@ -139,7 +150,7 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
     };
     auto weights = [&](int tile) __attribute__((always_inline)) {
         const int key0 = tile * kKeys;
-        if (hides(tile, q_first + wave * 32)) {
+        if (tile >= hiding_wave) {
 #pragma unroll
             for (int c = 0; c < kKeys / 32; ++c)
 #pragma unroll
@@ -196,11 +207,9 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
             if (kAhead) __builtin_amdgcn_sched_barrier(0);
         }
     };
-    if (tid < kHiding)
-        for (unsigned& bad : s_bad[tid]) bad = 0;
-    __syncthreads();
     if (tiles) {
         fetch(0);
+        if (hiding == 0) __syncthreads();       // s_bad is clear
         put(0);
     }
 #pragma unroll
@@ -208,25 +217,27 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
     for (int tile = 0; tile < tiles; ++tile) {
         __syncthreads();
         if (tile + 1 < tiles) fetch(tile + 1);
-        if (!p.causal || tile * kKeys <= q_first + wave * 32 + 31 + shift) {       // else none of the wave's queries sees any of the tile
+        if (tile < unseen) {
             scores(tile);
             weights(tile);
             values(tile);
         }
         if (tile + 1 < tiles) put(tile + 1);
     }
-    for (int tile = hiding; tile < tiles; ++tile)
-        for (int part = 0; part < kKeys / 32; ++part)
-            for (unsigned bad = s_bad[tile - hiding][part]; __builtin_expect(bad != 0, 0); bad &= bad - 1) {
-                const int key = tile * kKeys + 32 * part + __ffs(bad) - 1;
-                if (key <= last) add_them<T, DP>(static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head, p.dim, half, o);
-            }
     const float total = sum + swapped(sum);
     if (query >= at.nq) return;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     const int64_t row = (at.q0 + query) * p.heads + head;
     if (half == 0) p.lse[row] = total == 0.0f ? -INFINITY : 0.69314718055994531f * (top + log2f(total));
-    store_row<T, DP>(static_cast<T*>(p.out) + row * p.dim, o, inv, p.dim, half);
+    T* const to = static_cast<T*>(p.out) + row * p.dim;
+    store_row<T, DP>(to, o, inv, p.dim, half);
+    if (__builtin_expect(s_any != 0, 0))
+        for (int tile = hiding; tile < tiles; ++tile)
+            for (int part = 0; part < kKeys / 32; ++part)
+                for (unsigned bad = s_bad[tile - hiding][part]; bad; bad &= bad - 1) {
+                    const int key = tile * kKeys + 32 * part + __ffs(bad) - 1;
+                    if (key <= last) add_them<T, T>(static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head, to, p.dim, half);
+                }
 }
 
 // ---- few queries to many keys: rows of a tile are the pairs (query, head) that share a key head ----
@@ -239,7 +250,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
     constexpr int kTileBytes = kTile * Tile<DP>::kRowBytes, kLoads = kTile * Tile<DP>::kChunks / 64;
     __shared__ __attribute__((aligned(16))) char s_tiles[kWaves][2][kTileBytes];
     __shared__ float s_top[kWaves][32], s_sum[kWaves][32];
-    __shared__ unsigned s_bad[4];            // of the tiles that hide keys from some of the pairs: keys whose values are not finite
+    __shared__ unsigned s_bad[4], s_any;     // of the tiles that hide keys from some of the pairs: keys whose values are not finite
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = p.heads / p.kv_heads, kv = blockIdx.x % p.kv_heads, split = blockIdx.x / p.kv_heads % p.splits;
     const Span at = find_tile(p.packed, Tiling{false, 32, group}, blockIdx.x / p.kv_heads / p.splits, Dear::kLast);
@@ -283,9 +294,10 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
     const int first_query = at.tile * 32 / group;
     auto hides = [&](int tile) { return (tile + 1) * kTile > past - begin || (p.causal && begin + (tile + 1) * kTile - 1 > first_query + shift); };
     const int hiding = min(p.causal ? max(first_query + shift + 1 - begin, 0) / kTile : tiles, tiles - 1);      // the first of them, or one before it
-    if (tid < 4) s_bad[tid] = 0;
-    __syncthreads();
     if (wave < tiles) fetch(wave);
+    if (tid < 4) s_bad[tid] = 0;
+    if (tid == 4) s_any = 0;
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < kSlices; ++k) arrive<T>(q[k]);
     for (int tile = wave; tile < tiles; tile += kWaves) {
@@ -293,7 +305,10 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
         if (hidden)
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
-                if (take_them_out<T>(next[1][i])) atomicOr(&s_bad[tile - hiding], 1u << (i * 64 + lane) / Tile<DP>::kChunks);
+                if (take_them_out<T>(next[1][i])) {
+                    atomicOr(&s_bad[tile - hiding], 1u << (i * 64 + lane) / Tile<DP>::kChunks);
+                    s_any = 1;
+                }
         // the wave's own tiles: shared memory serves a wave in order, no barrier is needed
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
@@ -376,11 +391,14 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
                 for (int i = 0; i < 16; ++i) o[d][i] += shared[wave * kPart + (d * 16 + i) * 64 + lane];
     }
     if (wave || pair >= pairs) return;
-    for (int tile = hiding; tile < tiles; ++tile)
-        for (unsigned bad = s_bad[tile - hiding]; __builtin_expect(bad != 0, 0); bad &= bad - 1) {
-            const int key = begin + tile * kTile + __ffs(bad) - 1;
-            if (key <= last) add_them<T, DP>(static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head, p.dim, half, o);
-        }
+    auto correct = [&](auto* to) {
+        if (__builtin_expect(s_any != 0, 0))
+            for (int tile = hiding; tile < tiles; ++tile)
+                for (unsigned bad = s_bad[max(tile - hiding, 0)]; bad; bad &= bad - 1) {
+                    const int key = begin + tile * kTile + __ffs(bad) - 1;
+                    if (key <= last) add_them(static_cast<const T*>(p.v) + (at.k0 + key) * p.v_token + kv * p.v_head, to, p.dim, half);
+                }
+    };
     const int64_t row = (at.q0 + query) * p.heads + head;
     if (p.splits > 1) {
         // [splits][q_rows * heads] of (maximum, sum), then [splits][q_rows * heads][dim]
@@ -400,11 +418,14 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
                     *reinterpret_cast<f32x4*>(to + ch) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
                 }
             }
+        correct(to);
         return;
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     if (half == 0) p.lse[row] = total == 0.0f ? -INFINITY : 0.69314718055994531f * (most + log2f(total));
-    store_row<T, DP>(static_cast<T*>(p.out) + row * p.dim, o, inv, p.dim, half);
+    T* const to = static_cast<T*>(p.out) + row * p.dim;
+    store_row<T, DP>(to, o, inv, p.dim, half);
+    correct(to);
 }
 
 // the splits of one (query, head) to a wave, a lane to one or two channels pairwise
