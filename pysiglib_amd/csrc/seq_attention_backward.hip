@@ -294,25 +294,30 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
         }
     };
     constexpr bool kAhead = DP == 128;
-    // 32 rows of a tile times the fixed operand; 128 channels: operands are read a group ahead, as in the forward
-    auto by_rows = [&](const char* tile, int row0) __attribute__((always_inline)) {
-        constexpr int kGroup = 4, kGroups = kSlices / kGroup;
-        Frag<T> f[2][kGroup];
+    // A tile's rows times the fixed operand, its parts of 32 rows side by side: products of one part wait for each other.  128
+    // channels: operands are read a group ahead, as in the forward.
+    auto by_rows = [&](const char* tile, f32x16* x) __attribute__((always_inline)) {
+        constexpr int kGroup = 4 / kParts, kGroups = kSlices / kGroup;
+        Frag<T> f[2][kGroup][kParts];
         auto read = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-            for (int k = 0; k < kGroup; ++k) f[n & 1][k] = rows.template get<T>(tile, row0, n * kGroup + k);
+            for (int k = 0; k < kGroup; ++k)
+#pragma unroll
+                for (int c = 0; c < kParts; ++c) f[n & 1][k][c] = rows.template get<T>(tile, 32 * c, n * kGroup + k);
             if (kAhead) __builtin_amdgcn_sched_barrier(0);
         };
-        f32x16 x = zeros16();
+#pragma unroll
+        for (int c = 0; c < kParts; ++c) x[c] = zeros16();
         read(0);
 #pragma unroll
         for (int n = 0; n < kGroups; ++n) {
             if (n + 1 < kGroups) read(n + 1);
 #pragma unroll
-            for (int k = 0; k < kGroup; ++k) x = product(f[n & 1][k], fixed[n * kGroup + k], x);
+            for (int k = 0; k < kGroup; ++k)
+#pragma unroll
+                for (int c = 0; c < kParts; ++c) x[c] = product(f[n & 1][k][c], fixed[n * kGroup + k], x[c]);
             if (kAhead) __builtin_amdgcn_sched_barrier(0);
         }
-        return x;
     };
     // adds the columns of 32 rows times the two operands
     auto by_columns = [&](const char* tile, int row0, const Frag<T>* w) __attribute__((always_inline)) {
@@ -341,9 +346,11 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
         if (++tile == tiles) tile = 0, ++head;
         if (step + 1 < steps) fetch(head, tile);
         if (!second && step < steps) {
+            f32x16 parts[kParts];
+            by_rows(s_tiles[now][0], parts);
 #pragma unroll
             for (int c = 0; c < kParts; ++c) {
-                f32x16 s = by_rows(s_tiles[now][0], 32 * c);
+                f32x16& s = parts[c];
                 if (p.causal && q0 + 32 * c + shift < key0 + 31)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
@@ -360,9 +367,11 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
             }
         }
         if (second && step > 0) {
+            f32x16 parts[kParts];
+            by_rows(s_tiles[before][1], parts);
 #pragma unroll
             for (int c = 0; c < kParts; ++c) {
-                const f32x16 dp = by_rows(s_tiles[before][1], 32 * c);
+                const f32x16& dp = parts[c];
                 Frag<T> ds[2];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {

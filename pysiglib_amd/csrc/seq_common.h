@@ -62,6 +62,17 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& r)
     __builtin_memcpy(p, r.w, sizeof r.w);
 }
 
+// the same past the caches, in whole lines: for results larger than the eight L2s, which would leave them unread
+template <typename T, int V>
+__device__ __forceinline__ void store_past(T* p, const Pack<T, V>& r)
+{
+    typedef unsigned Words __attribute__((ext_vector_type(Pack<T, V>::kWords), aligned(4)));
+    Words x;
+#pragma unroll
+    for (int i = 0; i < Pack<T, V>::kWords; ++i) x[i] = r.w[i];
+    __builtin_nontemporal_store(x, reinterpret_cast<Words*>(p));
+}
+
 // the first `count` of V elements, the others zero
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> load_some(const T* p, int count)
@@ -90,6 +101,10 @@ __device__ __forceinline__ void store_some(T* p, const Pack<T, V>& r, int count)
             else p[i] = __builtin_bit_cast(T, static_cast<unsigned short>(r.w[i / 2] >> (i & 1 ? 16 : 0)));
         }
 }
+
+// whether results of so many bytes, in rows of `row` bytes, are stored past the caches.  Lines that are written in pieces are not:
+// gradients of 23000 steps of 997 channels in float16 took 126 us instead of 89.
+inline bool goes_past(uint64_t bytes, uint64_t row) { return bytes >= (uint64_t(32) << 20) && row % 128 == 0; }
 
 inline void require(bool ok, const char* what)
 {

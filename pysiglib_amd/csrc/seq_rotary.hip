@@ -26,6 +26,7 @@ struct RotaryArgs {
     int64_t tokens, q_token, q_head, k_token, k_head, gq_token, gq_head, gk_token, gk_head, table;
     int heads, kv_heads, dim, rotary, split;
     float eps;
+    bool past;                    // results go past the caches
 };
 
 // The U pairs of a lane: elements a[i] and b[i] are turned against each other (or stay, past the rotary part).
@@ -78,7 +79,7 @@ __device__ __forceinline__ void load_pairs(const T* row, const Place& p, float* 
 }
 
 template <typename T, int U, bool NEAR>
-__device__ __forceinline__ void store_pairs(T* row, const Place& p, const float* a, const float* b)
+__device__ __forceinline__ void store_pairs(T* row, const Place& p, bool past, const float* a, const float* b)
 {
     if constexpr (NEAR) {
         float x[2 * U];
@@ -86,13 +87,19 @@ __device__ __forceinline__ void store_pairs(T* row, const Place& p, const float*
         for (int i = 0; i < U; ++i) x[2 * i] = a[i], x[2 * i + 1] = b[i];
         Pack<T, 2 * U> o;
         o.set(x);
-        store_some<T, 2 * U>(row + p.first, o, 2 * p.pairs);
+        if (past && p.pairs == U) store_past<T, 2 * U>(row + p.first, o);
+        else store_some<T, 2 * U>(row + p.first, o, 2 * p.pairs);
     } else {
-        Pack<T, U> o;
-        o.set(a);
-        store_some<T, U>(row + p.first, o, p.pairs);
-        o.set(b);
-        store_some<T, U>(row + p.second, o, p.pairs);
+        Pack<T, U> x, y;
+        x.set(a);
+        y.set(b);
+        if (past && p.pairs == U) {
+            store_past<T, U>(row + p.first, x);
+            store_past<T, U>(row + p.second, y);
+        } else {
+            store_some<T, U>(row + p.first, x, p.pairs);
+            store_some<T, U>(row + p.second, y, p.pairs);
+        }
     }
 }
 
@@ -152,7 +159,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(RotaryArgs p)
             a[i] = u * c[i] - v * s[i];
             b[i] = u * s[i] + v * c[i];
         }
-        store_pairs<T, U, NEAR>(o, at, a, b);
+        store_pairs<T, U, NEAR>(o, at, p.past, a, b);
     }
 }
 
@@ -204,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(RotaryArgs p)
                 a[i] = r * (ga[i] * (key ? wk[0][i] : wq[0][i]) - a[i] * back);
                 b[i] = r * (gb[i] * (key ? wk[1][i] : wq[1][i]) - b[i] * back);
             }
-            store_pairs<T, U, NEAR>(o, at, a, b);
+            store_pairs<T, U, NEAR>(o, at, p.past, a, b);
         }
     }
     // the block's piece of the weights' gradients
@@ -313,6 +320,8 @@ void run(int dtype, RotaryArgs& p, bool interleaved, bool back, float* dqw, floa
     require((p.heads == 0 || (p.q && p.oq && (!back || p.gq))) && (p.kv_heads == 0 || (p.k && p.ok && (!back || p.gk))), "a tensor is missing");
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
+        // (16384 tokens, 40 heads of 128 channels, bfloat16: 55 us, through the caches 70 us)
+        p.past = goes_past(uint64_t(p.tokens) * (p.heads + p.kv_heads) * p.dim * sizeof(T), uint64_t(p.dim) * sizeof(T));
         if (interleaved) by_lanes<T, true>(p, back, dqw, dkw, static_cast<hipStream_t>(stream));
         else by_lanes<T, false>(p, back, dqw, dkw, static_cast<hipStream_t>(stream));
     });
