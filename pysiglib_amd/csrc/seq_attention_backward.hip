@@ -10,7 +10,8 @@
 // Keys fixed: a wave cannot hold sums, keys and values of 64 keys of 128 channels at once with two waves to a SIMD, so waves
 // work in pairs.  The first forms P of a tile of queries and adds to dV, the second, one tile behind, takes P from shared
 // memory, forms dS and adds to dK.  Operands are rounded to the inputs' type (P, dS), sums are 32-bit.  In shared memory P is a
-// float16 whatever that type: in [0, 1] these are eight times as fine as bfloat16 at the same size.
+// float16 whatever that type: in [0, 1] these are eight times as fine as bfloat16 at the same size.  For float16 inputs that
+// rounding would weigh as much as dS's own; an 8-bit float of its error goes along.
 #include "seq_attention.h"
 
 namespace seqamd {
@@ -29,7 +30,8 @@ struct GradArgs {
 };
 
 constexpr float kLog2e = 1.44269504088896341f;
-constexpr int kExact = 512;               // keys up to which delta is summed from its definition
+constexpr int kExact = 512;               // keys up to which delta is summed from its definition, 128 channels, causal
+constexpr float kRest = 1048576.0f;       // a weight's rounding error in float16, at most 2^-12, times this fits 8 bits (at most 448)
 
 // float16 holds dS only near 1: it is formed from gradients multiplied by a power of two that brings the largest there
 __device__ __forceinline__ float towards_one(float largest)
@@ -39,7 +41,7 @@ __device__ __forceinline__ float towards_one(float largest)
 
 // ---- queries fixed: 32 to a wave, tiles of kKeys keys ----
 template <typename T, int DP, int WAVES, int kKeys>
-__global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 3 : 2) dq_kernel(GradArgs p)
+__global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
 {
     constexpr int kThreads = WAVES * 64, kRows = 32 * WAVES, kSlices = DP / 16, kBlocks = DP / 32;
     constexpr int kTileBytes = kKeys * Tile<DP>::kRowBytes, kLoads = kKeys * Tile<DP>::kChunks / kThreads;
@@ -93,9 +95,22 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 3 : 2) dq_kernel(GradAr
     }
     const float lse = p.lse[place] == -INFINITY ? INFINITY : p.lse[place] * kLog2e;
     const int last = p.causal && query + shift < at.nk - 1 ? query + shift : at.nk - 1;
-    f32x16 dq[kBlocks];
+    // The output's rounding makes delta wrong by u |dO| |O|, which matters where few keys share the weight: dS, differences from
+    // delta, is as small there as that.  64 channels: e, the sum of dS, is what delta is short of, and dQ is short of e P K, which
+    // is summed beside it (24 sequences of up to 2000, 16 heads on 4, the whole gradient: 418 us, without it 390; sequences of 17 to
+    // 129: 66 us, 74 when they went over their keys twice).  128 channels: no registers for these sums; queries go over up to
+    // `exact` keys twice.  Every query has them all where none are hidden, and the error's share falls with the channels: there
+    // they do so to longer lengths (8 sequences of 1000, 16 heads on 8, nothing hidden: 381 us, once 321; dQ's error against 64
+    // bits, in those of a result that is rounded once: 1.43 and 1.55).
+    constexpr bool kMend = DP == 64;
+    const int exact = kExact * (p.causal ? 1 : 4) * (p.dim > 96 ? 1 : 2);
+    f32x16 dq[kBlocks], pk[kMend ? kBlocks : 1];
+    float short_of = 0.0f;
 #pragma unroll
-    for (int d = 0; d < kBlocks; ++d) dq[d] = zeros16();
+    for (int d = 0; d < kBlocks; ++d) {
+        dq[d] = zeros16();
+        if (kMend) pk[d] = zeros16();
+    }
 
     u32x4 next[2][kLoads];
     unsigned k_at[kLoads], v_at[kLoads];
@@ -168,10 +183,8 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 3 : 2) dq_kernel(GradAr
                 if (key0 + row_in(i, half) > last) s[i] = -INFINITY;
     };
     int buffer = 0;
-    // The output's rounding makes delta wrong by u |dO| |O|, which matters where few keys share the weight: dS, differences from
-    // delta, is as small there as that.  Queries with up to kExact keys go over them twice, first to sum P dP, which is delta.
-    if (keys <= kExact && tiles) {
-        float exact = 0.0f;
+    if (!kMend && keys <= exact && tiles) {       // first to sum P dP, which is delta
+        float sum = 0.0f;
         for (int tile = 0; tile < tiles; ++tile, buffer ^= 1) {
             __syncthreads();
             fetch(tile + 1 < tiles ? tile + 1 : 0);
@@ -182,11 +195,11 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 3 : 2) dq_kernel(GradAr
                 pair_products(s_tiles[buffer][0], s_tiles[buffer][1], 32 * c, s, dp);
                 hide(s, key0);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) exact = fmaf(__builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -lse)), dp[i], exact);
+                for (int i = 0; i < 16; ++i) sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -lse)), dp[i], sum);
             }
             put(buffer ^ 1);
         }
-        delta = exact + swapped(exact);
+        delta = sum + swapped(sum);
     }
     for (int tile = 0; tile < tiles; ++tile, buffer ^= 1) {
         __syncthreads();
@@ -200,9 +213,13 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 3 : 2) dq_kernel(GradAr
             pair_products(kt, vt, 32 * c, s, dp);
             hide(s, key0);
 #pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -lse));
+            Frag<T> w[2];
+            if (kMend) w[0] = rounded<T>(s, 0), w[1] = rounded<T>(s, 8);
+#pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float w = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -lse));
-                s[i] = w * (__is_same(T, f16) ? lift * (dp[i] - delta) : dp[i] - delta);
+                s[i] *= __is_same(T, f16) ? lift * (dp[i] - delta) : dp[i] - delta;
+                if (kMend) short_of += s[i];
             }
             Frag<T> f[2][kBlocks];
             auto read = [&](int u) __attribute__((always_inline)) {
@@ -215,10 +232,21 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 3 : 2) dq_kernel(GradAr
             for (int u = 0; u < 2; ++u) {
                 const Frag<T> ds = rounded<T>(s, 8 * u);
 #pragma unroll
-                for (int d = 0; d < kBlocks; ++d) dq[d] = product(f[u][d], ds, dq[d]);
+                for (int d = 0; d < kBlocks; ++d) {
+                    dq[d] = product(f[u][d], ds, dq[d]);
+                    if (kMend) pk[d] = product(f[u][d], w[u], pk[d]);
+                }
             }
         }
         if (tile + 1 < tiles) put(buffer ^ 1);
+    }
+    if (kMend) {
+        short_of += swapped(short_of);
+        delta += short_of / lift;
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dq[d][i] = fmaf(-short_of, pk[d][i], dq[d][i]);
     }
     if (query < at.nq && half == 0) p.delta[place] = delta;
     if (query < at.nq) store_row<T, DP>(static_cast<T*>(p.dq) + place * p.dim, dq, p.scale / lift, p.dim, half);
@@ -233,7 +261,8 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
     static_assert(kLoads * kThreads == kQueries * Tile<DP>::kChunks, "");
     __shared__ __attribute__((aligned(16))) char s_tiles[3][2][kTileBytes];
     __shared__ __attribute__((aligned(16))) float s_lse[3][kQueries], s_delta[3][kQueries];
-    __shared__ __attribute__((aligned(16))) u32x4 s_weights[2][PAIRS][kParts][2][64];
+    constexpr bool kFiner = __is_same(T, f16);
+    __shared__ __attribute__((aligned(16))) u32x4 s_weights[2][PAIRS][kParts][kFiner ? 3 : 2][64];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave % PAIRS;
     const bool second = wave >= PAIRS;
     const int kv = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
@@ -363,6 +392,17 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
                     w[u] = rounded<T>(s, 8 * u);
                     s_weights[step & 1][pair][c][u][lane] = __builtin_bit_cast(u32x4, rounded<f16>(s, 8 * u));
                 }
+                if constexpr (kFiner) {
+                    u32x4 rest;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float r[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) r[j] = (s[4 * i + j] - static_cast<float>(w[i / 2][i % 2 * 4 + j])) * kRest;
+                        rest[i] = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false), true);
+                    }
+                    s_weights[step & 1][pair][c][2][lane] = rest;
+                }
                 by_columns(s_tiles[now][1], 32 * c, w);
             }
         }
@@ -373,13 +413,21 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
             for (int c = 0; c < kParts; ++c) {
                 const f32x16& dp = parts[c];
                 Frag<T> ds[2];
+                u32x4 rest;
+                if constexpr (kFiner) rest = s_weights[(step - 1) & 1][pair][c][2][lane];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const Frag<f16> w = __builtin_bit_cast(Frag<f16>, s_weights[(step - 1) & 1][pair][c][u][lane]);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float x = dp[8 * u + i] - s_delta[before][32 * c + row_in(8 * u + i, half)];
-                        ds[u][i] = T(static_cast<float>(w[i]) * (__is_same(T, f16) ? x * lift : x));
+                        if constexpr (kFiner) {
+                            const int word = static_cast<int>(rest[2 * u + i / 4]);
+                            const float r = i % 4 < 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(word, false)[i % 2] : __builtin_amdgcn_cvt_pk_f32_fp8(word, true)[i % 2];
+                            ds[u][i] = T(fmaf(r, 1.0f / kRest, static_cast<float>(w[i])) * (x * lift));
+                        } else {
+                            ds[u][i] = T(static_cast<float>(w[i]) * x);
+                        }
                     }
                 }
                 by_columns(s_tiles[before][0], 32 * c, ds);
@@ -397,8 +445,8 @@ constexpr uint64_t kHeadBytes = 256;
 
 // Blocks by the average length of the sequences, from times of whole calls (16 heads on 4 of 64 channels, 16000 tokens, and 32 on
 // 8 of 128, 8000 tokens).
-// Queries fixed, waves of a block: 64 channels, sequences of 64: 2 waves 92 us, 4 waves 100; of 250: 135 and 130; of 1000: 404 and 324.  128
-// channels, of 16: 2 waves 178 us, 8 waves 232; of 400: 4 waves 250; of 2000: 4 waves 466 us, 8 waves 480; one of 8192: 8 waves 1934 us.
+// Queries fixed, waves of a block: 64 channels, sequences of 64: 2 waves 90 us, 4 waves 99; of 400: 169 and 174; of 2000: 360 and 356;
+// one of 8192: 852 and 842.  128 channels, of 16: 2 waves 178 us, 8 waves 232; of 400: 4 waves 250; of 2000: 4 waves 466 us, 8 waves 480; one of 8192: 8 waves 1934 us.
 // Keys fixed: 64 channels, 2 pairs, sequences of 16: steps of 32 queries 94 us, of 64 132; of 400: 150 and 139; of 8192: 895
 // and 804.  128 channels, of 64: 2 pairs and 32 queries 172 us, 4 pairs and 64 queries 191; of 1000: 493 and 498; 4 of 1600 to
 // 2047: 546 and 508; two of 4096: 1057 and 955.
@@ -409,7 +457,7 @@ struct Blocks {
 Blocks blocks_of(int64_t q_rows, int64_t k_rows, int64_t n, int64_t dim)
 {
     const int64_t queries = q_rows / n, keys = k_rows / n;
-    if (dim <= 64) return Blocks{queries <= 150 ? 2 : 4, 2, keys <= 200 ? 32 : 64};
+    if (dim <= 64) return Blocks{queries <= 1400 ? 2 : 4, 2, keys <= 200 ? 32 : 64};
     return Blocks{queries <= 200 ? 2 : (queries <= 2048 ? 4 : 8), keys <= 700 ? 2 : 4, keys <= 700 ? 32 : 64};
 }
 
