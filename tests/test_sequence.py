@@ -471,6 +471,25 @@ def test_attention_gradients_are_differences(P, size):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("lengths,heads,kv,dim,causal", [([40] * 8, 4, 4, 64, True), ([600], 2, 1, 40, False), ([640], 2, 1, 80, False),
+                                                         ([900], 2, 1, 128, False), ([1300], 2, 1, 128, True)])
+def test_attention_gradients_are_off_by_few_roundings(P, dtype, lengths, heads, kv, dim, causal):
+    """The error's size as a whole, in that of the exact gradient rounded once to the type.  dV is a product of rounded
+    weights, rounded: 2 of these squared.  dQ and dK are products of rounded dS, rounded, where dS, whose sum is zero, meets
+    keys with a mean of their own: 0.2 more at these scores.  What else goes into dS may add half a rounding's: 2.7, 1.65."""
+    starts = starts_of(lengths)
+    q, k, v, g = attention_inputs(dtype, starts[-1], starts[-1], heads, kv, dim, seed=17)
+    offsets = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    out, lse = P.attention(q, k, v, offsets, offsets, causal=causal)
+    got = P.attention_backprop(g, q, k, v, out, lse, offsets, offsets, causal=causal)
+    want = attention_oracle(f64(q), f64(k), f64(v), lengths, starts, lengths, causal, dim ** -0.5, grad=f64(g))[0][2:]
+    for name, x, w in zip(("dq", "dk", "dv"), got, want):
+        once = f64(torch.tensor(w).to(dtype)) - w
+        assert np.linalg.norm(f64(x) - w) <= 1.65 * np.linalg.norm(once), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("lengths,heads,kv,dim", [([1], 1, 1, 64), ([0, 5, 64, 65, 700, 33], 8, 2, 128), ([2500, 1, 3000], 12, 1, 40),
                                                   ([129] * 40, 4, 4, 64), ([4100], 5, 1, 128), ([300, 0, 17], 48, 1, 64)])
 @pytest.mark.parametrize("queries", [1, 2, 5])
