@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const T* x, const T* gat
 }
 
 // Lanes take eight bytes of a row.  Where blocks publish, a chunk has kWide lanes to a row and 256 rows forward (100003 steps of 384
-// channels, float32: 116 us, with 128 rows 128 us, with 64 178 us) and 128 backward (registers), with few channels kNarrow lanes and 512 rows.
+// channels, float32: 107 us, with 128 rows 128 us, with 64 178 us) and 128 backward (registers), with few channels kNarrow lanes and 512 rows.
 // Where a block has its sequence to itself, kNarrow lanes, 256 rows forward and 128 backward, or 128 for short sequences.
 template <typename T>
 struct Shape {
@@ -537,7 +537,7 @@ struct Plan {
 };
 
 // A block to a sequence and 64 bytes of channels where these are blocks enough, or the sequences short: 8 sequences of 2048, 2048
-// channels, bfloat16: 42 us forward and 97 us backward, publishing 83 and 123; 4 of 512, 1024 channels, float32: 10 and 12, publishing 14
+// channels, bfloat16: 42 us forward and 65 us backward, publishing 83 and 123; 4 of 512, 1024 channels, float32: 10 and 12, publishing 14
 // and 17; but one of 4096, 4096 channels: 54 and 82, publishing 42 and 57; 2 of 4000, 64 channels: 32 and 53, publishing 15 and 17.
 template <typename T, bool BACK>
 Plan plan_of(int64_t rows, int64_t n, int channels)
@@ -586,7 +586,7 @@ void scan(ScanArgs p, void* workspace, size_t bytes, hipStream_t stream)
             "rows are at most 2^20 elements long and apart");
     p.chunks = plan.chunks;
     p.channel_blocks = plan.channel_blocks;
-    // (8 sequences of 2048 steps, 2048 channels, bfloat16: gradients 65 us, through the caches 96 us)
+    // (gradients of 8 sequences of 2048 steps, 2048 channels, bfloat16, alone: 65 us, through the caches 96 us)
     p.past = goes_past(uint64_t(p.rows) * p.channels * sizeof(T) * (BACK ? 2 : 1), uint64_t(p.channels) * sizeof(T));
     if (plan.columns) {
         const dim3 grid(unsigned(p.n) * unsigned(p.channel_blocks));
