@@ -8,6 +8,11 @@
 //
 // The products are formed transposed, S^T = K Q^T and O^T = V^T P^T: a lane then holds scores of a single query, its maximum
 // and sum need one exchange between lanes, and the weights are the second product's operand where they stand.
+//
+// Bound: 128 channels, the matrix units: one sequence of 8192, 32 heads on 8, bfloat16, 540 to 600 us (0.92 to 1.02 PFLOP/s; a large
+// library product reaches 1.19), and the order of reads around the products no longer changes that.  64 channels, the
+// softmax: 15 vector instructions to a matrix one, 24 sequences of up to 2000, 16 heads on 4, float16, 134 us (0.56 PFLOP/s).
+// Single queries, HBM: 48 against caches of up to 12000 keys of 8 heads of 128, 242 us (5.1 TB/s).
 #include "seq_attention.h"
 
 namespace seqamd {
@@ -26,7 +31,7 @@ struct AttentionArgs {
 
 constexpr float kSlack = 8.0f;   // the maximum is taken over where it grew by more than this (in powers of two): weights stay below 2^8
 
-// WAVES waves of 32 queries each, tiles of kKeys keys
+// WAVES waves of 32 queries each, tiles of kKeys keys: what a block reads serves all its waves, the next tile on its way meanwhile.
 template <typename T, int DP, int WAVES, int kKeys>
 __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel(AttentionArgs p)
 {
@@ -120,33 +125,14 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
     const int last = p.causal && query + shift < at.nk - 1 ? query + shift : at.nk - 1;
     f32x16 s[kKeys / 32];
     Frag<T> w[kKeys / 16];
-    // 128 channels: operands are read a group ahead of the products that take them, the compiler would read each right before
-    // its product and wait (two waves to a SIMD; 8192 tokens, 32 heads: 548 us, without 580).  64 channels: four waves to a SIMD
-    // hide the waits, and the registers read ahead into would cost one of them (365 us, without 350).
-    constexpr bool kAhead = DP == 128;
     auto scores = [&](int tile) __attribute__((always_inline)) {
         const char* kt = s_tiles[tile & 1][0];
-        constexpr int kGroup = kKeys == 64 ? 2 : 4, kGroups = kSlices / kGroup;
-        Frag<T> f[2][kGroup][kKeys / 32];
-        auto read = [&](int g) __attribute__((always_inline)) {
-#pragma unroll
-            for (int k = 0; k < kGroup; ++k)
-#pragma unroll
-                for (int c = 0; c < kKeys / 32; ++c) f[g & 1][k][c] = rows.template get<T>(kt, 32 * c, g * kGroup + k);
-            if (kAhead) __builtin_amdgcn_sched_barrier(0);
-        };
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c) s[c] = zeros16();
-        read(0);
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            if (g + 1 < kGroups) read(g + 1);
+        for (int k = 0; k < kSlices; ++k)
 #pragma unroll
-            for (int k = 0; k < kGroup; ++k)
-#pragma unroll
-                for (int c = 0; c < kKeys / 32; ++c) s[c] = product(f[g & 1][k][c], q[g * kGroup + k], s[c]);
-            if (kAhead) __builtin_amdgcn_sched_barrier(0);
-        }
+            for (int c = 0; c < kKeys / 32; ++c) s[c] = product(rows.template get<T>(kt, 32 * c, k), q[k], s[c]);
     };
     auto weights = [&](int tile) __attribute__((always_inline)) {
         const int key0 = tile * kKeys;
@@ -192,20 +178,10 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
     };
     auto values = [&](int tile) __attribute__((always_inline)) {
         const char* vt = s_tiles[tile & 1][1];
-        Frag<T> f[2][kBlocks];
-        auto read = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-            for (int d = 0; d < kBlocks; ++d) f[c & 1][d] = columns.template get<T>(vt, 16 * c, d);
-            if (kAhead) __builtin_amdgcn_sched_barrier(0);
-        };
-        read(0);
+        for (int c = 0; c < kKeys / 16; ++c)
 #pragma unroll
-        for (int c = 0; c < kKeys / 16; ++c) {
-            if (c + 1 < kKeys / 16) read(c + 1);
-#pragma unroll
-            for (int d = 0; d < kBlocks; ++d) o[d] = product(f[c & 1][d], w[c], o[d]);
-            if (kAhead) __builtin_amdgcn_sched_barrier(0);
-        }
+            for (int d = 0; d < kBlocks; ++d) o[d] = product(columns.template get<T>(vt, 16 * c, d), w[c], o[d]);
     };
     if (tiles) {
         fetch(0);

@@ -39,7 +39,8 @@ __device__ __forceinline__ float towards_one(float largest)
     return largest > 0.0f && largest < INFINITY ? ldexpf(1.0f, -ilogbf(largest)) : 1.0f;
 }
 
-// ---- queries fixed: 32 to a wave, tiles of kKeys keys ----
+// ---- queries fixed: 32 to a wave, tiles of kKeys keys.  Bound: the matrix units, busy 46 % of the cycles, between them the
+// exponentials that wait for the products (4 sequences of 1600 to 2047, 32 heads on 8 of 128, bfloat16: 239 us) ----
 template <typename T, int DP, int WAVES, int kKeys>
 __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
 {
@@ -141,30 +142,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
             *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + to) = next[1][i];
         }
     };
-    constexpr bool kAhead = DP == 128;
-    // S^T and dP^T of 32 keys; 128 channels: operands are read a group ahead, as in the forward
+    // S^T and dP^T of 32 keys
     auto pair_products = [&](const char* kt, const char* vt, int row0, f32x16& s, f32x16& dp) __attribute__((always_inline)) {
-        constexpr int kGroup = 1, kGroups = kSlices / kGroup;
-        Frag<T> kf[2][kGroup], vf[2][kGroup];
-        auto read = [&](int n) __attribute__((always_inline)) {
-#pragma unroll
-            for (int k = 0; k < kGroup; ++k) {
-                kf[n & 1][k] = rows.template get<T>(kt, row0, n * kGroup + k);
-                vf[n & 1][k] = rows.template get<T>(vt, row0, n * kGroup + k);
-            }
-            if (kAhead) __builtin_amdgcn_sched_barrier(0);
-        };
         s = zeros16(), dp = zeros16();
-        read(0);
 #pragma unroll
-        for (int n = 0; n < kGroups; ++n) {
-            if (n + 1 < kGroups) read(n + 1);
-#pragma unroll
-            for (int k = 0; k < kGroup; ++k) {
-                s = product(kf[n & 1][k], q[n * kGroup + k], s);
-                dp = product(vf[n & 1][k], g[n * kGroup + k], dp);
-            }
-            if (kAhead) __builtin_amdgcn_sched_barrier(0);
+        for (int k = 0; k < kSlices; ++k) {
+            s = product(rows.template get<T>(kt, row0, k), q[k], s);
+            dp = product(rows.template get<T>(vt, row0, k), g[k], dp);
         }
     };
     if (tiles) {
@@ -221,20 +205,14 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
                 s[i] *= __is_same(T, f16) ? lift * (dp[i] - delta) : dp[i] - delta;
                 if (kMend) short_of += s[i];
             }
-            Frag<T> f[2][kBlocks];
-            auto read = [&](int u) __attribute__((always_inline)) {
-#pragma unroll
-                for (int d = 0; d < kBlocks; ++d) f[u][d] = columns.template get<T>(kt, 32 * c + 16 * u, d);
-            };
-            read(0);
-            read(1);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const Frag<T> ds = rounded<T>(s, 8 * u);
 #pragma unroll
                 for (int d = 0; d < kBlocks; ++d) {
-                    dq[d] = product(f[u][d], ds, dq[d]);
-                    if (kMend) pk[d] = product(f[u][d], w[u], pk[d]);
+                    const Frag<T> f = columns.template get<T>(kt, 32 * c + 16 * u, d);
+                    dq[d] = product(f, ds, dq[d]);
+                    if (kMend) pk[d] = product(f, w[u], pk[d]);
                 }
             }
         }
@@ -252,7 +230,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
     if (query < at.nq) store_row<T, DP>(static_cast<T*>(p.dq) + place * p.dim, dq, p.scale / lift, p.dim, half);
 }
 
-// ---- keys fixed: 32 to a pair of waves, PAIRS pairs to a block; queries in steps of kQueries ----
+// ---- keys fixed: 32 to a pair of waves, PAIRS pairs to a block; queries in steps of kQueries.  Bound: as above, 44 % (the same
+// sequences: 325 us) ----
 template <typename T, int DP, int PAIRS, int kQueries>
 __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 {
@@ -322,43 +301,21 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
             s_delta[buffer][tid] = none ? 0.0f : next_delta;
         }
     };
-    constexpr bool kAhead = DP == 128;
-    // A tile's rows times the fixed operand, its parts of 32 rows side by side: products of one part wait for each other.  128
-    // channels: operands are read a group ahead, as in the forward.
+    // a tile's rows times the fixed operand, its parts of 32 rows side by side: products of one part wait for each other
     auto by_rows = [&](const char* tile, f32x16* x) __attribute__((always_inline)) {
-        constexpr int kGroup = 4 / kParts, kGroups = kSlices / kGroup;
-        Frag<T> f[2][kGroup][kParts];
-        auto read = [&](int n) __attribute__((always_inline)) {
-#pragma unroll
-            for (int k = 0; k < kGroup; ++k)
-#pragma unroll
-                for (int c = 0; c < kParts; ++c) f[n & 1][k][c] = rows.template get<T>(tile, 32 * c, n * kGroup + k);
-            if (kAhead) __builtin_amdgcn_sched_barrier(0);
-        };
 #pragma unroll
         for (int c = 0; c < kParts; ++c) x[c] = zeros16();
-        read(0);
 #pragma unroll
-        for (int n = 0; n < kGroups; ++n) {
-            if (n + 1 < kGroups) read(n + 1);
+        for (int k = 0; k < kSlices; ++k)
 #pragma unroll
-            for (int k = 0; k < kGroup; ++k)
-#pragma unroll
-                for (int c = 0; c < kParts; ++c) x[c] = product(f[n & 1][k][c], fixed[n * kGroup + k], x[c]);
-            if (kAhead) __builtin_amdgcn_sched_barrier(0);
-        }
+            for (int c = 0; c < kParts; ++c) x[c] = product(rows.template get<T>(tile, 32 * c, k), fixed[k], x[c]);
     };
     // adds the columns of 32 rows times the two operands
     auto by_columns = [&](const char* tile, int row0, const Frag<T>* w) __attribute__((always_inline)) {
-        Frag<T> f[2][kBlocks];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int d = 0; d < kBlocks; ++d) f[u][d] = columns.template get<T>(tile, row0 + 16 * u, d);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int d = 0; d < kBlocks; ++d) sums[d] = product(f[u][d], w[u], sums[d]);
+            for (int d = 0; d < kBlocks; ++d) sums[d] = product(columns.template get<T>(tile, row0 + 16 * u, d), w[u], sums[d]);
     };
     if (steps) {
         fetch(kv * group, 0);
