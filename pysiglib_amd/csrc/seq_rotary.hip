@@ -15,7 +15,7 @@ namespace seqamd {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kPieces = 512;      // of the tokens, for the gradients of the weights
+constexpr int kPieces = 1024;     // of the tokens at most, for the gradients of the weights
 
 struct RotaryArgs {
     const void *q, *k;            // [tokens][heads][dim], rows of a head contiguous
@@ -286,7 +286,9 @@ void launch(RotaryArgs& p, bool back, float* dqw, float* dkw, hipStream_t stream
         SIG_HIP(hipGetLastError());
         return;
     }
-    const int pieces = blocks < kPieces ? int(blocks) : kPieces;
+    // 32-bit loads fill the memory's queues with half the blocks, and fewer pieces are summed up sooner (8000 tokens, 20 heads of 128,
+    // float32: 46 us, with all pieces 49; 16384, 40 heads of 128, bfloat16: 99 us, with half of them 129)
+    const int most = sizeof(T) == 4 ? kPieces / 2 : kPieces, pieces = blocks < most ? int(blocks) : most;
     hipLaunchKernelGGL((backward_kernel<T, kUnit, G, NEAR>), dim3(pieces), dim3(kThreads), 0, stream, p);
     SIG_HIP(hipGetLastError());
     hipLaunchKernelGGL(weights_kernel, dim3((2 * p.dim + 3) / 4), dim3(kThreads), 0, stream, p.parts, pieces, p.dim, dqw, dkw);
