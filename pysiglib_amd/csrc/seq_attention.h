@@ -340,7 +340,6 @@ struct MapArgs {
     Tiling how[2];
     int* map[2];
     int room[2];             // tiles that a map holds: offsets that do not ascend could name more
-    unsigned* clear;         // a word to be cleared, or null
 };
 
 constexpr int kMapThreads = 1024;
@@ -352,8 +351,6 @@ static __global__ void __launch_bounds__(kMapThreads) map_kernel(MapArgs p)
     const Tiling how = blockIdx.x ? p.how[1] : p.how[0];
     int* const map = blockIdx.x ? p.map[1] : p.map[0];
     const int room = blockIdx.x ? p.room[1] : p.room[0];
-    if (p.clear && blockIdx.x == 0 && tid == 0) *p.clear = 0;
-    if (!map) return;
     int done = 0;
     for (int base = 0; base < p.packed.n; base += kMapThreads) {
         Span one{};

@@ -22,7 +22,6 @@ struct GradArgs {
     const float* lse;
     void *dq, *dk, *dv;                       // contiguous
     float* delta;                             // [q_rows][heads]
-    unsigned* largest;                        // float16: bits of the largest |grad|, zero at the start
     Packed packed, k_packed;                  // the second with the map of tiles of keys
     int64_t q_token, q_head, k_token, k_head, v_token, v_head, g_token, g_head;
     int heads, kv_heads, dim, causal;
@@ -33,10 +32,38 @@ constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kExact = 512;               // keys up to which delta is summed from its definition, 128 channels, causal
 constexpr float kRest = 1048576.0f;       // a weight's rounding error in float16, at most 2^-12, times this fits 8 bits (at most 448)
 
-// float16 holds dS only near 1: it is formed from gradients multiplied by a power of two that brings the largest there
-__device__ __forceinline__ float towards_one(float largest)
+// the power of two that brings a size near 1
+__device__ __forceinline__ float towards_one(float size)
 {
-    return largest > 0.0f && largest < INFINITY ? ldexpf(1.0f, -ilogbf(largest)) : 1.0f;
+    return size > 0.0f && size < INFINITY ? ldexpf(1.0f, min(-ilogbf(size), 126)) : 1.0f;
+}
+
+// float16 holds dS only near 1.  The dS of a lane's column go into their product multiplied by a power of two, of the lane's own,
+// that brought the largest so far near 1; one that is 2^10 times as large moves it, and what is summed up with it.  Smaller ones
+// lose bits only where they are small beside the largest of the same sum.
+struct Lift {
+    float times = 1.0f, most = 0.0f;          // most: of what it is good for
+};
+
+template <int BLOCKS>
+__device__ __forceinline__ void fit(Lift& lift, const f32x16& x, f32x16* sums)
+{
+    auto size = [&](int i) { return __builtin_fabsf(x[i]); };
+    float most = larger(size(0), size(1), size(2));
+#pragma unroll
+    for (int i = 3; i < 15; i += 2) most = larger(most, size(i), size(i + 1));
+    most = larger(most, size(15));
+    most = larger(most, swapped(most));
+    if (__any(most > lift.most)) {
+        const bool moves = most > lift.most;
+        const float times = moves ? towards_one(most) : lift.times, change = times / lift.times;
+        if (moves) lift.most = most < INFINITY ? 1024.0f / times : INFINITY;
+        lift.times = times;
+#pragma unroll
+        for (int d = 0; d < BLOCKS; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums[d][i] *= change;
+    }
 }
 
 // ---- queries fixed: 32 to a wave, tiles of kKeys keys.  Bound: the matrix units, busy 46 % of the cycles, between them the
@@ -87,12 +114,6 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
     if constexpr (__is_same(T, f16)) {
         largest = fmaxf(largest, swapped(largest));
         lift = towards_one(largest);
-        float most = largest;
-#pragma unroll
-        for (int m = 1; m < 32; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
-        // bits of positive numbers ascend like them; most waves find a larger one there and leave the address alone
-        if (lane == 0 && most < INFINITY && __float_as_uint(most) > __hip_atomic_load(p.largest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-            atomicMax(p.largest, __float_as_uint(most));
     }
     const float lse = p.lse[place] == -INFINITY ? INFINITY : p.lse[place] * kLog2e;
     const int last = p.causal && query + shift < at.nk - 1 ? query + shift : at.nk - 1;
@@ -266,8 +287,7 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d) sums[d] = zeros16();
     }
-    float lift = 1.0f;
-    if constexpr (__is_same(T, f16)) lift = towards_one(__uint_as_float(*p.largest));
+    Lift lift;
 
     u32x4 next[2][kLoads];
     float next_lse, next_delta;
@@ -368,8 +388,7 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
             by_rows(s_tiles[before][1], parts);
 #pragma unroll
             for (int c = 0; c < kParts; ++c) {
-                const f32x16& dp = parts[c];
-                Frag<T> ds[2];
+                f32x16& x = parts[c];
                 u32x4 rest;
                 if constexpr (kFiner) rest = s_weights[(step - 1) & 1][pair][c][2][lane];
 #pragma unroll
@@ -377,16 +396,22 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
                     const Frag<f16> w = __builtin_bit_cast(Frag<f16>, s_weights[(step - 1) & 1][pair][c][u][lane]);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float x = dp[8 * u + i] - s_delta[before][32 * c + row_in(8 * u + i, half)];
+                        x[8 * u + i] -= s_delta[before][32 * c + row_in(8 * u + i, half)];
                         if constexpr (kFiner) {
                             const int word = static_cast<int>(rest[2 * u + i / 4]);
                             const float r = i % 4 < 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(word, false)[i % 2] : __builtin_amdgcn_cvt_pk_f32_fp8(word, true)[i % 2];
-                            ds[u][i] = T(fmaf(r, 1.0f / kRest, static_cast<float>(w[i])) * (x * lift));
+                            x[8 * u + i] *= fmaf(r, 1.0f / kRest, static_cast<float>(w[i]));
                         } else {
-                            ds[u][i] = T(static_cast<float>(w[i]) * x);
+                            x[8 * u + i] *= static_cast<float>(w[i]);
                         }
                     }
                 }
+                if constexpr (kFiner) {
+                    fit<kBlocks>(lift, x, sums);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] *= lift.times;
+                }
+                const Frag<T> ds[2] = {rounded<T>(x, 0), rounded<T>(x, 8)};
                 by_columns(s_tiles[before][0], 32 * c, ds);
             }
         }
@@ -395,10 +420,8 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
         now = after;
     }
     if (key < at.nk)
-        store_row<T, DP>(static_cast<T*>(second ? p.dk : p.dv) + ((at.k0 + key) * p.kv_heads + kv) * p.dim, sums, second ? p.scale / lift : 1.0f, p.dim, half);
+        store_row<T, DP>(static_cast<T*>(second ? p.dk : p.dv) + ((at.k0 + key) * p.kv_heads + kv) * p.dim, sums, second ? p.scale / lift.times : 1.0f, p.dim, half);
 }
-
-constexpr uint64_t kHeadBytes = 256;
 
 // Blocks by the average length of the sequences, from times of whole calls (16 heads on 4 of 64 channels, 16000 tokens, and 32 on
 // 8 of 128, 8000 tokens).
@@ -428,7 +451,7 @@ Space space_of(int64_t q_rows, int64_t k_rows, int64_t n, int64_t heads, int64_t
     Space s;
     s.q_map = map_bytes(most_tiles(q_rows, n, 32 * b.waves), n);
     s.k_map = map_bytes(most_tiles(k_rows, n, 32 * b.pairs), n);
-    s.all = kHeadBytes + s.q_map + s.k_map + size_t(q_rows) * heads * sizeof(float);
+    s.all = s.q_map + s.k_map + size_t(q_rows) * heads * sizeof(float);
     return s;
 }
 
@@ -438,27 +461,23 @@ void backward(GradArgs& p, void* workspace, hipStream_t stream)
     const Blocks b = blocks_of(p.packed.q_rows, p.packed.k_rows, p.packed.n, p.dim);
     const Space space = space_of(p.packed.q_rows, p.packed.k_rows, p.packed.n, p.heads, p.dim);
     char* const at = static_cast<char*>(workspace);
-    p.largest = reinterpret_cast<unsigned*>(at);
-    p.delta = reinterpret_cast<float*>(at + kHeadBytes + space.q_map + space.k_map);
+    p.delta = reinterpret_cast<float*>(at + space.q_map + space.k_map);
     const int64_t q_blocks = most_tiles(p.packed.q_rows, p.packed.n, 32 * b.waves) * p.heads;
     const int64_t k_blocks = most_tiles(p.packed.k_rows, p.packed.n, 32 * b.pairs) * p.kv_heads;
     require(q_blocks < (int64_t(1) << 31) && k_blocks < (int64_t(1) << 31), "too many queries and heads");
     p.k_packed = p.packed;
-    if (space.q_map || __is_same(T, f16)) {
+    if (space.q_map) {
         MapArgs m{};
         m.packed = p.packed;
-        m.clear = p.largest;
-        if (space.q_map) {
-            m.how[0] = Tiling{false, 32 * b.waves, 1};
-            m.how[1] = Tiling{true, 32 * b.pairs, 1};
-            m.map[0] = reinterpret_cast<int*>(at + kHeadBytes);
-            m.map[1] = reinterpret_cast<int*>(at + kHeadBytes + space.q_map);
-            m.room[0] = int(most_tiles(p.packed.q_rows, p.packed.n, 32 * b.waves));
-            m.room[1] = int(most_tiles(p.packed.k_rows, p.packed.n, 32 * b.pairs));
-            p.packed.map = m.map[0];
-            p.k_packed.map = m.map[1];
-        }
-        hipLaunchKernelGGL(map_kernel, dim3(space.q_map ? 2 : 1), dim3(space.q_map ? kMapThreads : 64), 0, stream, m);
+        m.how[0] = Tiling{false, 32 * b.waves, 1};
+        m.how[1] = Tiling{true, 32 * b.pairs, 1};
+        m.map[0] = reinterpret_cast<int*>(at);
+        m.map[1] = reinterpret_cast<int*>(at + space.q_map);
+        m.room[0] = int(most_tiles(p.packed.q_rows, p.packed.n, 32 * b.waves));
+        m.room[1] = int(most_tiles(p.packed.k_rows, p.packed.n, 32 * b.pairs));
+        p.packed.map = m.map[0];
+        p.k_packed.map = m.map[1];
+        hipLaunchKernelGGL(map_kernel, dim3(2), dim3(kMapThreads), 0, stream, m);
         SIG_HIP(hipGetLastError());
     }
     if (q_blocks) {
@@ -487,7 +506,9 @@ extern "C" {
 
 __attribute__((visibility("default"))) uint64_t cusig_amd_attention_backprop_workspace(uint64_t q_rows, uint64_t k_rows, uint64_t sequences, uint64_t heads, uint64_t dim) noexcept
 {
-    return sequences ? space_of(int64_t(q_rows), int64_t(k_rows), int64_t(sequences), int64_t(heads), int64_t(dim)).all : kHeadBytes;
+    // never nothing: the workspace is a pointer in every call
+    const uint64_t bytes = sequences ? space_of(int64_t(q_rows), int64_t(k_rows), int64_t(sequences), int64_t(heads), int64_t(dim)).all : 0;
+    return bytes ? bytes : 256;
 }
 
 __attribute__((visibility("default"))) int cusig_amd_attention_backprop(

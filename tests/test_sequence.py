@@ -796,3 +796,42 @@ def test_the_entry_points_report_what_is_wrong(P):
     assert L.CUSIG_ATTENTION_WORKSPACE(100000, 100000, 100, 2, 1, 64) > 0
     assert L.CUSIG_ATTENTION(*many) == 2 and "workspace" in L.last_error_message()
     assert L.CUSIG_ATTENTION_WORKSPACE(4, 4, 0, 2, 1, 64) == 0 and L.CUSIG_ATTENTION_BACKPROP_WORKSPACE(4, 4, 0, 2, 64) > 0
+
+
+# ---- gradients of very different sizes in one call ----
+
+def gradients_of(P, q, k, v, g, lengths, causal):
+    starts = starts_of(lengths)
+    offsets = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    out, lse = P.attention(q, k, v, offsets, offsets, causal=causal)
+    got = P.attention_backprop(g, q, k, v, out, lse, offsets, offsets, causal=causal)
+    dim = q.shape[2]
+    want = attention_oracle(f64(q), f64(k), f64(v), lengths, starts, lengths, causal, dim ** -0.5, grad=f64(g))[0][2:]
+    return got, want
+
+
+def few_roundings(got, want, dtype, what):
+    """As in test_attention_gradients_are_off_by_few_roundings, of a part of the rows: their error in that of one rounding."""
+    once = f64(torch.tensor(want).to(dtype)) - want
+    off = f64(got) - want
+    assert np.linalg.norm(off) <= 1.65 * np.linalg.norm(once), (what, float(np.linalg.norm(off) / np.linalg.norm(once)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("small,large", [(0.1, 4000.0), (0.01, 400.0), (0.1, 8.0)])
+def test_attention_gradients_beside_much_larger_ones(P, dtype, dim, small, large):
+    """A sequence's gradients have the same error whatever the other sequences' are, and a key's whatever those of queries
+    that do not see it are."""
+    lengths, heads, kv = [300, 200, 300], 2, 1
+    starts = starts_of(lengths)
+    q, k, v, g = attention_inputs(dtype, 800, 800, heads, kv, dim, seed=dim)
+    g[:starts[1]] *= small
+    g[starts[1]:starts[2]] *= large
+    g[starts[2]:starts[2] + 40] *= large        # keys from 40 on are seen by queries of small gradients alone
+    g[starts[2] + 40:] *= small
+    got, want = gradients_of(P, q, k, v, g, lengths, True)
+    for name, x, w in zip(("dq", "dk", "dv"), got, want):
+        for rows in (slice(0, starts[1]), slice(starts[1], starts[2]), slice(starts[2] + 40, starts[3])):
+            few_roundings(x[rows], w[rows], dtype, (name, rows))
