@@ -38,9 +38,9 @@ __device__ __forceinline__ float towards_one(float size)
     return size > 0.0f && size < INFINITY ? ldexpf(1.0f, min(-ilogbf(size), 126)) : 1.0f;
 }
 
-// float16 holds dS only near 1.  The dS of a lane's column go into their product multiplied by a power of two, of the lane's own,
-// that brought the largest so far near 1; one that is 2^10 times as large moves it, and what is summed up with it.  Smaller ones
-// lose bits only where they are small beside the largest of the same sum.
+// float16 holds dS, as large as gradients times values, only near 1.  The dS of a lane's column go into their product multiplied by
+// a power of two, of the lane's own, that brought the largest so far near 1; one that is 2^10 times as large moves it, and what is
+// summed up with it.  Smaller ones lose bits only where they are small beside the largest of the same sum.
 struct Lift {
     float times = 1.0f, most = 0.0f;          // most: of what it is good for
 };
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
     const ColumnRead<DP> columns(lane);
     const int query = q_first + wave * 32 + (lane & 31), row = query < at.nq ? query : at.nq - 1;
     Frag<T> q[kSlices], g[kSlices];
-    float delta = 0.0f, largest = 0.0f;
+    float delta = 0.0f;
     {
         const T* from = static_cast<const T*>(p.q) + (at.q0 + row) * p.q_token + head * p.q_head;
         const T* grad = static_cast<const T*>(p.grad) + (at.q0 + row) * p.g_token + head * p.g_head;
@@ -101,20 +101,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
             g[k] = load_row<T>(grad, d, p.dim);
             const Frag<T> y = load_row<T>(out, d, p.dim);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = static_cast<float>(g[k][i]);
-                delta = fmaf(x, static_cast<float>(y[i]), delta);
-                if constexpr (__is_same(T, f16)) largest = fmaxf(largest, fabsf(x));
-            }
+            for (int i = 0; i < 8; ++i) delta = fmaf(static_cast<float>(g[k][i]), static_cast<float>(y[i]), delta);
         }
         delta += swapped(delta);
     }
     const int64_t place = (at.q0 + row) * p.heads + head;
-    float lift = 1.0f;
-    if constexpr (__is_same(T, f16)) {
-        largest = fmaxf(largest, swapped(largest));
-        lift = towards_one(largest);
-    }
+    Lift lift;
     const float lse = p.lse[place] == -INFINITY ? INFINITY : p.lse[place] * kLog2e;
     const int last = p.causal && query + shift < at.nk - 1 ? query + shift : at.nk - 1;
     // The output's rounding makes delta wrong by u |dO| |O|, which matters where few keys share the weight: dS, differences from
@@ -223,8 +215,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
             if (kMend) w[0] = rounded<T>(s, 0), w[1] = rounded<T>(s, 8);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[i] *= __is_same(T, f16) ? lift * (dp[i] - delta) : dp[i] - delta;
+                s[i] *= dp[i] - delta;
                 if (kMend) short_of += s[i];
+            }
+            if constexpr (__is_same(T, f16)) {
+                fit<kBlocks>(lift, s, dq);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] *= lift.times;
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -241,14 +238,15 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
     }
     if (kMend) {
         short_of += swapped(short_of);
-        delta += short_of / lift;
+        delta += short_of;
+        short_of *= lift.times;
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) dq[d][i] = fmaf(-short_of, pk[d][i], dq[d][i]);
     }
     if (query < at.nq && half == 0) p.delta[place] = delta;
-    if (query < at.nq) store_row<T, DP>(static_cast<T*>(p.dq) + place * p.dim, dq, p.scale / lift, p.dim, half);
+    if (query < at.nq) store_row<T, DP>(static_cast<T*>(p.dq) + place * p.dim, dq, p.scale / lift.times, p.dim, half);
 }
 
 // ---- keys fixed: 32 to a pair of waves, PAIRS pairs to a block; queries in steps of kQueries.  Bound: as above, 44 % (the same

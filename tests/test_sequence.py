@@ -835,3 +835,17 @@ def test_attention_gradients_beside_much_larger_ones(P, dtype, dim, small, large
     for name, x, w in zip(("dq", "dk", "dv"), got, want):
         for rows in (slice(0, starts[1]), slice(starts[1], starts[2]), slice(starts[2] + 40, starts[3])):
             few_roundings(x[rows], w[rows], dtype, (name, rows))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("v_size,g_size", [(30000.0, 1e-4), (1e-3, 1000.0)])
+def test_attention_gradients_where_values_are_large_or_small(P, dtype, dim, v_size, g_size):
+    """What float16 has to hold between the products is as large as gradients times values, not as the gradients."""
+    lengths, heads, kv = [300, 37], 2, 1
+    q, k, v, g = attention_inputs(dtype, 337, 337, heads, kv, dim, seed=dim + 1)
+    v = v.sign() * v_size if v_size > 1 else v * v_size
+    got, want = gradients_of(P, q, k, v, g * g_size, lengths, True)
+    for name, x, w in zip(("dq", "dk"), got, want):
+        few_roundings(x, w, dtype, name)
