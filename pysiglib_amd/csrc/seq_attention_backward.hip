@@ -9,9 +9,9 @@
 //
 // Keys fixed: a wave cannot hold sums, keys and values of 64 keys of 128 channels at once with two waves to a SIMD, so waves
 // work in pairs.  The first forms P of a tile of queries and adds to dV, the second, one tile behind, takes P from shared
-// memory, forms dS and adds to dK.  Operands are rounded to the inputs' type (P, dS), sums are 32-bit.  In shared memory P is a
-// float16 whatever that type: in [0, 1] these are eight times as fine as bfloat16 at the same size.  For float16 inputs that
-// rounding would weigh as much as dS's own; an 8-bit float of its error goes along.
+// memory, forms dS and adds to dK.  Operands are rounded to the inputs' type (P, dS), sums are 32-bit.  In shared memory P is the
+// upper three bytes of its 32-bit float: its whole range, so that keys with little weight beside another have dK as exact as
+// others, and 2^-15 of its size, an eighth of float16's rounding at the least, which dS gets next.
 #include "seq_attention.h"
 
 namespace seqamd {
@@ -30,7 +30,31 @@ struct GradArgs {
 
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kExact = 512;               // keys up to which delta is summed from its definition, 128 channels, causal
-constexpr float kRest = 1048576.0f;       // a weight's rounding error in float16, at most 2^-12, times this fits 8 bits (at most 448)
+
+// Weights between two waves: the upper halves of eight floats in four words, the bytes below these of four floats in one
+__device__ __forceinline__ u32x4 upper_halves(const f32x16& x, int first)
+{
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(__float_as_uint(x[first + 2 * i + 1]), __float_as_uint(x[first + 2 * i]), 0x07060302u);
+    return w;
+}
+
+__device__ __forceinline__ u32x4 third_bytes(const f32x16& x)
+{
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = __builtin_amdgcn_perm(__float_as_uint(x[4 * i + 1]), __float_as_uint(x[4 * i]), 0x0c0c0501u) |
+               __builtin_amdgcn_perm(__float_as_uint(x[4 * i + 3]), __float_as_uint(x[4 * i + 2]), 0x05010c0cu);
+    return w;
+}
+
+// the i-th of the eight
+__device__ __forceinline__ float weight_of(u32x4 upper, unsigned third, int i)
+{
+    return __uint_as_float(__builtin_amdgcn_perm(upper[i / 2], third, (i & 1 ? 0x07060000u : 0x05040000u) | unsigned(i & 3) << 8 | 0x0cu));
+}
 
 // the power of two that brings a size near 1
 __device__ __forceinline__ float towards_one(float size)
@@ -259,8 +283,7 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
     static_assert(kLoads * kThreads == kQueries * Tile<DP>::kChunks, "");
     __shared__ __attribute__((aligned(16))) char s_tiles[3][2][kTileBytes];
     __shared__ __attribute__((aligned(16))) float s_lse[3][kQueries], s_delta[3][kQueries];
-    constexpr bool kFiner = __is_same(T, f16);
-    __shared__ __attribute__((aligned(16))) u32x4 s_weights[2][PAIRS][kParts][kFiner ? 3 : 2][64];
+    __shared__ __attribute__((aligned(16))) u32x4 s_weights[2][PAIRS][kParts][3][64];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave % PAIRS;
     const bool second = wave >= PAIRS;
     const int kv = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
@@ -365,19 +388,9 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     w[u] = rounded<T>(s, 8 * u);
-                    s_weights[step & 1][pair][c][u][lane] = __builtin_bit_cast(u32x4, rounded<f16>(s, 8 * u));
+                    s_weights[step & 1][pair][c][u][lane] = upper_halves(s, 8 * u);
                 }
-                if constexpr (kFiner) {
-                    u32x4 rest;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float r[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) r[j] = (s[4 * i + j] - static_cast<float>(w[i / 2][i % 2 * 4 + j])) * kRest;
-                        rest[i] = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false), true);
-                    }
-                    s_weights[step & 1][pair][c][2][lane] = rest;
-                }
+                s_weights[step & 1][pair][c][2][lane] = third_bytes(s);
                 by_columns(s_tiles[now][1], 32 * c, w);
             }
         }
@@ -387,24 +400,17 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 #pragma unroll
             for (int c = 0; c < kParts; ++c) {
                 f32x16& x = parts[c];
-                u32x4 rest;
-                if constexpr (kFiner) rest = s_weights[(step - 1) & 1][pair][c][2][lane];
+                const u32x4 third = s_weights[(step - 1) & 1][pair][c][2][lane];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const Frag<f16> w = __builtin_bit_cast(Frag<f16>, s_weights[(step - 1) & 1][pair][c][u][lane]);
+                    const u32x4 upper = s_weights[(step - 1) & 1][pair][c][u][lane];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        x[8 * u + i] -= s_delta[before][32 * c + row_in(8 * u + i, half)];
-                        if constexpr (kFiner) {
-                            const int word = static_cast<int>(rest[2 * u + i / 4]);
-                            const float r = i % 4 < 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(word, false)[i % 2] : __builtin_amdgcn_cvt_pk_f32_fp8(word, true)[i % 2];
-                            x[8 * u + i] *= fmaf(r, 1.0f / kRest, static_cast<float>(w[i]));
-                        } else {
-                            x[8 * u + i] *= static_cast<float>(w[i]);
-                        }
+                        const float d = x[8 * u + i] - s_delta[before][32 * c + row_in(8 * u + i, half)];
+                        x[8 * u + i] = weight_of(upper, third[2 * u + i / 4], i) * d;
                     }
                 }
-                if constexpr (kFiner) {
+                if constexpr (__is_same(T, f16)) {
                     fit<kBlocks>(lift, x, sums);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) x[i] *= lift.times;

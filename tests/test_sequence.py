@@ -849,3 +849,20 @@ def test_attention_gradients_where_values_are_large_or_small(P, dtype, dim, v_si
     got, want = gradients_of(P, q, k, v, g * g_size, lengths, True)
     for name, x, w in zip(("dq", "dk"), got, want):
         few_roundings(x, w, dtype, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim,causal", [(64, True), (64, False), (128, False)])
+@pytest.mark.parametrize("ahead", [8.0, 16.0, 24.0, 40.0])
+def test_attention_gradients_of_keys_with_little_weight(P, dtype, dim, causal, ahead):
+    """One key takes nearly all the weight of each query: the others' gradients are small, and as exact as the type holds
+    them."""
+    q, k, v, g = attention_inputs(dtype, 600, 600, 2, 1, dim, seed=int(ahead))
+    q *= 0.3
+    k *= 0.3
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    k[0, :, 0] = ahead * dim ** 0.5 / 8.0
+    got, want = gradients_of(P, q, k, v, g * 256.0, [600], causal)
+    few_roundings(got[1][1:], want[1][1:], dtype, "dk")
