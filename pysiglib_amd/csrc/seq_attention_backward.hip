@@ -62,9 +62,9 @@ __device__ __forceinline__ float towards_one(float size)
     return size > 0.0f && size < INFINITY ? ldexpf(1.0f, min(-ilogbf(size), 126)) : 1.0f;
 }
 
-// float16 holds dS, as large as gradients times values, only near 1.  The dS of a lane's column go into their product multiplied by
-// a power of two, of the lane's own, that brought the largest so far near 1; one that is 2^10 times as large moves it, and what is
-// summed up with it.  Smaller ones lose bits only where they are small beside the largest of the same sum.
+// float16 holds dS, as large as gradients times values, only near 1, and P only down to 2^-24.  Those of a lane's column go into their
+// product multiplied by a power of two, of the lane's own, that brought the largest so far near 1; one that is 2^10 times as large
+// moves it, and what is summed up with it.  Smaller ones lose bits only where they are small beside the largest of the same sum.
 struct Lift {
     float times = 1.0f, most = 0.0f;          // most: of what it is good for
 };
@@ -384,13 +384,15 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
                         if (key > q0 + 32 * c + row_in(i, half) + shift) s[i] = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -s_lse[now][32 * c + row_in(i, half)]));
-                Frag<T> w[2];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    w[u] = rounded<T>(s, 8 * u);
-                    s_weights[step & 1][pair][c][u][lane] = upper_halves(s, 8 * u);
-                }
+                for (int u = 0; u < 2; ++u) s_weights[step & 1][pair][c][u][lane] = upper_halves(s, 8 * u);
                 s_weights[step & 1][pair][c][2][lane] = third_bytes(s);
+                if constexpr (__is_same(T, f16)) {
+                    fit<kBlocks>(lift, s, sums);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] *= lift.times;
+                }
+                const Frag<T> w[2] = {rounded<T>(s, 0), rounded<T>(s, 8)};
                 by_columns(s_tiles[now][1], 32 * c, w);
             }
         }
@@ -424,7 +426,7 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
         now = after;
     }
     if (key < at.nk)
-        store_row<T, DP>(static_cast<T*>(second ? p.dk : p.dv) + ((at.k0 + key) * p.kv_heads + kv) * p.dim, sums, second ? p.scale / lift.times : 1.0f, p.dim, half);
+        store_row<T, DP>(static_cast<T*>(second ? p.dk : p.dv) + ((at.k0 + key) * p.kv_heads + kv) * p.dim, sums, (second ? p.scale : 1.0f) / lift.times, p.dim, half);
 }
 
 // Blocks by the average length of the sequences, from times of whole calls (16 heads on 4 of 64 channels, 16000 tokens, and 32 on
