@@ -153,8 +153,9 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
             for (int j = 0; j < 4; ++j) part[j] = larger(larger(part[j], s[1][j + 4], s[1][j + 8]), s[1][j + 12]);
         float most = larger(larger(part[0], part[1], part[2]), part[3]);
         most = larger(most, swapped(most)) * p.scale;
-        if (__any(most > top + kSlack || (top == -INFINITY && most > top))) {
-            const float now = fmaxf(top, most), shrink = top == now ? 1.0f : exp2f(top - now);
+        const bool grows = most > top + kSlack || (top == -INFINITY && most > top);
+        if (__any(grows)) {             // each query by itself: its roundings are no matter of the others'
+            const float now = grows ? most : top, shrink = top == now ? 1.0f : exp2f(top - now);
             top = now;
             sum *= shrink;
 #pragma unroll
@@ -307,8 +308,9 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
         for (int i = 3; i < 15; i += 2) most = larger(most, s[i], s[i + 1]);
         most = larger(most, s[15]);
         most = larger(most, swapped(most)) * p.scale;
-        if (__any(most > top + kSlack || (top == -INFINITY && most > top))) {
-            const float now = fmaxf(top, most), shrink = top == now ? 1.0f : exp2f(top - now);
+        const bool grows = most > top + kSlack || (top == -INFINITY && most > top);
+        if (__any(grows)) {             // each query by itself: its roundings are no matter of the others'
+            const float now = grows ? most : top, shrink = top == now ? 1.0f : exp2f(top - now);
             top = now;
             sum *= shrink;
 #pragma unroll

@@ -90,6 +90,22 @@ __device__ __forceinline__ void fit(Lift& lift, const f32x16& x, f32x16* sums)
     }
 }
 
+// A weight times what it weighs: zero where it has no weight, also of what is not finite (v_mul_legacy_f32)
+extern "C" __device__ __attribute__((const)) float weighed(float weight, float x) __asm("llvm.amdgcn.fmul.legacy");
+
+// Operands that are not finite, of keys that a query does not see or queries that do not see a key: neither a weight of zero nor dS,
+// set to zero there, makes zero with them in the second product.  They are taken out of the tiles that hide some from others, and put
+// back at the end into the sums that they belong to.  P knows of them all the same: by the log-sum of a query that is or sees such a
+// one, which is not finite then, unless the key's score was -infinity: P is set to zero there.  Where they are multiplied with dS, which
+// they make zero or not finite, it is not a number that they leave.
+template <typename T>
+__device__ __attribute__((noinline)) void spoil(const T* row, T* to, int dim, int half)
+{
+#pragma unroll 1
+    for (int ch = 4 * half; ch < dim; ch += (ch & 3) == 3 ? 5 : 1)
+        if (!__builtin_isfinite(static_cast<float>(row[ch]))) to[ch] = T(__builtin_nanf(""));
+}
+
 // ---- queries fixed: 32 to a wave, tiles of kKeys keys.  Bound: the matrix units, busy 46 % of the cycles, between them the
 // exponentials that wait for the products (4 sequences of 1600 to 2047, 32 heads on 8 of 128, bfloat16: 239 us) ----
 template <typename T, int DP, int WAVES, int kKeys>
@@ -98,8 +114,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
     constexpr int kThreads = WAVES * 64, kRows = 32 * WAVES, kSlices = DP / 16, kBlocks = DP / 32;
     constexpr int kTileBytes = kKeys * Tile<DP>::kRowBytes, kLoads = kKeys * Tile<DP>::kChunks / kThreads;
     static_assert(kLoads * kThreads == kKeys * Tile<DP>::kChunks, "");
+    static_assert(kKeys == 32, "");
     __shared__ __attribute__((aligned(16))) char s_tiles[2][2][kTileBytes];
+    constexpr int kHiding = kRows / kKeys + 2;          // tiles that hide keys from some queries of the block, at most
+    __shared__ unsigned s_bad[kHiding], s_any;          // their keys that are not finite, and whether there are any
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (tid < kHiding) s_bad[tid] = 0;
+    if (tid == 0) s_any = 0;
     const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
     const Span at = find_tile(p.packed, Tiling{false, kRows, 1}, blockIdx.x / p.heads, Dear::kLast);
     if (at.seq < 0) return;
@@ -171,12 +192,24 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
             next[1][i] = load_at(vp, v_at[i]);
         }
     };
-    auto put = [&](int buffer) __attribute__((always_inline)) {
+    const int hiding = min(at.nk, p.causal ? max(q_first + shift + 1, 0) : at.nk) / kKeys;       // the first tile that hides a key from a query
+    auto put = [&](int buffer, int tile) __attribute__((always_inline)) {
+        auto place = [&](int i) { return Tile<DP>::at((i * kThreads + tid) / Tile<DP>::kChunks, (i * kThreads + tid) % Tile<DP>::kChunks); };
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int e = i * kThreads + tid, to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
-            *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + to) = next[0][i];
-            *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + to) = next[1][i];
+        for (int i = 0; i < kLoads; ++i) *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + place(i)) = next[1][i];
+        if (tile >= hiding) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                u32x4 x = next[0][i];
+                if (take_them_out<T>(x)) {
+                    atomicOr(&s_bad[tile - hiding], 1u << (i * kThreads + tid) / Tile<DP>::kChunks);
+                    s_any = 1;
+                }
+                *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + place(i)) = x;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + place(i)) = next[0][i];
         }
     };
     // S^T and dP^T of 32 keys
@@ -190,35 +223,42 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
     };
     if (tiles) {
         fetch(0);
-        put(0);
+        if (hiding == 0) __syncthreads();       // s_bad is clear
+        put(0, 0);
     }
 #pragma unroll
     for (int k = 0; k < kSlices; ++k) {
         arrive<T>(q[k]);
         arrive<T>(g[k]);
     }
-    auto hide = [&](f32x16& s, int key0) __attribute__((always_inline)) {
-        if (key0 + 32 > at.nk || (p.causal && key0 + 31 > q_first + wave * 32 + shift))
+    auto hides = [&](int key0) { return key0 + 32 > at.nk || (p.causal && key0 + 31 > q_first + wave * 32 + shift); };
+    // P of 32 keys from their S; hidden ones have none, and no dP
+    auto weigh = [&](f32x16& s, f32x16& dp, int tile) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (key0 + row_in(i, half) > last) s[i] = -INFINITY;
+        for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -lse));
+        if (hides(tile * kKeys)) {
+            const unsigned bad = s_bad[tile - hiding] >> 4 * half;
+            const int past = last - tile * kKeys - 4 * half;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (row_in(i, 0) > past) s[i] = dp[i] = 0.0f;
+                if ((bad >> row_in(i, 0) & 1) != 0 && s[i] == s[i]) s[i] = 0.0f;
+            }
+        }
     };
     int buffer = 0;
     if (!kMend && keys <= exact && tiles) {       // first to sum P dP, which is delta
         float sum = 0.0f;
         for (int tile = 0; tile < tiles; ++tile, buffer ^= 1) {
             __syncthreads();
-            fetch(tile + 1 < tiles ? tile + 1 : 0);
-#pragma unroll 1
-            for (int c = 0; c < kKeys / 32; ++c) {
-                const int key0 = tile * kKeys + 32 * c;
-                f32x16 s, dp;
-                pair_products(s_tiles[buffer][0], s_tiles[buffer][1], 32 * c, s, dp);
-                hide(s, key0);
+            const int after = tile + 1 < tiles ? tile + 1 : 0;
+            fetch(after);
+            f32x16 s, dp;
+            pair_products(s_tiles[buffer][0], s_tiles[buffer][1], 0, s, dp);
+            weigh(s, dp, tile);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -lse)), dp[i], sum);
-            }
-            put(buffer ^ 1);
+            for (int i = 0; i < 16; ++i) sum = fmaf(s[i], dp[i], sum);
+            put(buffer ^ 1, after);
         }
         delta = sum + swapped(sum);
     }
@@ -226,15 +266,11 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
         __syncthreads();
         if (tile + 1 < tiles) fetch(tile + 1);
         const char *kt = s_tiles[buffer][0], *vt = s_tiles[buffer][1];
-#pragma unroll
-        for (int c = 0; c < kKeys / 32; ++c) {
-            const int key0 = tile * kKeys + 32 * c;
-            if (p.causal && key0 > q_first + wave * 32 + 31 + shift) continue;       // none of the wave's queries sees these
+        const int key0 = tile * kKeys;
+        if (!p.causal || key0 <= q_first + wave * 32 + 31 + shift) {        // otherwise none of the wave's queries sees these
             f32x16 s, dp;
-            pair_products(kt, vt, 32 * c, s, dp);
-            hide(s, key0);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -lse));
+            pair_products(kt, vt, 0, s, dp);
+            weigh(s, dp, tile);
             Frag<T> w[2];
             if (kMend) w[0] = rounded<T>(s, 0), w[1] = rounded<T>(s, 8);
 #pragma unroll
@@ -252,13 +288,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
                 const Frag<T> ds = rounded<T>(s, 8 * u);
 #pragma unroll
                 for (int d = 0; d < kBlocks; ++d) {
-                    const Frag<T> f = columns.template get<T>(kt, 32 * c + 16 * u, d);
+                    const Frag<T> f = columns.template get<T>(kt, 16 * u, d);
                     dq[d] = product(f, ds, dq[d]);
                     if (kMend) pk[d] = product(f, w[u], pk[d]);
                 }
             }
         }
-        if (tile + 1 < tiles) put(buffer ^ 1);
+        if (tile + 1 < tiles) put(buffer ^ 1, tile + 1);
     }
     if (kMend) {
         short_of += swapped(short_of);
@@ -269,8 +305,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
 #pragma unroll
             for (int i = 0; i < 16; ++i) dq[d][i] = fmaf(-short_of, pk[d][i], dq[d][i]);
     }
-    if (query < at.nq && half == 0) p.delta[place] = delta;
-    if (query < at.nq) store_row<T, DP>(static_cast<T*>(p.dq) + place * p.dim, dq, p.scale / lift.times, p.dim, half);
+    if (query >= at.nq) return;
+    if (half == 0) p.delta[place] = delta;
+    T* const to = static_cast<T*>(p.dq) + place * p.dim;
+    store_row<T, DP>(to, dq, p.scale / lift.times, p.dim, half);
+    if (__builtin_expect(s_any != 0, 0))
+        for (int k = hiding * kKeys; k <= last; ++k) spoil(static_cast<const T*>(p.k) + (at.k0 + k) * p.k_token + kv * p.k_head, to, p.dim, half);
 }
 
 // ---- keys fixed: 32 to a pair of waves, PAIRS pairs to a block; queries in steps of kQueries.  Bound: as above, 44 % (the same
@@ -284,8 +324,10 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
     __shared__ __attribute__((aligned(16))) char s_tiles[3][2][kTileBytes];
     __shared__ __attribute__((aligned(16))) float s_lse[3][kQueries], s_delta[3][kQueries];
     __shared__ __attribute__((aligned(16))) u32x4 s_weights[2][PAIRS][kParts][3][64];
+    __shared__ unsigned s_any;          // whether operands that are not finite were taken out
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave % PAIRS;
     const bool second = wave >= PAIRS;
+    if (tid == 0) s_any = 0;
     const int kv = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
     const Span at = find_tile(p.k_packed, Tiling{true, kRows, 1}, blockIdx.x / p.kv_heads, Dear::kFirst);
     if (at.seq < 0) return;
@@ -312,7 +354,9 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 
     u32x4 next[2][kLoads];
     float next_lse, next_delta;
-    bool next_in;
+    bool next_in, next_hides;
+    // queries up to `seen` and of the tiles that begin before it: some of them do not see some of the block's keys
+    const int seen = p.causal ? k_first + kRows - 1 - shift : 0;
     auto fetch = [&](int head, int tile) __attribute__((always_inline)) {
         const int q0 = q_begin + tile * kQueries, left = at.nq - q0 - 1;
         const char* qp = reinterpret_cast<const char*>(static_cast<const T*>(p.q) + (at.q0 + q0) * p.q_token + head * p.q_head);
@@ -328,13 +372,26 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
         next_lse = p.lse[first + place];
         next_delta = p.delta[first + place];
         next_in = mine <= left;
+        next_hides = q0 < seen;
     };
     auto put = [&](int buffer) __attribute__((always_inline)) {
+        auto place = [&](int i) { return Tile<DP>::at((i * kThreads + tid) / Tile<DP>::kChunks, (i * kThreads + tid) % Tile<DP>::kChunks); };
+        if (next_hides) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int e = i * kThreads + tid, to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
-            *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + to) = next[0][i];
-            *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + to) = next[1][i];
+            for (int i = 0; i < kLoads; ++i) {
+                u32x4 x = next[0][i], y = next[1][i];
+                // a query that is not finite has a log-sum that is not either, and P from that
+                const bool one = take_them_out<T>(x), two = take_them_out<T>(y);
+                if (one || two) s_any = 1;
+                *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + place(i)) = x;
+                *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + place(i)) = y;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + place(i)) = next[0][i];
+                *reinterpret_cast<u32x4*>(s_tiles[buffer][1] + place(i)) = next[1][i];
+            }
         }
         if (tid < kQueries) {           // queries past the end, and those that see nothing, have no weights
             const bool none = !next_in || next_lse == -INFINITY;
@@ -358,8 +415,16 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 #pragma unroll
             for (int d = 0; d < kBlocks; ++d) sums[d] = product(columns.template get<T>(tile, row0 + 16 * u, d), w[u], sums[d]);
     };
+    // nothing of the 32 queries from q0 on that do not see the key
+    auto hide = [&](f32x16& x, int q0) __attribute__((always_inline)) {
+        if (p.causal && q0 + shift < key0 + 31)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (key > q0 + row_in(i, half) + shift) x[i] = 0.0f;
+    };
     if (steps) {
         fetch(kv * group, 0);
+        __syncthreads();                // s_any is clear
         put(0);
     }
 #pragma unroll
@@ -378,12 +443,9 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 #pragma unroll
             for (int c = 0; c < kParts; ++c) {
                 f32x16& s = parts[c];
-                if (p.causal && q0 + 32 * c + shift < key0 + 31)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (key > q0 + 32 * c + row_in(i, half) + shift) s[i] = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -s_lse[now][32 * c + row_in(i, half)]));
+                hide(s, q0 + 32 * c);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) s_weights[step & 1][pair][c][u][lane] = upper_halves(s, 8 * u);
                 s_weights[step & 1][pair][c][2][lane] = third_bytes(s);
@@ -409,7 +471,7 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float d = x[8 * u + i] - s_delta[before][32 * c + row_in(8 * u + i, half)];
-                        x[8 * u + i] = weight_of(upper, third[2 * u + i / 4], i) * d;
+                        x[8 * u + i] = weighed(weight_of(upper, third[2 * u + i / 4], i), d);
                     }
                 }
                 if constexpr (__is_same(T, f16)) {
@@ -425,8 +487,15 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
         before = now;
         now = after;
     }
-    if (key < at.nk)
-        store_row<T, DP>(static_cast<T*>(second ? p.dk : p.dv) + ((at.k0 + key) * p.kv_heads + kv) * p.dim, sums, (second ? p.scale : 1.0f) / lift.times, p.dim, half);
+    if (key >= at.nk) return;
+    T* const to = static_cast<T*>(second ? p.dk : p.dv) + ((at.k0 + key) * p.kv_heads + kv) * p.dim;
+    store_row<T, DP>(to, sums, (second ? p.scale : 1.0f) / lift.times, p.dim, half);
+    if (__builtin_expect(steps != 0 && s_any != 0, 0))
+        for (int h = kv * group; h < (kv + 1) * group; ++h)
+            for (int i = max(key - shift, 0); i < min(seen + kQueries, at.nq); ++i) {
+                if (second) spoil(static_cast<const T*>(p.q) + (at.q0 + i) * p.q_token + h * p.q_head, to, p.dim, half);
+                else add_them(static_cast<const T*>(p.grad) + (at.q0 + i) * p.g_token + h * p.g_head, to, p.dim, half);
+            }
 }
 
 // Blocks by the average length of the sequences, from times of whole calls (16 heads on 4 of 64 channels, 16000 tokens, and 32 on

@@ -868,3 +868,56 @@ def test_attention_gradients_of_keys_with_little_weight(P, dtype, dim, causal, a
     got, want = gradients_of(P, q, k, v, g * 256.0, [600], causal)
     which = ("dq", "dk", "dv").index(name)
     few_roundings(got[which][1:], want[which][1:], dtype, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("lengths,heads,kv,dim", [([100, 40], 4, 2, 64), ([150], 2, 1, 128), ([90, 5, 33], 2, 2, 40), ([33] * 70, 1, 1, 64),
+                                                  ([1500, 40], 1, 1, 96)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("which", ["q", "k", "v", "grad"])
+@pytest.mark.parametrize("first", [False, True])
+def test_attention_gradients_of_what_is_not_finite(P, dtype, lengths, heads, kv, dim, bad, which, first):
+    """One element that is not finite reaches what the formula sums it into, over the visible pairs, and nothing else."""
+    starts = starts_of(lengths)
+    offsets = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    tensors = dict(zip(("q", "k", "v", "grad"), attention_inputs(dtype, starts[-1], starts[-1], heads, kv, dim, seed=dim)))
+
+    def gradients():
+        q, k, v, g = (tensors[n] for n in ("q", "k", "v", "grad"))
+        out, lse = P.attention(q, k, v, offsets, offsets)
+        return P.attention_backprop(g, q, k, v, out, lse, offsets, offsets)
+
+    clean = [f64(t) for t in gradients()]
+    n = 0
+    t, ch = 0 if first else lengths[0] // 2, 3
+    row = starts[n] + t
+    tensors[which][row, 0, ch] = bad
+    got = [f64(x) for x in gradients()]
+    q, k, v, g = (f64(tensors[x])[starts[n]:starts[n + 1]] for x in ("q", "k", "v", "grad"))
+    # sums over visible pairs alone, of the head that has it
+    m, scale = lengths[n], dim ** -0.5
+    want = [np.zeros((m, dim)) for _ in range(3)]
+    K, V, Q, G = k[:, 0], v[:, 0], q[:, 0], g[:, 0]
+    with np.errstate(all="ignore"):
+        for i in range(m):
+            s = K[:i + 1] @ Q[i] * scale
+            # scores of -infinity alone are those of a query that sees nothing: no weights
+            p = np.zeros(i + 1) if (s == -np.inf).all() else np.exp(s - s.max()) / np.exp(s - s.max()).sum()
+            out = (p[:, None] * V[:i + 1]).sum(0)
+            ds = p * ((V[:i + 1] * G[i]).sum(1) - (G[i] * out).sum())
+            want[0][i] = (ds[:, None] * K[:i + 1]).sum(0)
+            want[1][:i + 1] += ds[:, None] * Q[i]
+            want[2][:i + 1] += p[:, None] * G[i]
+    group = heads // kv
+    for name, x, c, w in zip(("dq", "dk", "dv"), got, clean, want):
+        fine = np.isfinite(w)
+        here = x[starts[n]:starts[n + 1], 0]
+        assert (np.isfinite(here) == fine).all(), (name, np.argwhere(np.isfinite(here) != fine)[:5])
+        # what lies before (queries) or behind (keys) the element's token has nothing to do with it
+        apart = slice(0, t) if name == "dq" else slice(t + 1, m)
+        if which in ("q", "grad") or name == "dq":
+            assert (here[apart] == c[starts[n]:starts[n + 1], 0][apart]).all(), name
+        assert (x[starts[1]:] == c[starts[1]:]).all(), name
+        others = slice(group if name == "dq" and which in ("k", "v") else 1, None)
+        assert (x[:, others] == c[:, others]).all(), name
