@@ -303,7 +303,7 @@ void by_lanes(RotaryArgs& p, bool back, float* dqw, float* dkw, hipStream_t stre
     case 8: return launch<T, 8, NEAR>(p, back, dqw, dkw, stream);
     case 16: return launch<T, 16, NEAR>(p, back, dqw, dkw, stream);
     case 32: return launch<T, 32, NEAR>(p, back, dqw, dkw, stream);
-    default: throw std::invalid_argument("heads of more than 256 channels are not supported");
+    default: return launch<T, 64, NEAR>(p, back, dqw, dkw, stream);       // 252 channels and more whose two parts both end inside a lane's
     }
 }
 

@@ -921,3 +921,11 @@ def test_attention_gradients_of_what_is_not_finite(P, dtype, lengths, heads, kv,
         assert (x[starts[1]:] == c[starts[1]:]).all(), name
         others = slice(group if name == "dq" and which in ("k", "v") else 1, None)
         assert (x[:, others] == c[:, others]).all(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,rotary", [(256, 100), (256, 250), (254, 4), (252, 2), (254, 254)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_norm_rotary_of_the_widest_heads(P, dtype, dim, rotary, interleaved):
+    test_norm_rotary(P, dtype, 5, 3, 2, dim, rotary, interleaved)
