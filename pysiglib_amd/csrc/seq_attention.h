@@ -220,8 +220,6 @@ struct Span {
     int tile, seq;       // tile among the sequence's; seq < 0: none
 };
 
-__device__ __forceinline__ int64_t kept(int64_t x, int64_t low, int64_t high) { return x < low ? low : (x > high ? high : x); }
-
 __device__ __forceinline__ void span_of(const Packed& p, int seq, Span& s)
 {
     s.seq = seq;

@@ -70,6 +70,13 @@ __device__ __forceinline__ float chain(float a1, float a2) { return a1 == 0.0f |
 // The hardware's exponential of the scaled argument: off by |g| 2^-24 of its size from the scaling and one rounding
 __device__ __forceinline__ float decay(float g) { return __builtin_amdgcn_exp2f(g * 1.44269504088896341f); }
 
+// The rows [first, past) of a packed sequence, kept inside the tensors whatever the offsets hold
+__device__ __forceinline__ void rows_of(const int* offsets, int64_t i, int64_t rows, int64_t& first, int64_t& past)
+{
+    first = kept(offsets[i], 0, rows);
+    past = kept(offsets[i + 1], first, rows);
+}
+
 // Rows [t0, t0 + ROWS) of the packed rows: at[r] = the sequence that begins (forward) or ends (backward) at row t0 + r,
 // ends[r] = the sequence that ends (forward) or begins (backward) there, -1: none.  Returns whether there is any.
 template <int ROWS, bool BACK>
@@ -102,11 +109,10 @@ __device__ bool find_edges(const ScanArgs& p, int64_t t0, int* at, int* ends)
             lo = 0;
         for (int64_t base = lo; base < p.n; base += kThreads) {
             const int64_t i = base + tid;
-            int64_t first = t0 + ROWS;
+            int64_t first = t0 + ROWS, past;
             if (i < p.n) {
-                first = p.offsets[i];
-                const int64_t past = p.offsets[i + 1];
-                if (first >= 0 && past > first && past <= p.rows) mark(i, first, past - 1);
+                rows_of(p.offsets, i, p.rows, first, past);
+                if (past > first) mark(i, first, past - 1);
             }
             if (__syncthreads_and(first >= t0 + ROWS)) break;
         }
@@ -145,6 +151,12 @@ __global__ void __launch_bounds__(kThreads, PART ? 1 : (BACK || R > 16 ? 3 : 4))
     // first row in memory of the chunk; mirrored, chunk 0 holds the last rows
     const int64_t t0 = BACK ? p.rows - int64_t(chunk + 1) * kRows : int64_t(chunk) * kRows;
     auto row_of = [&](int r) { return BACK ? t0 + kRows - 1 - r : t0 + r; };
+    // rows of sequences: those before and behind them are not written
+    int first_row = 0, past_row = int(p.rows);
+    if (p.offsets) {
+        first_row = __builtin_amdgcn_readfirstlane(int(kept(p.offsets[0], 0, p.rows)));
+        past_row = __builtin_amdgcn_readfirstlane(int(kept(p.offsets[p.n], first_row, p.rows)));
+    }
 
     P gate[R], in[R], prev[BACK ? R : 1];
     const bool whole = t0 >= (BACK ? 1 : 0) && t0 + kRows <= p.rows;
@@ -286,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, PART ? 1 : (BACK || R > 16 ? 3 : 4))
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t t = row_of(group * R + r);
-            if (!kAll && (t < 0 || t >= p.rows)) continue;
+            if (!kAll && (t < first_row || t >= past_row)) continue;
             int last = -1;
             if (edges) {
                 const int seq = at_of(group * R + r);
@@ -322,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, PART ? 1 : (BACK || R > 16 ? 3 : 4))
                     if (v < count) p.end[int64_t(last) * p.channels + ch0 + v] = state[v];
         }
     };
-    if (whole && !PART) walk(std::true_type{});
+    if (whole && !PART && t0 >= first_row && t0 + kRows <= past_row) walk(std::true_type{});
     else walk(std::false_type{});
 }
 
@@ -344,9 +356,8 @@ __global__ void __launch_bounds__(kThreads, 2) column_kernel(ScanArgs p)
     const int seq = id / p.channel_blocks, cb = id % p.channel_blocks;
     int64_t begin = int64_t(seq) * p.length, rows = p.length;
     if (p.offsets) {
-        begin = p.offsets[seq];
-        rows = p.offsets[seq + 1] - begin;
-        if (begin < 0 || begin + rows > p.rows) rows = 0;
+        rows_of(p.offsets, seq, p.rows, begin, rows);
+        rows -= begin;
     }
     begin = __builtin_amdgcn_readfirstlane(int(begin));
     rows = __builtin_amdgcn_readfirstlane(int(rows));
@@ -504,7 +515,9 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(unsigned long long* w
     if (offsets || length == 0)
         for (int64_t i = first; i < n * channels; i += step) {
             const int64_t s = i / channels;
-            if (length == 0 || offsets[s] >= offsets[s + 1]) end[i] = begin ? begin[i] : 0.0f;
+            int64_t first = 0, past = length;
+            if (offsets) rows_of(offsets, s, rows, first, past);
+            if (first == past) end[i] = begin ? begin[i] : 0.0f;
         }
 }
 

@@ -7,7 +7,9 @@ enqueued on the current stream of the tensors' device and not waited for; scratc
 may have gaps between their rows (parts of one projection, say); only the last axis has to be contiguous, others are copied.
 
 Sequences of different lengths are packed behind each other, with ``offsets`` (int32, on the GPU): sequence ``i`` has the rows
-``offsets[i]`` to ``offsets[i + 1]``; the offsets ascend from 0 to the number of rows.  They are not read on the host.
+``offsets[i]`` to ``offsets[i + 1]``; the offsets ascend, usually from 0 to the number of rows.  They are not read on the host.
+Where there are rows before the first or behind the last of them, outputs and gradients hold no values there; offsets that leave
+the tensors are cut to them.
 """
 import math
 

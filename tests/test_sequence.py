@@ -929,3 +929,48 @@ def test_attention_gradients_of_what_is_not_finite(P, dtype, lengths, heads, kv,
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_norm_rotary_of_the_widest_heads(P, dtype, dim, rotary, interleaved):
     test_norm_rotary(P, dtype, 5, 3, 2, dim, rotary, interleaved)
+
+
+# ---- rows that belong to no sequence, offsets that leave the tensors ----
+
+def whole_numbers(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def raw(fn, *args):
+    """A C entry point on the current stream, tensors as their addresses."""
+    code = fn(*(a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args), torch.cuda.current_stream().cuda_stream)
+    assert code == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels", [(300, 24), (5000, 24), (5000, 3), (9000, 70)])
+@pytest.mark.parametrize("offsets,cut", [([7, 100, 100, 290], None), ([-5, 100, 290], [0, 100, 290]), ([20, 100, 1 << 30], [20, 100, -1]),
+                                         ([-9, -7, 60, 1 << 30, (1 << 30) + 5], [0, 0, 60, -1, -1])])
+def test_recurrence_leaves_other_rows_alone(P, dtype, rows, channels, offsets, cut):
+    """Straight calls on buffers that hold a mark: rows of no sequence keep it, sequences are cut to the rows there are, and
+    every sequence has a state behind it.  Short calls walk sequences, long ones publish: both alike."""
+    from pysiglib_amd import _loader as L
+    offsets, n = ([x if x > 1 << 20 or x < 0 else x * rows // 300 for x in offsets]), len(offsets) - 1
+    cut = [rows if x == -1 else x * rows // 300 for x in cut] if cut else offsets
+    x, g, h0, grad, gf = (t.to(DEV) for t in recurrence_inputs(dtype, rows, channels, n, seed=rows))
+    code = L.SEQUENCE_DTYPES[str(dtype).split(".")[1]]
+    size = L.CUSIG_LINEAR_RECURRENCE_WORKSPACE(code, rows, n, channels)
+    space = torch.zeros(max(size, 1), dtype=torch.uint8, device=DEV)
+    marked = lambda shape, t=dtype: torch.full(shape, 77.0, dtype=t, device=DEV)       # noqa: E731
+    h, final = marked(x.shape), marked(h0.shape, torch.float32)
+    at = whole_numbers(offsets)
+    raw(L.CUSIG_LINEAR_RECURRENCE, code, x, g, h0, h, final, at, n, 0, rows, channels, channels, channels, space, size)
+    dx, dg, d0 = marked(x.shape), marked(x.shape), marked(h0.shape, torch.float32)
+    raw(L.CUSIG_LINEAR_RECURRENCE_BACKPROP, code, h, g, grad, gf, h0, dx, dg, d0, at, n, 0, rows, channels, channels, channels, space, size)
+    first, past = cut[0], cut[-1]
+    part = slice(first, past)
+    inside = [c - first for c in cut]
+    want, bound = recurrence_oracle(f64(x)[part], f64(g)[part], f64(h0), inside, f64(grad)[part], f64(gf), f64(h)[part])
+    for name, got, w, b in zip(("h", "final", "dx", "dg", "d0"), (h, final, dx, dg, d0), want, bound):
+        mine = got[part] if name in ("h", "dx", "dg") else got
+        u, tiny = (ROUND[dtype], SMALL[dtype]) if name in ("h", "dx", "dg") else (U32, SMALL[torch.float32])
+        within(mine, w, b + u * (np.abs(w) + b) + tiny, name)
+        if name in ("h", "dx", "dg"):
+            assert (got[:first] == 77.0).all() and (got[past:] == 77.0).all(), name
