@@ -412,7 +412,9 @@ __global__ void __launch_bounds__(256) join_kernel(AttentionArgs p)
 {
     const int64_t all = p.packed.q_rows * p.heads, row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    if (row >= all) return;
+    // rows before the first sequence and behind the last have no parts
+    const int64_t first_row = kept(p.packed.q_offsets[0], 0, p.packed.q_rows), past_row = kept(p.packed.q_offsets[p.packed.n], first_row, p.packed.q_rows);
+    if (row < first_row * p.heads || row >= past_row * p.heads) return;
     float most = -INFINITY;
     for (int s = lane; s < p.splits; s += 64) most = fmaxf(most, p.parts[2 * (s * all + row)]);
 #pragma unroll

@@ -974,3 +974,30 @@ def test_recurrence_leaves_other_rows_alone(P, dtype, rows, channels, offsets, c
         within(mine, w, b + u * (np.abs(w) + b) + tiny, name)
         if name in ("h", "dx", "dg"):
             assert (got[:first] == 77.0).all() and (got[past:] == 77.0).all(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("room", [40, 3000])
+@pytest.mark.parametrize("n", [2, 70])
+def test_attention_leaves_other_rows_alone(P, dtype, room, n):
+    """Rows of queries before the first sequence and behind the last keep what they held, with the keys in one piece and
+    in several."""
+    from pysiglib_amd import _loader as L
+    heads, kv, dim, before, behind = 4, 2, 64, 3, 6
+    q_rows, k_rows = before + n + behind, n * room
+    q, k, v, _ = attention_inputs(dtype, q_rows, k_rows, heads, kv, dim, seed=room)
+    out = torch.full(q.shape, 77.0, dtype=dtype, device=DEV)
+    lse = torch.full(q.shape[:2], 77.0, dtype=torch.float32, device=DEV)
+    sizes = (q_rows, k_rows, n, heads, kv, dim)
+    size = L.CUSIG_ATTENTION_WORKSPACE(*sizes)
+    space = torch.full((max(size, 4),), 255, dtype=torch.uint8, device=DEV)          # no number anywhere
+    at, places = whole_numbers(range(before, before + n + 1)), whole_numbers([i * room for i in range(n + 1)])
+    raw(L.CUSIG_ATTENTION, L.SEQUENCE_DTYPES[str(dtype).split(".")[1]], q, k, v, at, places, 0, out, lse, *sizes, heads * dim, dim, kv * dim, dim,
+        kv * dim, dim, dim ** -0.5, True, space, size)
+    mine = slice(before, before + n)
+    want, _ = P.attention(q[mine], k, v, at - before, places)
+    bound = 4 * ROUND[dtype] * f64(v).max()         # cut in ranges differently: weights rounded at other maxima
+    assert np.abs(f64(out[mine]) - f64(want)).max() <= bound
+    for t in (out, lse):
+        assert (t[:before] == 77.0).all() and (t[before + n:] == 77.0).all()
