@@ -435,10 +435,11 @@ __global__ void __launch_bounds__(256) join_kernel(AttentionArgs p)
         for (int s = 0; s < count; s += 8)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float ws = __shfl(w, s + j);              // zero past the last split
+                const float ws = __shfl(w, s + j);
                 const Pack<float, 2> v = load_pack<float, 2>(from + min(first + s + j, p.splits - 1) * all * p.dim);
-                x[0] = fmaf(ws, v.get(0), x[0]);
-                x[1] = fmaf(ws, v.get(1), x[1]);
+                const bool there = s + j < count;               // the last split's values in the place of those past it may be infinite
+                x[0] = there ? fmaf(ws, v.get(0), x[0]) : x[0];
+                x[1] = there ? fmaf(ws, v.get(1), x[1]) : x[1];
             }
     }
 #pragma unroll

@@ -1001,3 +1001,18 @@ def test_attention_leaves_other_rows_alone(P, dtype, room, n):
     assert np.abs(f64(out[mine]) - f64(want)).max() <= bound
     for t in (out, lse):
         assert (t[:before] == 77.0).all() and (t[before + n:] == 77.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("keys", [700, 2560, 3000, 6000])
+def test_an_infinite_value_stays_infinite_over_ranges_of_keys(P, dtype, keys):
+    """Keys cut in any number of ranges: an infinite value in the last one gives infinity, as in one piece."""
+    q, k, v, _ = attention_inputs(dtype, 1, keys, 1, 1, 64, seed=keys)
+    clean, _ = P.attention(q, k, v, whole_numbers([0, 1]), whole_numbers([0, keys]))
+    v[keys - 1, 0, 5], v[keys - 1, 0, 6], v[0, 0, 7] = float("inf"), -float("inf"), float("inf")
+    out, lse = P.attention(q, k, v, whole_numbers([0, 1]), whole_numbers([0, keys]))
+    got = f64(out)[0, 0]
+    assert got[5] == np.inf and got[6] == -np.inf and got[7] == np.inf
+    same = [c for c in range(64) if c not in (5, 6, 7)]
+    assert (got[same] == f64(clean)[0, 0, same]).all()
