@@ -397,7 +397,8 @@ CUSIG_AMD_API int cusig_amd_norm_rotary_backprop(int dtype, const void* grad_q, 
 /* Softmax attention over packed sequences, bfloat16 or float16: q [q_rows, heads, dim], k and v [k_rows, kv_heads, dim]; heads / kv_heads
  * neighbouring heads share keys and values; dim a multiple of 8 up to 128.  causal: query j of n sees the keys up to j + m - n of
  * m.  k_lengths (may be null): keys in use from each sequence's first on, as in a cache.  out [q_rows, heads, dim] and lse float32
- * [q_rows, heads] (the logarithm of the sum of exponentials), contiguous; 0 and -infinity where a query sees no key. */
+ * [q_rows, heads] (the logarithm of the sum of exponentials), contiguous; 0 and -infinity where a query sees no key.  Tokens are less
+ * than 2^23 elements apart. */
 CUSIG_AMD_API int cusig_amd_attention(int dtype, const void* q, const void* k, const void* v, const int* q_offsets,
                                       const int* k_offsets, const int* k_lengths, void* out, float* lse, uint64_t q_rows,
                                       uint64_t k_rows, uint64_t sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim,

@@ -223,12 +223,19 @@ def rotary_tables(length, rotary_dim, *, base=10000., scale=1., device="cuda"):
     return angle.cos().float(), angle.sin().float()
 
 
-def _heads(x, name, like, rows=None, dim=None):
-    """(tokens, heads, dim) whose last axis is contiguous, and the distances of its tokens and heads."""
+_APART = 1 << 23        # tokens of the attention are nearer than that: its kernels' offsets inside a tile are 32-bit
+
+
+def _heads(x, name, like, rows=None, dim=None, apart=None):
+    """(tokens, heads, dim) whose last axis is contiguous, and the distances of its tokens and heads; tokens that are ``apart``
+    or further are copied."""
     _tensor(x, name, 3, like)
     if (rows is not None and x.shape[0] != rows) or (dim is not None and x.shape[2] != dim):
         raise ValueError(name + " must have shape (" + str(rows) + ", heads, " + str(dim) + "), got " + str(tuple(x.shape)))
-    if x.stride(2) != 1 and x.shape[2] > 1:
+    if x.shape[0] <= 1:         # no next token: what the stride says has no meaning
+        x = x if x.stride(2) == 1 or x.shape[2] <= 1 else x.contiguous()
+        return x, x.shape[1] * x.shape[2], x.stride(1)
+    if (x.stride(2) != 1 and x.shape[2] > 1) or (apart is not None and x.stride(0) >= apart):
         x = x.contiguous()
     return x, x.stride(0), x.stride(1)
 
@@ -296,12 +303,12 @@ def norm_rotary_backprop(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin, pos
 
 def _attention_args(q, k, v, q_offsets, k_offsets, causal, scale):
     check_type(causal, "causal", bool)
-    q, q_token, q_head = _heads(q, "q", None)
+    q, q_token, q_head = _heads(q, "q", None, apart=_APART)
     if q.dtype == torch.float32:
         raise TypeError("q.dtype must be bfloat16 or float16, got torch.float32 instead")
     dim, device = q.shape[2], q.device
-    k, k_token, k_head = _heads(k, "k", q, None, dim)
-    v, v_token, v_head = _heads(v, "v", q, k.shape[0], dim)
+    k, k_token, k_head = _heads(k, "k", q, None, dim, _APART)
+    v, v_token, v_head = _heads(v, "v", q, k.shape[0], dim, _APART)
     heads, kv_heads = q.shape[1], k.shape[1]
     if v.shape[1] != kv_heads:
         raise ValueError("k and v must have the same heads")
@@ -351,7 +358,7 @@ def attention_backprop(grad_out, q, k, v, out, lse, q_offsets, k_offsets, *, cau
     outputs.  Returns ``(grad_q, grad_k, grad_v)``; the same inputs give the same bits."""
     q, k, v, q_offsets, k_offsets, sizes, rest = _attention_args(q, k, v, q_offsets, k_offsets, causal, scale)
     device, dtype = q.device, q.dtype
-    grad_out, g_token, g_head = _heads(grad_out, "grad_out", q, q.shape[0], q.shape[2])
+    grad_out, g_token, g_head = _heads(grad_out, "grad_out", q, q.shape[0], q.shape[2], _APART)
     if grad_out.shape != q.shape:
         raise ValueError("grad_out must have the shape of q")
     out = _other(out, "out", dtype, q.shape, device)

@@ -1016,3 +1016,27 @@ def test_an_infinite_value_stays_infinite_over_ranges_of_keys(P, dtype, keys):
     assert got[5] == np.inf and got[6] == -np.inf and got[7] == np.inf
     same = [c for c in range(64) if c not in (5, 6, 7)]
     assert (got[same] == f64(clean)[0, 0, same]).all()
+
+
+# ---- rows far apart, many blocks ----
+
+@pytest.mark.gpu
+def test_attention_of_tokens_far_apart(P):
+    """The last tokens of long sequences side by side: tokens 2^24 elements apart."""
+    n, length, heads, dim = 3, 4096, 32, 128
+    rows = torch.randn((n, length, heads, dim), device=DEV).to(torch.bfloat16)
+    last = rows[:, -1]
+    at = whole_numbers(range(n + 1))
+    dense = last.contiguous()
+    assert last.stride(0) == 1 << 24
+    for args in [(last, dense, dense), (dense, last, last), (last, last, last)]:
+        for got, want in zip(P.attention(*args, at, at), P.attention(dense, dense, dense, at, at)):
+            assert torch.equal(got, want)
+    out, lse = P.attention(dense, dense, dense, at, at)
+    for got, want in zip(P.attention_backprop(last, last, last, last, out, lse, at, at), P.attention_backprop(dense, dense, dense, dense, out, lse, at, at)):
+        assert torch.equal(got, want)
+    one = whole_numbers([0, 1])
+    single = rows[1:2, -1]                 # a single token: the distance to the next has no meaning
+    assert torch.equal(P.attention(single, single, single, one, one)[0], single)
+    out, lse = P.attention(single, single, single, one, one)
+    assert P.attention_backprop(single, single, single, single, out, lse, one, one)[0].shape == single.shape
