@@ -88,7 +88,7 @@ def _rows(x):
     shape = x.shape
     if x.is_contiguous():
         return x, shape[-1]
-    if x.stride(-1) == 1 or shape[-1] <= 1:
+    if (x.stride(-1) == 1 or shape[-1] <= 1) and x.stride(-2) <= 1 << 20:       # the scan's offsets inside a chunk are 32-bit
         step = x.stride(-2)
         want = step
         for axis in range(x.dim() - 2, -1, -1):

@@ -1040,3 +1040,22 @@ def test_attention_of_tokens_far_apart(P):
     assert torch.equal(P.attention(single, single, single, one, one)[0], single)
     out, lse = P.attention(single, single, single, one, one)
     assert P.attention_backprop(single, single, single, single, out, lse, one, one)[0].shape == single.shape
+
+
+@pytest.mark.gpu
+def test_recurrence_of_rows_far_apart(P):
+    """A few channels of very long rows."""
+    wide = torch.randn((12, (1 << 20) + 8), device=DEV).to(torch.bfloat16)
+    x, g, grad = wide[:, :16], -wide[:, 16:32].abs(), wide[:, 32:48]
+    far = torch.empty_like(wide)
+    far[:, :16] = g
+    g = far[:, :16]
+    assert min(t.stride(0) for t in (x, g, grad)) > 1 << 20
+    dense = [t.contiguous() for t in (x, g, grad)]
+    at = whole_numbers([0, 5, 12])
+    got, want = P.linear_recurrence(x, g, offsets=at), P.linear_recurrence(*dense[:2], offsets=at)
+    back, same = P.linear_recurrence_backprop(want[0], g, grad, offsets=at), P.linear_recurrence_backprop(want[0], *dense[1:], offsets=at)
+    for a, b in zip((*got, *back), (*want, *same)):
+        assert torch.equal(a, b)
+    state = torch.zeros((12, 16), device=DEV)
+    assert torch.equal(P.linear_recurrence_step(x, g, state), dense[0])
