@@ -27,6 +27,7 @@ struct AttentionArgs {
     float* parts;            // of the splits
     int heads, kv_heads, dim, causal, splits;
     float scale;             // times log2(e)
+    unsigned first_block;    // of a launch
 };
 
 constexpr float kSlack = 8.0f;   // the maximum is taken over where it grew by more than this (in powers of two): weights stay below 2^8
@@ -46,9 +47,10 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
         for (unsigned& bad : s_bad[tid]) bad = 0;
     if (tid == 0) s_any = 0;
     // the heads that share keys and values follow each other at a distance of kv_heads: on the same die where that is a multiple of 8
-    const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
+    const unsigned block = p.first_block + blockIdx.x;
+    const int turn = block % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
     // the last tiles see the most keys: they begin first
-    const Span at = find_tile(p.packed, Tiling{false, kRows, 1}, blockIdx.x / p.heads, Dear::kLast);
+    const Span at = find_tile(p.packed, Tiling{false, kRows, 1}, block / p.heads, Dear::kLast);
     if (at.seq < 0) return;
     const int q_first = at.tile * kRows, shift = at.nk - at.nq;
     // keys that any query of the block sees
@@ -229,8 +231,9 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
     __shared__ float s_top[kWaves][32], s_sum[kWaves][32];
     __shared__ unsigned s_bad[4], s_any;     // of the tiles that hide keys from some of the pairs: keys whose values are not finite
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int group = p.heads / p.kv_heads, kv = blockIdx.x % p.kv_heads, split = blockIdx.x / p.kv_heads % p.splits;
-    const Span at = find_tile(p.packed, Tiling{false, 32, group}, blockIdx.x / p.kv_heads / p.splits, Dear::kLast);
+    const unsigned block = p.first_block + blockIdx.x;
+    const int group = p.heads / p.kv_heads, kv = block % p.kv_heads, split = block / p.kv_heads % p.splits;
+    const Span at = find_tile(p.packed, Tiling{false, 32, group}, block / p.kv_heads / p.splits, Dear::kLast);
     if (at.seq < 0) return;
     const int pairs = at.nq * group, shift = at.nk - at.nq, pair = at.tile * 32 + (lane & 31);
     const int own = pair < pairs ? pair : pairs - 1, query = own / group, head = kv * group + own % group;
@@ -410,7 +413,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(AttentionArgs p)
 {
-    const int64_t all = p.packed.q_rows * p.heads, row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t all = p.packed.q_rows * p.heads, row = (int64_t(p.first_block) + blockIdx.x) * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     // rows before the first sequence and behind the last have no parts
     const int64_t first_row = kept(p.packed.q_offsets[0], 0, p.packed.q_rows), past_row = kept(p.packed.q_offsets[p.packed.n], first_row, p.packed.q_rows);
@@ -496,23 +499,17 @@ void forward(const AttentionArgs& p, const Cut& cut, hipStream_t stream)
     if (cut.few) {
         const int64_t blocks = cut.tiles * p.kv_heads * p.splits, rows = p.packed.q_rows * p.heads;
         require(blocks < (int64_t(1) << 31) && rows < (int64_t(1) << 32), "too many queries and heads");
-        hipLaunchKernelGGL((few_kernel<T, DP>), dim3(unsigned(blocks)), dim3(256), 0, stream, p);
-        SIG_HIP(hipGetLastError());
-        if (p.splits > 1) {
-            hipLaunchKernelGGL((join_kernel<T>), dim3(unsigned((rows + 3) / 4)), dim3(256), 0, stream, p);
-            SIG_HIP(hipGetLastError());
-        }
+        launch_all(few_kernel<T, DP>, blocks, 256, stream, p);
+        if (p.splits > 1) launch_all(join_kernel<T>, (rows + 3) / 4, 256, stream, p);
         return;
     }
     const int64_t blocks = cut.tiles * p.heads;
     require(blocks < (int64_t(1) << 31), "too many queries and heads");
-    const dim3 grid(static_cast<unsigned>(blocks));
     switch (cut.waves) {
-    case 2: hipLaunchKernelGGL((attention_kernel<T, DP, 2, 32>), grid, dim3(128), 0, stream, p); break;
-    case 4: hipLaunchKernelGGL((attention_kernel<T, 128, 4, 64>), grid, dim3(256), 0, stream, p); break;
-    default: hipLaunchKernelGGL((attention_kernel<T, DP, 8, 64>), grid, dim3(512), 0, stream, p); break;
+    case 2: return launch_all(attention_kernel<T, DP, 2, 32>, blocks, 128, stream, p);
+    case 4: return launch_all(attention_kernel<T, 128, 4, 64>, blocks, 256, stream, p);
+    default: return launch_all(attention_kernel<T, DP, 8, 64>, blocks, 512, stream, p);
     }
-    SIG_HIP(hipGetLastError());
 }
 
 }  // namespace

@@ -26,6 +26,7 @@ struct GradArgs {
     int64_t q_token, q_head, k_token, k_head, v_token, v_head, g_token, g_head;
     int heads, kv_heads, dim, causal;
     float scale, scale2;                      // scale2 = scale * log2(e)
+    unsigned first_block;                     // of a launch
 };
 
 constexpr float kLog2e = 1.44269504088896341f;
@@ -121,8 +122,9 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (tid < kHiding) s_bad[tid] = 0;
     if (tid == 0) s_any = 0;
-    const int turn = blockIdx.x % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
-    const Span at = find_tile(p.packed, Tiling{false, kRows, 1}, blockIdx.x / p.heads, Dear::kLast);
+    const unsigned block = p.first_block + blockIdx.x;
+    const int turn = block % p.heads, head = (turn % p.kv_heads) * (p.heads / p.kv_heads) + turn / p.kv_heads, kv = turn % p.kv_heads;
+    const Span at = find_tile(p.packed, Tiling{false, kRows, 1}, block / p.heads, Dear::kLast);
     if (at.seq < 0) return;
     const int q_first = at.tile * kRows, shift = at.nk - at.nq;
     const int q_past = q_first + kRows < at.nq ? q_first + kRows : at.nq;
@@ -328,8 +330,9 @@ __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6), pair = wave % PAIRS;
     const bool second = wave >= PAIRS;
     if (tid == 0) s_any = 0;
-    const int kv = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
-    const Span at = find_tile(p.k_packed, Tiling{true, kRows, 1}, blockIdx.x / p.kv_heads, Dear::kFirst);
+    const unsigned block = p.first_block + blockIdx.x;
+    const int kv = block % p.kv_heads, group = p.heads / p.kv_heads;
+    const Span at = find_tile(p.k_packed, Tiling{true, kRows, 1}, block / p.kv_heads, Dear::kFirst);
     if (at.seq < 0) return;
     const int k_first = at.tile * kRows, shift = at.nk - at.nq;
     // the first query that sees any of the block's keys
@@ -555,21 +558,13 @@ void backward(GradArgs& p, void* workspace, hipStream_t stream)
         hipLaunchKernelGGL(map_kernel, dim3(2), dim3(kMapThreads), 0, stream, m);
         SIG_HIP(hipGetLastError());
     }
-    if (q_blocks) {
-        const dim3 grid(static_cast<unsigned>(q_blocks));
-        switch (b.waves) {
-        case 2: hipLaunchKernelGGL((dq_kernel<T, DP, 2, 32>), grid, dim3(128), 0, stream, p); break;
-        case 4: hipLaunchKernelGGL((dq_kernel<T, DP, 4, 32>), grid, dim3(256), 0, stream, p); break;
-        default: hipLaunchKernelGGL((dq_kernel<T, 128, 8, 32>), grid, dim3(512), 0, stream, p); break;
-        }
-        SIG_HIP(hipGetLastError());
+    switch (b.waves) {
+    case 2: launch_all(dq_kernel<T, DP, 2, 32>, q_blocks, 128, stream, p); break;
+    case 4: launch_all(dq_kernel<T, DP, 4, 32>, q_blocks, 256, stream, p); break;
+    default: launch_all(dq_kernel<T, 128, 8, 32>, q_blocks, 512, stream, p); break;
     }
-    if (k_blocks) {
-        const dim3 grid(static_cast<unsigned>(k_blocks));
-        if (b.queries == 32) hipLaunchKernelGGL((dkv_kernel<T, DP, 2, 32>), grid, dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL((dkv_kernel<T, DP, DP == 64 ? 2 : 4, 64>), grid, dim3(DP == 64 ? 256 : 512), 0, stream, p);
-        SIG_HIP(hipGetLastError());
-    }
+    if (b.queries == 32) launch_all(dkv_kernel<T, DP, 2, 32>, k_blocks, 256, stream, p);
+    else launch_all(dkv_kernel<T, DP, DP == 64 ? 2 : 4, 64>, k_blocks, DP == 64 ? 256 : 512, stream, p);
 }
 
 }  // namespace

@@ -115,6 +115,27 @@ inline void require(bool ok, const char* what)
     if (!ok) throw std::invalid_argument(what);
 }
 
+// A launch numbers its threads with 32 bits: more blocks go in several, each of which tells its kernel what its first one is.
+// Multiples of eight: a block stays on its die.
+template <typename Launch>
+void in_launches(int64_t blocks, int threads, Launch&& launch)
+{
+    const int64_t most = ((int64_t(1) << 32) / threads - 1) / 8 * 8;
+    for (int64_t first = 0; first < blocks; first += most) {
+        launch(unsigned(first), dim3(static_cast<unsigned>(blocks - first < most ? blocks - first : most)));
+        SIG_HIP(hipGetLastError());
+    }
+}
+
+template <typename Args>
+void launch_all(void (*kernel)(Args), int64_t blocks, int threads, hipStream_t stream, Args p)
+{
+    in_launches(blocks, threads, [&](unsigned first, dim3 grid) {
+        p.first_block = first;
+        hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, p);
+    });
+}
+
 // calls body(T{}) with the element type of `dtype`
 template <typename F>
 void with_type(int dtype, F&& body)

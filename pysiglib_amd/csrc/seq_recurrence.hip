@@ -38,6 +38,7 @@ struct ScanArgs {
     int64_t length, n;
     int channels, channel_blocks, chunks;
     bool past;               // results go past the caches
+    unsigned first_block;    // of a launch
 };
 
 // A chunk's word for a channel: B in the low half, A in the high half with its sign bit set (A is a product of
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, PART ? 1 : (BACK || R > 16 ? 3 : 4))
     const int tid = threadIdx.x, lane = tid % LC, group = tid / LC;
     // The chunks of a channel block are counted by a number of its own: 2048 blocks on a single one took 18 ns each, one after
     // the other, a third of the call.
-    const int cb = blockIdx.x % p.channel_blocks;
+    const int cb = (p.first_block + blockIdx.x) % p.channel_blocks;
     if (tid == 0) s_ticket = atomicAdd(p.ticket + cb * kTicketStep, 1u);
     __syncthreads();
     const int chunk = s_ticket;
@@ -351,8 +352,8 @@ __global__ void __launch_bounds__(kThreads, 2) column_kernel(ScanArgs p)
     // Blocks go around the eight dies: each die takes neighbouring channel blocks, which share cache lines, a sequence's all together (37
     // of up to 1500 steps, 997 channels, float16, gradients: 90 us, an eighth of every sequence to a die 97, the longest first
     // besides 82; but of equal lengths 68, 84 and 86).
-    const unsigned all = unsigned(p.n) * unsigned(p.channel_blocks), die = blockIdx.x % 8, each = all / 8, more = all % 8;
-    const unsigned id = die * each + min(die, more) + blockIdx.x / 8;
+    const unsigned all = unsigned(p.n) * unsigned(p.channel_blocks), block = p.first_block + blockIdx.x, die = block % 8, each = all / 8, more = all % 8;
+    const unsigned id = die * each + min(die, more) + block / 8;
     const int seq = id / p.channel_blocks, cb = id % p.channel_blocks;
     int64_t begin = int64_t(seq) * p.length, rows = p.length;
     if (p.offsets) {
@@ -522,9 +523,10 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(unsigned long long* w
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) step_kernel(const T* x, const T* gate, float* state, T* out, int64_t n, int channels, int64_t x_stride, int64_t gate_stride, int packs)
+__global__ void __launch_bounds__(kThreads) step_kernel(const T* x, const T* gate, float* state, T* out, int64_t n, int channels, int64_t x_stride, int64_t gate_stride, int packs,
+                                                        unsigned first_block)
 {
-    const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+    const int64_t i = (int64_t(first_block) + blockIdx.x) * kThreads + threadIdx.x;
     if (i >= n * packs) return;
     const int64_t row = i / packs;
     const int ch = int(i - row * packs) * V, count = channels - ch > V ? V : channels - ch;
@@ -607,11 +609,8 @@ void scan(ScanArgs p, void* workspace, size_t bytes, hipStream_t stream)
     p.past = goes_past(uint64_t(p.rows) * p.channels * sizeof(T) * (BACK ? 2 : 1), uint64_t(p.channels) * sizeof(T));
     if (plan.columns) {
         require(p.n * p.channel_blocks < (int64_t(1) << 31), "too many sequences and channels");
-        const dim3 grid(unsigned(p.n) * unsigned(p.channel_blocks));
-        if (p.rows <= 128 * p.n) hipLaunchKernelGGL((column_kernel<T, S::V, 4, S::kNarrow, BACK>), grid, dim3(kThreads), 0, stream, p);
-        else hipLaunchKernelGGL((column_kernel<T, S::V, BACK ? 4 : 8, S::kNarrow, BACK>), grid, dim3(kThreads), 0, stream, p);
-        SIG_HIP(hipGetLastError());
-        return;
+        if (p.rows <= 128 * p.n) return launch_all(column_kernel<T, S::V, 4, S::kNarrow, BACK>, p.n * p.channel_blocks, kThreads, stream, p);
+        return launch_all(column_kernel<T, S::V, BACK ? 4 : 8, S::kNarrow, BACK>, p.n * p.channel_blocks, kThreads, stream, p);
     }
     p.ticket = static_cast<unsigned*>(workspace);
     p.words = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + ticket_bytes(plan));
@@ -622,12 +621,11 @@ void scan(ScanArgs p, void* workspace, size_t bytes, hipStream_t stream)
                        p.offsets, p.n, p.length, p.rows, p.channels);
     SIG_HIP(hipGetLastError());
     if (p.rows == 0) return;
-    const dim3 grid(unsigned(plan.chunks) * unsigned(plan.channel_blocks));
-    if (p.channels < S::V) hipLaunchKernelGGL((scan_kernel<T, S::V, S::kFew, S::kNarrow, BACK, true, false>), grid, dim3(kThreads), 0, stream, p);
-    else if (plan.lanes == S::kWide && p.past) hipLaunchKernelGGL((scan_kernel<T, S::V, BACK ? S::kBackward : S::kForward, S::kWide, BACK, false, true>), grid, dim3(kThreads), 0, stream, p);
-    else if (plan.lanes == S::kWide) hipLaunchKernelGGL((scan_kernel<T, S::V, BACK ? S::kBackward : S::kForward, S::kWide, BACK, false, false>), grid, dim3(kThreads), 0, stream, p);
-    else hipLaunchKernelGGL((scan_kernel<T, S::V, S::kFew, S::kNarrow, BACK, false, false>), grid, dim3(kThreads), 0, stream, p);
-    SIG_HIP(hipGetLastError());
+    const int64_t grid = int64_t(plan.chunks) * plan.channel_blocks;
+    if (p.channels < S::V) launch_all(scan_kernel<T, S::V, S::kFew, S::kNarrow, BACK, true, false>, grid, kThreads, stream, p);
+    else if (plan.lanes == S::kWide && p.past) launch_all(scan_kernel<T, S::V, BACK ? S::kBackward : S::kForward, S::kWide, BACK, false, true>, grid, kThreads, stream, p);
+    else if (plan.lanes == S::kWide) launch_all(scan_kernel<T, S::V, BACK ? S::kBackward : S::kForward, S::kWide, BACK, false, false>, grid, kThreads, stream, p);
+    else launch_all(scan_kernel<T, S::V, S::kFew, S::kNarrow, BACK, false, false>, grid, kThreads, stream, p);
 }
 
 void check_scan(uint64_t rows, uint64_t channels, uint64_t n, uint64_t length, const int* offsets)
@@ -717,9 +715,10 @@ __attribute__((visibility("default"))) int cusig_amd_linear_recurrence_step(
             constexpr int V = 4;
             const uint64_t packs = (channels + V - 1) / V, blocks = (rows * packs + kThreads - 1) / kThreads;
             require(blocks < (uint64_t(1) << 31), "too many rows and channels");
-            hipLaunchKernelGGL((step_kernel<T, V>), dim3(unsigned(blocks)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), static_cast<const T*>(x),
-                               static_cast<const T*>(log_decay), state, static_cast<T*>(h), int64_t(rows), int(channels), x_stride, log_decay_stride, int(packs));
-            SIG_HIP(hipGetLastError());
+            in_launches(int64_t(blocks), kThreads, [&](unsigned first, dim3 grid) {
+                hipLaunchKernelGGL((step_kernel<T, V>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), static_cast<const T*>(x),
+                                   static_cast<const T*>(log_decay), state, static_cast<T*>(h), int64_t(rows), int(channels), x_stride, log_decay_stride, int(packs), first);
+            });
         });
     });
 }

@@ -28,6 +28,7 @@ struct RotaryArgs {
     int heads, kv_heads, dim, rotary, split;
     float eps;
     bool past;                    // results go past the caches
+    unsigned first_block;         // of a launch
 };
 
 // The U pairs of a lane: elements a[i] and b[i] are turned against each other (or stay, past the rotary part).
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(RotaryArgs p)
 {
     constexpr int kHeads = 64 / G;
     const int lane = threadIdx.x & 63, unit = lane % G;
-    const int64_t wave = int64_t(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+    const int64_t wave = (int64_t(p.first_block) + blockIdx.x) * kWaves + (threadIdx.x >> 6);
     const int64_t token = wave / p.split;
     if (token >= p.tokens) return;
     const Place at = place_of<U, NEAR>(unit, p.dim, p.rotary);
@@ -282,8 +283,7 @@ void launch(RotaryArgs& p, bool back, float* dqw, float* dkw, hipStream_t stream
     const int64_t blocks = (p.tokens * p.split + kWaves - 1) / kWaves;
     if (!back) {
         require(blocks < (int64_t(1) << 31), "too many tokens");
-        hipLaunchKernelGGL((forward_kernel<T, kUnit, G, NEAR>), dim3(unsigned(blocks)), dim3(kThreads), 0, stream, p);
-        SIG_HIP(hipGetLastError());
+        launch_all(forward_kernel<T, kUnit, G, NEAR>, blocks, kThreads, stream, p);
         return;
     }
     // 32-bit loads fill the memory's queues with half the blocks, and fewer pieces are summed up sooner (8000 tokens, 20 heads of 128,

@@ -1059,3 +1059,43 @@ def test_recurrence_of_rows_far_apart(P):
         assert torch.equal(a, b)
     state = torch.zeros((12, 16), device=DEV)
     assert torch.equal(P.linear_recurrence_step(x, g, state), dense[0])
+
+
+@pytest.mark.gpu
+def test_more_threads_than_a_launch_has(P):
+    """A launch numbers its threads with 32 bits: these calls have more, and go in several."""
+    from pysiglib_amd import _loader as L
+    # 2^24 + 3 sequences of one step, a block of 256 threads to each
+    n = (1 << 24) + 3
+    x = torch.randn((n, 1, 4), device=DEV).to(torch.bfloat16)
+    g, start = torch.zeros_like(x), torch.randn((n, 4), device=DEV)
+    assert L.CUSIG_LINEAR_RECURRENCE_WORKSPACE(1, n, n, 4) == 0
+    h, final = P.linear_recurrence(x, g, initial_state=start)
+    want = start + x[:, 0].float()
+    assert torch.equal(final, want) and torch.equal(h[:, 0], want.to(torch.bfloat16))
+    dx, dg, d0 = P.linear_recurrence_backprop(h, g, x, grad_final=start, initial_state=start)
+    assert torch.equal(d0, want) and torch.equal(dx[:, 0], want.to(torch.bfloat16)) and torch.equal(dg[:, 0], (want * start).to(torch.bfloat16))
+    del x, g, start, h, final, want, dx, dg, d0
+    # 2^26 + 5 tokens, a wave to each
+    tokens = (1 << 26) + 5
+    q = torch.ones((tokens, 1, 2), dtype=torch.bfloat16, device=DEV)
+    q[-3:, 0, 1] = -1.0
+    w = torch.tensor([2.0, 3.0], device=DEV)
+    cos, sin = P.rotary_tables(1, 0, device=DEV)
+    out, _ = P.norm_rotary(q, q[:, :0], w, w, cos, sin, torch.zeros(tokens, dtype=torch.int32, device=DEV), eps=0.0)
+    assert (out[..., 0] == 2.0).all() and (out[:-3, 0, 1] == 3.0).all() and (out[-3:, 0, 1] == -3.0).all()
+    del q, out
+    # 65 sequences of one token, 2^19 heads: a block to each
+    heads, n = 1 << 19, 65
+    q, k, v, g = (torch.randn((n, heads, 8), device=DEV).to(torch.bfloat16) for _ in range(4))
+    at = whole_numbers(range(n + 1))
+    out, lse = P.attention(q, k, v, at, at, scale=0.5)
+    assert torch.equal(out, v)
+    score = (q.double() * k.double()).sum(-1) * 0.5
+    size = (q.double() * k.double()).abs().sum(-1) * 0.5
+    assert ((lse - score).abs() <= 16 * U32 * (size + 1)).all()
+    dq, dk, dv = P.attention_backprop(g, q, k, v, out, lse, at, at, scale=0.5)
+    assert torch.equal(dv, g)
+    # dp - delta, 8 terms each, is nothing but their roundings
+    most = 32 * U32 * (g.double() * v.double()).abs().sum(-1, keepdim=True) * 0.5
+    assert (dq.double().abs() <= most * k.double().abs() * 1.01).all() and (dk.double().abs() <= most * q.double().abs() * 1.01).all()
