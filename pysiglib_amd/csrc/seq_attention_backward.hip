@@ -91,9 +91,6 @@ __device__ __forceinline__ void fit(Lift& lift, const f32x16& x, f32x16* sums)
     }
 }
 
-// A weight times what it weighs: zero where it has no weight, also of what is not finite (v_mul_legacy_f32)
-extern "C" __device__ __attribute__((const)) float weighed(float weight, float x) __asm("llvm.amdgcn.fmul.legacy");
-
 // Operands that are not finite, of keys that a query does not see or queries that do not see a key: neither a weight of zero nor dS,
 // set to zero there, makes zero with them in the second product.  They are taken out of the tiles that hide some from others, and put
 // back at the end into the sums that they belong to.  P knows of them all the same: by the log-sum of a query that is or sees such a

@@ -65,8 +65,12 @@ __device__ __forceinline__ float word_b(unsigned long long v) { return __uint_as
 // A product that overflowed to infinity takes nothing from a state of zero, one of zero nothing from any state
 __device__ __forceinline__ float apply(float a, float b, float h) { return h == 0.0f || a == 0.0f ? b : fmaf(a, h, b); }
 
-// A run whose product is zero forgets whatever came before it, also after a product that overflowed
-__device__ __forceinline__ float chain(float a1, float a2) { return a1 == 0.0f || a2 == 0.0f ? 0.0f : a1 * a2; }
+// A decay that is zero forgets whatever came before it, also what is not finite, and a run's product is zero where it has one or a
+// sequence begins in it.  Other products stop at the smallest positive number, so that a state that is not finite goes through them
+// wherever in a chunk their steps lie; to a finite one that adds at most 5e-7.
+__device__ __forceinline__ float at_least(float a) { return a < 1.401298464e-45f ? 1.401298464e-45f : a; }
+
+__device__ __forceinline__ float chain(float a1, float a2) { return a1 == 0.0f || a2 == 0.0f ? 0.0f : at_least(a1 * a2); }
 
 // The hardware's exponential of the scaled argument: off by |g| 2^-24 of its size from the scaling and one rounding
 __device__ __forceinline__ float decay(float g) { return __builtin_amdgcn_exp2f(g * 1.44269504088896341f); }
@@ -77,6 +81,9 @@ __device__ __forceinline__ void rows_of(const int* offsets, int64_t i, int64_t r
     first = kept(offsets[i], 0, rows);
     past = kept(offsets[i + 1], first, rows);
 }
+
+// a step: a product with a decay of zero is zero, whatever the state
+__device__ __forceinline__ float next_state(float d, float h, float x) { return weighed(d, h) + x; }
 
 // Rows [t0, t0 + ROWS) of the packed rows: at[r] = the sequence that begins (forward) or ends (backward) at row t0 + r,
 // ends[r] = the sequence that ends (forward) or begins (backward) there, -1: none.  Returns whether there is any.
@@ -186,26 +193,29 @@ __global__ void __launch_bounds__(kThreads, PART ? 1 : (BACK || R > 16 ? 3 : 4))
     auto state_at = [&](const float* s, int64_t seq, int v) { return s && v < count ? s[seq * p.channels + ch0 + v] : 0.0f; };
 
     // the thread's rows as one map
-    float a[V], b[V];
+    float a[V], b[V], least[V];         // least: the smallest decay, zero where a sequence begins
 #pragma unroll
-    for (int v = 0; v < V; ++v) a[v] = 1.0f, b[v] = 0.0f;
+    for (int v = 0; v < V; ++v) a[v] = least[v] = 1.0f, b[v] = 0.0f;
     {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             if (edges) {
                 const int seq = at_of(group * R + r);
-                if (seq >= 0)
+                if (seq >= 0)       // a too: with no need of its own, but rows whose work is apart spill registers
 #pragma unroll
-                    for (int v = 0; v < V; ++v) a[v] = 0.0f, b[v] = state_at(p.begin, seq, v);
+                    for (int v = 0; v < V; ++v) a[v] = least[v] = 0.0f, b[v] = state_at(p.begin, seq, v);
             }
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float d = decay(gate[r].get(v)), x = in[r].get(v);
                 a[v] *= d;
-                b[v] = BACK ? d * (b[v] + x) : fmaf(d, b[v], x);
+                least[v] = fminf(least[v], d);
+                b[v] = BACK ? weighed(d, b[v] + x) : next_state(d, b[v], x);
             }
         }
     }
+#pragma unroll
+    for (int v = 0; v < V; ++v) a[v] = least[v] == 0.0f ? 0.0f : at_least(a[v]);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         s_a[group][lane * V + v] = a[v];
@@ -311,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, PART ? 1 : (BACK || R > 16 ? 3 : 4))
             P o;
             if constexpr (!BACK) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) state[v] = fmaf(decay(gate[r].get(v)), state[v], in[r].get(v));
+                for (int v = 0; v < V; ++v) state[v] = next_state(decay(gate[r].get(v)), state[v], in[r].get(v));
                 o.set(state);
                 put(op + t * p.channels, o);
             } else {
@@ -319,10 +329,10 @@ __global__ void __launch_bounds__(kThreads, PART ? 1 : (BACK || R > 16 ? 3 : 4))
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     e[v] = state[v] + in[r].get(v);
-                    state[v] = decay(gate[r].get(v)) * e[v];
+                    state[v] = weighed(decay(gate[r].get(v)), e[v]);
                     float h = prev[r].get(v);
                     if (last >= 0) h = state_at(p.init, last, v);
-                    dg[v] = state[v] * h;
+                    dg[v] = weighed(state[v], h);
                 }
                 o.set(e);
                 put(op + t * p.channels, o);
@@ -409,17 +419,20 @@ __global__ void __launch_bounds__(kThreads, 2) column_kernel(ScanArgs p)
             if constexpr (BACK) prev[r] = next_prev[r];
         }
         if (chunk + 1 < chunks) fetch(chunk + 1);
-        float a[V], b[V];
+        float a[V], b[V], least[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) a[v] = 1.0f, b[v] = 0.0f;
+        for (int v = 0; v < V; ++v) a[v] = least[v] = 1.0f, b[v] = 0.0f;
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float d = decay(gate[r].get(v)), x = in[r].get(v);
                 a[v] *= d;
-                b[v] = BACK ? d * (b[v] + x) : fmaf(d, b[v], x);
+                least[v] = fminf(least[v], d);
+                b[v] = BACK ? weighed(d, b[v] + x) : next_state(d, b[v], x);
             }
+#pragma unroll
+        for (int v = 0; v < V; ++v) a[v] = least[v] == 0.0f ? 0.0f : at_least(a[v]);
         // inclusive over the pieces before it in the wave, then the one before
 #pragma unroll
         for (int m = LC; m < 64; m *= 2)
@@ -477,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 2) column_kernel(ScanArgs p)
                 P o;
                 if constexpr (!BACK) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) state[v] = fmaf(decay(gate[r].get(v)), state[v], in[r].get(v));
+                    for (int v = 0; v < V; ++v) state[v] = next_state(decay(gate[r].get(v)), state[v], in[r].get(v));
                     o.set(state);
                     put(op + there, o);
                 } else {
@@ -485,10 +498,10 @@ __global__ void __launch_bounds__(kThreads, 2) column_kernel(ScanArgs p)
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
                         e[v] = state[v] + in[r].get(v);
-                        state[v] = decay(gate[r].get(v)) * e[v];
+                        state[v] = weighed(decay(gate[r].get(v)), e[v]);
                         float h = prev[r].get(v);
                         if (!decltype(all_there)::value && t == rows - 1) h = p.init ? p.init[int64_t(seq) * p.channels + ch0 + v] : 0.0f;
-                        dg[v] = state[v] * h;
+                        dg[v] = weighed(state[v], h);
                     }
                     o.set(e);
                     put(op + there, o);
@@ -535,7 +548,7 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const T* x, const T* gat
     Pack<T, V> o;
     float h[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = fmaf(decay(a.get(v)), s.get(v), b.get(v));
+    for (int v = 0; v < V; ++v) h[v] = next_state(decay(a.get(v)), s.get(v), b.get(v));
     s.set(h);
     o.set(h);
     store_some<float, V>(state + row * channels + ch, s, count);

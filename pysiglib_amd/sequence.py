@@ -122,7 +122,8 @@ def linear_recurrence(x, log_decay, *, initial_state=None, offsets=None):
     """``h_t = exp(log_decay_t) * h_{t-1} + x_t`` for each channel, over sequences of any length.
 
     ``x``, ``log_decay``: ``(..., length, channels)``, or with ``offsets`` ``(rows, channels)``, the sequences packed.
-    ``log_decay`` is meant to be at most 0; ``-inf`` forgets the state.  ``initial_state``: float32 ``(..., channels)``, with
+    ``log_decay`` is meant to be at most 0; where its exponential is zero in 32 bits (``-inf``, and below about -87) it forgets the
+    state, also one that is not finite.  ``initial_state``: float32 ``(..., channels)``, with
     ``offsets`` ``(sequences, channels)``; zero where it is not given.
 
     Returns ``(h, final_state)``: ``h`` like ``x``, the states behind the last steps like ``initial_state``.

@@ -1099,3 +1099,61 @@ def test_more_threads_than_a_launch_has(P):
     # dp - delta, 8 terms each, is nothing but their roundings
     most = 32 * U32 * (g.double() * v.double()).abs().sum(-1, keepdim=True) * 0.5
     assert (dq.double().abs() <= most * k.double().abs() * 1.01).all() and (dk.double().abs() <= most * q.double().abs() * 1.01).all()
+
+
+# ---- decays of -inf, states that are not finite ----
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels", [(700, 24), (6000, 24), (6000, 2), (9000, 70)])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_recurrence_forgets_at_minus_infinity_and_nowhere_else(P, dtype, rows, channels, bad):
+    """A state that is not finite goes on through any number of decays, and ends at one whose exponential is zero in 32 bits,
+    -inf or not; backwards alike.  Wherever in a block's rows that is."""
+    rng = np.random.default_rng(rows)
+    x, g, h0, grad, gf = recurrence_inputs(dtype, rows, channels, 1, seed=rows)
+    g = torch.minimum(g, torch.tensor(-0.25, dtype=dtype))
+    ends = np.full(channels, rows)
+    for c in range(channels):
+        begin = int(rng.integers(0, rows // 3))
+        x[begin, c] = bad
+        if c % 3:
+            ends[c] = int(rng.integers(begin + 1, rows))
+            g[ends[c], c] = -float("inf") if c % 3 == 1 else -300.0
+    put = lambda t: t.to(DEV)[None]              # noqa: E731
+    h, final = P.linear_recurrence(put(x), put(g), initial_state=put(h0)[0])
+    got, last = f64(h)[0], f64(final)[0]
+    for c in range(channels):
+        begin = int(np.flatnonzero(~np.isfinite(f64(x[:, c])))[0])
+        end = ends[c]
+        assert np.isfinite(got[:begin, c]).all() and np.isfinite(got[end:, c]).all(), c
+        assert (np.isinf if bad == bad else np.isnan)(got[begin:end, c]).all(), c
+        assert np.isfinite(last[c]) == (end < rows), c
+        if end < rows:
+            assert got[end, c] == f64(x[end, c]), c
+    # backwards from a gradient that is not finite
+    x, g, h0, grad, gf = recurrence_inputs(dtype, rows, channels, 1, seed=rows)
+    g = torch.minimum(g, torch.tensor(-0.25, dtype=dtype))
+    stops = np.full(channels, -1)
+    at = np.zeros(channels, int)
+    for c in range(channels):
+        at[c] = int(rng.integers(2 * rows // 3, rows))
+        grad[at[c], c] = bad
+        if c % 3:
+            stops[c] = int(rng.integers(0, at[c]))
+            g[stops[c], c] = -float("inf") if c % 3 == 1 else -300.0
+    h, _ = P.linear_recurrence(put(x), put(g), initial_state=put(h0)[0])
+    dx, dg, d0 = (f64(t)[0] for t in P.linear_recurrence_backprop(h, put(g), put(grad), grad_final=put(gf)[0], initial_state=put(h0)[0]))
+    for c in range(channels):
+        s = stops[c]
+        assert np.isfinite(dx[at[c] + 1:, c]).all() and np.isfinite(dx[:max(s, 0), c]).all(), c
+        assert not np.isfinite(dx[max(s, 0):at[c] + 1, c]).any(), c
+        assert not np.isfinite(dg[s + 1:at[c] + 1, c]).any() and np.isfinite(dg[at[c] + 1:, c]).all() and np.isfinite(dg[:s + 1, c]).all(), c
+        assert np.isfinite(d0[c]) == (s >= 0), c
+    # an infinite state meets a decay of -inf: neither gradient of that step depends on it
+    x, g, h0, grad, gf = recurrence_inputs(dtype, rows, channels, 1, seed=rows)
+    h, _ = P.linear_recurrence(put(x), put(g))
+    g[rows // 2] = -float("inf")
+    h[0, rows // 2 - 1] = float("inf")
+    _, dg, _ = P.linear_recurrence_backprop(h, put(g), put(grad))
+    assert (dg[0, rows // 2] == 0).all()
