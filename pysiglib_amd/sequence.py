@@ -208,6 +208,7 @@ def linear_recurrence_step(x, log_decay, state):
     channels = shape[-1]
     _call(CUSIG_LINEAR_RECURRENCE_STEP, "linear_recurrence_step", device, _CODES[x.dtype], x.data_ptr(), log_decay.data_ptr(),
           state.data_ptr(), h.data_ptr(), h.numel() // channels if channels else 0, channels, x_step, decay_step)
+    torch.autograd.graph.increment_version(state)       # written through its address: operations that kept it find out
     return h
 
 

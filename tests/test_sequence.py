@@ -1157,3 +1157,20 @@ def test_recurrence_forgets_at_minus_infinity_and_nowhere_else(P, dtype, rows, c
     h[0, rows // 2 - 1] = float("inf")
     _, dg, _ = P.linear_recurrence_backprop(h, put(g), put(grad))
     assert (dg[0, rows // 2] == 0).all()
+
+
+# ---- with autograd around them ----
+
+@pytest.mark.gpu
+def test_a_state_that_is_replaced_is_known_to_autograd(P):
+    """An operation that kept the state for its gradient finds out that it has changed."""
+    x, state = torch.randn((3, 8), device=DEV), torch.randn((3, 8), device=DEV)
+    w = torch.ones((3, 8), device=DEV, requires_grad=True)
+    kept = (w * state).sum()
+    before = state._version
+    P.linear_recurrence_step(x, x, state)
+    assert state._version > before
+    with pytest.raises(RuntimeError):
+        kept.backward()
+    with torch.inference_mode():
+        P.linear_recurrence_step(x, x, torch.zeros((3, 8), device=DEV))
