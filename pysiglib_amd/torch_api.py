@@ -158,6 +158,28 @@ def log_sig(path, degree, *, time_aug=False, lead_lag=False, end_time=1., method
     return sig_to_log_sig(sig_, path.shape[-1], degree, time_aug=time_aug, lead_lag=lead_lag, method=method)
 
 
+class _Gradients(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, anchor, *grads):
+        return grads
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("the gradients of pysiglib_amd's sequence layers are not differentiable")
+
+
+def _once(*grads):
+    """Gradients for a backward function to return.  Where a graph of them is asked for, they refuse to be differentiated
+    instead of being constants in it."""
+    if not torch.is_grad_enabled():
+        return grads
+    at = [i for i, g in enumerate(grads) if g is not None]
+    out = list(grads)
+    for i, g in zip(at, _Gradients.apply(torch.empty(0, requires_grad=True), *(grads[i] for i in at))):
+        out[i] = g
+    return tuple(out)
+
+
 class LinearRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, log_decay, initial_state, offsets):
@@ -174,7 +196,7 @@ class LinearRecurrence(torch.autograd.Function):
         grad_h = torch.zeros_like(h) if grad_h is None else grad_h
         dx, dg, d0 = _recurrence_backprop(h, log_decay, grad_h, grad_final=grad_final, initial_state=initial_state,
                                           offsets=offsets)
-        return dx, dg, d0 if initial_state is not None else None, None
+        return _once(dx, dg, d0 if initial_state is not None else None, None)
 
 
 def linear_recurrence(x, log_decay, *, initial_state=None, offsets=None):
@@ -195,7 +217,7 @@ class NormRotary(torch.autograd.Function):
         from .sequence import norm_rotary_backprop as _norm_rotary_backprop
         eps, interleaved = ctx.args
         grads = _norm_rotary_backprop(grad_q, grad_k, *ctx.saved_tensors, eps=eps, interleaved=interleaved)
-        return (*grads, None, None, None, None, None)
+        return _once(*grads, None, None, None, None, None)
 
 
 def norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, *, eps=1e-6, interleaved=False):
@@ -217,8 +239,8 @@ class Attention(torch.autograd.Function):
         from .sequence import attention_backprop as _attention_backprop
         q, k, v, out, lse, q_offsets, k_offsets = ctx.saved_tensors
         causal, scale = ctx.args
-        return (*_attention_backprop(grad_out, q, k, v, out, lse, q_offsets, k_offsets, causal=causal, scale=scale), None, None,
-                None, None)
+        grads = _attention_backprop(grad_out, q, k, v, out, lse, q_offsets, k_offsets, causal=causal, scale=scale)
+        return _once(*grads, None, None, None, None)
 
 
 def attention(q, k, v, q_offsets, k_offsets, *, causal=True, scale=None):

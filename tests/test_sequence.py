@@ -1174,3 +1174,24 @@ def test_a_state_that_is_replaced_is_known_to_autograd(P):
         kept.backward()
     with torch.inference_mode():
         P.linear_recurrence_step(x, x, torch.zeros((3, 8), device=DEV))
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused(P):
+    """The gradients are not differentiable: they say so, rather than leave a part of a second derivative out."""
+    A = P.torch_api
+    at = whole_numbers([0, 6])
+    q, k = (torch.randn((6, n, 64), device=DEV).half().requires_grad_(True) for n in (2, 1))
+    w = torch.ones(64, device=DEV, requires_grad=True)
+    cos, sin = P.rotary_tables(8, 64, device=DEV)
+    x = torch.randn((2, 6, 8), device=DEV, requires_grad=True)
+    positions = torch.arange(6, dtype=torch.int32, device=DEV)
+    for out, leaf in [(A.attention(q, k, k, at, at), q), (A.norm_rotary(q, k, w, w, cos, sin, positions)[0], q),
+                      (A.linear_recurrence(x, -x.detach().abs())[0], x)]:
+        for loss in (out.float().sum(), out.float().square().sum()):
+            grad, = torch.autograd.grad(loss, leaf, create_graph=True, retain_graph=True)
+            assert torch.isfinite(grad).all()
+            with pytest.raises(RuntimeError):
+                (grad.float().sum() + leaf.float().sum()).backward()
+        grad, = torch.autograd.grad(out.float().sum(), leaf)
+        assert not grad.requires_grad
