@@ -245,11 +245,11 @@ __device__ __forceinline__ int wave_max(int x)
 }
 
 // inclusive sum over the lanes
-__device__ __forceinline__ int wave_scan(int x)
+__device__ __forceinline__ long long wave_scan(long long x)
 {
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) {
-        const int left = __shfl_up(x, m);
+        const long long left = __shfl_up(x, m);
         if (int(threadIdx.x & 63) >= m) x += left;
     }
     return x;
@@ -344,30 +344,32 @@ constexpr int kMapThreads = 1024;
 
 static __global__ void __launch_bounds__(kMapThreads) map_kernel(MapArgs p)
 {
-    __shared__ int s_sums[kMapThreads / 64];
+    __shared__ long long s_sums[kMapThreads / 64];          // offsets that do not ascend can name more tiles than 32 bits count
     const int tid = threadIdx.x, lane = tid & 63;
     const Tiling how = blockIdx.x ? p.how[1] : p.how[0];
     int* const map = blockIdx.x ? p.map[1] : p.map[0];
     const int room = blockIdx.x ? p.room[1] : p.room[0];
-    int done = 0;
-    for (int base = 0; base < p.packed.n; base += kMapThreads) {
+    long long done = 0;
+    for (int64_t base = 0; base < p.packed.n; base += kMapThreads) {
         Span one{};
-        if (base + tid < p.packed.n) span_of(p.packed, base + tid, one);
-        const int own = base + tid < p.packed.n ? tiles_of(how, one) : 0, upto = wave_scan(own);
+        const int seq = int(base + tid);
+        if (base + tid < p.packed.n) span_of(p.packed, seq, one);
+        const int own = base + tid < p.packed.n ? tiles_of(how, one) : 0;
+        const long long upto = wave_scan(own);
         __syncthreads();
         if (lane == 63) s_sums[tid >> 6] = upto;
         __syncthreads();
-        int before = done + upto - own;
+        long long before = done + upto - own;
         for (int w = 0; w < kMapThreads / 64; ++w) {
             if (w < (tid >> 6)) before += s_sums[w];
             done += s_sums[w];
         }
         for (int i = 0; i < own && before + i < room; ++i) {
-            map[2 + 2 * (before + i)] = base + tid;
+            map[2 + 2 * (before + i)] = seq;
             map[3 + 2 * (before + i)] = i;
         }
     }
-    if (tid == 0) map[0] = min(done, room);
+    if (tid == 0) map[0] = done < room ? int(done) : room;
 }
 
 // offsets of a tile's rows are 32-bit

@@ -498,13 +498,11 @@ void forward(const AttentionArgs& p, const Cut& cut, hipStream_t stream)
 {
     if (cut.few) {
         const int64_t blocks = cut.tiles * p.kv_heads * p.splits, rows = p.packed.q_rows * p.heads;
-        require(blocks < (int64_t(1) << 31) && rows < (int64_t(1) << 32), "too many queries and heads");
         launch_all(few_kernel<T, DP>, blocks, 256, stream, p);
         if (p.splits > 1) launch_all(join_kernel<T>, (rows + 3) / 4, 256, stream, p);
         return;
     }
     const int64_t blocks = cut.tiles * p.heads;
-    require(blocks < (int64_t(1) << 31), "too many queries and heads");
     switch (cut.waves) {
     case 2: return launch_all(attention_kernel<T, DP, 2, 32>, blocks, 128, stream, p);
     case 4: return launch_all(attention_kernel<T, 128, 4, 64>, blocks, 256, stream, p);
@@ -550,6 +548,7 @@ __attribute__((visibility("default"))) int cusig_amd_attention(
         require(workspace_bytes >= cut.map + cut.parts && (workspace || cut.map + cut.parts == 0), "the workspace is too small");
         p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + cut.map);
         p.splits = cut.splits;
+        require(cut.tiles * (cut.few ? p.kv_heads * int64_t(p.splits) : p.heads) < (int64_t(1) << 31), "too many queries and heads");
         const hipStream_t s = static_cast<hipStream_t>(stream);
         if (cut.map) {
             p.packed.map = static_cast<const int*>(workspace);

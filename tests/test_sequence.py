@@ -1195,3 +1195,28 @@ def test_second_derivatives_are_refused(P):
                 (grad.float().sum() + leaf.float().sum()).backward()
         grad, = torch.autograd.grad(out.float().sum(), leaf)
         assert not grad.requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keys", [False, True])
+def test_lists_of_tiles_hold_what_offsets_that_do_not_ascend_name(P, keys):
+    """Offsets to and fro name more tiles than 32 bits count: the list keeps to its room, and nothing around it changes."""
+    from pysiglib_amd import _loader as L
+    rows, n, dim = 1 << 22, 140000, 8
+    at, none = torch.zeros(n + 1, dtype=torch.int32, device=DEV), torch.zeros(n + 1, dtype=torch.int32, device=DEV)
+    at[1::2] = rows
+    wide, small = torch.zeros((rows, 1, dim), dtype=torch.bfloat16, device=DEV), torch.zeros((4, 1, dim), dtype=torch.bfloat16, device=DEV)
+    out, one = torch.zeros_like(wide), torch.zeros_like(small)
+    if keys:
+        sizes, size = (4, rows, n, 1, 1, dim), L.CUSIG_ATTENTION_BACKPROP_WORKSPACE(4, rows, n, 1, dim)
+    else:
+        sizes, size = (rows, 4, n, 1, 1, dim), L.CUSIG_ATTENTION_WORKSPACE(rows, 4, n, 1, 1, dim)
+    space = torch.full((size + 2 * 4096,), 91, dtype=torch.uint8, device=DEV)
+    inner = space[4096:4096 + size]
+    lse = torch.zeros((rows, 1), device=DEV)
+    if keys:
+        raw(L.CUSIG_ATTENTION_BACKPROP, 1, small, small, wide, wide, small, lse, none, at, one, out, out, *sizes, dim, dim, dim, dim, dim, dim, dim, dim,
+            0.5, True, inner, size)
+    else:
+        raw(L.CUSIG_ATTENTION, 1, wide, small, small, at, none, 0, out, lse, *sizes, dim, dim, dim, dim, dim, dim, 0.5, True, inner, size)
+    assert (space[:4096] == 91).all() and (space[4096 + size:] == 91).all() and (out == 0).all()
