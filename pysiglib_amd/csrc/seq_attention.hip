@@ -104,10 +104,13 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
     const int hiding = min(at.nk, p.causal ? max(q_first + shift + 1, 0) : at.nk) / kKeys;
     const int hiding_wave = min(at.nk, p.causal ? max(q_first + wave * 32 + shift + 1, 0) : at.nk) / kKeys;
     const int unseen = p.causal ? min(max(q_first + wave * 32 + 31 + shift + kKeys, 0) / kKeys, tiles) : tiles;
+    // keys' channels past the head's are zero: zeros of the query make no zero with what is not finite
+    static_assert(kThreads % Tile<DP>::kChunks == 0, "");
+    const bool there = tid % Tile<DP>::kChunks * 8 < p.dim;
     auto put = [&](int tile) __attribute__((always_inline)) {
         auto place = [&](int i) { return Tile<DP>::at((i * kThreads + tid) / Tile<DP>::kChunks, (i * kThreads + tid) % Tile<DP>::kChunks); };
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) *reinterpret_cast<u32x4*>(s_tiles[tile & 1][0] + place(i)) = next[0][i];
+        for (int i = 0; i < kLoads; ++i) *reinterpret_cast<u32x4*>(s_tiles[tile & 1][0] + place(i)) = there ? next[0][i] : u32x4{0, 0, 0, 0};
         if (tile >= hiding) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
@@ -260,6 +263,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
     const int last = p.causal && query + shift < past - 1 ? query + shift : past - 1;
 
     char *kt = s_tiles[wave][0], *vt = s_tiles[wave][1];
+    const bool there = lane % Tile<DP>::kChunks * 8 < p.dim;          // keys' channels past the head's are zero, as above
     u32x4 next[2][kLoads];
     auto fetch = [&](int tile) {
 #pragma unroll
@@ -293,7 +297,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int e = i * 64 + lane, to = Tile<DP>::at(e / Tile<DP>::kChunks, e % Tile<DP>::kChunks);
-            *reinterpret_cast<u32x4*>(kt + to) = next[0][i];
+            *reinterpret_cast<u32x4*>(kt + to) = there ? next[0][i] : u32x4{0, 0, 0, 0};
             *reinterpret_cast<u32x4*>(vt + to) = next[1][i];
         }
         __builtin_amdgcn_wave_barrier();

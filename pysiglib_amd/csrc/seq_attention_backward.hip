@@ -192,6 +192,9 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
         }
     };
     const int hiding = min(at.nk, p.causal ? max(q_first + shift + 1, 0) : at.nk) / kKeys;       // the first tile that hides a key from a query
+    // keys' channels past the head's are zero: zeros of the query make no zero with what is not finite
+    static_assert(kThreads % Tile<DP>::kChunks == 0, "");
+    const bool there = tid % Tile<DP>::kChunks * 8 < p.dim;
     auto put = [&](int buffer, int tile) __attribute__((always_inline)) {
         auto place = [&](int i) { return Tile<DP>::at((i * kThreads + tid) / Tile<DP>::kChunks, (i * kThreads + tid) % Tile<DP>::kChunks); };
 #pragma unroll
@@ -199,7 +202,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
         if (tile >= hiding) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                u32x4 x = next[0][i];
+                u32x4 x = there ? next[0][i] : u32x4{0, 0, 0, 0};
                 if (take_them_out<T>(x)) {
                     atomicOr(&s_bad[tile - hiding], 1u << (i * kThreads + tid) / Tile<DP>::kChunks);
                     s_any = 1;
@@ -208,7 +211,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + place(i)) = next[0][i];
+            for (int i = 0; i < kLoads; ++i) *reinterpret_cast<u32x4*>(s_tiles[buffer][0] + place(i)) = there ? next[0][i] : u32x4{0, 0, 0, 0};
         }
     };
     // S^T and dP^T of 32 keys

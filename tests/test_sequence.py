@@ -1220,3 +1220,31 @@ def test_lists_of_tiles_hold_what_offsets_that_do_not_ascend_name(P, keys):
     else:
         raw(L.CUSIG_ATTENTION, 1, wide, small, small, at, none, 0, out, lse, *sizes, dim, dim, dim, dim, dim, dim, 0.5, True, inner, size)
     assert (space[:4096] == 91).all() and (space[4096 + size:] == 91).all() and (out == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim", [8, 40, 64, 96, 128])
+@pytest.mark.parametrize("queries,keys", [(300, 300), (1, 700), (2, 40)])
+def test_keys_of_minus_infinity_have_no_weight(P, dtype, dim, queries, keys):
+    """A key that is infinite in one channel, against queries that make its score -infinity: as if it were not there, in any
+    channel of heads of any width."""
+    q, k, v, _ = attention_inputs(dtype, queries, keys, 2, 1, dim, seed=dim)
+    at = [whole_numbers([0, n]) for n in (queries, keys)]
+    for channel in sorted({0, dim - 8, dim - 1}):
+        key, query = k.clone(), q.clone()
+        query[..., channel] = query[..., channel].abs() + 0.5
+        key[3:keys - 1:5, 0, channel] = -float("inf")
+        without = f64(key)
+        without[3:keys - 1:5] = 0.0
+        without[3:keys - 1:5, 0, channel] = -1e30
+        out, lse = P.attention(query, key, v, *at, causal=False)
+        u = ROUND[dtype]
+        with np.errstate(over="ignore"):
+            want, bound = attention_oracle(f64(query), without, f64(v), [queries], [0, keys], [keys], False, dim ** -0.5, u=u)
+        sizes = f64(key)
+        sizes[~np.isfinite(sizes)] = 0.0
+        _, bound = attention_oracle(f64(query), sizes, f64(v), [queries], [0, keys], [keys], False, dim ** -0.5, u=u)
+        # the weights are those of the other keys: at most 5 / 4 of what the bound takes them to be
+        within(out, want[0], 2 * (bound[0] + u * (np.abs(want[0]) + bound[0])) + SMALL[dtype], "out")
+        within(lse, want[1], 2 * bound[1], "lse")
