@@ -353,17 +353,17 @@ CUSIG_AMD_API int cusig_amd_kernel_choice(int backward, int is_f64, uint64_t dim
  * the device, sequence i has the rows offsets[i] to offsets[i + 1].  They are not read on the host; numbers outside the tensors
  * are cut to them, rows that belong to no sequence are not written. */
 
-/* h_t = exp(log_decay_t) h_{t-1} + x_t for each channel.  x, log_decay, h [rows, channels] (h contiguous), offsets, or null: `sequences`
- * of `length` rows each.  initial_state (may be null: zero) and final_state float32 [sequences, channels].  Rows of at most 2^20
- * elements. */
+/* h_t = exp(log_decay_t) h_{t-1} + x_t for each channel; an exponential that is zero in 32 bits forgets any state.  x, log_decay, h
+ * [rows, channels] (h contiguous), offsets, or null: `sequences` of `length` rows each.  initial_state (may be null: zero) and
+ * final_state float32 [sequences, channels].  Rows of at most 2^20 elements. */
 CUSIG_AMD_API int cusig_amd_linear_recurrence(int dtype, const void* x, const void* log_decay, const float* initial_state, void* h,
                                               float* final_state, const int* offsets, uint64_t sequences, uint64_t length,
                                               uint64_t rows, uint64_t channels, int64_t x_stride, int64_t log_decay_stride,
                                               void* workspace, uint64_t workspace_bytes, void* stream) CUSIG_AMD_NOEXCEPT;
 CUSIG_AMD_API uint64_t cusig_amd_linear_recurrence_workspace(int dtype, uint64_t rows, uint64_t sequences,
                                                              uint64_t channels) CUSIG_AMD_NOEXCEPT;
-/* Its gradients, from the output h (contiguous) and the gradients of both outputs (grad_final may be null: zero); grad_x and
- * grad_log_decay contiguous, grad_initial float32 [sequences, channels].  The same workspace. */
+/* Its gradients, from the output h (contiguous, as it was rounded) and the gradients of both outputs (grad_final may be null: zero);
+ * grad_x and grad_log_decay contiguous, grad_initial float32 [sequences, channels].  The same workspace. */
 CUSIG_AMD_API int cusig_amd_linear_recurrence_backprop(int dtype, const void* h, const void* log_decay, const void* grad_h,
                                                        const float* grad_final, const float* initial_state, void* grad_x,
                                                        void* grad_log_decay, float* grad_initial, const int* offsets,

@@ -9,9 +9,11 @@
 // The products are formed transposed, S^T = K Q^T and O^T = V^T P^T: a lane then holds scores of a single query, its maximum
 // and sum need one exchange between lanes, and the weights are the second product's operand where they stand.
 //
-// Bound: 128 channels, the matrix units: one sequence of 8192, 32 heads on 8, bfloat16, 540 to 600 us (0.92 to 1.02 PFLOP/s; a large
-// library product reaches 1.19), and the order of reads around the products no longer changes that.  64 channels, the
-// softmax: 15 vector instructions to a matrix one, 24 sequences of up to 2000, 16 heads on 4, float16, 134 us (0.56 PFLOP/s).
+// Bound: 128 channels, the matrix units: one sequence of 8192, 32 heads on 8, bfloat16, 525 to 605 us by the card (0.91 to 1.05 PFLOP/s;
+// a large library product reaches 1.19), and the order of reads around the products no longer changes that.  64 channels, the
+// softmax: 15 vector instructions to a matrix one, 24 sequences of up to 2000, 16 heads on 4, float16, 141 us (0.53 PFLOP/s).  Heads of
+// other widths take the time of the next of these two (4 sequences of 2000, 16 heads on 4, bfloat16: 32 channels 61 us, 64 58, 80 89, 96 91,
+// 128 95).
 // Single queries, HBM: 48 against caches of up to 12000 keys of 8 heads of 128, 242 us (5.1 TB/s).
 #include "seq_attention.h"
 
@@ -462,7 +464,8 @@ __global__ void __launch_bounds__(256) join_kernel(AttentionArgs p)
     }
 }
 
-// How a call is cut.  few: pairs of (query, head) in tiles of 32 instead of a head's queries in tiles of 32 to a wave.
+// How a call is cut, by averages: the lengths are not known here.  (A prompt of 4096 beside 63 single tokens against 2000 keys, 32 heads
+// on 8 of 128, bfloat16: 384 us; the prompt in a call of its own 152, the tokens 121.)  few: pairs of (query, head) in tiles of 32 instead of a head's queries in tiles of 32 to a wave.
 struct Cut {
     bool few;
     int waves, splits;

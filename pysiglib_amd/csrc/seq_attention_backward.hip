@@ -104,8 +104,8 @@ __device__ __attribute__((noinline)) void spoil(const T* row, T* to, int dim, in
         if (!__builtin_isfinite(static_cast<float>(row[ch]))) to[ch] = T(__builtin_nanf(""));
 }
 
-// ---- queries fixed: 32 to a wave, tiles of kKeys keys.  Bound: the matrix units, busy 46 % of the cycles, between them the
-// exponentials that wait for the products (4 sequences of 1600 to 2047, 32 heads on 8 of 128, bfloat16: 239 us) ----
+// ---- queries fixed: 32 to a wave, tiles of kKeys keys.  Bound: the matrix units, busy 40 % of the cycles, between them the
+// exponentials that wait for the products (4 sequences of 1600 to 2047, 32 heads on 8 of 128, bfloat16: 248 to 268 us) ----
 template <typename T, int DP, int WAVES, int kKeys>
 __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
 {
@@ -155,8 +155,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
     const int last = p.causal && query + shift < at.nk - 1 ? query + shift : at.nk - 1;
     // The output's rounding makes delta wrong by u |dO| |O|, which matters where few keys share the weight: dS, differences from
     // delta, is as small there as that.  64 channels: e, the sum of dS, is what delta is short of, and dQ is short of e P K, which
-    // is summed beside it (24 sequences of up to 2000, 16 heads on 4, the whole gradient: 418 us, without it 390; sequences of 17 to
-    // 129: 66 us, 74 when they went over their keys twice).  128 channels: no registers for these sums; queries go over up to
+    // is summed beside it (when it was chosen, 24 sequences of up to 2000, 16 heads on 4, the whole gradient: 418 us, without it 390;
+    // sequences of 17 to 129: 66 us, 74 when they went over their keys twice; now 440 and 69).  128 channels: no registers for these sums; queries go over up to
     // `exact` keys twice.  Every query has them all where none are hidden, and the error's share falls with the channels: there
     // they do so to longer lengths (8 sequences of 1000, 16 heads on 8, nothing hidden: 381 us, once 321; dQ's error against 64
     // bits, in those of a result that is rounded once: 1.43 and 1.55).
@@ -315,8 +315,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dq_kernel(GradArgs p)
         for (int k = hiding * kKeys; k <= last; ++k) spoil(static_cast<const T*>(p.k) + (at.k0 + k) * p.k_token + kv * p.k_head, to, p.dim, half);
 }
 
-// ---- keys fixed: 32 to a pair of waves, PAIRS pairs to a block; queries in steps of kQueries.  Bound: as above, 44 % (the same
-// sequences: 325 us) ----
+// ---- keys fixed: 32 to a pair of waves, PAIRS pairs to a block; queries in steps of kQueries.  Bound: as above, 41 % (the same
+// sequences: 319 to 348 us) ----
 template <typename T, int DP, int PAIRS, int kQueries>
 __global__ void __launch_bounds__(PAIRS * 128, 2) dkv_kernel(GradArgs p)
 {

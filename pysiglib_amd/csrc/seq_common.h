@@ -102,10 +102,11 @@ __device__ __forceinline__ void store_some(T* p, const Pack<T, V>& r, int count)
         }
 }
 
-// Whether results of so many bytes, in rows of `row` bytes, are stored past the caches.  Those of up to half of the last one's 256 MB
-// stay there for the call that reads them: 8 sequences of 2048 steps of 2048 channels in bfloat16, forward and gradients in turn over
-// three sets of inputs, 148 us, with the forward's 67 MB past the caches 160, with the gradients' 134 MB kept 157.  Lines that are
-// written in pieces are kept: gradients of 23000 steps of 997 channels in float16 took 126 us instead of 89.
+// Whether results of so many bytes, in rows of `row` bytes, are stored past the caches.  Those of less than half of the last one's 256 MB
+// stay there for the call that reads them.  8 sequences, 2048 channels, bfloat16, forward and gradients in turn over three sets of
+// inputs, the gradients' results kept and past the caches: of 96 MB 108 us both, of 120 MB 141 and 137, of 128 MB (2048 steps) 157 and 148,
+// of 256 MB 333 and 311; with 2048 steps and the forward's 64 MB past the caches too 160.  Lines that are written in pieces are kept:
+// gradients of 23000 steps of 997 channels in float16 took 126 us instead of 89.
 inline bool goes_past(uint64_t bytes, uint64_t row) { return bytes >= (uint64_t(128) << 20) && row % 128 == 0; }
 
 // A weight times what it weighs: zero where it has no weight, also of what is not finite (v_mul_legacy_f32)

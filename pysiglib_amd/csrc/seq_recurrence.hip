@@ -10,8 +10,8 @@
 // Bound: HBM.  Every element is read once and written once: a block holds a chunk of steps of its channels in registers,
 // publishes the chunk's (A, B), collects those of the chunks before it back to one that is the state itself, and only then
 // walks its steps.  States, products and sums are 32-bit whatever the element type.  One sequence of 100003 steps of 384 channels,
-// float32: 108 us, 4.3 TB/s; forward and gradients of 8 of 2048 steps of 2048 channels, bfloat16: 143 us, 3.8 TB/s.  Odd rows of
-// 16 bits lie across the words that lanes load: 37 of up to 1500 steps of 997 channels, float16, 142 us, 2.6 TB/s.
+// float32: 110 us, 4.2 TB/s; forward and gradients of 8 of 2048 steps of 2048 channels, bfloat16: 147 us, 3.7 TB/s.  Odd rows of
+// 16 bits lie across the words that lanes load: 37 of up to 1500 steps of 997 channels, float16, 146 us, 2.5 TB/s.
 #include "seq_common.h"
 
 #include <type_traits>
@@ -568,8 +568,9 @@ struct Plan {
     bool columns;
 };
 
-// A block to a sequence and 64 bytes of channels where these are blocks enough, or the sequences short: 8 sequences of 2048, 2048
-// channels, bfloat16: 42 us forward and 65 us backward, publishing 83 and 123; 4 of 512, 1024 channels, float32: 10 and 12, publishing 14
+// A block to a sequence and 64 bytes of channels where these are blocks enough, or the sequences short, on average: the lengths are
+// not known here.  (A sequence of 100000 steps beside 199 of 30, 64 channels, bfloat16, is walked by two blocks, 1.2 ms; alone it
+// publishes, 76 us.)  When it was chosen, 8 sequences of 2048, 2048 channels, bfloat16: 42 us forward and 65 us backward, publishing 83 and 123; 4 of 512, 1024 channels, float32: 10 and 12, publishing 14
 // and 17; but one of 4096, 4096 channels: 54 and 82, publishing 42 and 57; 2 of 4000, 64 channels: 32 and 53, publishing 15 and 17.
 template <typename T, bool BACK>
 Plan plan_of(int64_t rows, int64_t n, int channels)
