@@ -32,7 +32,12 @@ struct AttentionArgs {
     unsigned first_block;    // of a launch
 };
 
-constexpr float kSlack = 8.0f;   // the maximum is taken over where it grew by more than this (in powers of two): weights stay below 2^8
+// The maximum is taken over where it grew by more than kSlack, in powers of two.  Weights in float16 stand 2^kRaise above what they are: up
+// to 2^15, so that those of keys with little weight beside another's keep their bits down to 2^-25 of the largest, not to 2^-14.
+template <typename T>
+constexpr float kSlack = __is_same(T, f16) ? 4.0f : 8.0f;
+template <typename T>
+constexpr float kRaise = __is_same(T, f16) ? 11.0f : 0.0f;
 
 // WAVES waves of 32 queries each, tiles of kKeys keys: what a block reads serves all its waves, the next tile on its way meanwhile.
 template <typename T, int DP, int WAVES, int kKeys>
@@ -160,7 +165,7 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
             for (int j = 0; j < 4; ++j) part[j] = larger(larger(part[j], s[1][j + 4], s[1][j + 8]), s[1][j + 12]);
         float most = larger(larger(part[0], part[1], part[2]), part[3]);
         most = larger(most, swapped(most)) * p.scale;
-        const bool grows = most > top + kSlack || (top == -INFINITY && most > top);
+        const bool grows = most > top + kSlack<T> || (top == -INFINITY && most > top);
         if (__any(grows)) {             // each query by itself: its roundings are no matter of the others'
             const float now = grows ? most : top, shrink = top == now ? 1.0f : exp2f(top - now);
             top = now;
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= shrink;
         }
-        const float base = top == -INFINITY ? 0.0f : top;
+        const float base = top == -INFINITY ? 0.0f : top - kRaise<T>;
 #pragma unroll
         for (int j = 0; j < 4; ++j) part[j] = 0.0f;
 #pragma unroll
@@ -208,6 +213,7 @@ __global__ void __launch_bounds__(WAVES * 64, DP == 64 ? 4 : 2) attention_kernel
         }
         if (tile + 1 < tiles) put(tile + 1);
     }
+    top -= kRaise<T>;
     const float total = sum + swapped(sum);
     if (query >= at.nq) return;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
@@ -317,7 +323,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
         for (int i = 3; i < 15; i += 2) most = larger(most, s[i], s[i + 1]);
         most = larger(most, s[15]);
         most = larger(most, swapped(most)) * p.scale;
-        const bool grows = most > top + kSlack || (top == -INFINITY && most > top);
+        const bool grows = most > top + kSlack<T> || (top == -INFINITY && most > top);
         if (__any(grows)) {             // each query by itself: its roundings are no matter of the others'
             const float now = grows ? most : top, shrink = top == now ? 1.0f : exp2f(top - now);
             top = now;
@@ -327,7 +333,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= shrink;
         }
-        const float base = top == -INFINITY ? 0.0f : top;
+        const float base = top == -INFINITY ? 0.0f : top - kRaise<T>;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale, -base));
@@ -343,6 +349,7 @@ __global__ void __launch_bounds__(256, 2) few_kernel(AttentionArgs p)
     }
     // the waves' parts together: maxima and sums of all, then the weighted values, two waves into two, one into one
     sum += swapped(sum);
+    top -= kRaise<T>;
     if (half == 0) {
         s_top[wave][lane] = top;
         s_sum[wave][lane] = sum;

@@ -1248,3 +1248,24 @@ def test_keys_of_minus_infinity_have_no_weight(P, dtype, dim, queries, keys):
         # the weights are those of the other keys: at most 5 / 4 of what the bound takes them to be
         within(out, want[0], 2 * (bound[0] + u * (np.abs(want[0]) + bound[0])) + SMALL[dtype], "out")
         within(lse, want[1], 2 * bound[1], "lse")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim,queries,keys,causal", [(64, 600, 600, True), (64, 600, 600, False), (128, 300, 600, False), (128, 1, 8000, True), (40, 3, 3000, True)])
+@pytest.mark.parametrize("ahead", [8.0, 12.0, 16.0])
+def test_attention_beside_a_key_that_takes_the_weight(P, dtype, dim, queries, keys, causal, ahead):
+    """One key takes nearly all of each query's weight and has no value: the output is that of the others, as exact as the
+    type holds it."""
+    q, k, v, _ = attention_inputs(dtype, queries, keys, 2, 1, dim, seed=int(ahead))
+    q *= 0.3
+    k *= 0.3
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    k[0, :, 0] = ahead * dim ** 0.5 / 8.0
+    v[0] = 0.0
+    v *= 256.0
+    at = [whole_numbers([0, n]) for n in (queries, keys)]
+    out, _ = P.attention(q, k, v, *at, causal=causal)
+    want = attention_oracle(f64(q), f64(k), f64(v), [queries], [0, keys], [keys], causal, dim ** -0.5)[0][0]
+    few_roundings(out, want, dtype, "out")
