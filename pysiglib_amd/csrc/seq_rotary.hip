@@ -312,6 +312,7 @@ void run(int dtype, RotaryArgs& p, bool interleaved, bool back, float* dqw, floa
     require(p.dim >= 2 && p.dim % 2 == 0 && p.dim <= 256, "a head has 2 to 256 channels, an even number");
     require(p.rotary >= 0 && p.rotary % 2 == 0 && p.rotary <= p.dim, "the rotary part is an even number of a head's channels");
     require(p.heads >= 0 && p.kv_heads >= 0 && p.heads + p.kv_heads < (1 << 20) && p.tokens < (int64_t(1) << 31), "too many heads or tokens");
+    require(!back || (dqw && dkw), "a tensor is missing");
     if (p.tokens == 0 || p.heads + p.kv_heads == 0) {
         if (back) {        // no pieces: zeros
             hipLaunchKernelGGL(weights_kernel, dim3((2 * p.dim + 3) / 4), dim3(kThreads), 0, static_cast<hipStream_t>(stream), p.parts, 0, p.dim, dqw, dkw);

@@ -1269,3 +1269,14 @@ def test_attention_beside_a_key_that_takes_the_weight(P, dtype, dim, queries, ke
     out, _ = P.attention(q, k, v, *at, causal=causal)
     want = attention_oracle(f64(q), f64(k), f64(v), [queries], [0, keys], [keys], causal, dim ** -0.5)[0][0]
     few_roundings(out, want, dtype, "out")
+
+
+def test_weights_without_a_place_for_their_gradients_are_refused(P):
+    """Before anything reaches the GPU, also where there are no tokens and the gradients are zero."""
+    from pysiglib_amd import _loader as L
+    size = L.CUSIG_NORM_ROTARY_BACKPROP_WORKSPACE(8)
+    for tokens in (2, 0):
+        for at in (12, 13):
+            args = [0] + [256] * 13 + [tokens, 2, 2, 8, 8, 4, 16, 8, 16, 8, 16, 8, 16, 8, 1e-6, False, 256, size, 0]
+            args[at] = 0
+            assert L.CUSIG_NORM_ROTARY_BACKPROP(*args) == 2 and "missing" in L.last_error_message(), (tokens, at)
