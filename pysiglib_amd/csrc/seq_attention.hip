@@ -559,7 +559,7 @@ __attribute__((visibility("default"))) int cusig_amd_attention(
         p.heads = int(heads), p.kv_heads = int(kv_heads), p.dim = int(dim), p.causal = causal;
         p.scale = scale * 1.44269504088896341f;
         const Cut cut = cut_of(p.packed.q_rows, p.packed.k_rows, p.packed.n, p.heads, p.kv_heads, p.dim);
-        require(workspace_bytes >= cut.map + cut.parts && (workspace || cut.map + cut.parts == 0), "the workspace is too small");
+        check_workspace(workspace, workspace_bytes, cut.map + cut.parts);
         p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + cut.map);
         p.splits = cut.splits;
         require(cut.tiles * (cut.few ? p.kv_heads * int64_t(p.splits) : p.heads) < (int64_t(1) << 31), "too many queries and heads");

@@ -592,7 +592,7 @@ __attribute__((visibility("default"))) int cusig_amd_attention_backprop(
         require(dim >= 8 && dim <= 128 && dim % 8 == 0, "a head has 8 to 128 channels, a multiple of 8");
         require(kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads < (1u << 20), "heads are a multiple of the key heads");
         require(scale > 0.0f && std::isfinite(scale), "the scale is positive and finite");
-        require(workspace && workspace_bytes >= cusig_amd_attention_backprop_workspace(q_rows, k_rows, sequences, heads, dim), "the workspace is too small");
+        check_workspace(workspace, workspace_bytes, cusig_amd_attention_backprop_workspace(q_rows, k_rows, sequences, heads, dim));
         check_strides({q_token, k_token, v_token, grad_token});
         if (sequences == 0) return;
         require(q_offsets && k_offsets && (q_rows == 0 || (grad_out && q && out && lse && dq)) && (k_rows == 0 || (k && v && dk && dv)), "a tensor is missing");

@@ -119,6 +119,12 @@ inline void require(bool ok, const char* what)
     if (!ok) throw std::invalid_argument(what);
 }
 
+inline void check_workspace(const void* workspace, uint64_t bytes, uint64_t need)
+{
+    require(bytes >= need && (workspace || need == 0), "the workspace is too small");
+    require(reinterpret_cast<uintptr_t>(workspace) % 256 == 0 || need == 0, "the workspace is not aligned to 256 bytes");
+}
+
 // A launch numbers its threads with 32 bits: more blocks go in several, each of which tells its kernel what its first one is.
 // Multiples of eight: a block stays on its die.
 template <typename Launch>

@@ -613,10 +613,10 @@ void scan(ScanArgs p, void* workspace, size_t bytes, hipStream_t stream)
     require(p.end && (p.rows == 0 || (p.gate && p.in && p.out && (!BACK || (p.h && p.out2)))), "a tensor is missing");
     const Plan plan = plan_of<T, BACK>(p.rows, p.n, p.channels);
     const size_t need = scan_workspace<T, BACK>(p.rows, p.n, p.channels);
-    require(bytes >= need && (workspace || need == 0), "the workspace is too small");
     const int64_t widest = p.gate_stride > p.in_stride ? p.gate_stride : p.in_stride;
     require(p.gate_stride >= 0 && p.in_stride >= 0 && (widest > p.channels ? widest : p.channels) <= (int64_t(1) << 20),
             "rows are at most 2^20 elements long and apart");
+    check_workspace(workspace, bytes, need);
     p.chunks = plan.chunks;
     p.channel_blocks = plan.channel_blocks;
     // (gradients of 8 sequences of 2048 steps, 2048 channels, bfloat16, alone: 65 us, through the caches 96 us)

@@ -367,7 +367,7 @@ __attribute__((visibility("default"))) int cusig_amd_norm_rotary_backprop(
 {
     return sigamd::guarded([&] {
         require(heads < (1u << 20) && kv_heads < (1u << 20) && dim <= 256 && rotary_dim <= dim && tokens < (uint64_t(1) << 31) && table < (uint64_t(1) << 31), "too many heads, channels or tokens");
-        require(workspace && workspace_bytes >= cusig_amd_norm_rotary_backprop_workspace(dim), "the workspace is too small");
+        check_workspace(workspace, workspace_bytes, cusig_amd_norm_rotary_backprop_workspace(dim));
         RotaryArgs p{};
         p.q = q, p.k = k, p.gq = grad_q, p.gk = grad_k, p.qw = q_weight, p.kw = k_weight, p.cos = cos, p.sin = sin, p.positions = positions, p.oq = dq, p.ok = dk;
         p.parts = static_cast<float*>(workspace);

@@ -1280,3 +1280,17 @@ def test_weights_without_a_place_for_their_gradients_are_refused(P):
             args = [0] + [256] * 13 + [tokens, 2, 2, 8, 8, 4, 16, 8, 16, 8, 16, 8, 16, 8, 1e-6, False, 256, size, 0]
             args[at] = 0
             assert L.CUSIG_NORM_ROTARY_BACKPROP(*args) == 2 and "missing" in L.last_error_message(), (tokens, at)
+
+
+def test_a_workspace_that_is_not_aligned_is_refused(P):
+    """Words of it are 64-bit and accessed at once; before anything reaches the GPU."""
+    from pysiglib_amd import _loader as L
+    far = 1 << 40
+    calls = [(L.CUSIG_LINEAR_RECURRENCE, [0, 256, 256, 0, 256, 256, 0, 1, 100000, 100000, 8, 8, 8]),
+             (L.CUSIG_LINEAR_RECURRENCE_BACKPROP, [0, 256, 256, 256, 0, 0, 256, 256, 256, 0, 1, 100000, 100000, 8, 8, 8]),
+             (L.CUSIG_NORM_ROTARY_BACKPROP, [0] + [256] * 13 + [2, 2, 2, 8, 8, 4, 16, 8, 16, 8, 16, 8, 16, 8, 1e-6, False]),
+             (L.CUSIG_ATTENTION, [1] + [256] * 5 + [0, 256, 256, 100000, 100000, 100, 2, 1, 64, 128, 64, 64, 64, 64, 64, 0.1, True]),
+             (L.CUSIG_ATTENTION_BACKPROP, [1] + [256] * 11 + [4, 4, 1, 2, 1, 64, 128, 64, 64, 64, 64, 64, 128, 64, 0.1, True])]
+    for fn, args in calls:
+        assert fn(*args, 260, far, 0) == 2 and "aligned" in L.last_error_message(), fn
+        assert fn(*args, 256, 0, 0) == 2 and "too small" in L.last_error_message(), fn
