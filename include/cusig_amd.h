@@ -418,6 +418,75 @@ CUSIG_AMD_API int cusig_amd_attention_backprop(int dtype, const void* grad_out, 
 CUSIG_AMD_API uint64_t cusig_amd_attention_backprop_workspace(uint64_t q_rows, uint64_t k_rows, uint64_t sequences, uint64_t heads,
                                                               uint64_t dim) CUSIG_AMD_NOEXCEPT;
 
+/* s = x + residual as it is stored in the residual's type (residual_dtype: dtype or float32), out = s (mean s^2 + eps)^-1/2 weight for each
+ * row; residual null: s is x, total is not written.  out and total contiguous, weight float32 [channels]; 1 to 16384 channels.
+ * scales not null: out is float8 e4m3 with the scale max |out| / 448 of each row (1 where the row is zero or holds NaN). */
+CUSIG_AMD_API int cusig_amd_norm_residual(int dtype, int residual_dtype, const void* x, const void* residual, const float* weight, void* out,
+                                          void* total, float* scales, uint64_t rows, uint64_t channels, int64_t x_stride,
+                                          int64_t residual_stride, float eps, void* stream) CUSIG_AMD_NOEXCEPT;
+CUSIG_AMD_API uint64_t cusig_amd_norm_residual_backprop_workspace(uint64_t channels) CUSIG_AMD_NOEXCEPT;
+/* Its gradients, from s (`total`) and the gradients of out and s (grad_total may be null: zero): dx in dtype, dresidual in residual_dtype,
+ * contiguous (dresidual may be null where the types are the same: it is dx), dweight. */
+CUSIG_AMD_API int cusig_amd_norm_residual_backprop(int dtype, int residual_dtype, const void* grad_out, const void* grad_total,
+                                                   const void* total, const float* weight, void* dx, void* dresidual, float* dweight,
+                                                   uint64_t rows, uint64_t channels, int64_t grad_out_stride,
+                                                   int64_t grad_total_stride, int64_t total_stride, float eps, void* workspace,
+                                                   uint64_t workspace_bytes, void* stream) CUSIG_AMD_NOEXCEPT;
+
+/* y_t = f(bias + sum_k weight[k] x_{t - width + 1 + k}) for each channel, f(v) = v / (1 + exp(-v)) (silu) or v; rows before a sequence's
+ * first are those of its initial state.  x, y [rows, channels] (y contiguous), offsets or null as above, weight float32
+ * [channels, width], bias float32 [channels] or null, width 1 to 8; initial_state (may be null: zero) and final_state (the last width - 1
+ * rows) [sequences, width - 1, channels] in x's type. */
+CUSIG_AMD_API int cusig_amd_causal_conv(int dtype, const void* x, const float* weight, const float* bias, const void* initial_state, void* y,
+                                        void* final_state, const int* offsets, uint64_t sequences, uint64_t length, uint64_t rows,
+                                        uint64_t channels, uint64_t width, int64_t x_stride, bool silu, void* stream) CUSIG_AMD_NOEXCEPT;
+CUSIG_AMD_API uint64_t cusig_amd_causal_conv_backprop_workspace(uint64_t rows, uint64_t channels, uint64_t width) CUSIG_AMD_NOEXCEPT;
+/* Its gradients from the inputs and the gradients of both outputs (grad_final may be null: zero); grad_bias may be null. */
+CUSIG_AMD_API int cusig_amd_causal_conv_backprop(int dtype, const void* grad_y, const void* x, const float* weight, const float* bias,
+                                                 const void* initial_state, const void* grad_final, void* grad_x, float* grad_weight,
+                                                 float* grad_bias, void* grad_initial, const int* offsets, uint64_t sequences,
+                                                 uint64_t length, uint64_t rows, uint64_t channels, uint64_t width,
+                                                 int64_t grad_stride, int64_t x_stride, bool silu, void* workspace,
+                                                 uint64_t workspace_bytes, void* stream) CUSIG_AMD_NOEXCEPT;
+/* One row of each sequence: y from x and state [rows, width - 1, channels], which becomes the rows behind it. */
+CUSIG_AMD_API int cusig_amd_causal_conv_step(int dtype, const void* x, void* state, const float* weight, const float* bias, void* y,
+                                             uint64_t rows, uint64_t channels, uint64_t width, int64_t x_stride, bool silu,
+                                             void* stream) CUSIG_AMD_NOEXCEPT;
+
+/* h_t = exp(dt_t a) h_{t-1} + dt_t x_t b_t for each channel and state, y_t = (sum over states of c_t h_t + d x_t) f(z_t), with dt = softplus(delta +
+ * delta_bias) or delta + delta_bias and f(z) = z / (1 + exp(-z)); d, z and delta_bias may be null.  x, delta, z, y [rows, channels]
+ * (y contiguous), offsets or null as above; a float32 [channels, states], d and delta_bias float32 [channels]; b, c [rows, groups,
+ * states], the last axis contiguous: neighbouring channels share a group's; 1 to 64 states.  initial_state (may be null: zero) and
+ * final_state float32 [sequences, channels, states]. */
+CUSIG_AMD_API int cusig_amd_selective_scan(int dtype, const void* x, const void* delta, const float* a, const void* b, const void* c,
+                                           const float* d, const void* z, const float* delta_bias, const float* initial_state, void* y,
+                                           float* final_state, const int* offsets, uint64_t sequences, uint64_t length, uint64_t rows,
+                                           uint64_t channels, uint64_t states, uint64_t groups, int64_t x_stride, int64_t delta_stride,
+                                           int64_t z_stride, int64_t b_stride, int64_t b_group, int64_t c_stride, int64_t c_group,
+                                           bool softplus, void* workspace, uint64_t workspace_bytes, void* stream) CUSIG_AMD_NOEXCEPT;
+CUSIG_AMD_API uint64_t cusig_amd_selective_scan_workspace(bool packed, uint64_t sequences, uint64_t length, uint64_t rows, uint64_t channels,
+                                                          uint64_t states, uint64_t groups) CUSIG_AMD_NOEXCEPT;
+/* Its gradients from the inputs and the gradients of both outputs (grad_final may be null: zero); all contiguous, those of d, z and
+ * delta_bias only where these are given; those of a, d, delta_bias and the initial state float32. */
+CUSIG_AMD_API int cusig_amd_selective_scan_backprop(int dtype, const void* grad_y, const void* x, const void* delta, const float* a,
+                                                    const void* b, const void* c, const float* d, const void* z,
+                                                    const float* delta_bias, const float* grad_final, const float* initial_state,
+                                                    void* grad_x, void* grad_delta, float* grad_a, void* grad_b, void* grad_c,
+                                                    float* grad_d, void* grad_z, float* grad_delta_bias, float* grad_initial,
+                                                    const int* offsets, uint64_t sequences, uint64_t length, uint64_t rows,
+                                                    uint64_t channels, uint64_t states, uint64_t groups, int64_t grad_stride,
+                                                    int64_t x_stride, int64_t delta_stride, int64_t z_stride, int64_t b_stride,
+                                                    int64_t b_group, int64_t c_stride, int64_t c_group, bool softplus,
+                                                    void* workspace, uint64_t workspace_bytes, void* stream) CUSIG_AMD_NOEXCEPT;
+CUSIG_AMD_API uint64_t cusig_amd_selective_scan_backprop_workspace(bool packed, uint64_t sequences, uint64_t length, uint64_t rows,
+                                                                   uint64_t channels, uint64_t states, uint64_t groups) CUSIG_AMD_NOEXCEPT;
+/* One row of each sequence: state [rows, channels, states] float32 becomes the one behind it. */
+CUSIG_AMD_API int cusig_amd_selective_scan_step(int dtype, const void* x, const void* delta, const float* a, const void* b, const void* c,
+                                                const float* d, const void* z, const float* delta_bias, float* state, void* y,
+                                                uint64_t rows, uint64_t channels, uint64_t states, uint64_t groups, int64_t x_stride,
+                                                int64_t delta_stride, int64_t z_stride, int64_t b_stride, int64_t b_group,
+                                                int64_t c_stride, int64_t c_group, bool softplus, void* stream) CUSIG_AMD_NOEXCEPT;
+
 #ifdef __cplusplus
 }
 #endif

@@ -144,6 +144,25 @@ CUSIG_ATTENTION_BACKPROP = _sequence("attention_backprop", "ipppppppppppuuuuuuss
 CUSIG_ATTENTION_BACKPROP_WORKSPACE = _sequence("attention_backprop_workspace", "uuuuu")
 CUSIG_ATTENTION_BACKPROP_WORKSPACE.restype = c_uint64
 
+CUSIG_NORM_RESIDUAL = _sequence("norm_residual", "iippppppuussfp")
+CUSIG_NORM_RESIDUAL_BACKPROP = _sequence("norm_residual_backprop", "iipppppppuusssfpup")
+CUSIG_NORM_RESIDUAL_BACKPROP_WORKSPACE = _sequence("norm_residual_backprop_workspace", "u")
+CUSIG_NORM_RESIDUAL_BACKPROP_WORKSPACE.restype = c_uint64
+
+CUSIG_CAUSAL_CONV = _sequence("causal_conv", "ipppppppuuuuusbp")
+CUSIG_CAUSAL_CONV_BACKPROP = _sequence("causal_conv_backprop", "ipppppppppppuuuuussbpup")
+CUSIG_CAUSAL_CONV_BACKPROP_WORKSPACE = _sequence("causal_conv_backprop_workspace", "uuu")
+CUSIG_CAUSAL_CONV_BACKPROP_WORKSPACE.restype = c_uint64
+CUSIG_CAUSAL_CONV_STEP = _sequence("causal_conv_step", "ipppppuuusbp")
+
+CUSIG_SELECTIVE_SCAN = _sequence("selective_scan", "ippppppppppppuuuuuusssssssbpup")
+CUSIG_SELECTIVE_SCAN_WORKSPACE = _sequence("selective_scan_workspace", "buuuuuu")
+CUSIG_SELECTIVE_SCAN_WORKSPACE.restype = c_uint64
+CUSIG_SELECTIVE_SCAN_BACKPROP = _sequence("selective_scan_backprop", "ipppppppppppppppppppppuuuuuussssssssbpup")
+CUSIG_SELECTIVE_SCAN_BACKPROP_WORKSPACE = _sequence("selective_scan_backprop_workspace", "buuuuuu")
+CUSIG_SELECTIVE_SCAN_BACKPROP_WORKSPACE.restype = c_uint64
+CUSIG_SELECTIVE_SCAN_STEP = _sequence("selective_scan_step", "ippppppppppuuuusssssssbp")
+
 
 def last_error_message():
     msg = CUSIG.cusig_last_error_message()

@@ -1,5 +1,6 @@
 """Layers of a sequence model over path features: the gated linear recurrence, norms of queries and keys with the rotation by
-position, and causal attention over packed sequences, each with its gradients and its form for single tokens.
+position, and causal attention over packed sequences; the norm of the residual stream, the short causal convolution and the selective scan
+of a state space block; each with its gradients and its form for single tokens.
 
 They take the place after the signature: windows of a path give signatures, these are the tokens.  No counterpart in the
 reference.  Tensors are float32, bfloat16 or float16 on one GPU; sums, states and norms are 32-bit throughout.  The work is
@@ -16,9 +17,12 @@ import math
 import torch
 
 from ._loader import (CUSIG_ATTENTION, CUSIG_ATTENTION_BACKPROP, CUSIG_ATTENTION_BACKPROP_WORKSPACE,
-                      CUSIG_ATTENTION_WORKSPACE, CUSIG_LINEAR_RECURRENCE, CUSIG_LINEAR_RECURRENCE_BACKPROP, CUSIG_LINEAR_RECURRENCE_STEP,
+                      CUSIG_ATTENTION_WORKSPACE, CUSIG_CAUSAL_CONV, CUSIG_CAUSAL_CONV_BACKPROP, CUSIG_CAUSAL_CONV_BACKPROP_WORKSPACE,
+                      CUSIG_CAUSAL_CONV_STEP, CUSIG_LINEAR_RECURRENCE, CUSIG_LINEAR_RECURRENCE_BACKPROP, CUSIG_LINEAR_RECURRENCE_STEP,
                       CUSIG_LINEAR_RECURRENCE_WORKSPACE, CUSIG_NORM_ROTARY, CUSIG_NORM_ROTARY_BACKPROP,
-                      CUSIG_NORM_ROTARY_BACKPROP_WORKSPACE, SEQUENCE_DTYPES)
+                      CUSIG_NORM_ROTARY_BACKPROP_WORKSPACE, CUSIG_NORM_RESIDUAL, CUSIG_NORM_RESIDUAL_BACKPROP,
+                      CUSIG_NORM_RESIDUAL_BACKPROP_WORKSPACE, CUSIG_SELECTIVE_SCAN, CUSIG_SELECTIVE_SCAN_BACKPROP,
+                      CUSIG_SELECTIVE_SCAN_BACKPROP_WORKSPACE, CUSIG_SELECTIVE_SCAN_STEP, CUSIG_SELECTIVE_SCAN_WORKSPACE, SEQUENCE_DTYPES)
 from .data_handlers import on_device
 from .error_codes import err_msg
 from .param_checks import check_type
@@ -375,3 +379,331 @@ def attention_backprop(grad_out, q, k, v, out, lse, q_offsets, k_offsets, *, cau
           v.data_ptr(), out.data_ptr(), lse.data_ptr(), q_offsets.data_ptr(), k_offsets.data_ptr(), dq.data_ptr(), dk.data_ptr(),
           dv.data_ptr(), *sizes, *rest[:6], g_token, g_head, *rest[6:], space.data_ptr(), size)
     return dq, dk, dv
+
+
+def _norm_args(x, residual, weight):
+    """(x, its rows' distance, residual or None, its rows' distance, the sum's type, weight, rows, channels)."""
+    _tensor(x, "x")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 16384:
+        raise ValueError("x must have rows of 1 to 16384 channels")
+    channels, device = x.shape[-1], x.device
+    weight = _other(weight, "weight", torch.float32, (channels,), device)
+    step = 0
+    if residual is not None:
+        if not isinstance(residual, torch.Tensor):
+            raise TypeError("residual must be a torch tensor, got " + type(residual).__name__ + " instead")
+        if residual.dtype not in (x.dtype, torch.float32):
+            raise TypeError("residual.dtype must be " + str(x.dtype) + " or torch.float32, got " + str(residual.dtype) + " instead")
+        if residual.shape != x.shape:
+            raise ValueError("x and residual must have the same shape")
+        if residual.device != device:
+            raise ValueError("residual must be on " + str(device) + ", got " + str(residual.device))
+        residual, step = _rows(residual if residual.dim() > 1 else residual[None])
+    rows = x.numel() // channels
+    x, x_step = _rows(x if x.dim() > 1 else x[None])
+    return x, x_step, residual, step, x.dtype if residual is None else residual.dtype, weight, rows, channels
+
+
+def norm_residual(x, residual, weight, *, eps=1e-6):
+    """``total = x + residual`` and its root-mean-square norm with a weight for each channel, in one pass.
+
+    ``x`` ``(..., channels)``, up to 16384 of them; ``residual`` of the same shape, in the type of ``x`` or float32, or None: ``total`` is then
+    ``x`` itself; ``weight`` float32 ``(channels,)``.  The norm is of ``total`` as it is stored, in the residual's type.
+
+    Returns ``(out, total)``: ``out`` in the type of ``x``, contiguous.
+    """
+    shape, like = x.shape if isinstance(x, torch.Tensor) else None, x
+    x, x_step, residual, step, kind, weight, rows, channels = _norm_args(x, residual, weight)
+    out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    total = like if residual is None else torch.empty(shape, dtype=kind, device=x.device)
+    _call(CUSIG_NORM_RESIDUAL, "norm_residual", x.device, _CODES[x.dtype], _CODES[kind], x.data_ptr(),
+          0 if residual is None else residual.data_ptr(), weight.data_ptr(), out.data_ptr(), 0 if residual is None else total.data_ptr(),
+          0, rows, channels, x_step, step, eps)
+    return out, total
+
+
+def norm_residual_float8(x, residual, weight, *, eps=1e-6):
+    """``norm_residual`` with its output in 8 bits: ``out`` is ``float8_e4m3fn`` and stands for ``out * scales``, ``scales`` float32
+    ``(..., 1)`` the largest value of each row divided by 448 (1 where a row is zero or holds NaN).  Returns ``(out, scales, total)``."""
+    shape, like = x.shape if isinstance(x, torch.Tensor) else None, x
+    x, x_step, residual, step, kind, weight, rows, channels = _norm_args(x, residual, weight)
+    out = torch.empty(shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((*shape[:-1], 1), dtype=torch.float32, device=x.device)
+    total = like if residual is None else torch.empty(shape, dtype=kind, device=x.device)
+    if rows:
+        _call(CUSIG_NORM_RESIDUAL, "norm_residual_float8", x.device, _CODES[x.dtype], _CODES[kind], x.data_ptr(),
+              0 if residual is None else residual.data_ptr(), weight.data_ptr(), out.data_ptr(), 0 if residual is None else total.data_ptr(),
+              scales.data_ptr(), rows, channels, x_step, step, eps)
+    return out, scales, total
+
+
+def norm_residual_backprop(grad_out, total, weight, *, grad_total=None, eps=1e-6):
+    """Gradients of ``norm_residual`` from the gradients of its outputs (``grad_total`` like ``total``, zero where it is not given) and
+    ``total``.  Returns ``(grad_x, grad_residual, grad_weight)``: the first in the type of ``grad_out``, which is that of ``x``, the second in that of
+    ``total`` (where the types are the same, both are one tensor); the weight's is summed over the rows in a fixed order."""
+    _tensor(grad_out, "grad_out")
+    shape, dtype = grad_out.shape, grad_out.dtype
+    if not isinstance(total, torch.Tensor):
+        raise TypeError("total must be a torch tensor, got " + type(total).__name__ + " instead")
+    total_step = _norm_args(grad_out, total, weight)
+    grad_out, grad_step, total, step, kind, weight, rows, channels = total_step
+    after = 0
+    if grad_total is not None:
+        _tensor(grad_total, "grad_total", like=total)
+        if grad_total.shape != shape:
+            raise ValueError("grad_total must have the shape of total")
+        grad_total, after = _rows(grad_total if grad_total.dim() > 1 else grad_total[None])
+    device = grad_out.device
+    dx = torch.empty(shape, dtype=dtype, device=device)
+    dr = dx if kind == dtype else torch.empty(shape, dtype=kind, device=device)
+    dw = torch.empty(channels, dtype=torch.float32, device=device)
+    size = CUSIG_NORM_RESIDUAL_BACKPROP_WORKSPACE(channels)
+    space = _workspace(size, device)
+    _call(CUSIG_NORM_RESIDUAL_BACKPROP, "norm_residual_backprop", device, _CODES[dtype], _CODES[kind], grad_out.data_ptr(),
+          0 if grad_total is None else grad_total.data_ptr(), total.data_ptr(), weight.data_ptr(), dx.data_ptr(), dr.data_ptr(), dw.data_ptr(),
+          rows, channels, grad_step, after, step, eps, space.data_ptr(), size)
+    return dx, dr, dw
+
+
+def _conv_args(x, weight, bias, silu, offsets):
+    check_type(silu, "silu", bool)
+    _tensor(x, "x")
+    if x.dim() < 2:
+        raise ValueError("x must have at least rank 2, got rank " + str(x.dim()) + ".")
+    device, channels = x.device, x.shape[-1]
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError("weight must have shape (" + str(channels) + ", width)")
+    width = weight.shape[1]
+    if not 1 <= width <= 8:
+        raise ValueError("weight must have 1 to 8 taps for each channel, got " + str(width))
+    weight = _other(weight, "weight", torch.float32, (channels, width), device)
+    if bias is not None:
+        bias = _other(bias, "bias", torch.float32, (channels,), device)
+    if offsets is not None:
+        offsets = _offsets(offsets, "offsets", device)
+    return weight, bias, offsets, width, _sequences(x, offsets, "x")
+
+
+def causal_conv(x, weight, bias=None, *, initial_state=None, offsets=None, silu=True):
+    """Short causal convolution of each channel, ``y_t = f(bias + sum_k weight[:, k] * x_{t - width + 1 + k})`` with ``f(v) = v * sigmoid(v)``
+    (``silu``) or ``f(v) = v``.
+
+    ``x``: ``(..., length, channels)``, or with ``offsets`` ``(rows, channels)``, the sequences packed.  ``weight`` float32 ``(channels,
+    width)``, 1 to 8 taps, the last for the row itself; ``bias`` float32 ``(channels,)``.  ``initial_state``: the ``width - 1`` rows before
+    each sequence, in the type of ``x``, ``(..., width - 1, channels)``, with ``offsets`` ``(sequences, width - 1, channels)``; zero where it is not
+    given.
+
+    Returns ``(y, final_state)``: ``y`` like ``x``, and the last ``width - 1`` rows of each sequence like ``initial_state``.
+    """
+    weight, bias, offsets, width, (n, length, rows, lead, at) = _conv_args(x, weight, bias, silu, offsets)
+    device, dtype, channels = x.device, x.dtype, x.shape[-1]
+    state = (*lead, width - 1, channels)
+    if initial_state is not None:
+        initial_state = _other(initial_state, "initial_state", dtype, state, device)
+    y = torch.empty(x.shape, dtype=dtype, device=device)
+    final = torch.empty(state, dtype=dtype, device=device)
+    x, x_step = _rows(x)
+    _call(CUSIG_CAUSAL_CONV, "causal_conv", device, _CODES[dtype], x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+          0 if initial_state is None else initial_state.data_ptr(), y.data_ptr(), final.data_ptr(), at, n, length, rows, channels, width,
+          x_step, silu)
+    return y, final
+
+
+def causal_conv_backprop(grad_y, x, weight, bias=None, *, grad_final=None, initial_state=None, offsets=None, silu=True):
+    """Gradients of ``causal_conv`` from the gradients of its outputs (``grad_final`` like the final state, zero where it is not given) and its
+    inputs.  Returns ``(grad_x, grad_weight, grad_bias, grad_initial_state)``, the third None where there is no bias; the weights' are
+    summed over the rows in a fixed order."""
+    weight, bias, offsets, width, (n, length, rows, lead, at) = _conv_args(x, weight, bias, silu, offsets)
+    _tensor(grad_y, "grad_y", like=x)
+    if grad_y.shape != x.shape:
+        raise ValueError("grad_y and x must have the same shape")
+    device, dtype, channels = x.device, x.dtype, x.shape[-1]
+    state = (*lead, width - 1, channels)
+    if initial_state is not None:
+        initial_state = _other(initial_state, "initial_state", dtype, state, device)
+    if grad_final is not None:
+        grad_final = _other(grad_final, "grad_final", dtype, state, device)
+    dx = torch.empty(x.shape, dtype=dtype, device=device)
+    dw = torch.empty((channels, width), dtype=torch.float32, device=device)
+    db = None if bias is None else torch.empty(channels, dtype=torch.float32, device=device)
+    d0 = torch.empty(state, dtype=dtype, device=device)
+    x, x_step = _rows(x)
+    grad_y, grad_step = _rows(grad_y)
+    size = CUSIG_CAUSAL_CONV_BACKPROP_WORKSPACE(rows, channels, width)
+    space = _workspace(size, device) if size else None
+    _call(CUSIG_CAUSAL_CONV_BACKPROP, "causal_conv_backprop", device, _CODES[dtype], grad_y.data_ptr(), x.data_ptr(), weight.data_ptr(),
+          0 if bias is None else bias.data_ptr(), 0 if initial_state is None else initial_state.data_ptr(),
+          0 if grad_final is None else grad_final.data_ptr(), dx.data_ptr(), dw.data_ptr(), 0 if bias is None else db.data_ptr(), d0.data_ptr(),
+          at, n, length, rows, channels, width, grad_step, x_step, silu, space.data_ptr() if size else 0, size)
+    return dx, dw, db, d0
+
+
+def causal_conv_step(x, state, weight, bias=None, *, silu=True):
+    """One row of ``causal_conv`` for single tokens: ``x`` ``(..., channels)``; ``state`` ``(..., width - 1, channels)``, the rows before it, of
+    the same type, contiguous, is replaced by the rows before the next.  Returns ``y`` like ``x``."""
+    _tensor(x, "x")
+    shape, device, dtype = x.shape, x.device, x.dtype
+    if len(shape) < 1:
+        raise ValueError("x must have at least rank 1, got rank 0.")
+    weight, bias, _, width, _ = _conv_args(x if len(shape) > 1 else x[None], weight, bias, silu, None)
+    if _other(state, "state", dtype, (*shape[:-1], width - 1, shape[-1]), device) is not state:
+        raise ValueError("state must be contiguous: it is written")
+    y = torch.empty(shape, dtype=dtype, device=device)
+    x, x_step = _rows(x if len(shape) > 1 else x[None])
+    channels = shape[-1]
+    _call(CUSIG_CAUSAL_CONV_STEP, "causal_conv_step", device, _CODES[dtype], x.data_ptr(), state.data_ptr(), weight.data_ptr(),
+          0 if bias is None else bias.data_ptr(), y.data_ptr(), y.numel() // channels if channels else 0, channels, width, x_step, silu)
+    torch.autograd.graph.increment_version(state)
+    return y
+
+
+def _shared(value, name, like, groups, states):
+    """``b`` or ``c``, ``(..., groups, states)``: (tensor, distance of its rows, of its groups)."""
+    _tensor(value, name, like=like)
+    shape = (*like.shape[:-1], groups, states)
+    if value.shape != shape:
+        raise ValueError(name + " must have shape " + str(shape) + ", got " + str(tuple(value.shape)))
+    if value.stride(-1) != 1 and states > 1:
+        value = value.contiguous()
+    # rows a fixed distance apart
+    want = None
+    for axis in range(value.dim() - 3, -1, -1):
+        if value.shape[axis] == 1:
+            continue
+        if want is not None and value.stride(axis) != want:
+            value = value.contiguous()
+            return value, groups * states, states
+        want = value.stride(axis) * value.shape[axis]
+    step = next((value.stride(axis) for axis in range(value.dim() - 3, -1, -1) if value.shape[axis] != 1), groups * states)
+    return value, step, value.stride(-2)
+
+
+def _scan_args(x, delta, a, b, c, d, z, delta_bias, softplus):
+    """Checked inputs, and (states, groups) and the strides that the entry points take."""
+    check_type(softplus, "softplus", bool)
+    _tensor(x, "x")
+    _tensor(delta, "delta", like=x)
+    if delta.shape != x.shape:
+        raise ValueError("x and delta must have the same shape")
+    device, channels = x.device, x.shape[-1]
+    if not isinstance(a, torch.Tensor) or a.dim() != 2 or not 1 <= a.shape[1] <= 64:
+        raise ValueError("a must have shape (" + str(channels) + ", states), with 1 to 64 states")
+    states = a.shape[1]
+    a = _other(a, "a", torch.float32, (channels, states), device)
+    if not isinstance(b, torch.Tensor) or b.dim() != x.dim() + 1:
+        raise ValueError("b must have shape (..., groups, states)")
+    groups = b.shape[-2]
+    if groups < 1 or channels % groups:
+        raise ValueError("the channels must be a multiple of the groups, got " + str(channels) + " and " + str(groups))
+    b, b_step, b_group = _shared(b, "b", x, groups, states)
+    c, c_step, c_group = _shared(c, "c", x, groups, states)
+    if d is not None:
+        d = _other(d, "d", torch.float32, (channels,), device)
+    if delta_bias is not None:
+        delta_bias = _other(delta_bias, "delta_bias", torch.float32, (channels,), device)
+    x, x_step = _rows(x)
+    delta, delta_step = _rows(delta)
+    z_step = 0
+    if z is not None:
+        _tensor(z, "z", like=x)
+        if z.shape != delta.shape:
+            raise ValueError("x and z must have the same shape")
+        z, z_step = _rows(z)
+    tensors = (x, delta, a, b, c, d, z, delta_bias)
+    return tensors, states, groups, (x_step, delta_step, z_step, b_step, b_group, c_step, c_group)
+
+
+def _addresses(tensors):
+    return tuple(0 if t is None else t.data_ptr() for t in tensors)
+
+
+def selective_scan(x, delta, a, b, c, *, d=None, z=None, delta_bias=None, softplus=True, initial_state=None, offsets=None):
+    """Scan of a selective state space model: for each channel and state ``h_t = exp(dt_t * a) * h_{t-1} + dt_t * b_t * x_t``, and
+    ``y_t = (sum over states of c_t * h_t + d * x_t) * z_t * sigmoid(z_t)``, with ``dt = softplus(delta + delta_bias)``, or without ``softplus``
+    ``delta + delta_bias``.
+
+    ``x``, ``delta``, ``z`` (the gate, or None): ``(..., length, channels)``, or with ``offsets`` ``(rows, channels)``, the sequences packed.
+    ``a`` float32 ``(channels, states)``, meant to be negative, 1 to 64 states; ``b``, ``c``: ``(..., length, groups, states)`` or
+    ``(rows, groups, states)``, each group's for ``channels / groups`` neighbouring channels; ``d``, ``delta_bias``: float32 ``(channels,)`` or None.
+    ``initial_state``: float32 ``(..., channels, states)``, with ``offsets`` ``(sequences, channels, states)``; zero where it is not given.
+
+    Returns ``(y, final_state)``: ``y`` like ``x``, the states behind the last steps like ``initial_state``.
+    """
+    _tensor(x, "x")
+    if x.dim() < 2:
+        raise ValueError("x must have at least rank 2, got rank " + str(x.dim()) + ".")
+    shape, device = x.shape, x.device
+    tensors, states, groups, strides = _scan_args(x, delta, a, b, c, d, z, delta_bias, softplus)
+    if offsets is not None:
+        offsets = _offsets(offsets, "offsets", device)
+    n, length, rows, lead, at = _sequences(x, offsets, "x")
+    channels = shape[-1]
+    state = (*lead, channels, states)
+    if initial_state is not None:
+        initial_state = _other(initial_state, "initial_state", torch.float32, state, device)
+    y = torch.empty(shape, dtype=x.dtype, device=device)
+    final = torch.empty(state, dtype=torch.float32, device=device)
+    size = CUSIG_SELECTIVE_SCAN_WORKSPACE(offsets is not None, n, length, rows, channels, states, groups)
+    space = _workspace(size, device) if size else None
+    _call(CUSIG_SELECTIVE_SCAN, "selective_scan", device, _CODES[x.dtype], *_addresses(tensors),
+          0 if initial_state is None else initial_state.data_ptr(), y.data_ptr(), final.data_ptr(), at, n, length, rows, channels, states, groups,
+          *strides, softplus, space.data_ptr() if size else 0, size)
+    return y, final
+
+
+def selective_scan_backprop(grad_y, x, delta, a, b, c, *, d=None, z=None, delta_bias=None, softplus=True, grad_final=None, initial_state=None,
+                            offsets=None):
+    """Gradients of ``selective_scan`` from the gradients of its outputs (``grad_final`` float32 like the final state, zero where it is not
+    given) and its inputs; the states are formed again.  Returns ``(grad_x, grad_delta, grad_a, grad_b, grad_c, grad_d, grad_z,
+    grad_delta_bias, grad_initial_state)``, None for what was not given; those of float32 inputs and of the initial state are float32.  The
+    same inputs give the same bits."""
+    _tensor(x, "x")
+    if x.dim() < 2:
+        raise ValueError("x must have at least rank 2, got rank " + str(x.dim()) + ".")
+    shape, device, dtype = x.shape, x.device, x.dtype
+    _tensor(grad_y, "grad_y", like=x)
+    if grad_y.shape != shape:
+        raise ValueError("grad_y and x must have the same shape")
+    tensors, states, groups, strides = _scan_args(x, delta, a, b, c, d, z, delta_bias, softplus)
+    if offsets is not None:
+        offsets = _offsets(offsets, "offsets", device)
+    n, length, rows, lead, at = _sequences(x, offsets, "x")
+    channels = shape[-1]
+    state = (*lead, channels, states)
+    if initial_state is not None:
+        initial_state = _other(initial_state, "initial_state", torch.float32, state, device)
+    if grad_final is not None:
+        grad_final = _other(grad_final, "grad_final", torch.float32, state, device)
+    grad_y, grad_step = _rows(grad_y)
+    make = lambda shape, kind=torch.float32: torch.empty(shape, dtype=kind, device=device)          # noqa: E731
+    grads = (make(shape, dtype), make(shape, dtype), make((channels, states)), make((*shape[:-1], groups, states), dtype),
+             make((*shape[:-1], groups, states), dtype), None if d is None else make(channels), None if z is None else make(shape, dtype),
+             None if delta_bias is None else make(channels), make(state))
+    size = CUSIG_SELECTIVE_SCAN_BACKPROP_WORKSPACE(offsets is not None, n, length, rows, channels, states, groups)
+    space = _workspace(size, device) if size else None
+    _call(CUSIG_SELECTIVE_SCAN_BACKPROP, "selective_scan_backprop", device, _CODES[dtype], grad_y.data_ptr(), *_addresses(tensors),
+          0 if grad_final is None else grad_final.data_ptr(), 0 if initial_state is None else initial_state.data_ptr(), *_addresses(grads),
+          at, n, length, rows, channels, states, groups, grad_step, *strides, softplus, space.data_ptr() if size else 0, size)
+    return grads
+
+
+def selective_scan_step(x, delta, a, b, c, state, *, d=None, z=None, delta_bias=None, softplus=True):
+    """One step of ``selective_scan`` for single tokens: ``x``, ``delta``, ``z`` ``(..., channels)``, ``b``, ``c`` ``(..., groups, states)``; ``state``
+    float32 ``(..., channels, states)``, contiguous, is replaced by the state behind the step.  Returns ``y`` like ``x``."""
+    _tensor(x, "x")
+    shape, device = x.shape, x.device
+    if len(shape) < 1:
+        raise ValueError("x must have at least rank 1, got rank 0.")
+    if len(shape) == 1:
+        if not all(isinstance(t, torch.Tensor) for t in (delta, b, c)):
+            raise TypeError("delta, b and c must be torch tensors")
+        x, delta, b, c, z = x[None], delta[None], b[None], c[None], z if z is None else z[None]
+    tensors, states, groups, strides = _scan_args(x, delta, a, b, c, d, z, delta_bias, softplus)
+    if _other(state, "state", torch.float32, (*shape, states), device) is not state:
+        raise ValueError("state must be contiguous: it is written")
+    y = torch.empty(shape, dtype=x.dtype, device=device)
+    channels = shape[-1]
+    _call(CUSIG_SELECTIVE_SCAN_STEP, "selective_scan_step", device, _CODES[x.dtype], *_addresses(tensors), state.data_ptr(), y.data_ptr(),
+          y.numel() // channels if channels else 0, channels, states, groups, *strides, softplus)
+    torch.autograd.graph.increment_version(state)
+    return y

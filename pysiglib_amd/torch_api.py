@@ -246,3 +246,81 @@ class Attention(torch.autograd.Function):
 def attention(q, k, v, q_offsets, k_offsets, *, causal=True, scale=None):
     """Differentiable ``attention`` of whole sequences; the output alone, without the sums' logarithms."""
     return Attention.apply(q, k, v, q_offsets, k_offsets, causal, scale)
+
+
+class NormResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        from .sequence import norm_residual as _norm_residual
+        out, total = _norm_residual(x, residual, weight, eps=eps)
+        ctx.save_for_backward(total, weight)
+        ctx.eps, ctx.alone, ctx.dtype = eps, residual is None, x.dtype
+        ctx.set_materialize_grads(False)
+        return (out, None) if ctx.alone else (out, total)
+
+    @staticmethod
+    def backward(ctx, grad_out, grad_total):
+        from .sequence import norm_residual_backprop as _norm_residual_backprop
+        total, weight = ctx.saved_tensors
+        if grad_out is None:
+            if grad_total is None:
+                return None, None, None, None
+            grad_out = torch.zeros(total.shape, dtype=ctx.dtype, device=total.device)
+        dx, dr, dw = _norm_residual_backprop(grad_out, total, weight, grad_total=grad_total, eps=ctx.eps)
+        return _once(dx, None if ctx.alone else dr, dw, None)
+
+
+def norm_residual(x, residual, weight, *, eps=1e-6):
+    """Differentiable ``norm_residual``; without a residual ``total`` is ``x`` itself."""
+    out, total = NormResidual.apply(x, residual, weight, eps)
+    return out, x if residual is None else total
+
+
+class CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, initial_state, offsets, silu):
+        from .sequence import causal_conv as _causal_conv
+        y, final = _causal_conv(x, weight, bias, initial_state=initial_state, offsets=offsets, silu=silu)
+        ctx.save_for_backward(x, weight, bias, initial_state, offsets)
+        ctx.silu = silu
+        ctx.set_materialize_grads(False)
+        return y, final
+
+    @staticmethod
+    def backward(ctx, grad_y, grad_final):
+        from .sequence import causal_conv_backprop as _causal_conv_backprop
+        x, weight, bias, initial_state, offsets = ctx.saved_tensors
+        grad_y = torch.zeros_like(x) if grad_y is None else grad_y
+        dx, dw, db, d0 = _causal_conv_backprop(grad_y, x, weight, bias, grad_final=grad_final, initial_state=initial_state, offsets=offsets,
+                                               silu=ctx.silu)
+        return _once(dx, dw, db, d0 if initial_state is not None else None, None, None)
+
+
+def causal_conv(x, weight, bias=None, *, initial_state=None, offsets=None, silu=True):
+    """Differentiable ``causal_conv``."""
+    return CausalConv.apply(x, weight, bias, initial_state, offsets, silu)
+
+
+class SelectiveScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, delta, a, b, c, d, z, delta_bias, initial_state, softplus, offsets):
+        from .sequence import selective_scan as _selective_scan
+        y, final = _selective_scan(x, delta, a, b, c, d=d, z=z, delta_bias=delta_bias, softplus=softplus, initial_state=initial_state, offsets=offsets)
+        ctx.save_for_backward(x, delta, a, b, c, d, z, delta_bias, initial_state, offsets)
+        ctx.softplus = softplus
+        ctx.set_materialize_grads(False)
+        return y, final
+
+    @staticmethod
+    def backward(ctx, grad_y, grad_final):
+        from .sequence import selective_scan_backprop as _selective_scan_backprop
+        x, delta, a, b, c, d, z, delta_bias, initial_state, offsets = ctx.saved_tensors
+        grad_y = torch.zeros_like(x) if grad_y is None else grad_y
+        grads = _selective_scan_backprop(grad_y, x, delta, a, b, c, d=d, z=z, delta_bias=delta_bias, softplus=ctx.softplus, grad_final=grad_final,
+                                         initial_state=initial_state, offsets=offsets)
+        return _once(*grads[:8], grads[8] if initial_state is not None else None, None, None)
+
+
+def selective_scan(x, delta, a, b, c, *, d=None, z=None, delta_bias=None, softplus=True, initial_state=None, offsets=None):
+    """Differentiable ``selective_scan``."""
+    return SelectiveScan.apply(x, delta, a, b, c, d, z, delta_bias, initial_state, softplus, offsets)
