@@ -137,6 +137,32 @@ void in_launches(int64_t blocks, int threads, Launch&& launch)
     }
 }
 
+// Sums over pieces: parts [pieces][columns], each column's sum goes to put(column, sum).  A block to 32 columns; 32 threads for each add up
+// every 32nd piece, then each other's sums: the order is fixed.
+constexpr int kSumThreads = 1024;
+
+template <typename F>
+__device__ __forceinline__ void sum_pieces(const float* parts, int pieces, int64_t columns, F&& put)
+{
+    __shared__ float s_sum[32][33];
+    const int lane = threadIdx.x % 32, row = threadIdx.x / 32;
+    const int64_t e = int64_t(blockIdx.x) * 32 + lane;
+    float sum = 0.0f;
+    if (e < columns)
+#pragma unroll 8
+        for (int n = row; n < pieces; n += 32) sum += parts[n * columns + e];
+    s_sum[row][lane] = sum;
+    __syncthreads();
+    // turned: a half wave to a column
+    sum = s_sum[lane][row];
+#pragma unroll
+    for (int m = 16; m; m /= 2) sum += __shfl_xor(sum, m);
+    const int64_t to = int64_t(blockIdx.x) * 32 + row;
+    if (lane == 0 && to < columns) put(to, sum);
+}
+
+inline dim3 sum_blocks(int64_t columns) { return dim3(static_cast<unsigned>((columns + 31) / 32)); }
+
 template <typename Args>
 void launch_all(void (*kernel)(Args), int64_t blocks, int threads, hipStream_t stream, Args p)
 {

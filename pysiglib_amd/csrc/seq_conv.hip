@@ -350,21 +350,13 @@ __global__ void __launch_bounds__(kThreads) conv_back_kernel(ConvArgs a)
     }
 }
 
-// a block to 64 numbers: four threads for each add up every fourth piece, then each other's sums
-__global__ void __launch_bounds__(kThreads) conv_weight_kernel(const float* parts, int pieces, int channels, int width, float* dw, float* db)
+__global__ void __launch_bounds__(kSumThreads) conv_weight_kernel(const float* parts, int pieces, int channels, int width, float* dw, float* db)
 {
-    __shared__ float s_sum[4][64];
-    const int at = threadIdx.x % 64, row = threadIdx.x / 64, all = (width + 1) * channels, e = int(blockIdx.x) * 64 + at;
-    float sum = 0.0f;
-    if (e < all)
-        for (int n = row; n < pieces; n += 4) sum += parts[int64_t(n) * all + e];
-    s_sum[row][at] = sum;
-    __syncthreads();
-    if (row || e >= all) return;
-    sum = (s_sum[0][at] + s_sum[1][at]) + (s_sum[2][at] + s_sum[3][at]);
-    const int k = e / channels, ch = e % channels;
-    if (k < width) dw[int64_t(ch) * width + k] = sum;
-    else if (db) db[ch] = sum;
+    sum_pieces(parts, pieces, int64_t(width + 1) * channels, [&](int64_t e, float sum) {
+        const int k = int(e / channels), ch = int(e % channels);
+        if (k < width) dw[int64_t(ch) * width + k] = sum;
+        else if (db) db[ch] = sum;
+    });
 }
 
 template <typename T, int V, int W>
@@ -546,7 +538,7 @@ __attribute__((visibility("default"))) int cusig_amd_causal_conv_backprop(
                     else launch_all(conv_back_kernel<T, V, W, R, false>, blocks, kThreads, static_cast<hipStream_t>(stream), a);
                 });
             });
-        hipLaunchKernelGGL(conv_weight_kernel, dim3(unsigned(((width + 1) * channels + 63) / 64)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a.parts, pieces,
+        hipLaunchKernelGGL(conv_weight_kernel, sum_blocks(int64_t(width + 1) * a.channels), dim3(kSumThreads), 0, static_cast<hipStream_t>(stream), a.parts, pieces,
                            a.channels, int(width), grad_weight, grad_bias);
         SIG_HIP(hipGetLastError());
     });

@@ -252,17 +252,9 @@ __global__ void __launch_bounds__(W > 4 ? 64 * W : kThreads) norm_back_kernel(No
     }
 }
 
-// a block to 64 channels: four threads for each add up every fourth piece, then each other's sums
-__global__ void __launch_bounds__(kThreads) norm_weight_kernel(const float* parts, int pieces, int channels, float* dw)
+__global__ void __launch_bounds__(kSumThreads) norm_weight_kernel(const float* parts, int pieces, int channels, float* dw)
 {
-    __shared__ float s_sum[4][64];
-    const int ch = threadIdx.x % 64, row = threadIdx.x / 64, e = blockIdx.x * 64 + ch;
-    float sum = 0.0f;
-    if (e < channels)
-        for (int n = row; n < pieces; n += 4) sum += parts[int64_t(n) * channels + e];
-    s_sum[row][ch] = sum;
-    __syncthreads();
-    if (row == 0 && e < channels) dw[e] = (s_sum[0][ch] + s_sum[1][ch]) + (s_sum[2][ch] + s_sum[3][ch]);
+    sum_pieces(parts, pieces, channels, [&](int64_t e, float sum) { dw[e] = sum; });
 }
 
 // Waves to a row and packs to a lane: a wave holds up to two packs a lane, four waves up to eight, and eight waves what float32
@@ -356,7 +348,7 @@ void backward(int dtype, int residual, NormArgs& p, float* dw, hipStream_t strea
             });
         });
     }
-    hipLaunchKernelGGL(norm_weight_kernel, dim3((p.channels + 63) / 64), dim3(kThreads), 0, stream, p.parts, pieces, p.channels, dw);
+    hipLaunchKernelGGL(norm_weight_kernel, sum_blocks(p.channels), dim3(kSumThreads), 0, stream, p.parts, pieces, p.channels, dw);
     SIG_HIP(hipGetLastError());
 }
 

@@ -4,9 +4,12 @@
 // h_t = exp(dt_t a) h_{t-1} + dt_t x_t b_t for each channel and state, y_t = sum over the states of c_t h_t, plus d x_t, times
 // z_t sigmoid(z_t); dt = softplus(delta + bias), or delta + bias.  Every channel has its own a, x, delta; b and c are those of its group.
 //
-// Layout.  Q lanes share a channel, four states each (4 Q are at least the states); a lane has four channels.  So a wave holds 256 / Q
-// channels with all their states in 16 registers a lane, b and c are read once for four channels, dt and dt x once for four
-// states, and the sums over states (y) and over channels (the gradients of b and c) each cross few lanes.
+// Layout.  Four lanes (a quad) hold four channels: their registers the channels, the lanes neighbouring states, so that a step's
+// dt x_i b_n of 16 pairs is one matrix instruction (16 blocks of 4 x 4, one product each) that adds them to the decayed states.  A lane holds
+// four such quadruples: four groups of four states of four channels (16 states), two groups of eight channels (8), one of 16 (4);
+// 32 and 64 states are those of 2 and 4 quads.  Q = states / 4 counts lanes to a channel, 16 pairs being a lane's: a wave has 256 / Q channels,
+// b and c are read once for four channels, dt once for four states, and the sums over states (y) and over channels (the
+// gradients of b and c) each cross few lanes.
 #pragma once
 #include "seq_common.h"
 
@@ -18,20 +21,29 @@ namespace selective {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
+typedef float Four __attribute__((ext_vector_type(4)));
+
 template <int Q>
 struct Shape {
     static constexpr int kRows = Q == 1 ? 4 : (Q == 2 ? 8 : 16);        // of a tile
     static constexpr int kChannels = 256 / Q;                           // of a wave
-    static constexpr int kEach = kRows * kChannels / 64;                // elements of a tile to a lane
-    static constexpr int kOwn = kChannels >= 64 ? kChannels / 64 : 1;   // different channels among them
+    static constexpr int kEach = kRows * kChannels / 128;               // pairs of neighbouring channels of a tile's rows to a lane
+    static constexpr int kOwn = kChannels > 128 ? 2 : 1;                // different channels among them: so many pairs
     static constexpr int kStates = 4 * Q;
     static constexpr int kPacks = kRows * 2 * Q;                        // of four values of b or c in a tile
     static constexpr int kPacksEach = (kPacks + 63) / 64;
+    static constexpr int kGroups = Q < 4 ? Q : 4;                       // of four states of a lane
+    static constexpr int kSets = 4 / kGroups;                           // of four channels of a lane
+    static constexpr int kQuads = Q < 4 ? 1 : Q / 4;                    // with the same channels
+    static constexpr int kSaved = kRows < 8 ? kRows : 8;                // backward: rows between two states that are stored
 
-    // element i of a lane: its row in the tile and its channel in the wave
-    static __device__ __forceinline__ int row(int i, int lane) { return i * 64 / kChannels + (kChannels < 64 ? lane / kChannels : 0); }
-    static __device__ __forceinline__ int channel(int i, int lane) { return kChannels < 64 ? lane % kChannels : i * 64 % kChannels + lane; }
-    static constexpr int own(int i) { return kChannels < 64 ? 0 : i * 64 % kChannels / 64; }
+    // pair i of a lane: its row in the tile, and its first channel in the wave
+    static constexpr int kRowsAtOnce = kChannels < 128 ? 128 / kChannels : 1;
+    static constexpr int row(int i) { return i * 128 / kChannels; }      // of the wave's first lanes
+    static __device__ __forceinline__ int row(int i, int lane) { return row(i) + (kRowsAtOnce > 1 ? lane / (kChannels / 2) : 0); }
+
+    // where state n lies among the wave's in shared memory: a lane's groups beside each other
+    static __host__ __device__ constexpr int place(int n) { return n / 16 * 16 + n % 4 * kGroups + n % 16 / 4; }
 };
 
 struct Args {
@@ -42,10 +54,11 @@ struct Args {
     float* end;                                 // final states; backward: gradients of the initial ones
     void *out, *ddelta, *dz;                    // y; backward: the gradients of x, delta and z
     const int* offsets;                         // [n + 1] rows where sequences begin, or null: n sequences of `length` rows
-    float* carry;                               // [slots][channels][states] the segments' own last states, then the ones before them
-    float* back;                                // the same for the gradients of states, the other way
+    // states as the lanes hold them: [columns][4][64 lanes][4], columns: a wave's channels
+    Four* carry;                                // [slots] the segments' own last states, then the states before them
+    Four* back;                                 // the same for the gradients of states, the other way
     float* span;                                // [slots][channels] sum of dt over a segment
-    float* tile_state;                          // backward: [tiles][channels][states] states at the tiles' first rows, from zero ones at the segment's
+    Four* tile_state;                           // backward: [tiles] states before a tile's rows, of a segment's own
     float* tile_span;                           // [tiles][channels] sum of dt from the segment's first row on
     float* shared_parts;                        // backward: [blocks of a group][rows][groups][2][4 Q] sums of the gradients of b and c
     float* own_parts;                           // [pieces][channels][states + 2] those of a, d and bias
@@ -75,16 +88,19 @@ __device__ __forceinline__ float moved(float v)
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
 
-// the sum over the Q lanes of a channel, in all of them
+// the sum over the lanes of a channel, in all of them
 template <int Q>
 __device__ __forceinline__ float over_states(float v)
 {
-    if constexpr (Q >= 2) v += moved<0xB1>(v);      // neighbours
-    if constexpr (Q >= 4) v += moved<0x4E>(v);      // pairs
+    v += moved<0xB1>(v);                            // neighbours
+    v += moved<0x4E>(v);                            // pairs
     if constexpr (Q >= 8) v += moved<0x141>(v);     // mirrored halves of a row of 16: the other four
     if constexpr (Q >= 16) v += moved<0x140>(v);    // the other eight
     return v;
 }
+
+// state + x_i b_n for 16 pairs of a quad: x the channels' in its four lanes, b the states'
+__device__ __forceinline__ Four add_products(float x, float b, Four state) { return __builtin_amdgcn_mfma_f32_4x4x1f32(x, b, state, 0, 0, 0); }
 
 // The rows of a segment: `first` up to `past` of the sequence `seq`, number `k` of its segments
 struct Segment {
@@ -138,84 +154,153 @@ __device__ __forceinline__ Segment segment_of(const Args& p, int64_t slot)
 // the tiles of a segment are numbered like slots: those of the rows before it, and one more for every slot
 __device__ __forceinline__ int64_t tile_of(int64_t slot, const Segment& s, int rows) { return s.first / rows + slot; }
 
-// What the wave's lanes have of the channels
+// What the wave's lanes have of the channels and states
 template <typename T, int Q>
 struct Column {
     using S = Shape<Q>;
-    int lane, q, at;                // at: the lane's first channel in the wave
+    static constexpr int kG = S::kGroups, kSets = S::kSets;
+    int lane, j, part, at;          // j: in the quad, part: which 16 states, at: the lane's first channel in the wave
     int first, count;               // the wave's channels: the first, and how many there are
-    int group;
-    float a[4][4];                  // a log2(e), zero where there is no channel or state
-    float bias[S::kOwn], d[S::kOwn];
+    int group, column;
+    int pair[S::kOwn];              // the first channels of the lane's pairs.  Where the last one would be behind the channels it is the last two
+                                    // again: what two lanes form, they form alike
+    Four a[4];                      // a log2(e), zero where there is no channel or state; of set u / kG, group u % kG
+    float bias[S::kOwn][2], d[S::kOwn][2];
+
+    __device__ __forceinline__ int channel(int u) const { return at + 4 * (u / kG); }
+    __device__ __forceinline__ int state(int u) const { return part * 16 + 4 * (u % kG) + j; }
 
     __device__ __forceinline__ void init(const Args& p, int group_, int tile)
     {
         lane = threadIdx.x & 63;
-        q = lane % Q;
-        at = lane / Q * 4;
+        j = lane % 4;
+        part = lane / 4 % S::kQuads;
+        at = lane / 4 / S::kQuads * 4 * kSets;
         group = group_;
+        column = group * p.tiles + tile;
         first = group * p.per_group + tile * S::kChannels;
         count = p.per_group - tile * S::kChannels;
         count = count < S::kChannels ? count : S::kChannels;
+        load_state(p, p.a, a);
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-            const bool there = at + ch < count;
-            Pack<float, 4> v{};
-            if (there && 4 * q < p.states) v = load_some<float, 4>(p.a + int64_t(first + at + ch) * p.states + 4 * q, p.states - 4 * q);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) a[ch][k] = v.get(k) * kLog2e;
-        }
+        for (int u = 0; u < 4; ++u) a[u] *= kLog2e;
 #pragma unroll
         for (int i = 0; i < S::kOwn; ++i) {
-            const int ch = S::channel(i, lane);
-            bias[i] = p.bias && ch < count ? p.bias[first + ch] : 0.0f;
-            d[i] = p.d && ch < count ? p.d[first + ch] : 0.0f;
+            const int ch = 2 * ((lane + 64 * i) % (S::kChannels / 2));
+            pair[i] = max(min(ch, count - 2), 0);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const bool there = pair[i] + k < count;
+                bias[i][k] = p.bias && there ? p.bias[first + pair[i] + k] : 0.0f;
+                d[i][k] = p.d && there ? p.d[first + pair[i] + k] : 0.0f;
+            }
         }
+    }
+    __device__ __forceinline__ int channel_of(int i) const { return pair[i % S::kOwn]; }
+    // whether the lane is the one that counts this channel of its pair i
+    __device__ __forceinline__ bool counts(int i, int k) const
+    {
+        const int ch = 2 * ((lane + 64 * (i % S::kOwn)) % (S::kChannels / 2));
+        return channel_of(i) + k >= ch && channel_of(i) + k < count;
     }
 
-    // a state of the lane's channels and states, [channels][states] from `from` on
-    __device__ __forceinline__ void load_state(const Args& p, const float* from, float (&h)[4][4]) const
+    // the lane's values of [channels][states] from `from` on; zero where there are none
+    __device__ __forceinline__ void load_state(const Args& p, const float* from, Four (&h)[4]) const
     {
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-            Pack<float, 4> v{};
-            if (from && at + ch < count && 4 * q < p.states) v = load_some<float, 4>(from + int64_t(first + at + ch) * p.states + 4 * q, p.states - 4 * q);
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) h[ch][k] = v.get(k);
-        }
+            for (int i = 0; i < 4; ++i)
+                h[u][i] = from && channel(u) + i < count && state(u) < p.states ? from[int64_t(first + channel(u) + i) * p.states + state(u)] : 0.0f;
     }
-    __device__ __forceinline__ void store_state(const Args& p, float* to, const float (&h)[4][4]) const
+    __device__ __forceinline__ void store_state(const Args& p, float* to, const Four (&h)[4]) const
     {
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-            if (at + ch >= count || 4 * q >= p.states) continue;
-            Pack<float, 4> v;
-            v.set(h[ch]);
-            store_some<float, 4>(to + int64_t(first + at + ch) * p.states + 4 * q, v, p.states - 4 * q);
-        }
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (channel(u) + i < count && state(u) < p.states) to[int64_t(first + channel(u) + i) * p.states + state(u)] = h[u][i];
+    }
+    // the same as the lanes hold it
+    __device__ __forceinline__ int64_t place(const Args& p, int64_t row) const { return (row * p.groups * p.tiles + column) * 256 + lane; }
+    __device__ __forceinline__ void load_own(const Args& p, const Four* from, int64_t row, Four (&h)[4]) const
+    {
+        const Four* const q = from + place(p, row);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) h[u] = q[64 * u];
+    }
+    __device__ __forceinline__ void store_own(const Args& p, Four* to, int64_t row, const Four (&h)[4]) const
+    {
+        Four* const q = to + place(p, row);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) q[64 * u] = h[u];
+    }
+    // one number for each of the lane's channels, [channels] from `from` on
+    __device__ __forceinline__ void load_line(const float* from, Four (&v)[kSets]) const
+    {
+#pragma unroll
+        for (int s = 0; s < kSets; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[s][i] = at + 4 * s + i < count ? from[first + at + 4 * s + i] : 0.0f;
+    }
+    __device__ __forceinline__ void store_line(float* to, const Four (&v)[kSets]) const
+    {
+        if (j == 0 && part == 0)
+#pragma unroll
+            for (int s = 0; s < kSets; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (at + 4 * s + i < count) to[first + at + 4 * s + i] = v[s][i];
     }
 
-    // the lane's elements of a tile of rows from t0 on; rows from `past` on are the last one again, as are channels behind the last
-    __device__ __forceinline__ void load(const void* from, int64_t step, int64_t t0, int64_t past, T (&to)[S::kEach]) const
+    // the lane's pairs of `rows` rows from t0 on; rows behind them are the last one again.  The rows' address is the same for all lanes, each at a
+    // distance of its own.
+    __device__ __forceinline__ void load(const void* from, int64_t step, int64_t t0, int rows, Pack<T, 2> (&to)[S::kEach]) const
     {
+        const T* const base = static_cast<const T*>(from) + t0 * step + first;
+        if (rows == S::kRows && count >= 2) {
+            const unsigned more = S::kRowsAtOnce > 1 ? unsigned(lane / (S::kChannels / 2) * int(step)) : 0u;
 #pragma unroll
-        for (int i = 0; i < S::kEach; ++i) {
-            const int64_t t = t0 + S::row(i, lane), row = t < past ? t : past - 1;
-            const int ch = S::channel(i, lane);
-            to[i] = static_cast<const T*>(from)[row * step + first + (ch < count ? ch : 0)];
+            for (int i = 0; i < S::kEach; ++i) to[i] = load_pack<T, 2>(base + S::row(i) * step + (more + channel_of(i)));
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::kEach; ++i) to[i] = load_some<T, 2>(base + unsigned(min(S::row(i, lane), rows - 1) * int(step) + channel_of(i)), count);
         }
+    }
+    __device__ __forceinline__ void store(void* to, int64_t channels, int64_t t0, int rows, const float (&v)[S::kEach][2]) const
+    {
+        T* const base = static_cast<T*>(to) + t0 * channels + first;
+        Pack<T, 2> o;
+        if (rows == S::kRows && count >= 2) {
+            const unsigned more = S::kRowsAtOnce > 1 ? unsigned(lane / (S::kChannels / 2) * int(channels)) : 0u;
+#pragma unroll
+            for (int i = 0; i < S::kEach; ++i) {
+                o.set(v[i]);
+                store_pack<T, 2>(base + S::row(i) * channels + (more + channel_of(i)), o);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::kEach; ++i) {
+                o.set(v[i]);
+                if (S::row(i, lane) < rows) store_some<T, 2>(base + unsigned(S::row(i, lane) * int(channels) + channel_of(i)), o, count);
+            }
+        }
+    }
+    // a pair's two numbers in a row of shared memory
+    __device__ __forceinline__ void put(float* row, int i, float a, float b) const
+    {
+        row[channel_of(i)] = a;
+        row[channel_of(i) + 1] = b;
     }
     // the packs of b and c
-    __device__ __forceinline__ void load_shared(const Args& p, int64_t t0, int64_t past, Pack<T, 4> (&to)[S::kPacksEach]) const
+    __device__ __forceinline__ void load_shared(const Args& p, int64_t t0, int rows, Pack<T, 4> (&to)[S::kPacksEach]) const
     {
+        const T *const b = static_cast<const T*>(p.b) + t0 * p.b_step + group * p.b_group, *const c = static_cast<const T*>(p.c) + t0 * p.c_step + group * p.c_group;
 #pragma unroll
         for (int i = 0; i < S::kPacksEach; ++i) {
-            const int e = i * 64 + lane, r = e / (2 * Q), n = e % Q * 4;
-            const bool c = e / Q % 2;
-            const int64_t t = t0 + r, row = t < past ? t : past - 1;
+            const int e = i * 64 + lane, r = min(e / (2 * Q), rows - 1), n = e % Q * 4;
             to[i] = Pack<T, 4>{};
-            if (e < S::kPacks && n < p.states)
-                to[i] = load_some<T, 4>(c ? static_cast<const T*>(p.c) + row * p.c_step + group * p.c_group + n : static_cast<const T*>(p.b) + row * p.b_step + group * p.b_group + n, p.states - n);
+            if (e < S::kPacks && n < p.states) to[i] = load_some<T, 4>(e / Q % 2 ? c + r * p.c_step + n : b + r * p.b_step + n, p.states - n);
         }
     }
     __device__ __forceinline__ void put_shared(const Pack<T, 4> (&from)[S::kPacksEach], float (*to)[2][S::kStates]) const
@@ -223,18 +308,57 @@ struct Column {
 #pragma unroll
         for (int i = 0; i < S::kPacksEach; ++i) {
             const int e = i * 64 + lane;
-            if (e < S::kPacks) *reinterpret_cast<float4*>(&to[e / (2 * Q)][e / Q % 2][e % Q * 4]) = float4{from[i].get(0), from[i].get(1), from[i].get(2), from[i].get(3)};
+            if (e < S::kPacks)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) to[e / (2 * Q)][e / Q % 2][S::place(e % Q * 4 + k)] = from[i].get(k);
         }
+    }
+    // the lane's values of b or c of one row
+    __device__ __forceinline__ void read_shared(const float* row, float (&to)[kG]) const
+    {
+        const float* const q = row + part * 16 + j * kG;
+        if constexpr (kG == 4) {
+            const Four v = *reinterpret_cast<const Four*>(q);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) to[g] = v[g];
+        } else {
+#pragma unroll
+            for (int g = 0; g < kG; ++g) to[g] = q[g];
+        }
+    }
+    // dt of the pairs
+    __device__ __forceinline__ void steps(const Args& p, const Pack<T, 2> (&delta)[S::kEach], float (&dt)[S::kEach][2]) const
+    {
+#pragma unroll
+        for (int i = 0; i < S::kEach; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) dt[i][k] = delta[i].get(k) + bias[i % S::kOwn][k];
+        if (p.softplus)
+#pragma unroll
+            for (int i = 0; i < S::kEach; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) dt[i][k] = softplus_of(dt[i][k]);
+    }
+    // v times the gates
+    __device__ __forceinline__ void gate(const Pack<T, 2> (&z)[S::kEach], float (&v)[S::kEach][2]) const
+    {
+#pragma unroll
+        for (int i = 0; i < S::kEach; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) v[i][k] *= z[i].get(k) * sigmoid(z[i].get(k));
     }
 };
 
-__device__ __forceinline__ void read4(const float* from, float (&to)[4])
+// the decays of a quadruple
+__device__ __forceinline__ Four decays(Four dt, Four a)
 {
-    const float4 v = *reinterpret_cast<const float4*>(from);
-    to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+    Four e;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(dt[i] * a[i]);
+    return e;
 }
 
-// how the rows are cut, for `most` waves in all
+// how the rows are cut
 struct Plan {
     int q, tiles;
     int64_t segment, slots, per_sequence;

@@ -19,10 +19,10 @@ template <typename T, int Q, bool OUT>
 __global__ void __launch_bounds__(kThreads, 2) scan_kernel(Args p)
 {
     using S = Shape<Q>;
-    constexpr int R = S::kRows, E = S::kEach;
+    constexpr int R = S::kRows, E = S::kEach, G = S::kGroups, kSets = S::kSets;
     __shared__ __attribute__((aligned(16))) float s_in[kWaves][R][2][S::kChannels];
     __shared__ __attribute__((aligned(16))) float s_bc[kWaves][R][2][S::kStates];
-    const int wave = threadIdx.x / 64, columns = p.groups * p.tiles;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), columns = p.groups * p.tiles;
     const int64_t id = (int64_t(p.first_block) + blockIdx.x) * kWaves + wave, slot = id / columns;
     if (slot >= p.slots) return;
     const Segment s = segment_of(p, slot);
@@ -30,111 +30,165 @@ __global__ void __launch_bounds__(kThreads, 2) scan_kernel(Args p)
     Column<T, Q> col;
     col.init(p, int(id % columns) / p.tiles, int(id % columns) % p.tiles);
     const int64_t size = int64_t(p.channels) * p.states;
-    float h[4][4], span[4];
-    col.load_state(p, !OUT ? nullptr : (s.first_one ? (p.begin ? p.begin + s.seq * size : nullptr) : p.carry + slot * size), h);
+    Four h[4], span[kSets];
+    if (s.first_one) {
+        col.load_state(p, p.begin ? p.begin + s.seq * size : nullptr, h);
+    } else if constexpr (OUT) {
+        col.load_own(p, p.carry, slot, h);
+    } else {
 #pragma unroll
-    for (int ch = 0; ch < 4; ++ch) span[ch] = 0.0f;
+        for (int u = 0; u < 4; ++u) h[u] = Four{};
+    }
+#pragma unroll
+    for (int i = 0; i < kSets; ++i) span[i] = Four{};
     auto& in = s_in[wave];
     auto& bc = s_bc[wave];
-    T x[E], delta[E], z[E];
+    Pack<T, 2> x[E], delta[E], z[E];
     Pack<T, 4> shared[S::kPacksEach];
     auto fetch = [&](int64_t t0) __attribute__((always_inline)) {
-        col.load(p.x, p.x_step, t0, s.past, x);
-        col.load(p.delta, p.delta_step, t0, s.past, delta);
-        if (OUT && p.z) col.load(p.z, p.z_step, t0, s.past, z);
-        col.load_shared(p, t0, s.past, shared);
+        const int rows = s.past - t0 < R ? int(s.past - t0) : R;
+        col.load(p.x, p.x_step, t0, rows, x);
+        col.load(p.delta, p.delta_step, t0, rows, delta);
+        if (OUT && p.z) col.load(p.z, p.z_step, t0, rows, z);
+        col.load_shared(p, t0, rows, shared);
     };
     if (s.first < s.past) fetch(s.first);
     for (int64_t t0 = s.first; t0 < s.past; t0 += R) {
-        T x_now[E], z_now[E];
+        const int rows = s.past - t0 < R ? int(s.past - t0) : R;
+        Pack<T, 2> x_now[E], z_now[E];
+        {
+            float dt[E][2];
+            col.steps(p, delta, dt);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float raw = float(delta[i]) + col.bias[S::own(i)], dt = p.softplus ? softplus_of(raw) : raw;
-            in[S::row(i, col.lane)][0][S::channel(i, col.lane)] = dt;
-            in[S::row(i, col.lane)][1][S::channel(i, col.lane)] = dt * float(x[i]);
-            x_now[i] = x[i], z_now[i] = z[i];
+            for (int i = 0; i < E; ++i) {
+                auto& row = in[S::row(i, col.lane)];
+                col.put(row[0], i, dt[i][0], dt[i][1]);
+                col.put(row[1], i, dt[i][0] * x[i].get(0), dt[i][1] * x[i].get(1));
+                x_now[i] = x[i], z_now[i] = z[i];
+            }
         }
         col.put_shared(shared, bc);
         if (t0 + R < s.past) fetch(t0 + R);
         auto step = [&](int t) __attribute__((always_inline)) {
-            float dt[4], du[4], b[4], c[4], y[4];
-            read4(&in[t][0][col.at], dt);
-            read4(&in[t][1][col.at], du);
-            read4(&bc[t][0][4 * col.q], b);
-            if constexpr (OUT) read4(&bc[t][1][4 * col.q], c);
+            float b[G], c[G];
+            col.read_shared(bc[t][0], b);
+            if constexpr (OUT) col.read_shared(bc[t][1], c);
 #pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-                y[ch] = 0.0f;
+            for (int i = 0; i < kSets; ++i) {
+                const Four dt = *reinterpret_cast<const Four*>(&in[t][0][col.at + 4 * i]);
+                const float du = in[t][1][col.at + 4 * i + col.j];
+                Four y{};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    h[ch][k] = fmaf(h[ch][k], __builtin_amdgcn_exp2f(dt[ch] * col.a[ch][k]), du[ch] * b[k]);
-                    if constexpr (OUT) y[ch] = fmaf(c[k], h[ch][k], y[ch]);
+                for (int g = 0; g < G; ++g) {
+                    Four& state = h[i * G + g];
+                    state = add_products(du, b[g], state * decays(dt, col.a[i * G + g]));
+                    if constexpr (OUT)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) y[k] = fmaf(c[g], state[k], y[k]);
                 }
-                if constexpr (OUT) y[ch] = over_states<Q>(y[ch]);
-                else span[ch] += dt[ch];
+                if constexpr (OUT) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[k] = over_states<Q>(y[k]);
+                    *reinterpret_cast<Four*>(&in[t][0][col.at + 4 * i]) = y;
+                } else {
+                    span[i] += dt;
+                }
             }
-            if constexpr (OUT) *reinterpret_cast<float4*>(&in[t][0][col.at]) = float4{y[0], y[1], y[2], y[3]};
         };
-        const int count = s.past - t0 < R ? int(s.past - t0) : R;
-        if (count == R) {
+        if (rows == R) {
 #pragma unroll 4
             for (int t = 0; t < R; ++t) step(t);
         } else {
 #pragma unroll 1
-            for (int t = 0; t < count; ++t) step(t);
+            for (int t = 0; t < rows; ++t) step(t);
         }
         if constexpr (OUT) {
+            float y[E][2];
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const int r = S::row(i, col.lane), ch = S::channel(i, col.lane);
-                float y = fmaf(col.d[S::own(i)], float(x_now[i]), in[r][0][ch]);
-                if (p.z) y *= float(z_now[i]) * sigmoid(float(z_now[i]));
-                if (r < count && ch < col.count) static_cast<T*>(p.out)[(t0 + r) * p.channels + col.first + ch] = T(y);
-            }
+            for (int i = 0; i < E; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) y[i][k] = fmaf(col.d[i % S::kOwn][k], x_now[i].get(k), in[S::row(i, col.lane)][0][col.channel_of(i) + k]);
+            if (p.z) col.gate(z_now, y);
+            col.store(p.out, p.channels, t0, rows, y);
         }
     }
     if constexpr (OUT) {
         if (s.last_one) col.store_state(p, p.end + s.seq * size, h);
     } else {
-        col.store_state(p, p.carry + slot * size, h);
-        if (col.q == 0)
-#pragma unroll
-            for (int ch = 0; ch < 4; ++ch)
-                if (col.at + ch < col.count) p.span[slot * p.channels + col.first + col.at + ch] = span[ch];
+        col.store_own(p, p.carry, slot, h);
+        col.store_line(p.span + slot * p.channels, span);
     }
 }
 
-// A thread to a state of a sequence with several segments: their own last states become the states before them, and (BACK) their own gradients
-// the gradients behind them
-template <bool BACK>
-__global__ void __launch_bounds__(kThreads) join_kernel(Args p)
+// Sequences with several segments: the segments' own last states become the states before them, and (BACK) their own gradients the gradients behind
+// them.  P threads to a state take neighbouring segments, whose maps meet in shared memory; eight segments' numbers are on their way at once.
+template <bool BACK, int Q, int P>
+__global__ void __launch_bounds__(kThreads) join_kernel(Args p, int blocks)
 {
-    const int64_t size = int64_t(p.channels) * p.states, blocks = (size + kThreads - 1) / kThreads, block = int64_t(p.first_block) + blockIdx.x;
-    const int64_t seq = block / blocks, e = (block - seq * blocks) * kThreads + threadIdx.x;
-    if (seq >= p.n || e >= size) return;
+    using S = Shape<Q>;
+    constexpr int kLanes = kThreads / P, kAtOnce = 8;
+    __shared__ float s_a[P][kLanes], s_b[P][kLanes];
+    const int64_t block = int64_t(p.first_block) + blockIdx.x, seq = block / blocks;
+    if (seq >= p.n) return;
     int64_t first, past;
     rows_of(p, seq, first, past);
     const int64_t count = (past - first + p.segment - 1) / p.segment, slot = slot_of(p, seq, first);
     if (count < 2 || slot + count > p.slots) return;
-    const float a = p.a[e] * kLog2e;
-    const float* const span = p.span + e / p.states;
-    float h = p.begin ? p.begin[seq * size + e] : 0.0f;
-    for (int64_t k = slot; k < slot + count; ++k) {
-        const float own = k + 1 < slot + count ? p.carry[k * size + e] : 0.0f;
-        p.carry[k * size + e] = h;
-        if (k + 1 < slot + count) h = fmaf(h, __builtin_amdgcn_exp2f(a * span[k * p.channels]), own);
-    }
-    if constexpr (BACK) {
-        float g = p.grad_end ? p.grad_end[seq * size + e] : 0.0f;
-        for (int64_t k = slot + count - 1; k >= slot; --k) {
-            const float own = k > slot ? p.back[k * size + e] : 0.0f;
-            p.back[k * size + e] = g;
-            if (k > slot) g = fmaf(g, __builtin_amdgcn_exp2f(a * span[k * p.channels]), own);
-        }
+    const int lane = threadIdx.x % kLanes, piece = threadIdx.x / kLanes;
+    const int64_t each = (count + P - 1) / P, size = int64_t(p.groups) * p.tiles * 1024;
+    for (int64_t base = (block % blocks) * kLanes; base < size; base += int64_t(blocks) * kLanes) {
+        // e as the lanes hold it: column, quadruple, lane, channel of it
+        const int64_t e = base + lane;
+        const int column = int(e / 1024), u = int(e / 256) % 4, l = int(e / 4) % 64, i = int(e % 4);
+        const int ch = (column % p.tiles) * S::kChannels + l / 4 / S::kQuads * 4 * S::kSets + 4 * (u / S::kGroups) + i;
+        const int state = l / 4 % S::kQuads * 16 + 4 * (u % S::kGroups) + l % 4;
+        const bool there = ch < p.per_group && state < p.states;
+        const int channel = column / p.tiles * p.per_group + ch;
+        const float a = there ? p.a[int64_t(channel) * p.states + state] * kLog2e : 0.0f;
+        // BACKWARD: from the last segment to the first.  A segment's map takes the state before it to the one behind it; the last one's is not
+        // known, and not asked for.
+        auto join = [&](Four* at, auto backward) __attribute__((always_inline)) {
+            constexpr bool kBackward = decltype(backward)::value;
+            float* const own = reinterpret_cast<float*>(at) + e;
+            const int64_t low = min(piece * each, count), high = min(low + each, count);        // in the order of the walk
+            auto segment = [&](int64_t k) { return slot + (kBackward ? count - 1 - k : k); };
+            auto walk = [&](auto&& take) __attribute__((always_inline)) {
+                for (int64_t k0 = low; k0 < high; k0 += kAtOnce) {
+                    float v[kAtOnce], d[kAtOnce];
+#pragma unroll
+                    for (int n = 0; n < kAtOnce; ++n) {
+                        const bool known = k0 + n < high && k0 + n < count - 1;
+                        v[n] = known ? own[segment(k0 + n) * size] : 0.0f;
+                        d[n] = known && there ? p.span[segment(k0 + n) * p.channels + channel] : 0.0f;
+                    }
+#pragma unroll
+                    for (int n = 0; n < kAtOnce; ++n)
+                        if (k0 + n < high) take(k0 + n, __builtin_amdgcn_exp2f(a * d[n]), v[n]);
+                }
+            };
+            float h = 0.0f;
+            if constexpr (P > 1) {
+                float ma = 1.0f, mb = 0.0f;
+                walk([&](int64_t, float d, float v) {
+                    mb = fmaf(mb, d, v);
+                    ma *= d;
+                });
+                __syncthreads();
+                s_a[piece][lane] = ma, s_b[piece][lane] = mb;
+                __syncthreads();
+                for (int n = 0; n < piece; ++n) h = fmaf(h, s_a[n][lane], s_b[n][lane]);
+            }
+            walk([&](int64_t k, float d, float v) {
+                own[segment(k) * size] = h;
+                h = fmaf(h, d, v);
+            });
+        };
+        join(p.carry, std::false_type{});
+        if constexpr (BACK) join(p.back, std::true_type{});
     }
 }
 
-// One token of each row: Q lanes to a channel, four states to a lane
+// One token of each row: Q lanes to a channel, four neighbouring states to a lane
 template <typename T, int Q>
 __global__ void __launch_bounds__(kThreads) step_kernel(Args p)
 {
@@ -159,7 +213,8 @@ __global__ void __launch_bounds__(kThreads) step_kernel(Args p)
         now[k] = fmaf(h.get(k), __builtin_amdgcn_exp2f(dt * (a.get(k) * kLog2e)), du * b.get(k));
         y = fmaf(c.get(k), now[k], y);
     }
-    y = over_states<Q>(y);
+#pragma unroll
+    for (int m = 1; m < Q; m *= 2) y += __shfl_xor(y, m);
     if (p.d) y = fmaf(p.d[ch], x, y);
     if (p.z) {
         const float z = float(static_cast<const T*>(p.z)[row * p.z_step + ch]);
@@ -199,11 +254,24 @@ Plan plan_of(bool packed, int64_t rows, int64_t n, int64_t length, int channels,
     return p;
 }
 
+// Many segments to a sequence are joined by several threads to a state
 void join_segments(const Args& p, bool back, hipStream_t stream)
 {
-    const int64_t blocks = (int64_t(p.channels) * p.states + kThreads - 1) / kThreads * p.n;
-    if (back) launch_all(join_kernel<true>, blocks, kThreads, stream, p);
-    else launch_all(join_kernel<false>, blocks, kThreads, stream, p);
+    const int64_t states = int64_t(p.groups) * p.tiles * 1024, count = p.offsets ? p.rows / p.segment : p.per_sequence;
+    with_lanes(lanes_of(p.states), [&](auto q) {
+        constexpr int Q = decltype(q)::value;
+        auto launch = [&](auto kernel, int pieces) {
+            // no more blocks than some for every compute unit: most sequences may have one segment
+            const int64_t most = states * pieces / kThreads, blocks = std::max<int64_t>(std::min(most, 8192 / std::max<int64_t>(p.n, 1)), 1);
+            in_launches(blocks * p.n, kThreads, [&](unsigned first, dim3 grid) {
+                Args a = p;
+                a.first_block = first;
+                hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a, int(blocks));
+            });
+        };
+        if (count > 64) launch(back ? join_kernel<true, Q, 16> : join_kernel<false, Q, 16>, 16);
+        else launch(back ? join_kernel<true, Q, 1> : join_kernel<false, Q, 1>, 1);
+    });
 }
 
 }  // namespace selective
@@ -216,10 +284,9 @@ namespace {
 
 uint64_t up(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-uint64_t forward_workspace(const Plan& p, uint64_t channels, uint64_t states)
-{
-    return p.several ? up(uint64_t(p.slots) * channels * states * 4) + up(uint64_t(p.slots) * channels * 4) : 0;
-}
+uint64_t carry_bytes(const Plan& p, uint64_t groups) { return up(uint64_t(p.slots) * groups * p.tiles * 4096); }
+
+uint64_t forward_workspace(const Plan& p, uint64_t channels, uint64_t groups) { return p.several ? carry_bytes(p, groups) + up(uint64_t(p.slots) * channels * 4) : 0; }
 
 }  // namespace
 
@@ -231,7 +298,7 @@ __attribute__((visibility("default"))) uint64_t cusig_amd_selective_scan_workspa
     uint64_t bytes = 0;
     sigamd::guarded([&] {
         check_sizes(rows, sequences, channels, states, groups);
-        bytes = forward_workspace(plan_of(packed, int64_t(rows), int64_t(sequences), int64_t(length), int(channels), int(states), int(groups), false), channels, states);
+        bytes = forward_workspace(plan_of(packed, int64_t(rows), int64_t(sequences), int64_t(length), int(channels), int(states), int(groups), false), channels, groups);
     });
     return bytes;
 }
@@ -248,7 +315,7 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan(
         if (sequences * channels == 0) return;
         require(a && final_state && (rows == 0 || (x && delta && b && c && y)), "a tensor is missing");
         const Plan plan = plan_of(offsets, int64_t(rows), int64_t(sequences), int64_t(length), int(channels), int(states), int(groups), false);
-        check_workspace(workspace, workspace_bytes, forward_workspace(plan, channels, states));
+        check_workspace(workspace, workspace_bytes, forward_workspace(plan, channels, groups));
         Args p{};
         p.x = x, p.delta = delta, p.a = a, p.b = b, p.c = c, p.d = d, p.z = z, p.bias = delta_bias, p.begin = initial_state, p.out = y, p.end = final_state;
         p.offsets = offsets, p.n = int64_t(sequences), p.length = int64_t(length), p.rows = int64_t(rows);
@@ -256,8 +323,8 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan(
         p.x_step = x_stride, p.delta_step = delta_stride, p.z_step = z_stride, p.b_step = b_stride, p.b_group = b_group, p.c_step = c_stride, p.c_group = c_group;
         p.softplus = softplus;
         p.segment = plan.segment, p.slots = plan.slots, p.per_sequence = plan.per_sequence, p.several = plan.several;
-        p.carry = static_cast<float*>(workspace);
-        p.span = reinterpret_cast<float*>(static_cast<char*>(workspace) + up(uint64_t(plan.slots) * channels * states * 4));
+        p.carry = static_cast<Four*>(workspace);
+        p.span = reinterpret_cast<float*>(static_cast<char*>(workspace) + (plan.several ? carry_bytes(plan, groups) : 0));
         const int64_t waves = p.slots * p.groups * p.tiles, blocks = (waves + kWaves - 1) / kWaves;
         const auto s = static_cast<hipStream_t>(stream);
         with_type(dtype, [&](auto t) {

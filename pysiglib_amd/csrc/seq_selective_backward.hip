@@ -6,13 +6,14 @@
 // for each state da = sum over rows of G_t k_t h_{t-1} dt_t, and for each row of a group (sums over its channels) db_t = sum G_t dt_t x_t,
 // dc_t = sum gy_t h_t.  k_0 G_0 is the gradient of the initial state.  Nothing is taken from the forward pass: the states are formed again.
 //
-// Passes.  First every segment forward from a zero state: its state at each tile's first row, its own last state, and (where a
-// sequence has several) the gradient of the state before it that its own rows make, as sum over t of (k_first ... k_t) gy_t c_t, so one
-// exponential serves both.  Segments are joined; then each goes from its last tile to its first: the state before a tile is the stored one plus
-// exp(a sum dt) times the segment's; half a tile's states are formed and kept in registers, and its rows gone back through.
+// Passes.  First every segment forward, the first of a sequence from its initial state, others from zero: the state before every eighth
+// row, its own last state, and (where a sequence has several) the gradient of the state before it that its own rows make, as sum over t of
+// (k_first ... k_t) gy_t c_t, so one exponential serves both.  Segments are joined; then each goes from its last rows to its
+// first: the state before eight rows is the stored one plus exp(a sum dt) times the segment's; four rows' states are formed and kept in
+// registers, and these rows gone back through.
 // Sums over channels stay in a row's 64 lanes, then the block's waves, then the blocks, all in a fixed order.
 //
-// Bound: vector instructions, some fifteen and two and a half exponentials for each state and row.
+// Bound: vector instructions, some twenty for each state and row.
 #include "seq_selective.h"
 
 #include <algorithm>
@@ -22,143 +23,150 @@ namespace seqamd {
 namespace selective {
 namespace {
 
-__device__ __forceinline__ float slope(float v)
-{
-    const float s = sigmoid(v);
-    return s * fmaf(v, 1.0f - s, 1.0f);
-}
-
-// Every segment from a zero state: BACK: its own part of the gradients too
+// Every segment's own states; BACK: its own part of the gradients too
 template <typename T, int Q, bool BACK>
 __global__ void __launch_bounds__(kThreads, 2) states_kernel(Args p)
 {
     using S = Shape<Q>;
-    constexpr int R = S::kRows, E = S::kEach;
+    constexpr int R = S::kRows, E = S::kEach, G = S::kGroups, kSets = S::kSets, kSaved = S::kSaved;
     __shared__ __attribute__((aligned(16))) float s_in[kWaves][R][BACK ? 3 : 2][S::kChannels];
     __shared__ __attribute__((aligned(16))) float s_bc[kWaves][R][2][S::kStates];
-    const int wave = threadIdx.x / 64, columns = p.groups * p.tiles;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), columns = p.groups * p.tiles;
     const int64_t id = (int64_t(p.first_block) + blockIdx.x) * kWaves + wave, slot = id / columns;
     if (slot >= p.slots) return;
     const Segment s = segment_of(p, slot);
     if (!s.there || s.first >= s.past) return;
     Column<T, Q> col;
     col.init(p, int(id % columns) / p.tiles, int(id % columns) % p.tiles);
-    const int64_t size = int64_t(p.channels) * p.states, tile0 = tile_of(slot, s, R);
-    float h[4][4], span[4], decay[4][4], back[4][4];
+    const int64_t size = int64_t(p.channels) * p.states;
+    int64_t tile = tile_of(slot, s, kSaved);
+    Four h[4], decay[4], back[4], span[kSets];
+    col.load_state(p, s.first_one && p.begin ? p.begin + s.seq * size : nullptr, h);
 #pragma unroll
-    for (int ch = 0; ch < 4; ++ch) {
-        span[ch] = 0.0f;
+    for (int u = 0; u < 4; ++u) back[u] = Four{}, decay[u] = Four{1.0f, 1.0f, 1.0f, 1.0f};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) h[ch][k] = back[ch][k] = 0.0f, decay[ch][k] = 1.0f;
-    }
+    for (int i = 0; i < kSets; ++i) span[i] = Four{};
     auto& in = s_in[wave];
     auto& bc = s_bc[wave];
-    T x[E], delta[E], z[E], g[E];
+    Pack<T, 2> x[E], delta[E], z[E], g[E];
     Pack<T, 4> shared[S::kPacksEach];
     auto fetch = [&](int64_t t0) __attribute__((always_inline)) {
-        col.load(p.x, p.x_step, t0, s.past, x);
-        col.load(p.delta, p.delta_step, t0, s.past, delta);
-        if (BACK && p.z) col.load(p.z, p.z_step, t0, s.past, z);
-        if (BACK) col.load(p.grad, p.grad_step, t0, s.past, g);
-        col.load_shared(p, t0, s.past, shared);
-    };
-    auto store_span = [&](float* to) __attribute__((always_inline)) {
-        if (col.q == 0)
-#pragma unroll
-            for (int ch = 0; ch < 4; ++ch)
-                if (col.at + ch < col.count) to[col.first + col.at + ch] = span[ch];
+        const int rows = s.past - t0 < R ? int(s.past - t0) : R;
+        col.load(p.x, p.x_step, t0, rows, x);
+        col.load(p.delta, p.delta_step, t0, rows, delta);
+        if (BACK && p.z) col.load(p.z, p.z_step, t0, rows, z);
+        if (BACK) col.load(p.grad, p.grad_step, t0, rows, g);
+        col.load_shared(p, t0, rows, shared);
     };
     fetch(s.first);
-    int64_t tile = tile0;
-    for (int64_t t0 = s.first; t0 < s.past; t0 += R, ++tile) {
-        if (t0 > s.first) {
-            col.store_state(p, p.tile_state + tile * size, h);
-            store_span(p.tile_span + tile * p.channels);
-        }
-        if (t0 + R >= s.past && s.last_one && (!BACK || s.first_one)) break;      // nobody asks for its own last state
+    for (int64_t t0 = s.first; t0 < s.past; t0 += R) {
+        const int rows = s.past - t0 < R ? int(s.past - t0) : R;
+        {
+            float v[E][2];
+            col.steps(p, delta, v);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int r = S::row(i, col.lane), ch = S::channel(i, col.lane);
-            const float raw = float(delta[i]) + col.bias[S::own(i)], dt = p.softplus ? softplus_of(raw) : raw;
-            in[r][0][ch] = dt;
-            in[r][1][ch] = dt * float(x[i]);
-            if constexpr (BACK) in[r][2][ch] = p.z ? float(g[i]) * (float(z[i]) * sigmoid(float(z[i]))) : float(g[i]);
+            for (int i = 0; i < E; ++i) {
+                auto& row = in[S::row(i, col.lane)];
+                col.put(row[0], i, v[i][0], v[i][1]);
+                col.put(row[1], i, v[i][0] * x[i].get(0), v[i][1] * x[i].get(1));
+            }
+            if constexpr (BACK) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) v[i][0] = g[i].get(0), v[i][1] = g[i].get(1);
+                if (p.z) col.gate(z, v);
+#pragma unroll
+                for (int i = 0; i < E; ++i) col.put(in[S::row(i, col.lane)][2], i, v[i][0], v[i][1]);
+            }
         }
         col.put_shared(shared, bc);
         if (t0 + R < s.past) fetch(t0 + R);
         auto step = [&](int t) __attribute__((always_inline)) {
-            float dt[4], du[4], gy[4], b[4], c[4];
-            read4(&in[t][0][col.at], dt);
-            read4(&in[t][1][col.at], du);
-            read4(&bc[t][0][4 * col.q], b);
-            if constexpr (BACK) {
-                read4(&in[t][2][col.at], gy);
-                read4(&bc[t][1][4 * col.q], c);
-            }
+            float b[G], c[G];
+            col.read_shared(bc[t][0], b);
+            if constexpr (BACK) col.read_shared(bc[t][1], c);
 #pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
+            for (int i = 0; i < kSets; ++i) {
+                const Four dt = *reinterpret_cast<const Four*>(&in[t][0][col.at + 4 * i]);
+                const float du = in[t][1][col.at + 4 * i + col.j];
+                Four gy{};
+                if constexpr (BACK) gy = *reinterpret_cast<const Four*>(&in[t][2][col.at + 4 * i]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float e = __builtin_amdgcn_exp2f(dt[ch] * col.a[ch][k]);
-                    h[ch][k] = fmaf(h[ch][k], e, du[ch] * b[k]);
+                for (int g = 0; g < G; ++g) {
+                    const int u = i * G + g;
+                    const Four e = decays(dt, col.a[u]);
+                    h[u] = add_products(du, b[g], h[u] * e);
                     if constexpr (BACK) {
-                        decay[ch][k] *= e;
-                        back[ch][k] = fmaf(decay[ch][k], gy[ch] * c[k], back[ch][k]);
+                        decay[u] *= e;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) back[u][k] = fmaf(decay[u][k], gy[k] * c[g], back[u][k]);
                     }
                 }
-                span[ch] += dt[ch];
+                span[i] += dt;
             }
         };
-        const int count = s.past - t0 < R ? int(s.past - t0) : R;
-        if (count == R) {
-#pragma unroll 4
-            for (int t = 0; t < R; ++t) step(t);
-        } else {
 #pragma unroll 1
-            for (int t = 0; t < count; ++t) step(t);
+        for (int t = 0; t < rows; t += kSaved, ++tile) {
+            col.store_own(p, p.tile_state, tile, h);
+            if (!s.first_one) col.store_line(p.tile_span + tile * p.channels, span);
+            if (t + kSaved <= rows) {
+#pragma unroll 4
+                for (int k = 0; k < kSaved; ++k) step(t + k);
+            } else {
+#pragma unroll 1
+                for (int k = t; k < rows; ++k) step(k);
+            }
         }
     }
     if (s.first_one && s.last_one) return;
-    col.store_state(p, p.carry + slot * size, h);
-    store_span(p.span + slot * p.channels);
-    if constexpr (BACK) col.store_state(p, p.back + slot * size, back);
+    col.store_own(p, p.carry, slot, h);
+    col.store_line(p.span + slot * p.channels, span);
+    if constexpr (BACK) {
+        if (s.last_one && p.grad_end) {
+            Four end[4];
+            col.load_state(p, p.grad_end + s.seq * size, end);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) back[u][k] = fmaf(decay[u][k], end[u][k], back[u][k]);
+        }
+        col.store_own(p, p.back, slot, back);
+    }
 }
 
-// the sum over the channels of a wave, for eight values: of lane l's four states n = 4 (l % Q) + k of b (v[0][k]) and of c (v[1][k]).  Returns
-// two of them: lanes with l % 16 < Q hold those of states 4 q + 2 (row & 1) and the one behind, of b in rows 0 and 1 of 16 lanes, of c in rows 2 and 3
+// The sum over the channels of a wave of the lane's sums for b (v[0]) and c (v[1]).  Groups beside each other go to lanes with the lane's
+// place in its quads: lanes 0 to 31 hold b's, 32 to 63 c's; with four groups rows of 16 lanes hold two each, with two one each.
 template <int Q>
-__device__ __forceinline__ float2 over_channels(float (&v)[2][4])
+__device__ __forceinline__ float2 over_channels(const float (&v)[2][Shape<Q>::kGroups])
 {
-    float u[4];
+    constexpr int G = Shape<Q>::kGroups;
+    float u[G];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[0][k]), __float_as_uint(v[1][k]), false, false);
-        u[k] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    for (int g = 0; g < G; ++g) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[0][g]), __float_as_uint(v[1][g]), false, false);
+        u[g] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     }
-    float w[2];
+    float w[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(u[k]), __float_as_uint(u[2 + k]), false, false);
+    for (int k = 0; k < (G == 4 ? 2 : 1); ++k) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(u[k]), __float_as_uint(u[G == 1 ? 0 : G / 2 + k]), false, false);
         w[k] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-        if constexpr (Q <= 8) w[k] += moved<0x128>(w[k]);       // rows turned by 8, 4, 2, 1
+        if constexpr (Q <= 8) w[k] += moved<0x128>(w[k]);       // rows turned by 8 and 4
         if constexpr (Q <= 4) w[k] += moved<0x124>(w[k]);
-        if constexpr (Q <= 2) w[k] += moved<0x122>(w[k]);
-        if constexpr (Q <= 1) w[k] += moved<0x121>(w[k]);
     }
     return float2{w[0], w[1]};
 }
 
-// SOME: a wave may have fewer channels than there is room for.  What stands in their place takes no part in the sums over channels, not
-// even as a product with zero: b and c may hold what is not finite.
+// SOME: a wave may have fewer channels than there is room for.  What stands in their place is no
+// number in particular, and takes no part in the sums over channels.
 template <typename T, int Q, bool SOME>
 __global__ void __launch_bounds__(kThreads, 2) back_kernel(Args p)
 {
     using S = Shape<Q>;
-    constexpr int R = S::kRows, E = S::kEach, H = R < 8 ? R : 8, kParts = R / H;        // H: rows whose states are kept
+    constexpr int R = S::kRows, E = S::kEach, G = S::kGroups, kSets = S::kSets, kSaved = S::kSaved, H = 4;      // H: rows whose states are kept
     __shared__ __attribute__((aligned(16))) float s_in[kWaves][R][3][S::kChannels];
     __shared__ __attribute__((aligned(16))) float s_bc[kWaves][R][2][S::kStates];
     __shared__ __attribute__((aligned(16))) float s_part[kWaves][R][2][S::kStates];
-    const int wave = threadIdx.x / 64, blocks = p.groups * p.group_blocks;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), blocks = p.groups * p.group_blocks;
     const int64_t block = int64_t(p.first_block) + blockIdx.x;
     const int piece = int(block / blocks), group = int(block % blocks) / p.group_blocks, gb = int(block % blocks) % p.group_blocks;
     Column<T, Q> col;
@@ -166,155 +174,198 @@ __global__ void __launch_bounds__(kThreads, 2) back_kernel(Args p)
     const int64_t size = int64_t(p.channels) * p.states;
     auto& in = s_in[wave];
     auto& bc = s_bc[wave];
-    float da[4][4], dd[S::kOwn], dbias[S::kOwn];
+    Four da[4];
+    float dd[S::kOwn][2], dbias[S::kOwn][2];
 #pragma unroll
-    for (int ch = 0; ch < 4; ++ch)
+    for (int u = 0; u < 4; ++u) da[u] = Four{};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) da[ch][k] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < S::kOwn; ++i) dd[i] = dbias[i] = 0.0f;
+    for (int i = 0; i < S::kOwn; ++i) dd[i][0] = dd[i][1] = dbias[i][0] = dbias[i][1] = 0.0f;
     for (int64_t slot = piece; slot < p.slots; slot += p.pieces) {
         const Segment s = segment_of(p, slot);
         if (!s.there) continue;
-        const bool alone = s.first_one && s.last_one;
-        const float* const behind = alone ? (p.grad_end ? p.grad_end + s.seq * size : nullptr) : p.back + slot * size;
-        const float* const before = alone ? (p.begin ? p.begin + s.seq * size : nullptr) : p.carry + slot * size;
-        const int64_t tile0 = tile_of(slot, s, R);
-        float back[4][4];
-        col.load_state(p, behind, back);
-        const int64_t tiles = (s.past - s.first + R - 1) / R;
+        Four back[4];
+        if (s.last_one) col.load_state(p, p.grad_end ? p.grad_end + s.seq * size : nullptr, back);
+        else col.load_own(p, p.back, slot, back);
+        const int64_t tile0 = tile_of(slot, s, kSaved), tiles = (s.past - s.first + R - 1) / R;
         for (int64_t tile = tiles - 1; tile >= 0; --tile) {
             const int64_t t0 = s.first + tile * R;
-            const int count = s.past - t0 < R ? int(s.past - t0) : R;
+            const int rows = s.past - t0 < R ? int(s.past - t0) : R;
             {
-                T x[E], delta[E], z[E], g[E];
+                Pack<T, 2> x[E], delta[E], z[E], g[E];
                 Pack<T, 4> shared[S::kPacksEach];
-                col.load(p.x, p.x_step, t0, s.past, x);
-                col.load(p.delta, p.delta_step, t0, s.past, delta);
-                col.load(p.grad, p.grad_step, t0, s.past, g);
-                if (p.z) col.load(p.z, p.z_step, t0, s.past, z);
-                col.load_shared(p, t0, s.past, shared);
+                col.load(p.x, p.x_step, t0, rows, x);
+                col.load(p.delta, p.delta_step, t0, rows, delta);
+                col.load(p.grad, p.grad_step, t0, rows, g);
+                if (p.z) col.load(p.z, p.z_step, t0, rows, z);
+                col.load_shared(p, t0, rows, shared);
+                float v[E][2];
+                col.steps(p, delta, v);
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    const int r = S::row(i, col.lane), ch = S::channel(i, col.lane);
-                    const bool there = ch < col.count;
-                    const float raw = float(delta[i]) + col.bias[S::own(i)], dt = p.softplus ? softplus_of(raw) : raw;
-                    in[r][0][ch] = there ? dt : 0.0f;
-                    in[r][1][ch] = there ? dt * float(x[i]) : 0.0f;
-                    in[r][2][ch] = there ? (p.z ? float(g[i]) * (float(z[i]) * sigmoid(float(z[i]))) : float(g[i])) : 0.0f;
+                    auto& row = in[S::row(i, col.lane)];
+                    col.put(row[0], i, v[i][0], v[i][1]);
+                    col.put(row[1], i, v[i][0] * x[i].get(0), v[i][1] * x[i].get(1));
+                    v[i][0] = g[i].get(0), v[i][1] = g[i].get(1);
                 }
+                if (p.z) col.gate(z, v);
+#pragma unroll
+                for (int i = 0; i < E; ++i) col.put(in[S::row(i, col.lane)][2], i, v[i][0], v[i][1]);
                 col.put_shared(shared, bc);
             }
-            float h[4][4], y[4], dt[4], du[4], gy[4], b[4], c[4];
-            auto forward = [&](int t) __attribute__((always_inline)) {
-                read4(&in[t][0][col.at], dt);
-                read4(&in[t][1][col.at], du);
-                read4(&bc[t][0][4 * col.q], b);
+            auto forward = [&](int t, Four (&h)[4]) __attribute__((always_inline)) {
+                float b[G];
+                col.read_shared(bc[t][0], b);
 #pragma unroll
-                for (int ch = 0; ch < 4; ++ch)
+                for (int i = 0; i < kSets; ++i) {
+                    const Four dt = *reinterpret_cast<const Four*>(&in[t][0][col.at + 4 * i]);
+                    const float du = in[t][1][col.at + 4 * i + col.j];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) h[ch][k] = fmaf(h[ch][k], __builtin_amdgcn_exp2f(dt[ch] * col.a[ch][k]), du[ch] * b[k]);
+                    for (int g = 0; g < G; ++g) h[i * G + g] = add_products(du, b[g], h[i * G + g] * decays(dt, col.a[i * G + g]));
+                }
+            };
+            // back through up to four rows from `low` on, from the state before them
+            auto reverse = [&](int low, const Four (&start)[4]) __attribute__((always_inline)) {
+                Four kept_h[H][4];
+#pragma unroll
+                for (int k = 0; k < H; ++k)
+                    if (low + k < rows) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) kept_h[k][u] = k ? kept_h[k ? k - 1 : 0][u] : start[u];
+                        forward(low + k, kept_h[k]);
+                    }
+#pragma unroll
+                for (int k = H - 1; k >= 0; --k) {
+                    const int t = low + k;
+                    if (t >= rows) continue;
+                    float b[G], c[G], sums[2][G];
+                    col.read_shared(bc[t][0], b);
+                    col.read_shared(bc[t][1], c);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) sums[0][g] = sums[1][g] = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < kSets; ++i) {
+                        const int at = col.at + 4 * i;
+                        const Four dt = *reinterpret_cast<const Four*>(&in[t][0][at]), du = *reinterpret_cast<const Four*>(&in[t][1][at]),
+                                   gy = *reinterpret_cast<const Four*>(&in[t][2][at]);
+                        const float gy_own = in[t][2][at + col.j];
+                        Four through{}, rate{}, y{};
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            const int u = i * G + g;
+                            const Four now = add_products(gy_own, c[g], back[u]), e = decays(dt, col.a[u]);
+#pragma unroll
+                            for (int n = 0; n < 4; ++n) {
+                                const bool there = !SOME || at + n < col.count;
+                                const float h = kept_h[k][u][n];
+                                sums[0][g] = there ? fmaf(du[n], now[n], sums[0][g]) : sums[0][g];
+                                sums[1][g] = there ? fmaf(gy[n], h, sums[1][g]) : sums[1][g];
+                                y[n] = fmaf(c[g], h, y[n]);
+                                through[n] = fmaf(now[n], b[g], through[n]);
+                                back[u][n] = now[n] * e[n];
+                                const float r = back[u][n] * (k ? kept_h[k ? k - 1 : 0][u][n] : start[u][n]);
+                                rate[n] = fmaf(r, col.a[u][n], rate[n]);
+                                da[u][n] = fmaf(r, dt[n], da[u][n]);
+                            }
+                        }
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) through[n] = over_states<Q>(through[n]), rate[n] = over_states<Q>(rate[n]);
+                        *reinterpret_cast<Four*>(&in[t][0][at]) = through;
+                        *reinterpret_cast<Four*>(&in[t][1][at]) = rate;
+                        if (p.z) {
+#pragma unroll
+                            for (int n = 0; n < 4; ++n) y[n] = over_states<Q>(y[n]);
+                            *reinterpret_cast<Four*>(&in[t][2][at]) = y;
+                        }
+                    }
+                    const float2 two = over_channels<Q>(sums);
+                    const int row = col.lane / 16, l = col.lane % 16;       // of 16 lanes
+                    if (l < 4 * S::kQuads) {
+                        float* const to = &s_part[wave][t][row / 2][l / 4 * 16 + l % 4 * G];
+                        if constexpr (G == 4) *reinterpret_cast<float2*>(to + 2 * (row & 1)) = two;
+                        else if constexpr (G == 2) to[row & 1] = two.x;
+                        else to[0] = two.x;
+                    }
+                }
             };
 #pragma unroll 1
-            for (int part = (count - 1) / H; part >= 0; --part) {
-                // the state before the tile
-                col.load_state(p, before, h);
-                if (tile > 0) {
-                    float own[4][4], span[4];
-                    col.load_state(p, p.tile_state + (tile0 + tile) * size, own);
+            for (int low = (rows - 1) / kSaved * kSaved; low >= 0; low -= kSaved) {
+                // the state before these rows
+                Four h[4];
+                const int64_t at = tile0 + tile * (R / kSaved) + low / kSaved;
+                col.load_own(p, p.tile_state, at, h);
+                if (!s.first_one) {
+                    Four before[4], span[kSets];
+                    col.load_own(p, p.carry, slot, before);
+                    col.load_line(p.tile_span + at * p.channels, span);
 #pragma unroll
-                    for (int ch = 0; ch < 4; ++ch) {
-                        span[ch] = col.at + ch < col.count ? p.tile_span[(tile0 + tile) * p.channels + col.first + col.at + ch] : 0.0f;
+                    for (int u = 0; u < 4; ++u) {
+                        const Four e = decays(span[u / G], col.a[u]);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) h[ch][k] = fmaf(h[ch][k], __builtin_amdgcn_exp2f(span[ch] * col.a[ch][k]), own[ch][k]);
+                        for (int k = 0; k < 4; ++k) h[u][k] = fmaf(before[u][k], e[k], h[u][k]);
                     }
                 }
-#pragma unroll 1
-                for (int t = 0; t < part * H; ++t) forward(t);
-                float start[4][4], kept_h[H][4][4];
+                if constexpr (kSaved > H)
+                    if (low + H < rows) {
+                        Four middle[4];
 #pragma unroll
-                for (int ch = 0; ch < 4; ++ch)
+                        for (int u = 0; u < 4; ++u) middle[u] = h[u];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) start[ch][k] = h[ch][k];
-#pragma unroll
-                for (int j = 0; j < H; ++j)
-                    if (part * H + j < count) {
-                        forward(part * H + j);
-#pragma unroll
-                        for (int ch = 0; ch < 4; ++ch)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) kept_h[j][ch][k] = h[ch][k];
+                        for (int k = 0; k < H; ++k) forward(low + k, middle);
+                        reverse(low + H, middle);
                     }
-#pragma unroll
-                for (int j = H - 1; j >= 0; --j) {
-                    const int t = part * H + j;
-                    if (t >= count) continue;
-                    read4(&in[t][0][col.at], dt);
-                    read4(&in[t][1][col.at], du);
-                    read4(&in[t][2][col.at], gy);
-                    read4(&bc[t][0][4 * col.q], b);
-                    read4(&bc[t][1][4 * col.q], c);
-                    float sums[2][4], through[4], rate[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) sums[0][k] = sums[1][k] = 0.0f;
-#pragma unroll
-                    for (int ch = 0; ch < 4; ++ch) {
-                        through[ch] = rate[ch] = y[ch] = 0.0f;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float now = fmaf(gy[ch], c[k], back[ch][k]);
-                            const bool there = !SOME || col.at + ch < col.count;
-                            sums[0][k] = fmaf(du[ch], there ? now : 0.0f, sums[0][k]);
-                            sums[1][k] = fmaf(gy[ch], there ? kept_h[j][ch][k] : 0.0f, sums[1][k]);
-                            y[ch] = fmaf(c[k], kept_h[j][ch][k], y[ch]);
-                            through[ch] = fmaf(now, b[k], through[ch]);
-                            back[ch][k] = now * __builtin_amdgcn_exp2f(dt[ch] * col.a[ch][k]);
-                            const float r = back[ch][k] * (j ? kept_h[j ? j - 1 : 0][ch][k] : start[ch][k]);
-                            rate[ch] = fmaf(r, col.a[ch][k], rate[ch]);
-                            da[ch][k] = fmaf(r, dt[ch], da[ch][k]);
-                        }
-                        through[ch] = over_states<Q>(through[ch]);
-                        rate[ch] = over_states<Q>(rate[ch]);
-                        if (p.z) y[ch] = over_states<Q>(y[ch]);
-                    }
-                    *reinterpret_cast<float4*>(&in[t][0][col.at]) = float4{through[0], through[1], through[2], through[3]};
-                    *reinterpret_cast<float4*>(&in[t][1][col.at]) = float4{rate[0], rate[1], rate[2], rate[3]};
-                    if (p.z) *reinterpret_cast<float4*>(&in[t][2][col.at]) = float4{y[0], y[1], y[2], y[3]};
-                    const float2 two = over_channels<Q>(sums);
-                    const int row = col.lane / 16, q = col.lane % 16;
-                    if (q < Q) *reinterpret_cast<float2*>(&s_part[wave][t][row / 2][4 * q + 2 * (row & 1)]) = two;
-                }
+                reverse(low, h);
             }
             // the channels' gradients of these rows
             {
-                T x[E], delta[E], z[E], g[E];
-                col.load(p.x, p.x_step, t0, s.past, x);
-                col.load(p.delta, p.delta_step, t0, s.past, delta);
-                col.load(p.grad, p.grad_step, t0, s.past, g);
-                if (p.z) col.load(p.z, p.z_step, t0, s.past, z);
+                Pack<T, 2> x[E], delta[E], z[E], g[E];
+                col.load(p.x, p.x_step, t0, rows, x);
+                col.load(p.delta, p.delta_step, t0, rows, delta);
+                col.load(p.grad, p.grad_step, t0, rows, g);
+                if (p.z) col.load(p.z, p.z_step, t0, rows, z);
+                float dt[E][2], gy[E][2], v[E][2];
+                col.steps(p, delta, dt);
 #pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const int r = S::row(i, col.lane), ch = S::channel(i, col.lane), o = S::own(i);
-                    if (r >= count || ch >= col.count) continue;
-                    const float raw = float(delta[i]) + col.bias[o], dt = p.softplus ? softplus_of(raw) : raw, xv = float(x[i]), gv = float(g[i]);
-                    const float through = in[r][0][ch], ddt = fmaf(in[r][1][ch], kLn2, through * xv), ddelta = p.softplus ? ddt * sigmoid(raw) : ddt;
-                    const int64_t at = (t0 + r) * p.channels + col.first + ch;
-                    float gy = gv;
-                    if (p.z) {
-                        const float zv = float(z[i]);
-                        gy = gv * (zv * sigmoid(zv));
-                        static_cast<T*>(p.dz)[at] = T(gv * fmaf(col.d[o], xv, in[r][2][ch]) * slope(zv));
+                for (int i = 0; i < E; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const auto& row = in[S::row(i, col.lane)];
+                        gy[i][k] = g[i].get(k);
+                        v[i][k] = fmaf(row[1][col.channel_of(i) + k], kLn2, row[0][col.channel_of(i) + k] * x[i].get(k));
                     }
-                    static_cast<T*>(p.out)[at] = T(fmaf(through, dt, col.d[o] * gy));
-                    static_cast<T*>(p.ddelta)[at] = T(ddelta);
-                    dd[o] = fmaf(gy, xv, dd[o]);
-                    dbias[o] += ddelta;
+                if (p.softplus)
+#pragma unroll
+                    for (int i = 0; i < E; ++i)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) v[i][k] *= sigmoid(delta[i].get(k) + col.bias[i % S::kOwn][k]);
+                col.store(p.ddelta, p.channels, t0, rows, v);
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) dbias[i % S::kOwn][k] = S::row(i, col.lane) < rows ? dbias[i % S::kOwn][k] + v[i][k] : dbias[i % S::kOwn][k];
+                if (p.z) {
+#pragma unroll
+                    for (int i = 0; i < E; ++i)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const float gate = z[i].get(k), w = sigmoid(gate), y = fmaf(col.d[i % S::kOwn][k], x[i].get(k), in[S::row(i, col.lane)][2][col.channel_of(i) + k]);
+                            v[i][k] = gy[i][k] * y * (w * fmaf(gate, 1.0f - w, 1.0f));
+                            gy[i][k] *= gate * w;
+                        }
+                    col.store(p.dz, p.channels, t0, rows, v);
                 }
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        v[i][k] = fmaf(in[S::row(i, col.lane)][0][col.channel_of(i) + k], dt[i][k], col.d[i % S::kOwn][k] * gy[i][k]);
+                        dd[i % S::kOwn][k] = S::row(i, col.lane) < rows ? fmaf(gy[i][k], x[i].get(k), dd[i % S::kOwn][k]) : dd[i % S::kOwn][k];
+                    }
+                col.store(p.out, p.channels, t0, rows, v);
             }
             // the block's sums over channels
             __syncthreads();
             float* const to = p.shared_parts + ((gb * p.rows + t0) * p.groups + group) * 2 * S::kStates;
-            for (int e = threadIdx.x; e < count * 2 * S::kStates; e += blockDim.x) {
+            for (int e = threadIdx.x; e < rows * 2 * S::kStates; e += blockDim.x) {
                 const int t = e / (2 * S::kStates), n = e % (2 * S::kStates);
                 float sum = 0.0f;
                 for (int w = 0; w < p.waves; ++w) sum += (&s_part[w][t][0][0])[n];
@@ -328,28 +379,29 @@ __global__ void __launch_bounds__(kThreads, 2) back_kernel(Args p)
     const int each = p.states + 2;
     float* const own = p.own_parts + int64_t(piece) * p.channels * each;
 #pragma unroll
-    for (int ch = 0; ch < 4; ++ch)
+    for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (col.at + ch < col.count && 4 * col.q + k < p.states) own[int64_t(col.first + col.at + ch) * each + 4 * col.q + k] = da[ch][k];
+        for (int i = 0; i < 4; ++i)
+            if (col.channel(u) + i < col.count && col.state(u) < p.states) own[int64_t(col.first + col.channel(u) + i) * each + col.state(u)] = da[u][i];
     // lanes with the same channels add up
 #pragma unroll
-    for (int i = 0; i < S::kOwn; ++i) {
-        if constexpr (S::kChannels < 64)
+    for (int i = 0; i < S::kOwn; ++i)
 #pragma unroll
-            for (int m = S::kChannels; m < 64; m *= 2) dd[i] += __shfl_xor(dd[i], m), dbias[i] += __shfl_xor(dbias[i], m);
-        const int ch = S::kChannels < 64 ? col.lane % S::kChannels : i * 64 + col.lane;
-        if (ch < col.count && col.lane < S::kChannels) {
-            own[int64_t(col.first + ch) * each + p.states] = dd[i];
-            own[int64_t(col.first + ch) * each + p.states + 1] = dbias[i];
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int m = S::kChannels / 2; m < 64; m *= 2) dd[i][k] += __shfl_xor(dd[i][k], m), dbias[i][k] += __shfl_xor(dbias[i][k], m);
+            if (col.counts(i, k) && col.lane < S::kChannels / 2) {
+                own[int64_t(col.first + col.channel_of(i) + k) * each + p.states] = dd[i][k];
+                own[int64_t(col.first + col.channel_of(i) + k) * each + p.states + 1] = dbias[i][k];
+            }
         }
-    }
 }
 
 // the gradients of b and c: a thread to a value, over the blocks of its group
-template <typename T>
-__global__ void __launch_bounds__(kThreads) shared_kernel(Args p, int wide, T* db, T* dc)
+template <typename T, int Q>
+__global__ void __launch_bounds__(kThreads) shared_kernel(Args p, T* db, T* dc)
 {
+    using S = Shape<Q>;
     const int64_t e = (int64_t(p.first_block) + blockIdx.x) * kThreads + threadIdx.x, all = p.rows * p.groups * 2 * p.states;
     if (e >= all) return;
     const int64_t pair = e / (2 * p.states);            // row and group
@@ -359,23 +411,21 @@ __global__ void __launch_bounds__(kThreads) shared_kernel(Args p, int wide, T* d
         if (row < first || row >= kept(p.offsets[p.n], first, p.rows)) return;
     }
     float sum = 0.0f;
-    for (int g = 0; g < p.group_blocks; ++g) sum += p.shared_parts[((g * p.rows * p.groups + pair) * 2 + dir) * wide + state];
+    for (int g = 0; g < p.group_blocks; ++g) sum += p.shared_parts[((g * p.rows * p.groups + pair) * 2 + dir) * S::kStates + S::place(state)];
     (dir ? dc : db)[pair * p.states + state] = T(sum);
 }
 
-// those of a, d and bias: a thread to a value, over the pieces of the slots
-__global__ void __launch_bounds__(kThreads) own_kernel(Args p, float* da, float* dd, float* dbias)
+// those of a, d and bias, over the pieces of the slots
+__global__ void __launch_bounds__(kSumThreads) own_kernel(Args p, float* da, float* dd, float* dbias)
 {
     const int each = p.states + 2;
-    const int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x, all = int64_t(p.channels) * each;
-    if (e >= all) return;
-    float sum = 0.0f;
-    for (int n = 0; n < p.pieces; ++n) sum += p.own_parts[n * all + e];
-    const int64_t ch = e / each;
-    const int i = int(e - ch * each);
-    if (i < p.states) da[ch * p.states + i] = sum;
-    else if (i == p.states && dd) dd[ch] = sum;
-    else if (i > p.states && dbias) dbias[ch] = sum;
+    sum_pieces(p.own_parts, p.pieces, int64_t(p.channels) * each, [&](int64_t e, float sum) {
+        const int64_t ch = e / each;
+        const int i = int(e - ch * each);
+        if (i < p.states) da[ch * p.states + i] = sum;
+        else if (i == p.states && dd) dd[ch] = sum;
+        else if (i > p.states && dbias) dbias[ch] = sum;
+    });
 }
 
 uint64_t up(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -397,14 +447,15 @@ Layout layout_of(bool packed, int64_t rows, int64_t n, int64_t length, int chann
     // a piece of the slots to a block: enough of them for some waves to every SIMD
     const int64_t columns = int64_t(groups) * p.tiles, most = std::max<int64_t>(4096 / columns, 1);
     l.pieces = int(std::min(p.slots, most));
-    const uint64_t size = uint64_t(channels) * states * 4, line = uint64_t(channels) * 4, tiles = uint64_t(rows / tile_rows(p.q) + p.slots), several = p.several ? p.slots : 0;
+    const uint64_t size = uint64_t(groups) * p.tiles * 4096, line = uint64_t(channels) * 4, several = p.several ? p.slots : 0;
+    const uint64_t tiles = uint64_t(rows / std::min(tile_rows(p.q), 8) + p.slots);
     uint64_t at = 0;
     auto take = [&](uint64_t& where, uint64_t bytes) { where = at, at += up(bytes); };
     take(l.carry, several * size);
     take(l.back, several * size);
     take(l.span, several * line);
     take(l.tile_state, tiles * size);
-    take(l.tile_span, tiles * line);
+    take(l.tile_span, p.several ? tiles * line : 0);
     take(l.shared_parts, uint64_t(l.group_blocks) * rows * groups * 2 * 4 * p.q * 4);
     take(l.own_parts, uint64_t(l.pieces) * channels * (states + 2) * 4);
     l.all = at;
@@ -460,15 +511,16 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan_backprop(
         check_workspace(workspace, workspace_bytes, l.all);
         char* const w = static_cast<char*>(workspace);
         auto at = [&](uint64_t where) { return reinterpret_cast<float*>(w + where); };
-        p.carry = at(l.carry), p.back = at(l.back), p.span = at(l.span), p.tile_state = at(l.tile_state), p.tile_span = at(l.tile_span);
+        auto state_at = [&](uint64_t where) { return reinterpret_cast<Four*>(w + where); };
+        p.carry = state_at(l.carry), p.back = state_at(l.back), p.span = at(l.span), p.tile_state = state_at(l.tile_state), p.tile_span = at(l.tile_span);
         p.shared_parts = at(l.shared_parts), p.own_parts = at(l.own_parts);
         p.segment = l.plan.segment, p.slots = l.plan.slots, p.per_sequence = l.plan.per_sequence, p.several = l.plan.several, p.tiles = l.plan.tiles;
         p.waves = l.waves, p.group_blocks = l.group_blocks, p.pieces = l.pieces;
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
-            if (p.slots)
-                with_lanes(l.plan.q, [&](auto q) {
-                    constexpr int Q = decltype(q)::value;
+            with_lanes(l.plan.q, [&](auto q) {
+                constexpr int Q = decltype(q)::value;
+                if (p.slots) {
                     const int64_t blocks = (p.slots * p.groups * p.tiles + kWaves - 1) / kWaves;
                     if (p.several) {
                         launch_all(states_kernel<T, Q, true>, blocks, kThreads, s, p);
@@ -479,14 +531,15 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan_backprop(
                     const int64_t work = int64_t(p.pieces) * p.groups * p.group_blocks;
                     if (p.per_group % Shape<Q>::kChannels) launch_all(back_kernel<T, Q, true>, work, 64 * p.waves, s, p);
                     else launch_all(back_kernel<T, Q, false>, work, 64 * p.waves, s, p);
-                });
-            if (p.rows)
+                }
                 in_launches((p.rows * p.groups * 2 * p.states + kThreads - 1) / kThreads, kThreads, [&](unsigned first, dim3 grid) {
-                    p.first_block = first;
-                    hipLaunchKernelGGL(shared_kernel<T>, grid, dim3(kThreads), 0, s, p, 4 * l.plan.q, static_cast<T*>(grad_b), static_cast<T*>(grad_c));
+                    Args more = p;
+                    more.first_block = first;
+                    hipLaunchKernelGGL((shared_kernel<T, Q>), grid, dim3(kThreads), 0, s, more, static_cast<T*>(grad_b), static_cast<T*>(grad_c));
                 });
+            });
         });
-        hipLaunchKernelGGL(own_kernel, dim3(unsigned((int64_t(p.channels) * (p.states + 2) + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, p, grad_a, grad_d, grad_delta_bias);
+        hipLaunchKernelGGL(own_kernel, sum_blocks(int64_t(p.channels) * (p.states + 2)), dim3(kSumThreads), 0, s, p, grad_a, grad_d, grad_delta_bias);
         SIG_HIP(hipGetLastError());
     });
 }
