@@ -65,18 +65,17 @@ struct Args {
     int64_t rows, length, n, segment, slots, per_sequence;
     int64_t x_step, delta_step, z_step, grad_step, b_step, b_group, c_step, c_group;
     int channels, states, groups, per_group, tiles;     // tiles: of a group's channels
-    int waves, group_blocks, pieces;                    // backward: waves to a block (they divide the tiles), blocks to a group, pieces of the slots
+    int group_blocks, pieces;                           // backward: blocks to a group, pieces of the slots
     bool softplus, several;                             // several: a sequence may have more than one segment
     unsigned first_block;
 };
 
-// log(1 + e^v) = max(v, 0) + log1p(w), w = e^-|v|; log1p(w) = 2 atanh(s) with s = w / (2 + w) <= 1/3, and atanh(s) / s as a polynomial
-// in s^2, fitted on that range (off by 4e-9; the whole by four roundings)
+// log(1 + e^v) = max(v, 0) + log(1 + w), w = e^-|v|: the logarithm of u = 1 + w as it was rounded, and what the rounding left out, over u, which is 1
+// wherever that counts.  The hardware's logarithm is off by two roundings on all of [1, 2], the whole by |v| (the exponential's) and four.
 __device__ __forceinline__ float softplus_of(float v)
 {
-    const float w = __builtin_amdgcn_exp2f(-fabsf(v) * kLog2e), s = w * __builtin_amdgcn_rcpf(2.0f + w), u = s * s;
-    const float f = fmaf(fmaf(fmaf(fmaf(0.14089162647724152f, u, 0.13980302214622498f), u, 0.20012454688549042f), u, 0.3333315849304199f), u, 1.0f);
-    return fmaxf(v, 0.0f) + 2.0f * s * f;
+    const float w = __builtin_amdgcn_exp2f(-fabsf(v) * kLog2e), u = 1.0f + w;
+    return fmaxf(v, 0.0f) + fmaf(__builtin_amdgcn_logf(u), kLn2, w - (u - 1.0f));
 }
 
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * kLog2e)); }
@@ -177,10 +176,10 @@ struct Column {
         part = lane / 4 % S::kQuads;
         at = lane / 4 / S::kQuads * 4 * kSets;
         group = group_;
-        column = group * p.tiles + tile;
-        first = group * p.per_group + tile * S::kChannels;
-        count = p.per_group - tile * S::kChannels;
-        count = count < S::kChannels ? count : S::kChannels;
+        const int place = tile < p.tiles ? tile : p.tiles - 1;       // a wave behind the last tile has no channels
+        column = group * p.tiles + place;
+        first = group * p.per_group + place * S::kChannels;
+        count = tile < p.tiles ? min(p.per_group - place * S::kChannels, S::kChannels) : 0;
         load_state(p, p.a, a);
 #pragma unroll
         for (int u = 0; u < 4; ++u) a[u] *= kLog2e;

@@ -16,7 +16,7 @@ namespace {
 
 // OUT: the outputs and the sequences' last states; otherwise the segments' own last states and the sums of dt
 template <typename T, int Q, bool OUT>
-__global__ void __launch_bounds__(kThreads, 2) scan_kernel(Args p)
+__global__ void __launch_bounds__(kThreads, OUT && (sizeof(T) == 4 || Q == 1) ? 2 : 3) scan_kernel(Args p)
 {
     using S = Shape<Q>;
     constexpr int R = S::kRows, E = S::kEach, G = S::kGroups, kSets = S::kSets;
@@ -243,7 +243,7 @@ Plan plan_of(bool packed, int64_t rows, int64_t n, int64_t length, int channels,
     p.q = lanes_of(states);
     const int wide = 256 / p.q, tile = tile_rows(p.q);
     p.tiles = (channels / groups + wide - 1) / wide;
-    const int64_t most = 4096, columns = int64_t(groups) * p.tiles;
+    const int64_t most = back ? 2048 : 4096, columns = int64_t(groups) * p.tiles;
     int64_t segment = (rows * columns + most - 1) / most;
     segment = (std::max<int64_t>(segment, 4 * tile) + tile - 1) / tile * tile;
     const int64_t longest = packed ? rows : length;
@@ -257,7 +257,7 @@ Plan plan_of(bool packed, int64_t rows, int64_t n, int64_t length, int channels,
 // Many segments to a sequence are joined by several threads to a state
 void join_segments(const Args& p, bool back, hipStream_t stream)
 {
-    const int64_t states = int64_t(p.groups) * p.tiles * 1024, count = p.offsets ? p.rows / p.segment : p.per_sequence;
+    const int64_t states = int64_t(p.groups) * p.tiles * 1024, count = p.offsets ? p.rows / p.segment / p.n : p.per_sequence;        // on average
     with_lanes(lanes_of(p.states), [&](auto q) {
         constexpr int Q = decltype(q)::value;
         auto launch = [&](auto kernel, int pieces) {

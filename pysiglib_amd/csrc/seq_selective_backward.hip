@@ -156,21 +156,20 @@ __device__ __forceinline__ float2 over_channels(const float (&v)[2][Shape<Q>::kG
     return float2{w[0], w[1]};
 }
 
-// SOME: a wave may have fewer channels than there is room for.  What stands in their place is no
+// W waves to a block.  SOME: a wave may have fewer channels than there is room for.  What stands in their place is no
 // number in particular, and takes no part in the sums over channels.
-template <typename T, int Q, bool SOME>
-__global__ void __launch_bounds__(kThreads, 2) back_kernel(Args p)
+template <typename T, int Q, int W, bool SOME>
+__global__ void __launch_bounds__(64 * W, 2) back_kernel(Args p)
 {
     using S = Shape<Q>;
     constexpr int R = S::kRows, E = S::kEach, G = S::kGroups, kSets = S::kSets, kSaved = S::kSaved, H = 4;      // H: rows whose states are kept
-    __shared__ __attribute__((aligned(16))) float s_in[kWaves][R][3][S::kChannels];
-    __shared__ __attribute__((aligned(16))) float s_bc[kWaves][R][2][S::kStates];
-    __shared__ __attribute__((aligned(16))) float s_part[kWaves][R][2][S::kStates];
+    __shared__ __attribute__((aligned(16))) float s_in[W][R][4][S::kChannels];
+    __shared__ __attribute__((aligned(16))) float s_bc[W][R][2][S::kStates];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), blocks = p.groups * p.group_blocks;
     const int64_t block = int64_t(p.first_block) + blockIdx.x;
     const int piece = int(block / blocks), group = int(block % blocks) / p.group_blocks, gb = int(block % blocks) % p.group_blocks;
     Column<T, Q> col;
-    col.init(p, group, gb * p.waves + wave);
+    col.init(p, group, gb * W + wave);
     const int64_t size = int64_t(p.channels) * p.states;
     auto& in = s_in[wave];
     auto& bc = s_bc[wave];
@@ -205,6 +204,7 @@ __global__ void __launch_bounds__(kThreads, 2) back_kernel(Args p)
                     auto& row = in[S::row(i, col.lane)];
                     col.put(row[0], i, v[i][0], v[i][1]);
                     col.put(row[1], i, v[i][0] * x[i].get(0), v[i][1] * x[i].get(1));
+                    col.put(row[3], i, v[i][0], v[i][1]);       // again: the first three are overwritten
                     v[i][0] = g[i].get(0), v[i][1] = g[i].get(1);
                 }
                 if (p.z) col.gate(z, v);
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 2) back_kernel(Args p)
                     const float2 two = over_channels<Q>(sums);
                     const int row = col.lane / 16, l = col.lane % 16;       // of 16 lanes
                     if (l < 4 * S::kQuads) {
-                        float* const to = &s_part[wave][t][row / 2][l / 4 * 16 + l % 4 * G];
+                        float* const to = &bc[t][row / 2][l / 4 * 16 + l % 4 * G];          // in the place of b and c, which this row has read
                         if constexpr (G == 4) *reinterpret_cast<float2*>(to + 2 * (row & 1)) = two;
                         else if constexpr (G == 2) to[row & 1] = two.x;
                         else to[0] = two.x;
@@ -323,20 +323,21 @@ __global__ void __launch_bounds__(kThreads, 2) back_kernel(Args p)
                 col.load(p.grad, p.grad_step, t0, rows, g);
                 if (p.z) col.load(p.z, p.z_step, t0, rows, z);
                 float dt[E][2], gy[E][2], v[E][2];
-                col.steps(p, delta, dt);
 #pragma unroll
                 for (int i = 0; i < E; ++i)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const auto& row = in[S::row(i, col.lane)];
+                        const int ch = col.channel_of(i) + k;
+                        dt[i][k] = row[3][ch];
                         gy[i][k] = g[i].get(k);
-                        v[i][k] = fmaf(row[1][col.channel_of(i) + k], kLn2, row[0][col.channel_of(i) + k] * x[i].get(k));
+                        v[i][k] = fmaf(row[1][ch], kLn2, row[0][ch] * x[i].get(k));
                     }
-                if (p.softplus)
+                if (p.softplus)         // its slope: e^(raw - softplus(raw))
 #pragma unroll
                     for (int i = 0; i < E; ++i)
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) v[i][k] *= sigmoid(delta[i].get(k) + col.bias[i % S::kOwn][k]);
+                        for (int k = 0; k < 2; ++k) v[i][k] *= __builtin_amdgcn_exp2f((delta[i].get(k) + col.bias[i % S::kOwn][k] - dt[i][k]) * kLog2e);
                 col.store(p.ddelta, p.channels, t0, rows, v);
 #pragma unroll
                 for (int i = 0; i < E; ++i)
@@ -365,10 +366,10 @@ __global__ void __launch_bounds__(kThreads, 2) back_kernel(Args p)
             // the block's sums over channels
             __syncthreads();
             float* const to = p.shared_parts + ((gb * p.rows + t0) * p.groups + group) * 2 * S::kStates;
-            for (int e = threadIdx.x; e < rows * 2 * S::kStates; e += blockDim.x) {
+            for (int e = threadIdx.x; e < rows * 2 * S::kStates; e += 64 * W) {
                 const int t = e / (2 * S::kStates), n = e % (2 * S::kStates);
                 float sum = 0.0f;
-                for (int w = 0; w < p.waves; ++w) sum += (&s_part[w][t][0][0])[n];
+                for (int w = 0; w < W; ++w) sum += (&s_bc[w][t][0][0])[n];
                 to[int64_t(t) * p.groups * 2 * S::kStates + n] = sum;
             }
             __syncthreads();
@@ -441,9 +442,9 @@ Layout layout_of(bool packed, int64_t rows, int64_t n, int64_t length, int chann
     Layout l;
     l.plan = plan_of(packed, rows, n, length, channels, states, groups, true);
     const Plan& p = l.plan;
-    l.waves = kWaves;
-    while (p.tiles % l.waves) --l.waves;
-    l.group_blocks = p.tiles / l.waves;
+    // four waves to a block add up their sums over channels; groups of one or two tiles leave such blocks half empty
+    l.waves = p.tiles > 2 ? kWaves : 1;
+    l.group_blocks = (p.tiles + l.waves - 1) / l.waves;
     // a piece of the slots to a block: enough of them for some waves to every SIMD
     const int64_t columns = int64_t(groups) * p.tiles, most = std::max<int64_t>(4096 / columns, 1);
     l.pieces = int(std::min(p.slots, most));
@@ -515,7 +516,7 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan_backprop(
         p.carry = state_at(l.carry), p.back = state_at(l.back), p.span = at(l.span), p.tile_state = state_at(l.tile_state), p.tile_span = at(l.tile_span);
         p.shared_parts = at(l.shared_parts), p.own_parts = at(l.own_parts);
         p.segment = l.plan.segment, p.slots = l.plan.slots, p.per_sequence = l.plan.per_sequence, p.several = l.plan.several, p.tiles = l.plan.tiles;
-        p.waves = l.waves, p.group_blocks = l.group_blocks, p.pieces = l.pieces;
+        p.group_blocks = l.group_blocks, p.pieces = l.pieces;
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
             with_lanes(l.plan.q, [&](auto q) {
@@ -529,8 +530,10 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan_backprop(
                         launch_all(states_kernel<T, Q, false>, blocks, kThreads, s, p);
                     }
                     const int64_t work = int64_t(p.pieces) * p.groups * p.group_blocks;
-                    if (p.per_group % Shape<Q>::kChannels) launch_all(back_kernel<T, Q, true>, work, 64 * p.waves, s, p);
-                    else launch_all(back_kernel<T, Q, false>, work, 64 * p.waves, s, p);
+                    const bool some = p.per_group % (Shape<Q>::kChannels * l.waves);
+                    if (l.waves == 1) launch_all(back_kernel<T, Q, 1, true>, work, 64, s, p);
+                    else if (some) launch_all(back_kernel<T, Q, kWaves, true>, work, kThreads, s, p);
+                    else launch_all(back_kernel<T, Q, kWaves, false>, work, kThreads, s, p);
                 }
                 in_launches((p.rows * p.groups * 2 * p.states + kThreads - 1) / kThreads, kThreads, [&](unsigned first, dim3 grid) {
                     Args more = p;
