@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWidest = 8;
+constexpr int kAtOnce = 4;          // rows that a thread takes at once, backward
 
 struct ConvArgs {
     const void* x;              // [rows][channels], rows x_step apart
@@ -31,7 +32,7 @@ struct ConvArgs {
     const int* offsets;         // [n + 1] rows where sequences begin, or null: n sequences of `length` rows
     int64_t rows, x_step, grad_step, length, n;
     int channels, lanes, channel_blocks, pieces;
-    int64_t runs, blocks, idle; // blocks with runs; `idle` ones behind them serve sequences without rows
+    int64_t run, blocks, idle;  // backward: rows of a thread; blocks with rows; `idle` ones behind them serve sequences without rows
     bool silu, past;
     unsigned first_block;
 };
@@ -200,13 +201,14 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs a)
     }
 }
 
-// Gradients: a block goes through runs of R rows, a thread walks each from its last row to its first with the window of the W - 1 values e
-// behind the row and that of the W rows of x up to it.
-template <typename T, int V, int W, int R, bool PART>
+// Gradients: a thread walks a run of rows from its last to its first, U at a time, with the window of the W - 1 values e behind them; the next
+// rows are on their way meanwhile.  The W - 1 rows behind its own it goes through first, for their e.
+template <typename T, int V, int W, bool PART>
 __global__ void __launch_bounds__(kThreads) conv_back_kernel(ConvArgs a)
 {
     const int64_t block = int64_t(a.first_block) + blockIdx.x;
     if (block >= a.blocks) return without_rows<T, W>(a, a.grad_end, a.end);
+    constexpr int U = kAtOnce, kX = U + W - 1;
     __shared__ float s_sum[kThreads][V + 1];
     const int groups = kThreads / a.lanes, cb = int(block % a.channel_blocks), piece = int(block / a.channel_blocks), group = int(threadIdx.x) / a.lanes;
     const Lane<T, V, PART> lane((cb * a.lanes + int(threadIdx.x) % a.lanes) * V, a.channels);
@@ -220,14 +222,14 @@ __global__ void __launch_bounds__(kThreads) conv_back_kernel(ConvArgs a)
         for (int k = 0; k < W; ++k) dw[k][v] = 0.0f;
     }
     float e[W][V];              // e[j]: of the row j behind
-    // row t with the rows of x up to it: e, and where the row is the run's own its part of the sums and dx
-    auto value = [&](const float (&xs)[W][V], const float* g, bool own) __attribute__((always_inline)) {
+    // row t with the rows of x up to it: e, and where the row is the run's own its part of the sums
+    auto value = [&](const float (&xs)[W][V], const Pack<T, V>& g, bool own) __attribute__((always_inline)) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float sum = bias[v];
 #pragma unroll
             for (int k = 0; k < W; ++k) sum = fmaf(w[k][v], xs[k][v], sum);
-            e[0][v] = a.silu ? g[v] * slope(sum) : g[v];
+            e[0][v] = a.silu ? g.get(v) * slope(sum) : g.get(v);
             if (own) {
                 db[v] += e[0][v];
 #pragma unroll
@@ -255,81 +257,114 @@ __global__ void __launch_bounds__(kThreads) conv_back_kernel(ConvArgs a)
 #pragma unroll
             for (int j = 0; j < W; ++j) e[j][v] = 0.0f;
     };
-    for (int64_t run = int64_t(piece) * groups + group; run < a.runs; run += int64_t(a.pieces) * groups) {
-        const int64_t t0 = run * R, t1 = t0 + R < a.rows ? t0 + R : a.rows;
-        int64_t i = sequence_at(a, t0), first = 0, past = 0;
-        if (i >= a.n) continue;
-        rows_of(a, i, first, past);
-        if (t0 - (W - 1) >= first && t0 + R + W - 1 <= past) {
-            // nothing but rows of one sequence that are neither its first nor its last ones
-            constexpr int kX = R + 2 * (W - 1), kG = R + W - 1;
-            Pack<T, V> xs[kX], gs[kG];
+    auto load = [&](const T* from, int64_t step, int64_t t) __attribute__((always_inline)) {
+        return lane.template load<T>(from + (t < 0 ? 0 : (t < a.rows ? t : a.rows - 1)) * step);
+    };
+    const int64_t t0 = (int64_t(piece) * groups + group) * a.run, t1 = t0 + a.run < a.rows ? t0 + a.run : a.rows;
+    if (t0 < t1) {
+        int64_t i = -1, first = 0, past = 0;        // the sequence that the walk is in: none
+        // the gradient of the final state, which the last W - 1 positions have
+        auto add_end = [&](int64_t p, float* d) __attribute__((always_inline)) {
+            const int64_t place = p - (past - first - (W - 1));
+            if (!a.grad_end || place < 0) return;
+            const Pack<T, V> more = lane.template load<T>(static_cast<const T*>(a.grad_end) + (i * (W - 1) + place) * a.channels);
 #pragma unroll
-            for (int r = 0; r < kX; ++r) xs[r] = lane.template load<T>(x + (t0 - (W - 1) + r) * a.x_step);
-#pragma unroll
-            for (int r = 0; r < kG; ++r) gs[r] = lane.template load<T>(grad + (t0 + r) * a.grad_step);
-            clear();
-#pragma unroll
-            for (int r = kG - 1; r >= 0; --r) {
-                float taps[W][V], g[V], d[V];
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    g[v] = gs[r].get(v);
-#pragma unroll
-                    for (int k = 0; k < W; ++k) taps[k][v] = xs[r + k].get(v);
+            for (int v = 0; v < V; ++v) d[v] += more.get(v);
+        };
+        // a row near a sequence's first or last one; xs: the rows of memory up to it
+        auto one = [&](const Pack<T, V>* xs, const Pack<T, V>& g, int64_t t, bool own) __attribute__((always_inline)) {
+            if (i < 0 || t < first) {
+                i = sequence_at(a, t);
+                if (i < a.n) rows_of(a, i, first, past);
+                if (i >= a.n || t < first || t >= past) {       // of none
+                    i = -1;
+                    return;
                 }
-                value(taps, g, r < R);
-                if (r < R) {
-                    derivative(d);
-                    lane.template store<T>(static_cast<T*>(a.out) + (t0 + r) * a.channels, d, a.past);
-                }
-                shift();
+                clear();
+            } else if (t == past - 1) {
+                clear();
             }
-            continue;
-        }
-        for (; i < a.n; ++i) {
-            rows_of(a, i, first, past);
-            if (first >= t1) break;
-            const int64_t low = t0 > first ? t0 : first, high = t1 < past ? t1 : past;
-            if (low >= high) continue;
-            clear();
-            const int64_t len = past - first;
-            int64_t t = high + W - 2 < past - 1 ? high + W - 2 : past - 1;
-            float taps[W][V];
+            const int64_t p = t - first;
+            float taps[W][V], d[V];
 #pragma unroll
-            for (int k = 1; k < W; ++k) row_at<T, V, W, PART>(a, lane, i, first, t - first - (W - 1) + k, taps[k - 1]);
-            // down to the sequence's first row, and from there through the positions of the initial state
-            const int64_t lowest = low == first ? first - (W - 1) : low;
-            for (; t >= lowest; --t) {
-                const int64_t p = t - first;
-                float d[V];
-                if (p >= 0) {
-                    const Pack<T, V> gp = lane.template load<T>(grad + t * a.grad_step);
-                    float g[V];
+            for (int k = 0; k < W; ++k) {
+                if (p - (W - 1) + k >= 0)
 #pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        g[v] = gp.get(v);
+                    for (int v = 0; v < V; ++v) taps[k][v] = xs[k].get(v);
+                else row_at<T, V, W, PART>(a, lane, i, first, p - (W - 1) + k, taps[k]);
+            }
+            value(taps, g, own);
+            if (own) {
+                derivative(d);
+                add_end(p, d);
+                lane.template store<T>(static_cast<T*>(a.out) + t * a.channels, d, a.past);
+            }
+            shift();
+            if (own && p == 0) {            // on through the positions of the initial state
 #pragma unroll
-                        for (int k = W - 1; k > 0; --k) taps[k][v] = taps[k - 1][v];
-                    }
-                    row_at<T, V, W, PART>(a, lane, i, first, p - (W - 1), taps[0]);
-                    value(taps, g, t < high);
-                } else {
+                for (int k = 1; k < W; ++k) {
 #pragma unroll
                     for (int v = 0; v < V; ++v) e[0][v] = 0.0f;
-                }
-                if (t < high) {
                     derivative(d);
-                    if (a.grad_end && p >= len - (W - 1)) {
-                        const Pack<T, V> more = lane.template load<T>(static_cast<const T*>(a.grad_end) + (i * (W - 1) + p - (len - (W - 1))) * a.channels);
-#pragma unroll
-                        for (int v = 0; v < V; ++v) d[v] += more.get(v);
-                    }
-                    if (p >= 0) lane.template store<T>(static_cast<T*>(a.out) + t * a.channels, d, a.past);
-                    else lane.template store<T>(static_cast<T*>(a.end) + (i * (W - 1) + (W - 1) + p) * a.channels, d, false);
+                    add_end(-k, d);
+                    lane.template store<T>(static_cast<T*>(a.end) + (i * (W - 1) + (W - 1) - k) * a.channels, d, false);
+                    shift();
                 }
-                shift();
             }
+        };
+        clear();
+        if constexpr (W > 1) {
+            // the rows behind the run, as far as the sequence of its last row goes
+            Pack<T, V> xs[2 * (W - 1)], gs[W - 1];
+#pragma unroll
+            for (int k = 0; k < 2 * (W - 1); ++k) xs[k] = load(x, a.x_step, t1 - (W - 1) + k);
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) gs[k] = load(grad, a.grad_step, t1 + k);
+            i = sequence_at(a, t1 - 1);
+            if (i < a.n) rows_of(a, i, first, past);
+            if (i >= a.n || t1 - 1 < first || t1 - 1 >= past) i = -1;
+            else
+#pragma unroll
+                for (int k = W - 2; k >= 0; --k)
+                    if (t1 + k < past) one(xs + k, gs[k], t1 + k, false);
+        }
+        // x[k]: row t - (U - 1) - (W - 1) + k
+        Pack<T, V> xs[kX], gs[U], xn[U], gn[U];
+        int64_t t = t1 - 1;
+#pragma unroll
+        for (int k = 0; k < kX; ++k) xs[k] = load(x, a.x_step, t - (U - 1) - (W - 1) + k);
+#pragma unroll
+        for (int k = 0; k < U; ++k) gs[k] = load(grad, a.grad_step, t - (U - 1) + k);
+        for (; t >= t0; t -= U) {
+            if (t - U >= t0) {
+#pragma unroll
+                for (int k = 0; k < U; ++k) xn[k] = load(x, a.x_step, t - U - (U - 1) - (W - 1) + k);
+#pragma unroll
+                for (int k = 0; k < U; ++k) gn[k] = load(grad, a.grad_step, t - U - (U - 1) + k);
+            }
+            if (i >= 0 && t - (U - 1) >= t0 && t - (U - 1) - (W - 1) >= first && t < past - W) {
+                // nothing but rows of one sequence that are neither its first nor its last ones
+#pragma unroll
+                for (int r = 0; r < U; ++r) {
+                    float taps[W][V], d[V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v)
+#pragma unroll
+                        for (int k = 0; k < W; ++k) taps[k][v] = xs[U - 1 - r + k].get(v);
+                    value(taps, gs[U - 1 - r], true);
+                    derivative(d);
+                    lane.template store<T>(static_cast<T*>(a.out) + (t - r) * a.channels, d, a.past);
+                    shift();
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < U; ++r)
+                    if (t - r >= t0) one(xs + U - 1 - r, gs[U - 1 - r], t - r, true);
+            }
+#pragma unroll
+            for (int k = W - 2; k >= 0; --k) xs[U + k] = xs[k];
+#pragma unroll
+            for (int k = 0; k < U; ++k) xs[k] = xn[k], gs[k] = gn[k];
         }
     }
     // the block's piece of the weights' gradients, a tap after the other
@@ -405,8 +440,7 @@ void with_width(uint64_t width, F&& body)
     }
 }
 
-constexpr int kForwardRows = 16, kBackwardRows = 16;        // of a run
-constexpr int kBackwardBlocks = 1024;
+constexpr int kForwardRows = 16;        // of a thread
 
 // lanes to a row: a power of two, at most a wave
 int lanes_for(int packs)
@@ -416,14 +450,12 @@ int lanes_for(int packs)
     return lanes;
 }
 
-void place(ConvArgs& a, int v, int rows)
+// how a row's packs of v channels go to lanes and blocks
+void place(ConvArgs& a, int v)
 {
     const int packs = (a.channels + v - 1) / v;
     a.lanes = lanes_for(packs);
     a.channel_blocks = (packs + a.lanes - 1) / a.lanes;
-    a.runs = (a.rows + rows - 1) / rows;
-    const int64_t groups = kThreads / a.lanes;
-    a.pieces = int((a.runs + groups - 1) / groups);
 }
 
 int64_t idle_blocks(const ConvArgs& a, int width)
@@ -433,14 +465,28 @@ int64_t idle_blocks(const ConvArgs& a, int width)
     return blocks < 256 ? blocks : 256;
 }
 
-// pieces of the rows in the gradients' sums: enough blocks to fill the chip some times over
-int pieces_of(int64_t rows, int channels)
+// Backward: runs as long as make 4096 waves, of 16 rows at least.  A thread has v = 8 bytes of a row: 8 sequences of 2048, 1024 channels, float32, forward
+// and gradients 101 us, with 16 bytes, whose windows leave registers for fewer waves, 132.
+void place_back(ConvArgs& a, int v)
 {
-    ConvArgs a{};
-    a.rows = rows, a.channels = channels;
-    place(a, 4, kBackwardRows);
-    const int most = kBackwardBlocks / a.channel_blocks > 0 ? kBackwardBlocks / a.channel_blocks : 1;
-    return a.pieces < most ? a.pieces : most;
+    place(a, v);
+    const int64_t groups = kThreads / a.lanes, most = a.channel_blocks < 1024 ? 1024 / a.channel_blocks * groups : groups;
+    a.run = (a.rows + most - 1) / most;
+    a.run = ((a.run > 16 ? a.run : 16) + kAtOnce - 1) / kAtOnce * kAtOnce;
+    a.pieces = int((a.rows + a.run * groups - 1) / (a.run * groups));
+}
+
+// no fewer than those of any type
+int most_pieces(int64_t rows, int channels)
+{
+    int most = 0;
+    for (int v = 2; v <= 4; v += 2) {
+        ConvArgs a{};
+        a.rows = rows, a.channels = channels;
+        place_back(a, v);
+        most = a.pieces > most ? a.pieces : most;
+    }
+    return most;
 }
 
 void check(const ConvArgs& a, uint64_t width, uint64_t rows, uint64_t channels, uint64_t n, uint64_t length)
@@ -481,8 +527,9 @@ __attribute__((visibility("default"))) int cusig_amd_causal_conv(
             constexpr int V = 16 / sizeof(T);
             with_width(width, [&](auto w) {
                 constexpr int W = decltype(w)::value;
-                place(a, V, kForwardRows);
-                a.blocks = int64_t(a.pieces) * a.channel_blocks;
+                place(a, V);
+                const int64_t each = int64_t(kForwardRows) * (kThreads / a.lanes);
+                a.blocks = (a.rows + each - 1) / each * a.channel_blocks;
                 a.past = goes_past(uint64_t(a.rows) * a.channels * sizeof(T), uint64_t(a.channels) * sizeof(T));
                 a.idle = idle_blocks(a, W);
                 const int64_t blocks = a.blocks + a.idle;
@@ -501,7 +548,7 @@ __attribute__((visibility("default"))) uint64_t cusig_amd_causal_conv_backprop_w
         check(a, width, rows, channels, 0, 0);
     });
     if (width >= 1 && width <= kWidest && channels < (uint64_t(1) << 27) && rows < (uint64_t(1) << 31) && rows && channels)
-        bytes = uint64_t(pieces_of(int64_t(rows), int(channels))) * (width + 1) * channels * sizeof(float);
+        bytes = uint64_t(most_pieces(int64_t(rows), int(channels))) * (width + 1) * channels * sizeof(float);
     return bytes;
 }
 
@@ -523,19 +570,17 @@ __attribute__((visibility("default"))) int cusig_amd_causal_conv_backprop(
         if (a.n)
             with_type(dtype, [&](auto t) {
                 using T = decltype(t);
-                constexpr int V = 4;
+                constexpr int V = 8 / sizeof(T);
                 with_width(width, [&](auto w) {
-                    // windows of more than four taps leave registers for half the rows
-                    constexpr int W = decltype(w)::value, R = W > 4 ? kBackwardRows / 2 : kBackwardRows;
-                    place(a, V, R);
-                    pieces = a.rows ? pieces_of(a.rows, a.channels) : 0;
-                    a.pieces = pieces;
-                    a.blocks = int64_t(a.pieces) * a.channel_blocks;
+                    constexpr int W = decltype(w)::value;
+                    place_back(a, V);
+                    pieces = a.pieces;
+                    a.blocks = int64_t(pieces) * a.channel_blocks;
                     a.past = goes_past(uint64_t(a.rows) * a.channels * sizeof(T), uint64_t(a.channels) * sizeof(T));
                     a.idle = idle_blocks(a, W);
                     const int64_t blocks = a.blocks + a.idle;
-                    if (a.channels < V) launch_all(conv_back_kernel<T, V, W, R, true>, blocks, kThreads, static_cast<hipStream_t>(stream), a);
-                    else launch_all(conv_back_kernel<T, V, W, R, false>, blocks, kThreads, static_cast<hipStream_t>(stream), a);
+                    if (a.channels < V) launch_all(conv_back_kernel<T, V, W, true>, blocks, kThreads, static_cast<hipStream_t>(stream), a);
+                    else launch_all(conv_back_kernel<T, V, W, false>, blocks, kThreads, static_cast<hipStream_t>(stream), a);
                 });
             });
         hipLaunchKernelGGL(conv_weight_kernel, sum_blocks(int64_t(width + 1) * a.channels), dim3(kSumThreads), 0, static_cast<hipStream_t>(stream), a.parts, pieces,

@@ -565,6 +565,8 @@ def _shared(value, name, like, groups, states):
         raise ValueError(name + " must have shape " + str(shape) + ", got " + str(tuple(value.shape)))
     if value.stride(-1) != 1 and states > 1:
         value = value.contiguous()
+    if len(shape) == 3:
+        return value, value.stride(0) if shape[0] > 1 else groups * states, value.stride(1)
     # rows a fixed distance apart
     want = None
     for axis in range(value.dim() - 3, -1, -1):
