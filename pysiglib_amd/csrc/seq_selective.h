@@ -360,6 +360,7 @@ __device__ __forceinline__ Four decays(Four dt, Four a)
 // how the rows are cut
 struct Plan {
     int q, tiles;
+    int waves;              // to a block, backward: four add up their sums over channels; groups of one or two tiles would leave such blocks half empty
     int64_t segment, slots, per_sequence;
     bool several;
 };

@@ -304,16 +304,17 @@ __global__ void __launch_bounds__(64 * W, 2) back_kernel(Args p)
                         for (int k = 0; k < 4; ++k) h[u][k] = fmaf(before[u][k], e[k], h[u][k]);
                     }
                 }
-                if constexpr (kSaved > H)
-                    if (low + H < rows) {
-                        Four middle[4];
+                // its two halves, the second one first, in the same code
+#pragma unroll 1
+                for (int part = kSaved > H && low + H < rows ? 1 : 0; part >= 0; --part) {
+                    Four start[4];
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) middle[u] = h[u];
+                    for (int u = 0; u < 4; ++u) start[u] = h[u];
+                    if (part)
 #pragma unroll
-                        for (int k = 0; k < H; ++k) forward(low + k, middle);
-                        reverse(low + H, middle);
-                    }
-                reverse(low, h);
+                        for (int k = 0; k < H; ++k) forward(low + k, start);
+                    reverse(low + part * H, start);
+                }
             }
             // the channels' gradients of these rows
             {
@@ -442,8 +443,7 @@ Layout layout_of(bool packed, int64_t rows, int64_t n, int64_t length, int chann
     Layout l;
     l.plan = plan_of(packed, rows, n, length, channels, states, groups, true);
     const Plan& p = l.plan;
-    // four waves to a block add up their sums over channels; groups of one or two tiles leave such blocks half empty
-    l.waves = p.tiles > 2 ? kWaves : 1;
+    l.waves = p.waves;
     l.group_blocks = (p.tiles + l.waves - 1) / l.waves;
     // a piece of the slots to a block: enough of them for some waves to every SIMD
     const int64_t columns = int64_t(groups) * p.tiles, most = std::max<int64_t>(4096 / columns, 1);
