@@ -237,10 +237,11 @@ void check_sizes(uint64_t rows, uint64_t n, uint64_t channels, uint64_t states, 
 }
 
 // Segments: as long as makes 4096 waves over all rows forward, 2048 backward, where two waves fill a SIMD, and with up to eight states, whose
-// segments would be short; not shorter than four tiles.  (16 sequences of 1024, 2048 channels of 16, bfloat16: 258 us, with 2048 waves 270;
+// segments would be short; at least a tile: few rows end sooner in many short segments (3000 steps of 100 channels of 16, bfloat16, forward 27 us, with
+// four tiles to a segment 57; with gradients 95 and 200).  (16 sequences of 1024, 2048 channels of 16, bfloat16: 258 us, with 2048 waves 270;
 // 3 of 3000, 1000 channels of 64, float16: 265 and 287; but one of 50000, 256 channels of 8, bfloat16: 115 and 102, of 4: 119 and 94.)
 // Backward no more than that: the waves are all there at once, and one more would run behind them.  A packed sequence ends half a segment
-// early on average, and a block's idle waves count.  (24 sequences of up to 900, 770 channels in two groups, float16, forward and gradients: MEASURED us, with
+// early on average, and a block's idle waves count.  (24 sequences of up to 900, 770 channels in two groups, float16, forward and gradients: 416 us, with
 // 2352 waves 473.)
 Plan plan_of(bool packed, int64_t rows, int64_t n, int64_t length, int channels, int states, int groups, bool back)
 {
@@ -258,7 +259,7 @@ Plan plan_of(bool packed, int64_t rows, int64_t n, int64_t length, int channels,
         const int64_t each = std::max<int64_t>(most / std::max<int64_t>(n * columns, 1), 1);
         segment = (length + each - 1) / each;
     }
-    segment = (std::max<int64_t>(segment, 4 * tile) + tile - 1) / tile * tile;
+    segment = (std::max<int64_t>(segment, 1) + tile - 1) / tile * tile;
     const int64_t longest = packed ? rows : length;
     p.several = longest > segment;
     p.segment = p.several ? segment : std::max<int64_t>((longest + tile - 1) / tile * tile, tile);
