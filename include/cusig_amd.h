@@ -420,7 +420,8 @@ CUSIG_AMD_API uint64_t cusig_amd_attention_backprop_workspace(uint64_t q_rows, u
 
 /* s = x + residual as it is stored in the residual's type (residual_dtype: dtype or float32), out = s (mean s^2 + eps)^-1/2 weight for each
  * row; residual null: s is x, total is not written.  out and total contiguous, weight float32 [channels]; 1 to 16384 channels.
- * scales not null: out is float8 e4m3 with the scale max |out| / 448 of each row (1 where the row is zero or holds NaN). */
+ * scales not null: out is float8 e4m3 with the scale max |out| / 448 of each row (1 where that is zero, or the row holds NaN).
+ * None of the outputs of these operators may overlap an input, but for the states that a step replaces. */
 CUSIG_AMD_API int cusig_amd_norm_residual(int dtype, int residual_dtype, const void* x, const void* residual, const float* weight, void* out,
                                           void* total, float* scales, uint64_t rows, uint64_t channels, int64_t x_stride,
                                           int64_t residual_stride, float eps, void* stream) CUSIG_AMD_NOEXCEPT;
@@ -457,7 +458,7 @@ CUSIG_AMD_API int cusig_amd_causal_conv_step(int dtype, const void* x, void* sta
  * delta_bias) or delta + delta_bias and f(z) = z / (1 + exp(-z)); d, z and delta_bias may be null.  x, delta, z, y [rows, channels]
  * (y contiguous), offsets or null as above; a float32 [channels, states], d and delta_bias float32 [channels]; b, c [rows, groups,
  * states], the last axis contiguous: neighbouring channels share a group's; 1 to 64 states.  initial_state (may be null: zero) and
- * final_state float32 [sequences, channels, states]. */
+ * final_state float32 [sequences, channels, states].  Rows of x, delta, z (and of y's gradient) are 0 to 2^24 elements apart. */
 CUSIG_AMD_API int cusig_amd_selective_scan(int dtype, const void* x, const void* delta, const float* a, const void* b, const void* c,
                                            const float* d, const void* z, const float* delta_bias, const float* initial_state, void* y,
                                            float* final_state, const int* offsets, uint64_t sequences, uint64_t length, uint64_t rows,

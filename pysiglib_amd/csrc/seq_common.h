@@ -119,6 +119,12 @@ inline void require(bool ok, const char* what)
     if (!ok) throw std::invalid_argument(what);
 }
 
+// n sequences of `length` rows: the product may be beyond 64 bits
+inline void check_rows(uint64_t n, uint64_t length, uint64_t rows)
+{
+    require(n == 0 ? rows == 0 : rows % n == 0 && rows / n == length, "rows are not sequences times length");
+}
+
 inline void check_workspace(const void* workspace, uint64_t bytes, uint64_t need)
 {
     require(bytes >= need && (workspace || need == 0), "the workspace is too small");
@@ -142,11 +148,11 @@ void in_launches(int64_t blocks, int threads, Launch&& launch)
 constexpr int kSumThreads = 1024;
 
 template <typename F>
-__device__ __forceinline__ void sum_pieces(const float* parts, int pieces, int64_t columns, F&& put)
+__device__ __forceinline__ void sum_pieces(const float* parts, int pieces, int64_t columns, unsigned first_block, F&& put)
 {
     __shared__ float s_sum[32][33];
     const int lane = threadIdx.x % 32, row = threadIdx.x / 32;
-    const int64_t e = int64_t(blockIdx.x) * 32 + lane;
+    const int64_t at = (int64_t(first_block) + blockIdx.x) * 32, e = at + lane;
     float sum = 0.0f;
     if (e < columns)
 #pragma unroll 8
@@ -157,11 +163,10 @@ __device__ __forceinline__ void sum_pieces(const float* parts, int pieces, int64
     sum = s_sum[lane][row];
 #pragma unroll
     for (int m = 16; m; m /= 2) sum += __shfl_xor(sum, m);
-    const int64_t to = int64_t(blockIdx.x) * 32 + row;
-    if (lane == 0 && to < columns) put(to, sum);
+    if (lane == 0 && at + row < columns) put(at + row, sum);
 }
 
-inline dim3 sum_blocks(int64_t columns) { return dim3(static_cast<unsigned>((columns + 31) / 32)); }
+inline int64_t sum_blocks(int64_t columns) { return (columns + 31) / 32; }
 
 template <typename Args>
 void launch_all(void (*kernel)(Args), int64_t blocks, int threads, hipStream_t stream, Args p)

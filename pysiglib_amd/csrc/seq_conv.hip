@@ -385,9 +385,9 @@ __global__ void __launch_bounds__(kThreads) conv_back_kernel(ConvArgs a)
     }
 }
 
-__global__ void __launch_bounds__(kSumThreads) conv_weight_kernel(const float* parts, int pieces, int channels, int width, float* dw, float* db)
+__global__ void __launch_bounds__(kSumThreads) conv_weight_kernel(const float* parts, int pieces, int channels, int width, float* dw, float* db, unsigned first_block)
 {
-    sum_pieces(parts, pieces, int64_t(width + 1) * channels, [&](int64_t e, float sum) {
+    sum_pieces(parts, pieces, int64_t(width + 1) * channels, first_block, [&](int64_t e, float sum) {
         const int k = int(e / channels), ch = int(e % channels);
         if (k < width) dw[int64_t(ch) * width + k] = sum;
         else if (db) db[ch] = sum;
@@ -489,11 +489,16 @@ int most_pieces(int64_t rows, int channels)
     return most;
 }
 
-void check(const ConvArgs& a, uint64_t width, uint64_t rows, uint64_t channels, uint64_t n, uint64_t length)
+void check_sizes(uint64_t width, uint64_t rows, uint64_t channels, uint64_t n)
 {
     require(width >= 1 && width <= kWidest, "a convolution has 1 to 8 taps");
     require(channels < (uint64_t(1) << 27) && rows < (uint64_t(1) << 31) && n < (uint64_t(1) << 31), "too many rows, channels or sequences");
-    require(a.offsets || n * length == rows, "rows are not sequences times length");
+}
+
+void check(const ConvArgs& a, uint64_t width, uint64_t rows, uint64_t channels, uint64_t n, uint64_t length)
+{
+    check_sizes(width, rows, channels, n);
+    if (!a.offsets) check_rows(n, length, rows);
 }
 
 ConvArgs args_of(const void* x, const float* w, const float* bias, const int* offsets, uint64_t n, uint64_t length, uint64_t rows, uint64_t channels, int64_t x_step, bool silu)
@@ -544,11 +549,9 @@ __attribute__((visibility("default"))) uint64_t cusig_amd_causal_conv_backprop_w
 {
     uint64_t bytes = 0;
     sigamd::guarded([&] {
-        ConvArgs a{};
-        check(a, width, rows, channels, 0, 0);
+        check_sizes(width, rows, channels, 0);
+        if (rows && channels) bytes = uint64_t(most_pieces(int64_t(rows), int(channels))) * (width + 1) * channels * sizeof(float);
     });
-    if (width >= 1 && width <= kWidest && channels < (uint64_t(1) << 27) && rows < (uint64_t(1) << 31) && rows && channels)
-        bytes = uint64_t(most_pieces(int64_t(rows), int(channels))) * (width + 1) * channels * sizeof(float);
     return bytes;
 }
 
@@ -583,9 +586,10 @@ __attribute__((visibility("default"))) int cusig_amd_causal_conv_backprop(
                     else launch_all(conv_back_kernel<T, V, W, false>, blocks, kThreads, static_cast<hipStream_t>(stream), a);
                 });
             });
-        hipLaunchKernelGGL(conv_weight_kernel, sum_blocks(int64_t(width + 1) * a.channels), dim3(kSumThreads), 0, static_cast<hipStream_t>(stream), a.parts, pieces,
-                           a.channels, int(width), grad_weight, grad_bias);
-        SIG_HIP(hipGetLastError());
+        in_launches(sum_blocks(int64_t(width + 1) * a.channels), kSumThreads, [&](unsigned first, dim3 grid) {
+            hipLaunchKernelGGL(conv_weight_kernel, grid, dim3(kSumThreads), 0, static_cast<hipStream_t>(stream), a.parts, pieces, a.channels, int(width), grad_weight,
+                               grad_bias, first);
+        });
     });
 }
 

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(W > 4 ? 64 * W : kThreads) norm_kernel(NormArg
     if constexpr (EIGHT) {
         // NaN has larger bits than every number: one in the row makes the scale 1
         top = over_row<W>(top, s_top, [](unsigned a, unsigned b) { return max(a, b); });
-        const float most = __uint_as_float(top), scale = most > 0.0f ? most / 448.0f : 1.0f;
+        const float ratio = __uint_as_float(top) / 448.0f, scale = ratio > 0.0f ? ratio : 1.0f;       // of 3e-43 and less it is zero
         if (lane == 0) p.scales[row] = scale;
         // out / scale by the reciprocal and one correction from the remainder: the quotient's rounding, and not three, decides between two
         // neighbours of eight bits.  The reciprocal of a scale below 2^-64 may be beyond the numbers: both move.
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(W > 4 ? 64 * W : kThreads) norm_back_kernel(No
 
 __global__ void __launch_bounds__(kSumThreads) norm_weight_kernel(const float* parts, int pieces, int channels, float* dw)
 {
-    sum_pieces(parts, pieces, channels, [&](int64_t e, float sum) { dw[e] = sum; });
+    sum_pieces(parts, pieces, channels, 0, [&](int64_t e, float sum) { dw[e] = sum; });
 }
 
 // Waves to a row and packs to a lane: a wave holds up to two packs a lane, four waves up to eight, and eight waves what float32
@@ -348,7 +348,7 @@ void backward(int dtype, int residual, NormArgs& p, float* dw, hipStream_t strea
             });
         });
     }
-    hipLaunchKernelGGL(norm_weight_kernel, sum_blocks(p.channels), dim3(kSumThreads), 0, stream, p.parts, pieces, p.channels, dw);
+    hipLaunchKernelGGL(norm_weight_kernel, dim3(unsigned(sum_blocks(p.channels))), dim3(kSumThreads), 0, stream, p.parts, pieces, p.channels, dw);
     SIG_HIP(hipGetLastError());
 }
 

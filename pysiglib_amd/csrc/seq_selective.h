@@ -13,6 +13,7 @@
 #pragma once
 #include "seq_common.h"
 
+#include <initializer_list>
 #include <type_traits>
 
 namespace seqamd {
@@ -66,7 +67,7 @@ struct Args {
     int64_t x_step, delta_step, z_step, grad_step, b_step, b_group, c_step, c_group;
     int channels, states, groups, per_group, tiles;     // tiles: of a group's channels
     int group_blocks, pieces;                           // backward: blocks to a group, pieces of the slots
-    bool softplus, several;                             // several: a sequence may have more than one segment
+    bool softplus;
     unsigned first_block;
 };
 
@@ -362,7 +363,7 @@ struct Plan {
     int q, tiles;
     int waves;              // to a block, backward: four add up their sums over channels; groups of one or two tiles would leave such blocks half empty
     int64_t segment, slots, per_sequence;
-    bool several;
+    bool several;           // a sequence may have more than one segment
 };
 
 inline int lanes_of(int states)
@@ -376,9 +377,11 @@ inline int tile_rows(int q) { return q == 1 ? 4 : (q == 2 ? 8 : 16); }
 
 Plan plan_of(bool packed, int64_t rows, int64_t n, int64_t length, int channels, int states, int groups, bool back);
 void check_sizes(uint64_t rows, uint64_t n, uint64_t channels, uint64_t states, uint64_t groups);
+void check_strides(std::initializer_list<int64_t> strides);
 void join_segments(const Args& p, bool back, hipStream_t stream);
 
 constexpr int kMostStates = 64;
+constexpr int64_t kMostStride = 1 << 24;      // of x, delta, z and y's gradient: distances in a tile are 32-bit
 
 // calls body with the lanes to a channel as a type
 template <typename F>

@@ -232,8 +232,13 @@ __global__ void __launch_bounds__(kThreads) step_kernel(Args p)
 void check_sizes(uint64_t rows, uint64_t n, uint64_t channels, uint64_t states, uint64_t groups)
 {
     require(states >= 1 && states <= kMostStates, "a channel has 1 to 64 states");
-    require(rows < (uint64_t(1) << 31) && n < (uint64_t(1) << 31) && channels < (uint64_t(1) << 24), "too many rows, channels or sequences");
+    require(rows < (uint64_t(1) << 31) && n < (uint64_t(1) << 31) && channels < (uint64_t(1) << 24) && groups < (uint64_t(1) << 24), "too many rows, channels or sequences");
     require(groups >= 1 && channels % groups == 0, "the channels are a multiple of the groups");
+}
+
+void check_strides(std::initializer_list<int64_t> strides)
+{
+    for (const int64_t stride : strides) require(stride >= 0 && stride <= kMostStride, "rows are too far apart");
 }
 
 // Segments: as long as makes 4096 waves over all rows forward, 2048 backward, where two waves fill a SIMD, and with up to eight states, whose
@@ -325,7 +330,8 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan(
 {
     return sigamd::guarded([&] {
         check_sizes(rows, sequences, channels, states, groups);
-        require(offsets || sequences * length == rows, "rows are not sequences times length");
+        if (!offsets) check_rows(sequences, length, rows);
+        check_strides({x_stride, delta_stride, z_stride});
         if (sequences * channels == 0) return;
         require(a && final_state && (rows == 0 || (x && delta && b && c && y)), "a tensor is missing");
         const Plan plan = plan_of(offsets, int64_t(rows), int64_t(sequences), int64_t(length), int(channels), int(states), int(groups), false);
@@ -336,7 +342,7 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan(
         p.channels = int(channels), p.states = int(states), p.groups = int(groups), p.per_group = int(channels / groups), p.tiles = plan.tiles;
         p.x_step = x_stride, p.delta_step = delta_stride, p.z_step = z_stride, p.b_step = b_stride, p.b_group = b_group, p.c_step = c_stride, p.c_group = c_group;
         p.softplus = softplus;
-        p.segment = plan.segment, p.slots = plan.slots, p.per_sequence = plan.per_sequence, p.several = plan.several;
+        p.segment = plan.segment, p.slots = plan.slots, p.per_sequence = plan.per_sequence;
         p.carry = static_cast<Four*>(workspace);
         p.span = reinterpret_cast<float*>(static_cast<char*>(workspace) + (plan.several ? carry_bytes(plan, groups) : 0));
         const int64_t waves = p.slots * p.groups * p.tiles, blocks = (waves + kWaves - 1) / kWaves;
@@ -345,7 +351,7 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan(
             using T = decltype(t);
             with_lanes(plan.q, [&](auto q) {
                 constexpr int Q = decltype(q)::value;
-                if (p.several) {
+                if (plan.several) {
                     launch_all(scan_kernel<T, Q, false>, blocks, kThreads, s, p);
                     join_segments(p, false, s);
                 }

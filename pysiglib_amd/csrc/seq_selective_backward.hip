@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kThreads) shared_kernel(Args p, T* db, T* dc)
 __global__ void __launch_bounds__(kSumThreads) own_kernel(Args p, float* da, float* dd, float* dbias)
 {
     const int each = p.states + 2;
-    sum_pieces(p.own_parts, p.pieces, int64_t(p.channels) * each, [&](int64_t e, float sum) {
+    sum_pieces(p.own_parts, p.pieces, int64_t(p.channels) * each, p.first_block, [&](int64_t e, float sum) {
         const int64_t ch = e / each;
         const int i = int(e - ch * each);
         if (i < p.states) da[ch * p.states + i] = sum;
@@ -492,7 +492,8 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan_backprop(
 {
     return sigamd::guarded([&] {
         check_sizes(rows, sequences, channels, states, groups);
-        require(offsets || sequences * length == rows, "rows are not sequences times length");
+        if (!offsets) check_rows(sequences, length, rows);
+        check_strides({x_stride, delta_stride, z_stride, grad_stride});
         const auto s = static_cast<hipStream_t>(stream);
         Args p{};
         p.x = x, p.delta = delta, p.a = a, p.b = b, p.c = c, p.d = d, p.z = z, p.bias = delta_bias, p.grad = grad_y;
@@ -502,8 +503,17 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan_backprop(
         p.x_step = x_stride, p.delta_step = delta_stride, p.z_step = z_stride, p.grad_step = grad_stride;
         p.b_step = b_stride, p.b_group = b_group, p.c_step = c_stride, p.c_group = c_group;
         p.softplus = softplus;
-        if (channels == 0) {
+        auto shared = [&](auto t, auto q) {
+            using T = decltype(t);
+            in_launches((p.rows * p.groups * 2 * p.states + kThreads - 1) / kThreads, kThreads, [&](unsigned first, dim3 grid) {
+                Args more = p;
+                more.first_block = first;
+                hipLaunchKernelGGL((shared_kernel<T, decltype(q)::value>), grid, dim3(kThreads), 0, s, more, static_cast<T*>(grad_b), static_cast<T*>(grad_c));
+            });
+        };
+        if (channels == 0) {            // sums over nothing
             require(rows == 0 || (grad_b && grad_c), "a tensor is missing");
+            with_type(dtype, [&](auto t) { shared(t, std::integral_constant<int, 1>{}); });
             return;
         }
         require(a && grad_a && (sequences == 0 || grad_initial) && (!d || grad_d) && (!delta_bias || grad_delta_bias), "a tensor is missing");
@@ -515,7 +525,7 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan_backprop(
         auto state_at = [&](uint64_t where) { return reinterpret_cast<Four*>(w + where); };
         p.carry = state_at(l.carry), p.back = state_at(l.back), p.span = at(l.span), p.tile_state = state_at(l.tile_state), p.tile_span = at(l.tile_span);
         p.shared_parts = at(l.shared_parts), p.own_parts = at(l.own_parts);
-        p.segment = l.plan.segment, p.slots = l.plan.slots, p.per_sequence = l.plan.per_sequence, p.several = l.plan.several, p.tiles = l.plan.tiles;
+        p.segment = l.plan.segment, p.slots = l.plan.slots, p.per_sequence = l.plan.per_sequence, p.tiles = l.plan.tiles;
         p.group_blocks = l.group_blocks, p.pieces = l.pieces;
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
@@ -523,7 +533,7 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan_backprop(
                 constexpr int Q = decltype(q)::value;
                 if (p.slots) {
                     const int64_t blocks = (p.slots * p.groups * p.tiles + kWaves - 1) / kWaves;
-                    if (p.several) {
+                    if (l.plan.several) {
                         launch_all(states_kernel<T, Q, true>, blocks, kThreads, s, p);
                         join_segments(p, true, s);
                     } else {
@@ -535,15 +545,14 @@ __attribute__((visibility("default"))) int cusig_amd_selective_scan_backprop(
                     else if (some) launch_all(back_kernel<T, Q, kWaves, true>, work, kThreads, s, p);
                     else launch_all(back_kernel<T, Q, kWaves, false>, work, kThreads, s, p);
                 }
-                in_launches((p.rows * p.groups * 2 * p.states + kThreads - 1) / kThreads, kThreads, [&](unsigned first, dim3 grid) {
-                    Args more = p;
-                    more.first_block = first;
-                    hipLaunchKernelGGL((shared_kernel<T, Q>), grid, dim3(kThreads), 0, s, more, static_cast<T*>(grad_b), static_cast<T*>(grad_c));
-                });
+                shared(t, q);
             });
         });
-        hipLaunchKernelGGL(own_kernel, sum_blocks(int64_t(p.channels) * (p.states + 2)), dim3(kSumThreads), 0, s, p, grad_a, grad_d, grad_delta_bias);
-        SIG_HIP(hipGetLastError());
+        in_launches(sum_blocks(int64_t(p.channels) * (p.states + 2)), kSumThreads, [&](unsigned first, dim3 grid) {
+            Args more = p;
+            more.first_block = first;
+            hipLaunchKernelGGL(own_kernel, grid, dim3(kSumThreads), 0, s, more, grad_a, grad_d, grad_delta_bias);
+        });
     });
 }
 

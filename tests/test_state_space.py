@@ -919,6 +919,108 @@ def test_a_block_run_together(P):
                     assert float((y[i].double().cpu() - want[starts[i] + t].detach()).abs().max()) <= 1024 * U32 * float(want.detach().abs().max())
 
 
+@pytest.mark.gpu
+def test_gradients_of_shared_inputs_where_there_are_no_channels(P):
+    at = whole_numbers([1, 4])
+    for dtype in TYPES:
+        x, b = torch.zeros((5, 0), dtype=dtype, device=DEV), torch.ones((5, 2, 3), dtype=dtype, device=DEV)
+        a = torch.zeros((0, 3), device=DEV)
+        for offsets, first, past in ((None, 0, 5), (at, 1, 4)):
+            back = P.selective_scan_backprop(x, x, x, a, b, b, offsets=offsets)
+            assert (back[3][first:past] == 0).all() and (back[4][first:past] == 0).all()
+    b = torch.full((5, 2, 3), 7.0, device=DEV)
+    from pysiglib_amd import _loader as L
+    raw(L.CUSIG_SELECTIVE_SCAN_BACKPROP, 0, x, x, x, a, b, b, 0, 0, 0, 0, 0, x, x, a, b, b, 0, 0, 0, x, at, 1, 0, 5, 0, 3, 2, 0, 0, 0, 0, 6, 3, 6, 3, True, 0, 0)
+    assert (b[1:4] == 0).all() and (b[0] == 7).all() and (b[4] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("channels", [40, 2000])
+def test_norm_residual_in_8_bits_of_outputs_whose_scale_is_zero(P, channels):
+    """max |out| / 448 of less than half of 2^-149 is zero in 32 bits: the scale is 1, and the outputs, far below 2^-10, are zero."""
+    x = torch.ones((2, channels), device=DEV)
+    q, scales, _ = P.norm_residual_float8(x, None, torch.full((channels,), 2.0 ** -142, device=DEV), eps=0.0)
+    assert (scales == 1).all() and (q.float() == 0).all()
+
+
+@pytest.mark.gpu
+def test_weights_of_very_many_channels(P):
+    """Sums over the rows for more columns than one launch has threads for."""
+    channels = 1 << 25
+    x = torch.ones((2, channels), dtype=torch.bfloat16, device=DEV)
+    dw = P.causal_conv_backprop(x, x, torch.zeros((channels, 4), device=DEV), torch.zeros(channels, device=DEV), silu=False)[1:3]
+    # two rows: the last tap saw both, the one before it the first
+    assert (dw[0] == torch.tensor([0.0, 0.0, 1.0, 2.0], device=DEV)).all() and (dw[1] == 2).all()
+    del dw, x
+    channels, states = 1 << 22, 32
+    x = torch.ones((1, channels), dtype=torch.bfloat16, device=DEV)
+    one = torch.ones((1, 1, states), dtype=torch.bfloat16, device=DEV)
+    h = torch.ones((channels, states), device=DEV)
+    # one row, a = 0, dt = 1: da = h c dt, the gradient of d is x's product with g
+    back = P.selective_scan_backprop(x, x, x, torch.zeros_like(h), one, one, d=torch.zeros(channels, device=DEV), softplus=False, initial_state=h)
+    assert (back[2] == 1).all() and (back[5] == 1).all()
+
+
+@pytest.mark.gpu
+def test_tensors_of_more_than_32_bits_of_elements(P):
+    """A long sequence of zeros, and behind it a short one that starts beyond 2^31 elements: as alone."""
+    channels, rows, last = 8192, 270000, 50
+    assert (rows - last) * channels > 1 << 31
+    kind = torch.bfloat16
+    rng = np.random.default_rng(0)
+    small = {k: numbers(rng, last, channels, dtype=kind) for k in ("x", "delta", "z", "g")}
+    big = {}
+    for k, v in small.items():
+        big[k] = torch.zeros((rows, channels), dtype=kind, device=DEV)
+        big[k][-last:] = v
+    at, alone = whole_numbers([0, rows - last, rows]), whole_numbers([0, last])
+    w, bias = numbers(rng, channels, 4), numbers(rng, channels)
+    y, final = P.causal_conv(big["x"], w, bias, offsets=at)
+    want, end = P.causal_conv(small["x"], w, bias, offsets=alone)
+    assert torch.equal(y[-last:], want) and torch.equal(final[1:], end)
+    dx = P.causal_conv_backprop(big["g"], big["x"], w, bias, offsets=at)[0]
+    assert torch.equal(dx[-last:], P.causal_conv_backprop(small["g"], small["x"], w, bias, offsets=alone)[0])
+    del y, dx
+    out, total = P.norm_residual(big["x"], big["z"], bias)
+    want, sums = P.norm_residual(small["x"], small["z"], bias)
+    assert torch.equal(total[-last:], sums)
+    assert (out[-last:].float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()         # another split of a row: a step of the output
+    del out
+    dx = P.norm_residual_backprop(big["g"], total, bias)[0]
+    want = P.norm_residual_backprop(small["g"], sums, bias)[0]
+    assert (dx[-last:].float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+    del dx, total
+    states = 4
+    a, d = -numbers(rng, channels, states).abs(), numbers(rng, channels)
+    b = torch.zeros((rows, 1, states), dtype=kind, device=DEV)
+    b[-last:] = numbers(rng, last, 1, states, dtype=kind)
+    some = b[-last:].clone()
+    y, final = P.selective_scan(big["x"], big["delta"], a, b, b, d=d, z=big["z"], offsets=at)
+    want, end = P.selective_scan(small["x"], small["delta"], a, some, some, d=d, z=small["z"], offsets=alone)
+    # the segments may be others: a state is then a sum in another order, far below a step of bfloat16
+    assert (y[-last:].float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+    assert (final[1] - end[0]).abs().max() <= 2.0 ** -16 * end.abs().max() and (final[0] == 0).all()
+    del y
+    back = P.selective_scan_backprop(big["g"], big["x"], big["delta"], a, b, b, d=d, z=big["z"], offsets=at)
+    want = P.selective_scan_backprop(small["g"], small["x"], small["delta"], a, some, some, d=d, z=small["z"], offsets=alone)
+    for i in (0, 1, 3, 4, 6):
+        assert (back[i][-last:].float() - want[i].float()).abs().max() <= 2.0 ** -7 * want[i].float().abs().max(), i
+    for i in (2, 5):            # the zeros add nothing
+        assert (back[i] - want[i]).abs().max() <= 2.0 ** -14 * want[i].abs().max(), i
+
+
+@pytest.mark.gpu
+def test_gradients_of_two_inputs_are_two_tensors(P):
+    x, r = (torch.randn((3, 40), device=DEV, requires_grad=True) for _ in range(2))
+    w = torch.ones(40, device=DEV)
+    for _ in range(2):
+        P.torch_api.norm_residual(x, r, w)[0].square().sum().backward()
+    want = r.grad.clone()
+    assert torch.equal(x.grad, want)
+    x.grad.add_(1.0)
+    assert torch.equal(r.grad, want)
+
+
 # ---- refusals ----
 
 @pytest.mark.gpu
@@ -1034,3 +1136,27 @@ def test_the_entry_points_report_what_is_wrong(P):
     size = L.CUSIG_NORM_RESIDUAL_BACKPROP_WORKSPACE(8)
     for space, bytes_, dw, other, dr in ((0, size, at, 1, 0), (256, size - 1, at, 1, 0), (8, size, at, 1, 0), (256, size, 0, 1, 0), (256, size, at, 0, 0)):
         assert L.CUSIG_NORM_RESIDUAL_BACKPROP(1, other, at, 0, at, at, at, dr, dw, 2, 8, 8, 8, 8, 1e-6, space, bytes_, 0) == 2
+
+
+def test_the_entry_points_refuse_sizes_beyond_their_numbers(P):
+    from pysiglib_amd import _loader as L
+    at = 256
+    assert L.CUSIG_SELECTIVE_SCAN_WORKSPACE(False, 1, 5, 5, 0, 2, 1 << 32) == 0
+    assert L.CUSIG_SELECTIVE_SCAN_BACKPROP_WORKSPACE(False, 1, 5, 5, 0, 2, 1 << 32) == 0
+    # 2^30 sequences of 2^34 rows: the product is zero in 64 bits
+    n, length = 1 << 30, 1 << 34
+    assert L.CUSIG_SELECTIVE_SCAN(1, at, at, at, at, at, 0, 0, 0, 0, at, at, 0, n, length, 0, 4, 2, 1, *(4,) * 7, True, at, 1 << 62, 0) == 2
+    assert L.CUSIG_SELECTIVE_SCAN_BACKPROP(1, at, at, at, at, at, at, 0, 0, 0, 0, 0, at, at, at, at, at, 0, 0, 0, at, 0, n, length, 0, 4, 2, 1, 4, *(4,) * 7, True, at,
+                                           1 << 62, 0) == 2
+    assert L.CUSIG_CAUSAL_CONV(1, at, at, 0, 0, at, at, 0, n, length, 0, 4, 4, 4, True, 0) == 2
+    # distances of rows that 32 bits do not hold 16 times
+    for i in range(3):
+        for stride in (-4, (1 << 24) + 1):
+            strides = [4] * 7
+            strides[i] = stride
+            assert L.CUSIG_SELECTIVE_SCAN(1, at, at, at, at, at, 0, at, 0, 0, at, at, 0, 2, 3, 6, 4, 2, 1, *strides, True, at, 1 << 40, 0) == 2
+            assert L.CUSIG_SELECTIVE_SCAN_BACKPROP(1, at, at, at, at, at, at, 0, at, 0, 0, 0, at, at, at, at, at, 0, at, 0, at, 0, 2, 3, 6, 4, 2, 1, 4, *strides, True, at,
+                                                   1 << 40, 0) == 2
+    for stride in (-4, (1 << 24) + 1):
+        assert L.CUSIG_SELECTIVE_SCAN_BACKPROP(1, at, at, at, at, at, at, 0, 0, 0, 0, 0, at, at, at, at, at, 0, 0, 0, at, 0, 2, 3, 6, 4, 2, 1, stride, *(4,) * 7, True, at,
+                                               1 << 40, 0) == 2
