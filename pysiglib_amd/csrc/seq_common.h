@@ -107,7 +107,7 @@ __device__ __forceinline__ void store_some(T* p, const Pack<T, V>& r, int count)
 // inputs, the gradients' results kept and past the caches: of 96 MB 108 us both, of 120 MB 141 and 137, of 128 MB (2048 steps) 157 and 148,
 // of 256 MB 333 and 311; with 2048 steps and the forward's 64 MB past the caches too 160.  Lines that are written in pieces are kept:
 // gradients of 23000 steps of 997 channels in float16 took 126 us instead of 89.
-inline bool goes_past(uint64_t bytes, uint64_t row) { return bytes >= (uint64_t(128) << 20) && row % 128 == 0; }
+inline bool goes_past(uint64_t bytes, uint64_t row, uint64_t from = uint64_t(128) << 20) { return bytes >= from && row % 128 == 0; }
 
 // A weight times what it weighs: zero where it has no weight, also of what is not finite (v_mul_legacy_f32)
 extern "C" __device__ __attribute__((const)) float weighed(float weight, float x) __asm("llvm.amdgcn.fmul.legacy");

@@ -18,7 +18,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWidest = 8;
-constexpr int kAtOnce = 4;          // rows that a thread takes at once, backward
+// Rows that a thread takes at once, backward.  8 sequences of 2048, 2048 channels, bfloat16, both directions: 111 us, with 2 rows 128, with 8 109, but in float32, 1024
+// channels, 100 and 128.
+constexpr int kAtOnce = 4;
 
 struct ConvArgs {
     const void* x;              // [rows][channels], rows x_step apart
@@ -440,7 +442,9 @@ void with_width(uint64_t width, F&& body)
     }
 }
 
-constexpr int kForwardRows = 16;        // of a thread
+// Rows of a thread, of 16 bytes each.  8 sequences of 2048, 2048 channels, bfloat16: 38 us, with 8 rows 41, with 24 40; 37 of up to 1500, 997 channels, float16:
+// 30, 28 and 29; the first of 1024 channels, float32: 30, 28 and 28.
+constexpr int kForwardRows = 16;
 
 // lanes to a row: a power of two, at most a wave
 int lanes_for(int packs)
@@ -466,7 +470,8 @@ int64_t idle_blocks(const ConvArgs& a, int width)
 }
 
 // Backward: runs as long as make 4096 waves, of 16 rows at least.  A thread has v = 8 bytes of a row: 8 sequences of 2048, 1024 channels, float32, forward
-// and gradients 101 us, with 16 bytes, whose windows leave registers for fewer waves, 132.
+// and gradients 101 us, with 16 bytes, whose windows leave registers for fewer waves, 132.  Results past the caches from 128 MB on: 8 of 2048, 4096 channels,
+// bfloat16, both directions 190 us, kept 205; 2048 channels, float32, 178 and 175; forward alone, 8 of 4096, 4096 channels, bfloat16, 114 and 122.
 void place_back(ConvArgs& a, int v)
 {
     place(a, v);

@@ -17,7 +17,12 @@ namespace seqamd {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPieces = 1024;       // of the rows at most, for the gradient of the weight
+// Of the rows at most, for the gradient of the weight: 16384 rows of 2048 channels, bfloat16, both directions 109 us, with 512 pieces 112, with 2048 115
+constexpr int kPieces = 1024;
+
+// Results of this size leave the last cache before they are read.  16384 rows of 2048 channels, bfloat16 (134 MB), both directions, past the caches 111 us, kept 103;
+// 8192 rows of 8192 into 8 bits (201 MB) 90 and 92; 16384 of 4096 (268 MB) 94 and 96; 8192 of 8192, float32, both directions 371 and 395.
+constexpr uint64_t kPast = uint64_t(192) << 20;
 
 struct NormArgs {
     const void *x, *residual;       // residual null: the sum is x, and not written
@@ -258,7 +263,8 @@ __global__ void __launch_bounds__(kSumThreads) norm_weight_kernel(const float* p
 }
 
 // Waves to a row and packs to a lane: a wave holds up to two packs a lane, four waves up to eight, and eight waves what float32
-// rows have beyond that.  Few rows are spread over more waves, so that a call of few tokens has all its loads on their way at once.
+// rows have beyond that.  (32768 rows of 1024 channels, bfloat16, two packs to a lane of one wave 49 us, one pack to a lane of four 57;
+// gradients as well 107 and 115; 64 to 4096 rows alike.)
 struct NormPlan {
     int waves, packs;
 };
@@ -266,11 +272,11 @@ struct NormPlan {
 constexpr int kMost = 16384;        // channels
 
 template <typename T>
-NormPlan plan_of(int64_t rows, int channels)
+NormPlan plan_of(int channels)
 {
     const int packs = (channels + 16 / int(sizeof(T)) - 1) / (16 / int(sizeof(T)));
     NormPlan p;
-    p.waves = packs <= 128 && (rows > 1024 || packs <= 64) ? 1 : (packs <= 2048 ? 4 : 8);
+    p.waves = packs <= 128 ? 1 : (packs <= 2048 ? 4 : 8);
     const int each = (packs + 64 * p.waves - 1) / (64 * p.waves);
     p.packs = 1;
     while (p.packs < each) p.packs *= 2;
@@ -320,8 +326,8 @@ void forward(int dtype, int residual, NormArgs& p, hipStream_t stream)
         using T = decltype(t);
         using R = decltype(u);
         const uint64_t cells = uint64_t(p.rows) * p.channels;
-        p.past = goes_past(cells * ((EIGHT ? 1 : sizeof(T)) + (p.residual ? sizeof(R) : 0)), uint64_t(p.channels) * sizeof(T));
-        by_plan<T>(plan_of<T>(p.rows, p.channels), [&](auto w, auto k) {
+        p.past = goes_past(cells * ((EIGHT ? 1 : sizeof(T)) + (p.residual ? sizeof(R) : 0)), uint64_t(p.channels) * sizeof(T), kPast);
+        by_plan<T>(plan_of<T>(p.channels), [&](auto w, auto k) {
             constexpr int W = decltype(w)::value, K = decltype(k)::value, kBlock = W > 4 ? 64 * W : kThreads, kRows = kBlock / (64 * W);
             launch_all(norm_kernel<T, R, W, K, EIGHT>, (p.rows + kRows - 1) / kRows, kBlock, stream, p);
         });
@@ -338,8 +344,8 @@ void backward(int dtype, int residual, NormArgs& p, float* dw, hipStream_t strea
             using T = decltype(t);
             using R = decltype(u);
             const uint64_t cells = uint64_t(p.rows) * p.channels;
-            p.past = goes_past(cells * (sizeof(T) + (std::is_same_v<T, R> ? 0 : sizeof(R))), uint64_t(p.channels) * sizeof(T));
-            by_plan<T>(plan_of<T>(p.rows, p.channels), [&](auto w, auto k) {
+            p.past = goes_past(cells * (sizeof(T) + (std::is_same_v<T, R> ? 0 : sizeof(R))), uint64_t(p.channels) * sizeof(T), kPast);
+            by_plan<T>(plan_of<T>(p.channels), [&](auto w, auto k) {
                 constexpr int W = decltype(w)::value, K = decltype(k)::value, kBlock = W > 4 ? 64 * W : kThreads, kRows = kBlock / (64 * W);
                 const int64_t blocks = (p.rows + kRows - 1) / kRows;
                 pieces = int(blocks < kPieces ? blocks : kPieces);

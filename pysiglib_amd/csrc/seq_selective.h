@@ -177,10 +177,9 @@ struct Column {
         part = lane / 4 % S::kQuads;
         at = lane / 4 / S::kQuads * 4 * kSets;
         group = group_;
-        const int place = tile < p.tiles ? tile : p.tiles - 1;       // a wave behind the last tile has no channels
-        column = group * p.tiles + place;
-        first = group * p.per_group + place * S::kChannels;
-        count = tile < p.tiles ? min(p.per_group - place * S::kChannels, S::kChannels) : 0;
+        column = group * p.tiles + tile;
+        first = group * p.per_group + tile * S::kChannels;
+        count = min(p.per_group - tile * S::kChannels, S::kChannels);
         load_state(p, p.a, a);
 #pragma unroll
         for (int u = 0; u < 4; ++u) a[u] *= kLog2e;
@@ -361,7 +360,7 @@ __device__ __forceinline__ Four decays(Four dt, Four a)
 // how the rows are cut
 struct Plan {
     int q, tiles;
-    int waves;              // to a block, backward: four add up their sums over channels; groups of one or two tiles would leave such blocks half empty
+    int waves;              // to a block, backward
     int64_t segment, slots, per_sequence;
     bool several;           // a sequence may have more than one segment
 };

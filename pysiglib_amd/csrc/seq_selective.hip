@@ -246,16 +246,17 @@ void check_strides(std::initializer_list<int64_t> strides)
 // four tiles to a segment 57; with gradients 95 and 200).  (16 sequences of 1024, 2048 channels of 16, bfloat16: 258 us, with 2048 waves 270;
 // 3 of 3000, 1000 channels of 64, float16: 265 and 287; but one of 50000, 256 channels of 8, bfloat16: 115 and 102, of 4: 119 and 94.)
 // Backward no more than that: the waves are all there at once, and one more would run behind them.  A packed sequence ends half a segment
-// early on average, and a block's idle waves count.  (24 sequences of up to 900, 770 channels in two groups, float16, forward and gradients: 416 us, with
-// 2352 waves 473.)
+// early on average.  (24 sequences of up to 900, 770 channels in two groups, float16, forward and gradients: 385 us, with 2352 waves and an idle one in eight 473.)
+// Backward four waves to a block add up their sums over channels where all four have all their channels, which is 1 % sooner than each alone (4 sequences of
+// 2048, 2048 channels of 16, bfloat16, forward and gradients: 589 and 594 us); with idle ones it is slower (64 of 1024, 192 channels: 548 and 492; 64 channels: 439 and 215).
 Plan plan_of(bool packed, int64_t rows, int64_t n, int64_t length, int channels, int states, int groups, bool back)
 {
     Plan p;
     p.q = lanes_of(states);
     const int wide = 256 / p.q, tile = tile_rows(p.q);
     p.tiles = (channels / groups + wide - 1) / wide;
-    p.waves = p.tiles > 2 ? kWaves : 1;
-    const int64_t columns = int64_t(groups) * (back ? (p.tiles + p.waves - 1) / p.waves * p.waves : p.tiles);
+    p.waves = channels / groups % (kWaves * wide) ? 1 : kWaves;
+    const int64_t columns = int64_t(groups) * p.tiles;
     int64_t most = back || p.q <= 2 ? 2048 : 4096, segment;
     if (packed) {
         most = std::max(most - n * columns / 2, most / 2);
@@ -273,7 +274,9 @@ Plan plan_of(bool packed, int64_t rows, int64_t n, int64_t length, int channels,
     return p;
 }
 
-// Many segments to a sequence are joined by several threads to a state
+// Many segments to a sequence are joined by several threads to a state: one of 50003, 256 channels of 8, float32, forward with 16 threads to a state 108 us, with one
+// 197; 8 of 2048, 256 channels of 16, bfloat16, 128 segments each, 66 and 68; 64 segments of 16 such sequences 96 and 87: there are then threads enough, and
+// the maps go by shared memory for nothing.
 void join_segments(const Args& p, bool back, hipStream_t stream)
 {
     const int64_t states = int64_t(p.groups) * p.tiles * 1024, count = p.offsets ? p.rows / p.segment / p.n : p.per_sequence;        // on average
