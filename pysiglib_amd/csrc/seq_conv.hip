@@ -9,6 +9,9 @@
 // Bound: HBM.  A thread takes a run of R rows of a few channels with all its loads on their way at once and keeps the window of the last
 // W - 1 rows in registers; the W - 1 rows before (backward: and behind) its run it reads again, from the caches.  Sums are 32-bit;
 // those of dw go by fixed pieces of the rows, added up in a fixed order: the same inputs give the same bits.
+// Measured, 8 sequences of 2048, 2048 channels, 4 taps, bfloat16, inputs in turn: forward 38 us (134 MB, 3.5 TB/s), gradients 71 us (201 MB, 2.8 TB/s: the loads
+// of three or four blocks of a compute unit at once, and three times the forward's arithmetic) and 4.6 us for the weights' sums; one token of 64 streams of 4096
+// channels 4.0 us.
 #include "seq_common.h"
 
 #include <type_traits>

@@ -9,6 +9,8 @@
 // Bound: HBM.  A row belongs to W waves, which hold it in registers between the sum of its squares and the output, so everything is
 // read once and written once.  Everything between load and store is 32-bit; the sums of dw go by fixed pieces of the rows, added up in
 // a fixed order: the same inputs give the same bits.
+// Measured, inputs in turn: 16384 rows of 2048, bfloat16 with a residual in float32, 79 us (403 MB, 5.1 TB/s), gradients 108 us (537 MB, 5.0 TB/s) and 5 us for
+// the weight's sums; 16384 rows of 4096, bfloat16, into 8 bits 87 us (470 MB, 5.4 TB/s, a part of it found in the last cache); 32 rows of 4096 4.1 us.
 #include "seq_common.h"
 
 #include <type_traits>

@@ -5,6 +5,8 @@
 // wave puts into shared memory of its own, so no wave waits for another.
 // Sequences too few to fill the chip are cut into segments: each forms its own last state from a zero one at its beginning, these are
 // joined one after the other with the decay of whole segments, exp(a sum dt), and then every segment runs with the state before it.
+// Measured, one sequence of 8192 steps, 4096 channels of 16 states, bfloat16 (5.4e8 steps of states): the segments' own states 115 us, their joining 13, the outputs
+// 154, vector instructions issuing in 84 % of the two passes' cycles; the reads and writes alone would take 53.  One token of 64 such streams 12 us.
 #include "seq_selective.h"
 
 #include <algorithm>
@@ -188,7 +190,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Args p, int blocks)
     }
 }
 
-// One token of each row: Q lanes to a channel, four neighbouring states to a lane
+// One token of each row: Q lanes to a channel, four neighbouring states to a lane.  Bound: HBM, a state is read and written once (34 MB of the 64 streams above,
+// 2.9 TB/s; four rows to a thread, whose a is then read once, took 11.6 us in place of 12.3, and the call with its host side the same).
 template <typename T, int Q>
 __global__ void __launch_bounds__(kThreads) step_kernel(Args p)
 {

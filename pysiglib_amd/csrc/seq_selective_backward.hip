@@ -13,7 +13,9 @@
 // registers, and these rows gone back through.
 // Sums over channels stay in a row's 64 lanes, then the block's waves, then the blocks, all in a fixed order.
 //
-// Bound: vector instructions, some twenty for each state and row.
+// Bound: vector instructions, some twenty for each state and row.  Measured, 4 sequences of 2048 steps, 2048 channels of 16 states, bfloat16 (2.7e8 steps of states): states
+// 110 us, joining 12, back 324 (vector instructions in 62 % of its cycles: two waves to a SIMD, which is what the kept states leave registers for, do not cover all of
+// each other's waits), sums over blocks and pieces 7 and 7.
 #include "seq_selective.h"
 
 #include <algorithm>

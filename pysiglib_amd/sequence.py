@@ -625,7 +625,8 @@ def selective_scan(x, delta, a, b, c, *, d=None, z=None, delta_bias=None, softpl
     ``delta + delta_bias``.
 
     ``x``, ``delta``, ``z`` (the gate, or None): ``(..., length, channels)``, or with ``offsets`` ``(rows, channels)``, the sequences packed.
-    ``a`` float32 ``(channels, states)``, meant to be negative, 1 to 64 states; ``b``, ``c``: ``(..., length, groups, states)`` or
+    ``a`` float32 ``(channels, states)``, meant to be negative (decays of many steps are formed at once: where they grow past float32's
+    range, so do the results), 1 to 64 states; ``b``, ``c``: ``(..., length, groups, states)`` or
     ``(rows, groups, states)``, each group's for ``channels / groups`` neighbouring channels; ``d``, ``delta_bias``: float32 ``(channels,)`` or None.
     ``initial_state``: float32 ``(..., channels, states)``, with ``offsets`` ``(sequences, channels, states)``; zero where it is not given.
 
