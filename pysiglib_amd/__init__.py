@@ -17,6 +17,7 @@ from .sig_length import log_sig_length, sig_length
 __all__ = ["sig", "signature", "sig_backprop", "sig_length", "sig_combine", "sig_combine_backprop", "sig_join",
            "sig_join_backprop", "linear_sig", "transform_path", "transform_path_backprop", "sig_coef", "sig_coef_backprop",
            "extract_sig_coef", "word_to_idx", "log_sig", "sig_to_log_sig", "sig_to_log_sig_backprop", "prepare_log_sig", "clear_cache",
-           "log_sig_length", "attention", "attention_backprop", "causal_conv", "causal_conv_backprop", "causal_conv_step", "linear_recurrence", "linear_recurrence_backprop", "linear_recurrence_step", "norm_residual",
-           "norm_residual_backprop", "norm_residual_float8", "norm_rotary", "norm_rotary_backprop", "rotary_tables", "selective_scan",
-           "selective_scan_backprop", "selective_scan_step", "torch_api"]
+           "log_sig_length", "attention", "attention_backprop", "causal_conv", "causal_conv_backprop", "causal_conv_step",
+           "linear_recurrence", "linear_recurrence_backprop", "linear_recurrence_step", "norm_residual", "norm_residual_backprop",
+           "norm_residual_float8", "norm_rotary", "norm_rotary_backprop", "rotary_tables", "selective_scan", "selective_scan_backprop",
+           "selective_scan_step", "torch_api"]

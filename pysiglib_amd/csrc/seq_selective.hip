@@ -16,9 +16,15 @@ namespace seqamd {
 namespace selective {
 namespace {
 
+// Waves to a SIMD that registers are kept for: three, but two where float32's rows, twice as wide, and few states to a channel, so that a wave has many channels, would
+// spill.  (Forward, two and three: one sequence of 8192, 4096 channels of 16, bfloat16, 266 and 257 us; 16 of 1000, 1024 channels of 4, bfloat16, 87 and 86; in float32 50003
+// steps of 256 of 8 113 and 122, 16 of 1000, 1024 of 16, 158 and 173, 512 of 32 144 and 137; a segment's own states of 1024 of 4 with two 105, with three 108.)
+template <typename T>
+constexpr int waves_of(int q, bool out) { return sizeof(T) == 4 && q < (out ? 8 : 2) ? 2 : 3; }
+
 // OUT: the outputs and the sequences' last states; otherwise the segments' own last states and the sums of dt
 template <typename T, int Q, bool OUT>
-__global__ void __launch_bounds__(kThreads, OUT && (sizeof(T) == 4 || Q == 1) ? 2 : 3) scan_kernel(Args p)
+__global__ void __launch_bounds__(kThreads, waves_of<T>(Q, OUT)) scan_kernel(Args p)
 {
     using S = Shape<Q>;
     constexpr int R = S::kRows, E = S::kEach, G = S::kGroups, kSets = S::kSets;
