@@ -420,7 +420,8 @@ CUSIG_AMD_API uint64_t cusig_amd_attention_backprop_workspace(uint64_t q_rows, u
 
 /* s = x + residual as it is stored in the residual's type (residual_dtype: dtype or float32), out = s (mean s^2 + eps)^-1/2 weight for each
  * row; residual null: s is x, total is not written.  out and total contiguous, weight float32 [channels]; 1 to 16384 channels.
- * scales not null: out is float8 e4m3 with the scale max |out| / 448 of each row (1 where that is zero, or the row holds NaN).
+ * scales not null: out is float8 e4m3 with the scale max |out| / 448 of each row (1 where that is zero, or the row holds NaN; infinite
+ * where the row holds an infinity, finite values are then zero and infinities NaN).
  * None of the outputs of these operators may overlap an input, but for the states that a step replaces. */
 CUSIG_AMD_API int cusig_amd_norm_residual(int dtype, int residual_dtype, const void* x, const void* residual, const float* weight, void* out,
                                           void* total, float* scales, uint64_t rows, uint64_t channels, int64_t x_stride,

@@ -139,8 +139,9 @@ __global__ void __launch_bounds__(W > 4 ? 64 * W : kThreads) norm_kernel(NormArg
         const float ratio = __uint_as_float(top) / 448.0f, scale = ratio > 0.0f ? ratio : 1.0f;       // of 3e-43 and less it is zero
         if (lane == 0) p.scales[row] = scale;
         // out / scale by the reciprocal and one correction from the remainder: the quotient's rounding, and not three, decides between two
-        // neighbours of eight bits.  The reciprocal of a scale below 2^-64 may be beyond the numbers: both move.
-        const float move = scale < 5.421010862e-20f ? 7.922816251e28f : 1.0f, divisor = scale * move, inverse = 1.0f / divisor;
+        // neighbours of eight bits.  The reciprocal of a scale below 2^-64 may be beyond the numbers: both move.  An infinite scale has the reciprocal
+        // zero, and a remainder from zero instead of from itself: finite outputs are then zero, infinite ones NaN, as out / scale is.
+        const float move = scale < 5.421010862e-20f ? 7.922816251e28f : 1.0f, inverse = 1.0f / (scale * move), divisor = inverse > 0.0f ? scale * move : 0.0f;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int at = (k * W * 64 + lane) * V;

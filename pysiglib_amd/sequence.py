@@ -424,7 +424,8 @@ def norm_residual(x, residual, weight, *, eps=1e-6):
 
 def norm_residual_float8(x, residual, weight, *, eps=1e-6):
     """``norm_residual`` with its output in 8 bits: ``out`` is ``float8_e4m3fn`` and stands for ``out * scales``, ``scales`` float32
-    ``(..., 1)`` the largest value of each row divided by 448 (1 where that is zero, or the row holds NaN).  Returns ``(out, scales, total)``."""
+    ``(..., 1)`` the largest value of each row divided by 448 (1 where that is zero, or the row holds NaN).  A row that holds an infinity has that scale:
+    its finite values are then zero and its infinities NaN, the quotients by it.  Returns ``(out, scales, total)``."""
     shape, like = x.shape if isinstance(x, torch.Tensor) else None, x
     x, x_step, residual, step, kind, weight, rows, channels = _norm_args(x, residual, weight)
     out = torch.empty(shape, dtype=torch.float8_e4m3fn, device=x.device)
