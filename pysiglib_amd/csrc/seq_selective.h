@@ -102,6 +102,15 @@ __device__ __forceinline__ float over_states(float v)
 // state + x_i b_n for 16 pairs of a quad: x the channels' in its four lanes, b the states'
 __device__ __forceinline__ Four add_products(float x, float b, Four state) { return __builtin_amdgcn_mfma_f32_4x4x1f32(x, b, state, 0, 0, 0); }
 
+// Orders the shared memory of ONE wave.  The hardware serves its accesses in the order of their issue, so lanes see what others wrote before, and
+// no wait is needed; only the compiler, to which a lane's accesses are its own, has to be kept from moving them across this point.
+__device__ __forceinline__ void wave_sync()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // The rows of a segment: `first` up to `past` of the sequence `seq`, number `k` of its segments
 struct Segment {
     int64_t seq, first, past, begin, end;       // begin, end: of the sequence

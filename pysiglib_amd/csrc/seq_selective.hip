@@ -76,6 +76,7 @@ __global__ void __launch_bounds__(kThreads, waves_of<T>(Q, OUT)) scan_kernel(Arg
             }
         }
         col.put_shared(shared, bc);
+        wave_sync();
         if (t0 + R < s.past) fetch(t0 + R);
         auto step = [&](int t) __attribute__((always_inline)) {
             float b[G], c[G];
@@ -110,6 +111,7 @@ __global__ void __launch_bounds__(kThreads, waves_of<T>(Q, OUT)) scan_kernel(Arg
 #pragma unroll 1
             for (int t = 0; t < rows; ++t) step(t);
         }
+        wave_sync();
         if constexpr (OUT) {
             float y[E][2];
 #pragma unroll
@@ -118,6 +120,7 @@ __global__ void __launch_bounds__(kThreads, waves_of<T>(Q, OUT)) scan_kernel(Arg
                 for (int k = 0; k < 2; ++k) y[i][k] = fmaf(col.d[i % S::kOwn][k], x_now[i].get(k), in[S::row(i, col.lane)][0][col.channel_of(i) + k]);
             if (p.z) col.gate(z_now, y);
             col.store(p.out, p.channels, t0, rows, y);
+            wave_sync();
         }
     }
     if constexpr (OUT) {

@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(kThreads, 2) states_kernel(Args p)
             }
         }
         col.put_shared(shared, bc);
+        wave_sync();
         if (t0 + R < s.past) fetch(t0 + R);
         auto step = [&](int t) __attribute__((always_inline)) {
             float b[G], c[G];
@@ -118,6 +119,7 @@ __global__ void __launch_bounds__(kThreads, 2) states_kernel(Args p)
                 for (int k = t; k < rows; ++k) step(k);
             }
         }
+        wave_sync();
     }
     if (s.first_one && s.last_one) return;
     col.store_own(p, p.carry, slot, h);
@@ -214,6 +216,7 @@ __global__ void __launch_bounds__(64 * W, 2) back_kernel(Args p)
 #pragma unroll
                 for (int i = 0; i < E; ++i) col.put(in[S::row(i, col.lane)][2], i, v[i][0], v[i][1]);
                 col.put_shared(shared, bc);
+                wave_sync();
             }
             auto forward = [&](int t, Four (&h)[4]) __attribute__((always_inline)) {
                 float b[G];
@@ -319,6 +322,7 @@ __global__ void __launch_bounds__(64 * W, 2) back_kernel(Args p)
                     reverse(low + part * H, start);
                 }
             }
+            wave_sync();
             // the channels' gradients of these rows
             {
                 Pack<T, 2> x[E], delta[E], z[E], g[E];

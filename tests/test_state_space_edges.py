@@ -1,5 +1,8 @@
 """Values at the ends of the number formats, and places of the state space layers that only some sizes reach (see test_state_space.py,
 whose formulas, bounds and helpers these are)."""
+import os
+import re
+
 import numpy as np
 import pytest
 
@@ -37,3 +40,29 @@ def test_norm_in_8_bits_of_infinite_outputs(P, dtype, channels):
         out = P.norm_residual(x.float(), None, w, eps=1e-6)[0]
         want = (out / scales).clamp(-448, 448)[held]
         assert np.array_equal(f64(q[held]), f64(want), equal_nan=True)
+
+
+# ---- the scan ----
+
+def test_a_waves_accesses_to_shared_memory_are_kept_in_order():
+    """The scan's waves exchange values through shared memory without a barrier.  The compiler may move a lane's reads across what other lanes
+    write, to addresses that it can tell apart from the lane's own: between the phases of a tile (its values are put there; rows are gone through;
+    pairs of channels are read), and before the next tile's, the sources have to hold it back."""
+    here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pysiglib_amd", "csrc")
+    phases = re.compile(r"(?P<put>col\.put(?:_shared)?\()|(?P<rows>col\.read_shared\()|(?P<pairs>const auto& row = in\[|\]\[col\.channel_of\(i\) \+ k\])"
+                        r"|(?P<sync>wave_sync\(\);|__syncthreads\(\);)")
+    seen = 0
+    for name in ("seq_selective.hip", "seq_selective_backward.hip"):
+        with open(os.path.join(here, name)) as fh:
+            kernels = re.split(r"__global__ void", fh.read())[1:]
+        for text in kernels:
+            found = [m.lastgroup for m in phases.finditer(text)]
+            if "put" not in found:
+                continue
+            seen += 1
+            found = found[found.index("put"):]
+            last = None
+            for phase in found + ["put"]:           # the next tile's
+                assert last in (None, "sync", phase) or phase == "sync", (name, text.split("(")[1].split()[-1], last, phase)
+                last = phase
+    assert seen == 3
