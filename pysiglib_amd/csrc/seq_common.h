@@ -27,6 +27,12 @@ struct Pack {
         else if constexpr (__is_same(T, bf16)) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
         else return static_cast<float>(__builtin_bit_cast(f16, static_cast<unsigned short>(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu)));
     }
+    // one element into words that are zero
+    __device__ __forceinline__ void put(int i, T x)
+    {
+        if constexpr (sizeof(T) == 4) w[i] = __builtin_bit_cast(unsigned, x);
+        else w[i / 2] |= static_cast<unsigned>(__builtin_bit_cast(unsigned short, x)) << (i & 1 ? 16 : 0);
+    }
     // rounds to nearest, ties to even
     __device__ __forceinline__ void set(const float* x)
     {

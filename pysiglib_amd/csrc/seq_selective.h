@@ -10,6 +10,9 @@
 // 32 and 64 states are those of 2 and 4 quads.  Q = states / 4 counts lanes to a channel, 16 pairs being a lane's: a wave has 256 / Q channels,
 // b and c are read once for four channels, dt once for four states, and the sums over states (y) and over channels (the
 // gradients of b and c) each cross few lanes.
+// Room for more states than there are holds the first ones again.  Copies of a state go through the same steps, and each has an equal part of its c
+// and of its final gradient: 1, 1/2 or 1/4 of it, which rounds nothing.  Sums over the room are then sums over the states, and nothing infinite
+// meets a zero that the formula does not have.  Gradients that are not sums over states are those of one copy times the number of copies.
 #pragma once
 #include "seq_common.h"
 
@@ -46,6 +49,12 @@ struct Shape {
     // where state n lies among the wave's in shared memory: a lane's groups beside each other
     static __host__ __device__ constexpr int place(int n) { return n / 16 * 16 + n % 4 * kGroups + n % 16 / 4; }
 };
+
+// which state place n holds, where there are places for up to twice as many as there are (for four times one)
+__device__ __forceinline__ int state_at(int n, int states) { return n < states ? n : min(n - states, states - 1); }
+
+// how many of `room` places hold state n: a power of two
+__device__ __forceinline__ float copies_of(int n, int states, int room) { return n + states >= room ? 1.0f : (n + 2 * states >= room ? 2.0f : 4.0f); }
 
 struct Args {
     const void *x, *delta, *b, *c, *z, *grad;   // z may be null; grad: of y, backward
@@ -173,11 +182,19 @@ struct Column {
     int group, column;
     int pair[S::kOwn];              // the first channels of the lane's pairs.  Where the last one would be behind the channels it is the last two
                                     // again: what two lanes form, they form alike
-    Four a[4];                      // a log2(e), zero where there is no channel or state; of set u / kG, group u % kG
+    Four a[4];                      // a log2(e), zero where there is no channel; of set u / kG, group u % kG
     float bias[S::kOwn][2], d[S::kOwn][2];
 
     __device__ __forceinline__ int channel(int u) const { return at + 4 * (u / kG); }
     __device__ __forceinline__ int state(int u) const { return part * 16 + 4 * (u % kG) + j; }
+    // the lane's number, unknown to the compiler: what is formed from it is formed where it is used and takes no registers through a loop
+    __device__ __forceinline__ int lane_again() const
+    {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        return l;
+    }
+    __device__ __forceinline__ int state_of(int l, int u, int states) const { return state_at(l / 4 % S::kQuads * 16 + 4 * (u % kG) + l % 4, states); }
 
     __device__ __forceinline__ void init(const Args& p, int group_, int tile)
     {
@@ -215,11 +232,24 @@ struct Column {
     // the lane's values of [channels][states] from `from` on; zero where there are none
     __device__ __forceinline__ void load_state(const Args& p, const float* from, Four (&h)[4]) const
     {
+        const int l = lane_again();
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                h[u][i] = from && channel(u) + i < count && state(u) < p.states ? from[int64_t(first + channel(u) + i) * p.states + state(u)] : 0.0f;
+                h[u][i] = from && channel(u) + i < count ? from[int64_t(first + channel(u) + i) * p.states + state_of(l, u, p.states)] : 0.0f;
+    }
+    // each copy's part of its state's, or (ALL) what all copies of a state have, of one's
+    template <bool ALL>
+    __device__ __forceinline__ void over_copies(const Args& p, Four (&h)[4]) const
+    {
+        if (p.states == S::kStates) return;
+        const int l = lane_again();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float n = copies_of(state_of(l, u, p.states), p.states, S::kStates);
+            h[u] *= ALL ? n : 1.0f / n;
+        }
     }
     __device__ __forceinline__ void store_state(const Args& p, float* to, const Four (&h)[4]) const
     {
@@ -308,17 +338,35 @@ struct Column {
         for (int i = 0; i < S::kPacksEach; ++i) {
             const int e = i * 64 + lane, r = min(e / (2 * Q), rows - 1), n = e % Q * 4;
             to[i] = Pack<T, 4>{};
-            if (e < S::kPacks && n < p.states) to[i] = load_some<T, 4>(e / Q % 2 ? c + r * p.c_step + n : b + r * p.b_step + n, p.states - n);
+            if (e < S::kPacks) {
+                const T* const row = e / Q % 2 ? c + r * p.c_step : b + r * p.b_step;
+                if (n + 4 <= p.states) {
+                    to[i] = load_pack<T, 4>(row + n);
+                } else {
+                    const int from = lane_again() % Q * 4;          // 64 is a multiple of Q
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) to[i].put(k, row[state_at(from + k, p.states)]);
+                }
+            }
         }
     }
-    __device__ __forceinline__ void put_shared(const Pack<T, 4> (&from)[S::kPacksEach], float (*to)[2][S::kStates]) const
+    __device__ __forceinline__ void put_shared(const Args& p, const Pack<T, 4> (&from)[S::kPacksEach], float (*to)[2][S::kStates]) const
     {
 #pragma unroll
         for (int i = 0; i < S::kPacksEach; ++i) {
             const int e = i * 64 + lane;
-            if (e < S::kPacks)
+            if (e < S::kPacks) {
+                float v[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) to[e / (2 * Q)][e / Q % 2][S::place(e % Q * 4 + k)] = from[i].get(k);
+                for (int k = 0; k < 4; ++k) v[k] = from[i].get(k);
+                if (p.states != S::kStates) {           // each copy's part of c
+                    const int l = lane_again();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] *= (i * 64 + l) / Q % 2 ? 1.0f / copies_of(state_at(l % Q * 4 + k, p.states), p.states, S::kStates) : 1.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) to[e / (2 * Q)][e / Q % 2][S::place(e % Q * 4 + k)] = v[k];
+            }
         }
     }
     // the lane's values of b or c of one row

@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kThreads, waves_of<T>(Q, OUT)) scan_kernel(Arg
                 x_now[i] = x[i], z_now[i] = z[i];
             }
         }
-        col.put_shared(shared, bc);
+        col.put_shared(p, shared, bc);
         wave_sync();
         if (t0 + R < s.past) fetch(t0 + R);
         auto step = [&](int t) __attribute__((always_inline)) {
@@ -153,9 +153,9 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Args p, int blocks)
         const int column = int(e / 1024), u = int(e / 256) % 4, l = int(e / 4) % 64, i = int(e % 4);
         const int ch = (column % p.tiles) * S::kChannels + l / 4 / S::kQuads * 4 * S::kSets + 4 * (u / S::kGroups) + i;
         const int state = l / 4 % S::kQuads * 16 + 4 * (u % S::kGroups) + l % 4;
-        const bool there = ch < p.per_group && state < p.states;
+        const bool there = ch < p.per_group;
         const int channel = column / p.tiles * p.per_group + ch;
-        const float a = there ? p.a[int64_t(channel) * p.states + state] * kLog2e : 0.0f;
+        const float a = there ? p.a[int64_t(channel) * p.states + state_at(state, p.states)] * kLog2e : 0.0f;
         // BACKWARD: from the last segment to the first.  A segment's map takes the state before it to the one behind it; the last one's is not
         // known, and not asked for.
         auto join = [&](Four* at, auto backward) __attribute__((always_inline)) {
@@ -221,10 +221,12 @@ __global__ void __launch_bounds__(kThreads) step_kernel(Args p)
     const float dt = p.softplus ? softplus_of(raw) : raw, du = dt * x;
     float now[4], y = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        now[k] = fmaf(h.get(k), __builtin_amdgcn_exp2f(dt * (a.get(k) * kLog2e)), du * b.get(k));
-        y = fmaf(c.get(k), now[k], y);
-    }
+    for (int k = 0; k < 4; ++k) now[k] = fmaf(h.get(k), __builtin_amdgcn_exp2f(dt * (a.get(k) * kLog2e)), du * b.get(k));
+    if (count < 4)          // where there is no state an infinite du has made NaN
+#pragma unroll
+        for (int k = 0; k < 4; ++k) now[k] = k < count ? now[k] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y = fmaf(c.get(k), now[k], y);
 #pragma unroll
     for (int m = 1; m < Q; m *= 2) y += __shfl_xor(y, m);
     if (p.d) y = fmaf(p.d[ch], x, y);

@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kThreads, 2) states_kernel(Args p)
                 for (int i = 0; i < E; ++i) col.put(in[S::row(i, col.lane)][2], i, v[i][0], v[i][1]);
             }
         }
-        col.put_shared(shared, bc);
+        col.put_shared(p, shared, bc);
         wave_sync();
         if (t0 + R < s.past) fetch(t0 + R);
         auto step = [&](int t) __attribute__((always_inline)) {
@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kThreads, 2) states_kernel(Args p)
         if (s.last_one && p.grad_end) {
             Four end[4];
             col.load_state(p, p.grad_end + s.seq * size, end);
+            col.template over_copies<false>(p, end);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -188,8 +189,12 @@ __global__ void __launch_bounds__(64 * W, 2) back_kernel(Args p)
         const Segment s = segment_of(p, slot);
         if (!s.there) continue;
         Four back[4];
-        if (s.last_one) col.load_state(p, p.grad_end ? p.grad_end + s.seq * size : nullptr, back);
-        else col.load_own(p, p.back, slot, back);
+        if (s.last_one) {
+            col.load_state(p, p.grad_end ? p.grad_end + s.seq * size : nullptr, back);
+            col.template over_copies<false>(p, back);
+        } else {
+            col.load_own(p, p.back, slot, back);
+        }
         const int64_t tile0 = tile_of(slot, s, kSaved), tiles = (s.past - s.first + R - 1) / R;
         for (int64_t tile = tiles - 1; tile >= 0; --tile) {
             const int64_t t0 = s.first + tile * R;
@@ -215,7 +220,7 @@ __global__ void __launch_bounds__(64 * W, 2) back_kernel(Args p)
                 if (p.z) col.gate(z, v);
 #pragma unroll
                 for (int i = 0; i < E; ++i) col.put(in[S::row(i, col.lane)][2], i, v[i][0], v[i][1]);
-                col.put_shared(shared, bc);
+                col.put_shared(p, shared, bc);
                 wave_sync();
             }
             auto forward = [&](int t, Four (&h)[4]) __attribute__((always_inline)) {
@@ -382,8 +387,12 @@ __global__ void __launch_bounds__(64 * W, 2) back_kernel(Args p)
             }
             __syncthreads();
         }
-        if (s.first_one && p.end) col.store_state(p, p.end + s.seq * size, back);
+        if (s.first_one && p.end) {
+            col.template over_copies<true>(p, back);
+            col.store_state(p, p.end + s.seq * size, back);
+        }
     }
+    col.template over_copies<true>(p, da);
     // the piece's sums over rows
     const int each = p.states + 2;
     float* const own = p.own_parts + int64_t(piece) * p.channels * each;
@@ -421,6 +430,7 @@ __global__ void __launch_bounds__(kThreads) shared_kernel(Args p, T* db, T* dc)
     }
     float sum = 0.0f;
     for (int g = 0; g < p.group_blocks; ++g) sum += p.shared_parts[((g * p.rows * p.groups + pair) * 2 + dir) * S::kStates + S::place(state)];
+    if (!dir) sum *= copies_of(state, p.states, S::kStates);
     (dir ? dc : db)[pair * p.states + state] = T(sum);
 }
 

@@ -8,7 +8,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from tests.test_state_space import DEV, P, TYPES, f64, numbers  # noqa: E402,F401
+from tests.test_state_space import DEV, NAMES, P, TYPES, f64, numbers, rounded, scan_inputs, scan_oracle, starts_of, whole_numbers  # noqa: E402,F401
 
 
 # ---- the norm in 8 bits ----
@@ -66,3 +66,55 @@ def test_a_waves_accesses_to_shared_memory_are_kept_in_order():
                 assert last in (None, "sync", phase) or phase == "sync", (name, text.split("(")[1].split()[-1], last, phase)
                 last = phase
     assert seen == 3
+
+
+def like_the_formula(got, want, bound, dtype, name):
+    """The same infinities and NaN, and what is finite within its bound (where what it is bounded by is)."""
+    got = f64(got).reshape(want.shape)
+    assert (np.isnan(got) == np.isnan(want)).all() and (np.isposinf(got) == np.isposinf(want)).all() and (np.isneginf(got) == np.isneginf(want)).all(), name
+    at = np.isfinite(want) & np.isfinite(bound)
+    bound = rounded(np.where(at, want, 0.0), np.where(at, bound, 0.0), dtype)
+    assert (np.abs(got[at] - want[at]) <= bound[at]).all(), name
+
+
+def infinite_scan(P, t, starts, packed=True):
+    """Outputs and gradients beside those of the formula: [(name, got, want, bound, type)]."""
+    dtype, n = t["x"].dtype, len(starts) - 1
+    shape = lambda v: v if packed else v.reshape(n, -1, *v.shape[1:])          # noqa: E731
+    args = [shape(t["x"]), shape(t["delta"]), t["a"], shape(t["b"]), shape(t["c"])]
+    options = dict(d=t["d"], z=shape(t["z"]), delta_bias=t["bias"], initial_state=t["h0"], offsets=whole_numbers(starts) if packed else None)
+    got = (*P.selective_scan(*args, **options), *P.selective_scan_backprop(shape(t["g"]), *args, grad_final=t["gf"], **options))
+    with np.errstate(all="ignore"):
+        want, bound = scan_oracle(*(f64(t[k]) for k in ("x", "delta", "a", "b", "c", "d", "z", "bias", "h0")), starts, True, f64(t["g"]), f64(t["gf"]))
+    kinds = (dtype, torch.float32, dtype, dtype, torch.float32, dtype, dtype, torch.float32, dtype, torch.float32, torch.float32)
+    return list(zip(NAMES, got, want, bound, kinds))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("states", [1, 2, 3, 4, 5, 7, 8, 13, 16, 20, 33, 63, 64])
+@pytest.mark.parametrize("which", ["x", "g", "h0", "gf", "delta"])
+def test_selective_scan_of_infinities_with_any_number_of_states(P, dtype, states, which):
+    """A channel's room may be for more states than it has: an infinity meets nothing there that the formula does not have."""
+    starts = starts_of([20, 0, 33, 7])
+    t = scan_inputs(dtype, 60, 4, 6, states, 2, seed=states, decays=0.3)
+    at = (40, 3) if which in ("x", "g", "delta") else (2, 3, 0)
+    t[which][at] = float("inf")
+    for name, got, want, bound, kind in infinite_scan(P, t, starts):
+        if which != "delta" or name not in ("ddelta", "dbias"):
+            like_the_formula(got, want, bound, kind, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("states", [1, 2, 3, 4, 5, 7, 13, 16, 20, 33, 63])
+@pytest.mark.parametrize("which", ["x", "h0", "delta"])
+def test_selective_scan_step_of_infinities_with_any_number_of_states(P, dtype, states, which):
+    t = scan_inputs(dtype, 5, 5, 6, states, 2, seed=states, decays=0.3)
+    t[which][(2, 3) if which != "h0" else (2, 3, 0)] = float("inf")
+    state = t["h0"].clone()
+    y = P.selective_scan_step(t["x"], t["delta"], t["a"], t["b"], t["c"], state, d=t["d"], z=t["z"], delta_bias=t["bias"])
+    with np.errstate(all="ignore"):
+        want, bound = scan_oracle(*(f64(t[k]) for k in ("x", "delta", "a", "b", "c", "d", "z", "bias", "h0")), list(range(6)), True)
+    like_the_formula(y, want[0], bound[0], dtype, "y")
+    like_the_formula(state, want[1], bound[1], torch.float32, "state")
