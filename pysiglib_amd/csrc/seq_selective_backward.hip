@@ -346,11 +346,11 @@ __global__ void __launch_bounds__(64 * W, 2) back_kernel(Args p)
                         gy[i][k] = g[i].get(k);
                         v[i][k] = fmaf(row[1][ch], kLn2, row[0][ch] * x[i].get(k));
                     }
-                if (p.softplus)         // its slope: e^(raw - softplus(raw))
+                if (p.softplus)         // its slope: e^(raw - softplus(raw)), 1 where both are infinite (fminf takes the number; a raw NaN is in v already)
 #pragma unroll
                     for (int i = 0; i < E; ++i)
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) v[i][k] *= __builtin_amdgcn_exp2f((delta[i].get(k) + col.bias[i % S::kOwn][k] - dt[i][k]) * kLog2e);
+                        for (int k = 0; k < 2; ++k) v[i][k] *= __builtin_amdgcn_exp2f(fminf(delta[i].get(k) + col.bias[i % S::kOwn][k] - dt[i][k], 0.0f) * kLog2e);
                 col.store(p.ddelta, p.channels, t0, rows, v);
 #pragma unroll
                 for (int i = 0; i < E; ++i)

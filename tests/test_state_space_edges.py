@@ -118,3 +118,20 @@ def test_selective_scan_step_of_infinities_with_any_number_of_states(P, dtype, s
         want, bound = scan_oracle(*(f64(t[k]) for k in ("x", "delta", "a", "b", "c", "d", "z", "bias", "h0")), list(range(6)), True)
     like_the_formula(y, want[0], bound[0], dtype, "y")
     like_the_formula(state, want[1], bound[1], torch.float32, "state")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("states", [1, 4, 7, 16, 40])
+@pytest.mark.parametrize("row", [0, 19, 40, 59])
+def test_selective_scan_gradient_of_an_infinite_step(P, dtype, states, row):
+    """softplus has the slope 1 there, and everything before the step is forgotten: the gradient is that of x's product alone."""
+    t = scan_inputs(dtype, 60, 2, 6, states, 2, seed=states, decays=0.3)
+    t["delta"][row, 3] = float("inf")
+    for name, got, want, bound, kind in infinite_scan(P, t, [0, 20, 60]):
+        like_the_formula(got, want, bound, kind, name)
+        if name == "ddelta":
+            assert np.isfinite(want[row, 3])
+    t["delta"][row, 3] = float("nan")
+    _, got, want, _, _ = infinite_scan(P, t, [0, 20, 60])[3]
+    assert torch.isnan(got[row, 3]) and np.isnan(want[row, 3])
