@@ -8,7 +8,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from tests.test_state_space import DEV, NAMES, P, TYPES, f64, numbers, rounded, scan_inputs, scan_oracle, starts_of, whole_numbers  # noqa: E402,F401
+from tests.test_state_space import (DEV, NAMES, P, TYPES, U32, check_scan, f64, numbers, raw, rounded, scan_inputs, scan_oracle, starts_of,  # noqa: E402,F401
+                                    whole_numbers)
 
 
 # ---- the norm in 8 bits ----
@@ -40,6 +41,27 @@ def test_norm_in_8_bits_of_infinite_outputs(P, dtype, channels):
         out = P.norm_residual(x.float(), None, w, eps=1e-6)[0]
         want = (out / scales).clamp(-448, 448)[held]
         assert np.array_equal(f64(q[held]), f64(want), equal_nan=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("channels", [64, 2048, 16384])
+@pytest.mark.parametrize("scale", [2.0 ** -60, 1.1 * 2.0 ** -64, 2.0 ** -64, 0.9 * 2.0 ** -64, 1.3 * 2.0 ** -126, 2.0 ** -126, 0.7 * 2.0 ** -126, 2.0 ** -140, 5 * 2.0 ** -149,
+                                   2.0 ** -149, 1e30])
+def test_norm_in_8_bits_with_scales_at_the_ends_of_float32(P, dtype, channels, scale):
+    """Entries of one size in a row whose length is a power of two: the norm is 1, and the outputs are the weights.  The scale is off by its rounding,
+    half a step, which is all of a subnormal one's; the quotient by it is off by a correction's few roundings and by half a step of the format,
+    2^-4 of the value, or 2^-10 among the smallest."""
+    rng = np.random.default_rng(channels)
+    x = torch.tensor(rng.choice([-1.0, 1.0], (3, channels))).to(dtype).to(DEV)
+    w = np.float32(448 * scale * np.exp2(-12 * rng.random(channels)) * rng.choice([-1.0, 1.0], channels))
+    w[5] = np.float32(448 * scale)
+    q, scales, _ = P.norm_residual_float8(x, None, torch.tensor(w, device=DEV), eps=0.0)
+    out, top = f64(x) * w.astype(np.float64), float(np.abs(w).max())
+    assert (np.abs(f64(scales) - top / 448) <= np.maximum(U32 * top / 448, 2.0 ** -150)).all() and (f64(scales) > 0).all()
+    v = np.clip(out / f64(scales), -448, 448)
+    assert (np.abs(f64(q.float()) - v) <= np.maximum(2.0 ** -4 * np.abs(v), 2.0 ** -10) * (1 + 8 * U32) + 4 * U32 * np.abs(v)).all()
+    assert (np.sign(f64(q.float())) * np.sign(out) >= 0).all() and (np.abs(f64(q.float())).max(-1) >= 448 * 2 / 3).all()
 
 
 # ---- the scan ----
@@ -135,3 +157,74 @@ def test_selective_scan_gradient_of_an_infinite_step(P, dtype, states, row):
     t["delta"][row, 3] = float("nan")
     _, got, want, _, _ = infinite_scan(P, t, [0, 20, 60])[3]
     assert torch.isnan(got[row, 3]) and np.isnan(want[row, 3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("channels,states,groups", [(1024, 4, 1), (512, 8, 1), (256, 16, 1), (512, 16, 2), (128, 32, 1), (64, 64, 1), (256, 13, 1), (1024, 3, 1)])
+def test_selective_scan_with_four_full_waves_to_a_block(P, dtype, channels, states, groups):
+    """Channels of a group that fill four waves: their gradients come from blocks of four waves, which add up their sums over channels."""
+    t = scan_inputs(dtype, 100, 2, channels, states, groups, seed=channels + states)
+    check_scan(P, t, [0, 50, 100], False)
+    check_scan(P, t, [0, 37, 100], True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,channels,states", [([1200], 6, 16), ([1043], 5, 20), ([300], 9, 4), ([330], 7, 3), ([700], 300, 8), ([1500, 0, 1500, 1600], 4, 16),
+                                                     ([301, 2, 500], 3, 2)])
+def test_selective_scan_of_many_segments(P, dtype, lengths, channels, states):
+    """More than 64 segments to a sequence: several threads to a state join them."""
+    starts = starts_of(lengths)
+    t = scan_inputs(dtype, starts[-1], len(lengths), channels, states, 1, seed=channels)
+    if len(lengths) == 1:
+        check_scan(P, t, starts, False)
+    check_scan(P, t, starts, True)
+
+
+# ---- offsets that make no sense ----
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("states", [3, 16])
+def test_offsets_that_do_not_ascend_write_only_into_the_outputs(P, dtype, states):
+    """Every output and the workspace lies in a buffer that holds a mark before and behind it."""
+    from pysiglib_amd import _loader as L
+    rows, channels, code, margin = 500, 20, L.SEQUENCE_DTYPES[str(dtype).split(".")[1]], 65536
+    rng = np.random.default_rng(states)
+    buffers = []
+
+    def inside(like=None, size=0):
+        size = like.numel() * like.element_size() if like is not None else size
+        whole = torch.full((size + 2 * margin,), 0x5A, dtype=torch.uint8, device=DEV)
+        buffers.append((whole, size))
+        part = whole[margin:margin + size]
+        return part if like is None else part.view(like.dtype)
+
+    def untouched(what):
+        for whole, size in buffers:
+            assert (whole[:margin] == 0x5A).all() and (whole[margin + size:] == 0x5A).all(), what
+        buffers.clear()
+
+    w, bias = numbers(rng, channels, 4), numbers(rng, channels)
+    strides = (channels, channels, channels, 2 * states, 2 * states, 2 * states, 2 * states)
+    for offsets in ([300, 100, 500, 0], [0, 500, 0, 500], [500, 0, 0, 0], [1 << 30, -1 << 30, 7, 1 << 30], [0, 500, 100, 200, 300, 50, 500, -7], [499, 1, 498, 2, 497, 3],
+                    [7, 7, 7, 1, 1, 1, 500, 500, 9]):
+        at, n = whole_numbers(offsets), len(offsets) - 1
+        t = scan_inputs(dtype, rows, n, channels, states, 1, seed=1)
+        state = numbers(rng, n, 3, channels, dtype=dtype)
+        raw(L.CUSIG_CAUSAL_CONV, code, t["x"], w, bias, state, inside(t["x"]), inside(state), at, n, 0, rows, channels, 4, channels, True)
+        untouched(("conv", offsets))
+        size = L.CUSIG_CAUSAL_CONV_BACKPROP_WORKSPACE(rows, channels, 4)
+        raw(L.CUSIG_CAUSAL_CONV_BACKPROP, code, t["g"], t["x"], w, bias, state, state, inside(t["x"]), inside(w), inside(bias), inside(state), at, n, 0, rows, channels, 4,
+            channels, channels, True, inside(size=size), size)
+        untouched(("conv gradients", offsets))
+        inputs = [t[k] for k in ("x", "delta", "a", "b", "c", "d", "z", "bias")]
+        size = L.CUSIG_SELECTIVE_SCAN_WORKSPACE(True, n, 0, rows, channels, states, 1)
+        raw(L.CUSIG_SELECTIVE_SCAN, code, *inputs, t["h0"], inside(t["x"]), inside(t["h0"]), at, n, 0, rows, channels, states, 1, *strides, True, inside(size=size), size)
+        untouched(("scan", offsets))
+        size = L.CUSIG_SELECTIVE_SCAN_BACKPROP_WORKSPACE(True, n, 0, rows, channels, states, 1)
+        grads = [inside(t[k]) for k in ("x", "delta", "a")] + [inside(t["b"].contiguous()) for _ in range(2)] + [inside(t[k]) for k in ("d", "z", "bias", "h0")]
+        raw(L.CUSIG_SELECTIVE_SCAN_BACKPROP, code, t["g"], *inputs, t["gf"], t["h0"], *grads, at, n, 0, rows, channels, states, 1, channels, *strides, True,
+            inside(size=size), size)
+        untouched(("scan gradients", offsets))
