@@ -22,9 +22,11 @@ constexpr int kThreads = 256;
 // Of the rows at most, for the gradient of the weight: 16384 rows of 2048 channels, bfloat16, both directions 109 us, with 512 pieces 112, with 2048 115
 constexpr int kPieces = 1024;
 
-// Results of this size leave the last cache before they are read.  16384 rows of 2048 channels, bfloat16 (134 MB), both directions, past the caches 111 us, kept 103;
-// 8192 rows of 8192 into 8 bits (201 MB) 90 and 92; 16384 of 4096 (268 MB) 94 and 96; 8192 of 8192, float32, both directions 371 and 395.
-constexpr uint64_t kPast = uint64_t(192) << 20;
+// From how many bytes of results on they are stored past the caches, in MiB; of those that may be, which the 8-bit output is not.  Kept and past, us, inputs in
+// turn.  Forward, 2048 channels, bfloat16: 120 MiB 46 and 47, 136 51 and 53, 152 60 and 58, 200 79 and 76; with a copy that reads the results 136 98 and 104,
+// 152 117 and 115; forward and gradients 136 95 and 98, 168 115 and 117, 184 132 and 126; the sum in float32 136 136 and 123, 152 149 and 136.  Into 8 bits, 4096 channels,
+// where the layer behind reads the 8 bits and not the sum: 88 MiB of sums 63 and 58, 120 84 and 79; with a copy that reads the sum 88 90 and 99, 104 115 and 116, 120 132 and 130.
+constexpr uint64_t kPast = uint64_t(144) << 20, kPastEight = uint64_t(112) << 20;
 
 struct NormArgs {
     const void *x, *residual;       // residual null: the sum is x, and not written
@@ -329,7 +331,7 @@ void forward(int dtype, int residual, NormArgs& p, hipStream_t stream)
         using T = decltype(t);
         using R = decltype(u);
         const uint64_t cells = uint64_t(p.rows) * p.channels;
-        p.past = goes_past(cells * ((EIGHT ? 1 : sizeof(T)) + (p.residual ? sizeof(R) : 0)), uint64_t(p.channels) * sizeof(T), kPast);
+        p.past = goes_past(cells * ((EIGHT ? 0 : sizeof(T)) + (p.residual ? sizeof(R) : 0)), uint64_t(p.channels) * sizeof(T), EIGHT ? kPastEight : kPast);
         by_plan<T>(plan_of<T>(p.channels), [&](auto w, auto k) {
             constexpr int W = decltype(w)::value, K = decltype(k)::value, kBlock = W > 4 ? 64 * W : kThreads, kRows = kBlock / (64 * W);
             launch_all(norm_kernel<T, R, W, K, EIGHT>, (p.rows + kRows - 1) / kRows, kBlock, stream, p);

@@ -8,8 +8,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from tests.test_state_space import (DEV, NAMES, P, TYPES, U32, check_scan, f64, numbers, raw, rounded, scan_inputs, scan_oracle, starts_of,  # noqa: E402,F401
-                                    whole_numbers)
+from tests.test_state_space import (DEV, NAMES, P, TYPES, U32, check_scan, f64, numbers, raw, rounded, same_bits, scan_inputs, scan_oracle,  # noqa: E402,F401
+                                    starts_of, whole_numbers)
 
 
 # ---- the norm in 8 bits ----
@@ -62,6 +62,26 @@ def test_norm_in_8_bits_with_scales_at_the_ends_of_float32(P, dtype, channels, s
     v = np.clip(out / f64(scales), -448, 448)
     assert (np.abs(f64(q.float()) - v) <= np.maximum(2.0 ** -4 * np.abs(v), 2.0 ** -10) * (1 + 8 * U32) + 4 * U32 * np.abs(v)).all()
     assert (np.sign(f64(q.float())) * np.sign(out) >= 0).all() and (np.abs(f64(q.float())).max(-1) >= 448 * 2 / 3).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,stream", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.float32, torch.float32)])
+def test_norm_of_results_that_go_past_the_caches(P, dtype, stream):
+    """Large results are stored in another way: the bits are those of the same rows in small calls."""
+    rows, channels, part = 40000, 1024, 5000
+    assert rows * channels * 2 * (2 if stream == torch.float32 else 1) * 2 > 144 << 20 > part * channels * 8
+    gen = torch.Generator(DEV).manual_seed(1)
+    make = lambda kind: torch.randn((rows, channels), generator=gen, device=DEV).to(kind)          # noqa: E731
+    x, r, g, after, w = make(dtype), make(stream), make(dtype), make(stream), torch.randn(channels, generator=gen, device=DEV)
+    out, total = P.norm_residual(x, r, w)
+    dx, dr, _ = P.norm_residual_backprop(g, total, w, grad_total=after)
+    wide = torch.cat((x, x), 1), torch.cat((r, r), 1), torch.cat((w, w))
+    q, scales, sums = P.norm_residual_float8(*wide)
+    for i in range(0, rows, part):
+        at = slice(i, i + part)
+        same_bits((out[at], total[at]), P.norm_residual(x[at], r[at], w))
+        same_bits((dx[at], dr[at]), P.norm_residual_backprop(g[at], total[at], w, grad_total=after[at])[:2])
+        same_bits((q[at], scales[at], sums[at]), P.norm_residual_float8(wide[0][at], wide[1][at], wide[2]))
 
 
 # ---- the scan ----
