@@ -459,7 +459,8 @@ CUSIG_AMD_API int cusig_amd_causal_conv_step(int dtype, const void* x, void* sta
  * delta_bias) or delta + delta_bias and f(z) = z / (1 + exp(-z)); d, z and delta_bias may be null.  x, delta, z, y [rows, channels]
  * (y contiguous), offsets or null as above; a float32 [channels, states], d and delta_bias float32 [channels]; b, c [rows, groups,
  * states], the last axis contiguous: neighbouring channels share a group's; 1 to 64 states.  initial_state (may be null: zero) and
- * final_state float32 [sequences, channels, states].  Rows of x, delta, z (and of y's gradient) are 0 to 2^24 elements apart. */
+ * final_state float32 [sequences, channels, states].  Rows of x, delta, z (and of y's gradient) are 0 to 2^24 elements apart.  In time and scratch, numbers
+ * of states are rounded up to 4, 8, 16, 32 or 64, and each group's channels to 256, 128, 64, 32 or 16 of them. */
 CUSIG_AMD_API int cusig_amd_selective_scan(int dtype, const void* x, const void* delta, const float* a, const void* b, const void* c,
                                            const float* d, const void* z, const float* delta_bias, const float* initial_state, void* y,
                                            float* final_state, const int* offsets, uint64_t sequences, uint64_t length, uint64_t rows,

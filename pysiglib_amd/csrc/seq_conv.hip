@@ -6,12 +6,14 @@
 // dx_p = sum_j w_{W - 1 - j} e_{p + j} over the positions p + j of the sequence, plus the gradient of the final state where p is one of the
 // last W - 1 positions; for p < 0 that is the gradient of the initial state.  dw_k = sum_p e_p x_{p - W + 1 + k}, dbias = sum_p e_p.
 //
-// Bound: HBM.  A thread takes a run of R rows of a few channels with all its loads on their way at once and keeps the window of the last
+// Bound: forward HBM and the loads that are on their way, backward those and vector instructions (47 and 57 % of the cycles): a load's row is cut to the tensor and multiplied
+// in 64 bits, and short runs read their weights and the rows before them again.  A thread takes a run of R rows of a few channels with all its loads on their way at once and keeps the window of the last
 // W - 1 rows in registers; the W - 1 rows before (backward: and behind) its run it reads again, from the caches.  Sums are 32-bit;
 // those of dw go by fixed pieces of the rows, added up in a fixed order: the same inputs give the same bits.
 // Measured, 8 sequences of 2048, 2048 channels, 4 taps, bfloat16, inputs in turn: forward 38 us (134 MB, 3.5 TB/s), gradients 71 us (201 MB, 2.8 TB/s: the loads
 // of three or four blocks of a compute unit at once, and three times the forward's arithmetic) and 4.6 us for the weights' sums; one token of 64 streams of 4096
-// channels 4.0 us.
+// channels 3.9 us.  In memory instead of registers are the rows of float32's gradients (48 to 128 bytes a lane with 2 to 8 taps: the edges' path takes them by a pointer) and, forward, those of
+// fewer channels than a pack has (272 bytes).
 #include "seq_common.h"
 
 #include <type_traits>
@@ -22,7 +24,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWidest = 8;
 // Rows that a thread takes at once, backward.  8 sequences of 2048, 2048 channels, bfloat16, both directions: 111 us, with 2 rows 128, with 8 109, but in float32, 1024
-// channels, 100 and 128.
+// channels, whose rows the compiler keeps in memory, 100 and 128.
 constexpr int kAtOnce = 4;
 
 struct ConvArgs {

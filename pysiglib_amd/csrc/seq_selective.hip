@@ -5,8 +5,9 @@
 // wave puts into shared memory of its own, so no wave waits for another.
 // Sequences too few to fill the chip are cut into segments: each forms its own last state from a zero one at its beginning, these are
 // joined one after the other with the decay of whole segments, exp(a sum dt), and then every segment runs with the state before it.
-// Measured, one sequence of 8192 steps, 4096 channels of 16 states, bfloat16 (5.4e8 steps of states): the segments' own states 115 us, their joining 13, the outputs
-// 154, vector instructions issuing in 84 % of the two passes' cycles; the reads and writes alone would take 53.  One token of 64 such streams 12 us.
+// Measured, one sequence of 8192 steps, 4096 channels of 16 states, bfloat16 (5.4e8 steps of states): the segments' own states 111 us, their joining 13, the outputs
+// 148, each kernel by itself under a profiler; the call takes 254.  Vector instructions issue in 83 % of the two passes' cycles; the reads and writes alone would take
+// 53 us.  One token of 64 such streams 11 us.
 #include "seq_selective.h"
 
 #include <algorithm>
@@ -17,7 +18,8 @@ namespace selective {
 namespace {
 
 // Waves to a SIMD that registers are kept for: three, but two where float32's rows, twice as wide, and few states to a channel, so that a wave has many channels, would
-// spill.  (Forward, two and three: one sequence of 8192, 4096 channels of 16, bfloat16, 266 and 257 us; 16 of 1000, 1024 channels of 4, bfloat16, 87 and 86; in float32 50003
+// spill.  Three leave room for all but a few in five kernels: the outputs' of 16-bit types keep 10 registers in memory with 16 states and 7 with up to four, of float32 2 with
+// 32, outside their loops over rows.  (Forward, two and three: one sequence of 8192, 4096 channels of 16, bfloat16, 266 and 257 us; 16 of 1000, 1024 channels of 4, bfloat16, 87 and 86; in float32 50003
 // steps of 256 of 8 113 and 122, 16 of 1000, 1024 of 16, 158 and 173, 512 of 32 144 and 137; a segment's own states of 1024 of 4 with two 105, with three 108.)
 template <typename T>
 constexpr int waves_of(int q, bool out) { return sizeof(T) == 4 && q < (out ? 8 : 2) ? 2 : 3; }
@@ -199,8 +201,9 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Args p, int blocks)
     }
 }
 
-// One token of each row: Q lanes to a channel, four neighbouring states to a lane.  Bound: HBM, a state is read and written once (34 MB of the 64 streams above,
-// 2.9 TB/s; four rows to a thread, whose a is then read once, took 11.6 us in place of 12.3, and the call with its host side the same).
+// One token of each row: Q lanes to a channel, four neighbouring states to a lane.  Bound: vector instructions, in 72 % of the cycles, 213 to a wave, of which the formula
+// needs some 60 and the addresses the most: a division of 64 bits for the row, one for the group, products of rows and distances.  (34 MB of states of the 64 streams above,
+// read and written, at 3.0 TB/s; four rows to a thread, whose a is then read once, took 11.6 us in place of 12.3, and the call with its host side the same.)
 template <typename T, int Q>
 __global__ void __launch_bounds__(kThreads) step_kernel(Args p)
 {

@@ -14,8 +14,11 @@
 // Sums over channels stay in a row's 64 lanes, then the block's waves, then the blocks, all in a fixed order.
 //
 // Bound: vector instructions, some twenty for each state and row.  Measured, 4 sequences of 2048 steps, 2048 channels of 16 states, bfloat16 (2.7e8 steps of states): states
-// 110 us, joining 12, back 324 (vector instructions in 62 % of its cycles: two waves to a SIMD, which is what the kept states leave registers for, do not cover all of
-// each other's waits), sums over blocks and pieces 7 and 7.
+// 111 us, joining 12, back 328, sums over blocks and pieces 7 and 8, each kernel by itself under a profiler.  Vector instructions take 61 % of back's cycles: two waves to a
+// SIMD, which is what the kept states leave registers for, do not cover all of each other's waits, and their 256 registers do not hold everything that lives through a
+// tile.  back_kernel keeps 56 (bfloat16, 64 states) to 192 registers (float32, up to four) in memory, 228 to 764 bytes to a lane, 444 in the case above; its
+// loop over rows is free of that, but each tile of 16 rows stores some 20 words a lane there and loads 40, and the kernel writes 251 MB where its results and the partial
+// sums are 119.  states_kernel<float> with the gradients' part keeps 3 to 51 with up to 32 states.
 #include "seq_selective.h"
 
 #include <algorithm>

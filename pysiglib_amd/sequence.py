@@ -631,6 +631,10 @@ def selective_scan(x, delta, a, b, c, *, d=None, z=None, delta_bias=None, softpl
     ``(rows, groups, states)``, each group's for ``channels / groups`` neighbouring channels; ``d``, ``delta_bias``: float32 ``(channels,)`` or None.
     ``initial_state``: float32 ``(..., channels, states)``, with ``offsets`` ``(sequences, channels, states)``; zero where it is not given.
 
+    Numbers of states are rounded up to 4, 8, 16, 32 or 64, and each group's channels to 256, 128, 64, 32 or 16 of them, in time: many small groups cost
+    most.  States that are not finite stay so; long sequences are cut, and whether such a state is infinite or NaN behind a cut may differ from a walk
+    step by step.
+
     Returns ``(y, final_state)``: ``y`` like ``x``, the states behind the last steps like ``initial_state``.
     """
     _tensor(x, "x")
@@ -660,7 +664,11 @@ def selective_scan_backprop(grad_y, x, delta, a, b, c, *, d=None, z=None, delta_
     """Gradients of ``selective_scan`` from the gradients of its outputs (``grad_final`` float32 like the final state, zero where it is not
     given) and its inputs; the states are formed again.  Returns ``(grad_x, grad_delta, grad_a, grad_b, grad_c, grad_d, grad_z,
     grad_delta_bias, grad_initial_state)``, None for what was not given; those of float32 inputs and of the initial state are float32.  The
-    same inputs give the same bits."""
+    same inputs give the same bits.
+
+    Its scratch holds the states before every eighth row (every fourth with up to 4 states), half a byte (a byte) for each row, channel and state, these
+    rounded up as in ``selective_scan``, and each row's sums over 1024 or 4096 pairs of channel and state, 8 bytes for each state: 5.4 GB for 32768 rows of
+    4096 channels of 64 states."""
     _tensor(x, "x")
     if x.dim() < 2:
         raise ValueError("x must have at least rank 2, got rank " + str(x.dim()) + ".")
