@@ -11,7 +11,7 @@
 // b and c are read once for four channels, dt once for four states, and the sums over states (y) and over channels (the
 // gradients of b and c) each cross few lanes.
 // Room for more states than there are holds the first ones again.  Copies of a state go through the same steps, and each has an equal part of its c
-// and of its final gradient: 1, 1/2 or 1/4 of it, which rounds nothing.  Sums over the room are then sums over the states, and nothing infinite
+// and of its final gradient: 1, 1/2 or 1/4 of it, which rounds no normal number.  Sums over the room are then sums over the states, and nothing infinite
 // meets a zero that the formula does not have.  Gradients that are not sums over states are those of one copy times the number of copies.
 #pragma once
 #include "seq_common.h"
